@@ -281,6 +281,61 @@ int vk_select_update(const float *logits, const void *h, const void *norm_w, flo
                      void *stream);
 
 /*
+ * Rules on logits [B, V] (bf16 or fp32, row stride ld): penalties for repeated tokens, bias, grammar mask. For sequence b
+ * and token v, with x = logits[b, v] in fp32 and c = the number of t < hist_len[b] with hist[b * hist_ld + t] == v:
+ *   c > 0: z = x > 0 ? x / rep_b : x * rep_b;  z -= freq_b * c;  z -= pres_b;   then z += bias[b * bias_ld + v];
+ *   bit v % 32 of word v / 32 of the sequence's mask row clear: z = -inf, whatever it was;
+ * each step rounded to fp32 in this order, z rounded once to out's dtype. rep / pres / freq: [B] fp32, or NULL for the
+ * scalars rep0 / pres0 / freq0 (repetition penalties are positive; 1, 0 and 0 change nothing). hist [B, hist_cols] int64
+ * (at most 65535 columns; ids outside [0, V) count nowhere), hist_len [B] int32 clamped to 0 .. hist_cols; hist NULL: no
+ * penalties. bias NULL: none; bias_ld 0: one row for all. allowed [n_allowed, allowed_ld] 32-bit words; allowed_rows [B]
+ * int32 names each sequence's mask row, one outside 0 .. n_allowed - 1 meaning no mask; NULL: the one row, or row b of B.
+ * allowed NULL: no masks. out [B, V] bf16 or fp32 (row stride out_ld) may be logits itself (same dtype and stride).
+ * No reference counterpart: the reference's rules are the bias and the k-mer grammar of viktor/engine.py:79-116.
+ */
+int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, const int64_t *hist, int64_t hist_ld,
+                      int64_t hist_cols, const int32_t *hist_len, const float *rep, float rep0, const float *pres,
+                      float pres0, const float *freq, float freq0, const float *bias, int64_t bias_ld,
+                      const uint32_t *allowed, int64_t allowed_ld, int64_t n_allowed, const int32_t *allowed_rows,
+                      void *out, int32_t out_dtype, int64_t out_ld, int64_t B, int32_t V, void *stream);
+
+/*
+ * The token choice over a vocabulary of any size after the rules of vk_process_logits (z, in fp32; nothing of it is
+ * written). temp [B] fp32, or NULL for temp0; z' = z / T where T > 0, else z' = z and the choice is greedy.
+ *   mode 0: the first index of max z';
+ *   mode 1: the first index of max z'_v - log(-log(max(u_v, 1e-20))), u_v = uniforms[b * u_ld + v] (scores closer than
+ *           fp32 can tell are compared in fp64);
+ *   mode 2: the first v with u < sum_{w <= v} softmax(z')_w, u = uniforms[b * u_ld] (sums over slices in fp64).
+ * token[b] (int64) and logp[b] = log softmax(z')[token] (NULL: not written). NaN is never chosen and weighs nothing, +inf
+ * counts as the largest finite value; a row whose mask and bias leave nothing gives `fallback` and -inf.
+ * workspace: vk_choose_tokens_workspace() bytes, 16-byte aligned.
+ */
+int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t *bytes);
+int vk_choose_tokens(const void *logits, int32_t dtype, int64_t ld, const int64_t *hist, int64_t hist_ld,
+                     int64_t hist_cols, const int32_t *hist_len, const float *rep, float rep0, const float *pres,
+                     float pres0, const float *freq, float freq0, const float *bias, int64_t bias_ld,
+                     const uint32_t *allowed, int64_t allowed_ld, int64_t n_allowed, const int32_t *allowed_rows,
+                     const float *temp, float temp0, int32_t mode, const float *uniforms, int64_t u_ld,
+                     int64_t fallback, int64_t *token, float *logp, int64_t B, int32_t V, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+
+/*
+ * vk_select_update from logits at any vocabulary, with the rules of vk_process_logits: one decode step's choice
+ * (vk_choose_tokens) and bookkeeping (vk_select_update's: tail and homopolymer rules, PAD, output column, state). The
+ * history is what the sequence has produced, out[b, 0 .. pos[b] - plen[b] - 1]; the mask row is token_rows[tok[b]]
+ * ([V] int32, by the previous token). uniforms [B, u_cols] (mode 2) or [B, u_cols, V] (mode 1), row stride u_ld, read at
+ * the output column. A row with nothing left takes pad. Other arguments as vk_select_update's and vk_choose_tokens'.
+ */
+int vk_choose_update(const void *logits, int32_t dtype, int64_t ld, float rep0, float pres0, float freq0,
+                     const float *bias, const uint32_t *allowed, int64_t allowed_ld, int64_t n_allowed,
+                     const int32_t *token_rows, const uint8_t *is_tail, const uint8_t *is_homo, int32_t homo_stop,
+                     float temperature, int32_t mode, const float *uniforms, int64_t u_ld, int64_t u_cols, int64_t *tok,
+                     int64_t *run, int64_t *pos, const int64_t *plen, const int64_t *rope_off,
+                     const int64_t *cache_base, int64_t *out, int64_t out_stride, int64_t out_cols, int32_t *pos32,
+                     int32_t *seqlens, int32_t *rpos32, float *logp, int64_t logp_stride, int64_t B, int32_t V,
+                     int32_t eos, int32_t pad, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
  * Decode-step fusions (small M: one row per sequence). Same rounding points as the unfused ops.
  *
  * vk_norm_qkv_rope_cache: h = RMSNorm(x) * norm_w (x [M, K] bf16; or, with tok non-NULL, x = emb[tok] with
@@ -443,6 +498,25 @@ int vk_embed_grad_workspace(int64_t n, int32_t V, int32_t d, int64_t *bytes);
  */
 int vk_embed_grad(const void *d_rows, int32_t d_dtype, int64_t ld, const int64_t *tokens, int64_t n, int32_t V, int32_t d,
                   float *out, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * out[r, :] = scale * w[tokens[r], :] (product in fp32, one rounding; w [V, d] and out [n, d] bf16 or fp32, contiguous,
+ * any width). Ids outside [0, V) give zero rows. The lookup of nn.Embedding (viktor/decoder.py:127, viktor/model.py:77).
+ */
+int vk_embed_lookup(const void *w, int32_t w_dtype, const int64_t *tokens, int64_t n, int64_t V, int32_t d, float scale,
+                    void *out, int32_t out_dtype, void *stream);
+
+/*
+ * vk_embed_grad for large vocabularies, by sorted tokens: out[v, :] = scale * sum over tokens[r] == v of d_rows[r, :]
+ * (+ the old out[v, :] with accumulate != 0), fp32 sums in an order that n, V and the ids alone decide. d_rows [n, d] bf16
+ * or fp32, row stride ld, any width; ids outside [0, V) and rows of the id `pad` (negative: none) add nothing; a row
+ * without ids is zero (accumulate: left as it is). n < 2^31 - 2048; workspace: vk_embed_grad_sorted_workspace() bytes,
+ * 16-byte aligned.
+ */
+int vk_embed_grad_sorted_workspace(int64_t n, int32_t V, int32_t d, int64_t *bytes);
+int vk_embed_grad_sorted(const void *d_rows, int32_t d_dtype, int64_t ld, const int64_t *tokens, int64_t n, int32_t V,
+                         int32_t d, float scale, int64_t pad, float *out, int32_t accumulate, void *workspace,
+                         int64_t workspace_bytes, void *stream);
 
 /* Workgroups (= rows of the weight-gradient partials) vk_rmsnorm_backward uses for n rows. */
 int vk_rmsnorm_backward_blocks(int64_t n, int32_t *blocks);

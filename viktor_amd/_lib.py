@@ -67,6 +67,16 @@ SIGNATURES = {
     "vk_act_backward": [_P, _P, _P, _P, _I32, _I64, _I32, _I32, _P],
     "vk_embed_grad_workspace": [_I64, _I32, _I32, ctypes.POINTER(_I64)],
     "vk_embed_grad": [_P, _I32, _I64, _P, _I64, _I32, _I32, _P, _P, _I64, _P],
+    "vk_embed_lookup": [_P, _I32, _P, _I64, _I64, _I32, _F, _P, _I32, _P],
+    "vk_embed_grad_sorted_workspace": [_I64, _I32, _I32, ctypes.POINTER(_I64)],
+    "vk_embed_grad_sorted": [_P, _I32, _I64, _P, _I64, _I32, _I32, _F, _I64, _P, _I32, _P, _I64, _P],
+    "vk_process_logits": [_P, _I32, _I64, _P, _I64, _I64, _P, _P, _F, _P, _F, _P, _F, _P, _I64, _P, _I64, _I64, _P, _P, _I32,
+                          _I64, _I64, _I32, _P],
+    "vk_choose_tokens_workspace": [_I64, _I32, ctypes.POINTER(_I64)],
+    "vk_choose_tokens": [_P, _I32, _I64, _P, _I64, _I64, _P, _P, _F, _P, _F, _P, _F, _P, _I64, _P, _I64, _I64, _P, _P, _F,
+                         _I32, _P, _I64, _I64, _P, _P, _I64, _I32, _P, _I64, _P],
+    "vk_choose_update": [_P, _I32, _I64, _F, _F, _F, _P, _P, _I64, _I64, _P, _P, _P, _I32, _F, _I32, _P, _I64, _I64, _P, _P,
+                         _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _I64, _P],
     "vk_rmsnorm_backward_blocks": [_I64, ctypes.POINTER(_I32)],
     "vk_rmsnorm_backward": [_P, _I32, _P, _I32, _P, _I32, _P, _P, _P, _P, _I64, _I32, _F, _P],
     "vk_colsum": [_P, _P, _I32, _I32, _I32, _P],

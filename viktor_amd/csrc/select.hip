@@ -14,7 +14,7 @@
 // bf16 as an nn.Linear in bf16 would) or read as fp32 logits.
 #include <math.h>
 
-#include "common.h"
+#include "decode_state.h"
 
 namespace vk {
 
@@ -280,23 +280,8 @@ __global__ __launch_bounds__(SEL_THREADS) void select_update_kernel(
   }
 
   // 4. grammar and bookkeeping
-  if (prev_tail) nxt = eos;
-  if (homo_stop > 0) {
-    const bool same = nxt == prev && nxt >= 0 && nxt < V && homo_s[nxt];
-    const int64_t r = same ? run_raw + 1 : 0;
-    run[b] = r;
-    if (r + 1 >= homo_stop) nxt = eos;
-  }
-  if (prev == eos || prev == pad) nxt = pad;
-  if (ocol >= 0 && ocol < out_cols) out[b * out_stride + ocol] = nxt;
-  tok[b] = nxt;
-  const int64_t np = p + 1;
-  pos[b] = np;
-  // cache_base: the KV-cache row of position p is p - cache_base[b] (a per-sequence suffix cache)
-  const int64_t cp = np - (cache_base ? cb_raw : 0);
-  if (pos32) pos32[b] = static_cast<int32_t>(cp);
-  if (seqlens) seqlens[b] = static_cast<int32_t>(cp + 1);
-  if (rpos32) rpos32[b] = static_cast<int32_t>(np + (rope_off ? ro_raw : 0));
+  const DecodeState st = {tok, run, pos, cache_base, out, out_stride, out_cols, pos32, seqlens, rpos32, homo_stop, eos, pad};
+  advance_state(st, b, nxt, prev, prev_tail, homo_s, V, p, run_raw, ocol, rope_off ? ro_raw : 0, cache_base ? cb_raw : 0);
 }
 
 }  // namespace vk

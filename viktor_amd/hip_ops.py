@@ -856,6 +856,186 @@ def embed_grad(d_rows, tokens, vocab):
     return out
 
 
+def _here(what, *ts):
+    """Every tensor on the current device: launches go to its current stream."""
+    for t in ts:
+        if torch.is_tensor(t):
+            require_device(t, what)
+            _require(t.get_device() == torch.cuda.current_device(), f"{what}: tensors on the current device")
+
+
+def _vk_dtype(t):
+    return VK_DTYPE_F32 if t == torch.float32 else VK_DTYPE_BF16
+
+
+def embed_lookup(weight, tokens, scale=1.0, out_dtype=None):
+    """scale * weight[tokens]: weight [V, d] bf16 or fp32, tokens int64 of any shape -> [*tokens.shape, d] of out_dtype
+    (bf16 or fp32; default: the weight's). The product is fp32, rounded once. Ids outside [0, V) give zero rows.
+    Reference: nn.Embedding's gather, viktor/model.py:77."""
+    _here("embed_lookup", weight, tokens)
+    odt = out_dtype or weight.dtype
+    _require(weight.dim() == 2 and weight.dtype in (BF16, torch.float32) and odt in (BF16, torch.float32)
+             and weight.shape[0] > 0 and weight.shape[1] > 0, "embed_lookup: weight [V, d] and out bf16 or fp32")
+    _require(tokens.dtype == torch.long and _contig(weight, tokens), "embed_lookup: contiguous weight and int64 tokens")
+    V, d = weight.shape
+    out = torch.empty(*tokens.shape, d, dtype=odt, device=weight.device)
+    call("vk_embed_lookup", ptr(weight), _vk_dtype(weight.dtype), ptr(tokens), tokens.numel(), V, d, float(scale), ptr(out),
+         _vk_dtype(odt), stream_handle())
+    return out
+
+
+def embed_grad_sorted(d_rows, tokens, vocab, scale=1.0, pad=None, out=None, accumulate=False):
+    """embed_grad for large vocabularies, by sorted tokens: fp32 [vocab, d] with row v = scale * the sum of d_rows[r]
+    (bf16 or fp32 [n, d], any width and row stride, unit column stride) over tokens[r] == v (int64 [n]), in an order that
+    n, vocab and the ids alone decide. Rows of ids outside [0, vocab) and of the id `pad` add nothing. out: the caller's
+    contiguous fp32 [vocab, d]; accumulate: added to what it holds. Reference: the backward of nn.Embedding,
+    viktor/decoder.py:127, as viktor/model.py:77 gathers it."""
+    _here("embed_grad_sorted", d_rows, tokens, out)
+    _require(d_rows.dim() == 2 and d_rows.dtype in (BF16, torch.float32) and d_rows.shape[1] > 0
+             and (d_rows.stride(1) == 1 or d_rows.shape[1] == 1) and (d_rows.shape[0] < 2 or d_rows.stride(0) >= d_rows.shape[1]),
+             "embed_grad_sorted: d_rows [n, d] bf16 or fp32, rows side by side")
+    _require(tokens.shape == (d_rows.shape[0],) and tokens.dtype == torch.long and tokens.is_contiguous(),
+             "embed_grad_sorted: tokens [n] int64")
+    _require(vocab > 0 and (out is not None or not accumulate), "embed_grad_sorted: vocab > 0, accumulate into out")
+    n, d = d_rows.shape
+    _require(out is None or (out.dtype == torch.float32 and out.shape == (vocab, d) and out.is_contiguous()),
+             "embed_grad_sorted: out fp32 [vocab, d]")
+    nb = ctypes.c_int64(0)
+    call("vk_embed_grad_sorted_workspace", n, vocab, d, ctypes.byref(nb))
+    ws = torch.empty(nb.value, dtype=torch.uint8, device=d_rows.device)
+    if out is None:
+        out = torch.empty(vocab, d, dtype=torch.float32, device=d_rows.device)
+    call("vk_embed_grad_sorted", ptr(d_rows), _vk_dtype(d_rows.dtype), max(d_rows.stride(0), d), ptr(tokens), n, vocab, d,
+         float(scale), -1 if pad is None else int(pad), ptr(out), int(bool(accumulate)), ptr(ws), nb.value, stream_handle())
+    return out
+
+
+def pack_allowed(mask):
+    """Grammar masks bool [S, V] as process_logits and choose_tokens take them: int32 [S, ceil(V / 32)], bit v % 32 of word
+    v // 32 set where token v is allowed."""
+    _require(mask.dim() == 2 and mask.dtype == torch.bool, "pack_allowed: bool [S, V]")
+    S, V = mask.shape
+    words = -(-V // 32)
+    bits = torch.zeros(S, words * 32, dtype=torch.int64, device=mask.device)
+    bits[:, :V] = mask
+    w = (bits.view(S, words, 32) << torch.arange(32, device=mask.device)).sum(-1)
+    return torch.where(w >= 2 ** 31, w - 2 ** 32, w).to(torch.int32)
+
+
+def _per_row(x, B, what):
+    """A float, or fp32 [B] on the device -> (pointer or None, the float)."""
+    if not torch.is_tensor(x):
+        return None, float(x)
+    _require(x.dtype == torch.float32 and x.shape == (B,) and x.is_contiguous(), f"{what}: a float or fp32 [B]")
+    return x.data_ptr(), 0.0
+
+
+def _mask_args(allowed, V, what):
+    if allowed is None:
+        return None, 0, 0
+    _require(allowed.dim() == 2 and allowed.dtype == torch.int32 and allowed.shape[0] > 0
+             and allowed.shape[1] >= -(-V // 32) and allowed.is_contiguous(), f"{what}: allowed int32 [S, ceil(V / 32)]")
+    return allowed.data_ptr(), allowed.shape[1], allowed.shape[0]
+
+
+def _logit_rules(what, logits, history, lengths, repetition, presence, frequency, bias, allowed, allowed_rows):
+    """The checked arguments of the rules, in the C entry points' order."""
+    _here(what, logits, history, lengths, repetition, presence, frequency, bias, allowed, allowed_rows)
+    _require(logits.dim() == 2 and logits.dtype in (BF16, torch.float32) and logits.shape[1] > 0
+             and (logits.stride(1) == 1 or logits.shape[1] == 1)
+             and (logits.shape[0] < 2 or logits.stride(0) >= logits.shape[1]), f"{what}: logits [B, V] bf16 or fp32, rows side by side")
+    B, V = logits.shape
+    rep, pres, freq = (_per_row(x, B, f"{what}: {name}") for x, name in
+                       ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")))
+    _require(rep[0] is not None or rep[1] > 0, f"{what}: the repetition penalty must be positive")
+    hist = (None, 0, 0, None)
+    if history is None:
+        _require(lengths is None and rep == (None, 1.0) and pres == (None, 0.0) and freq == (None, 0.0),
+                 f"{what}: penalties need the history and its lengths")
+    else:
+        _require(history.dim() == 2 and history.shape[0] == B and history.dtype == torch.long
+                 and (history.stride(1) == 1 or history.shape[1] < 2)
+                 and (B < 2 or history.stride(0) >= history.shape[1]), f"{what}: history int64 [B, T], rows side by side")
+        _require(lengths is not None and lengths.shape == (B,) and lengths.dtype == torch.int32 and lengths.is_contiguous(),
+                 f"{what}: lengths int32 [B]")
+        if history.shape[1] > 0:
+            hist = (history.data_ptr(), max(history.stride(0), history.shape[1]), history.shape[1], lengths.data_ptr())
+    bp, bld = None, 0
+    if bias is not None:
+        _require(bias.dtype == torch.float32 and bias.shape in ((V,), (B, V)) and (bias.stride(-1) == 1 or V == 1)
+                 and (bias.dim() == 1 or B < 2 or bias.stride(0) >= V), f"{what}: bias fp32 [V] or [B, V]")
+        bp, bld = bias.data_ptr(), 0 if bias.dim() == 1 else max(bias.stride(0), V)
+    mask = _mask_args(allowed, V, what)
+    _require(allowed_rows is None or (allowed is not None and allowed_rows.shape == (B,) and allowed_rows.dtype == torch.int32
+                                      and allowed_rows.is_contiguous()), f"{what}: allowed_rows int32 [B], with allowed")
+    _require(allowed is None or allowed_rows is not None or allowed.shape[0] in (1, B),
+             f"{what}: allowed without allowed_rows has 1 row or one per sequence")
+    return B, V, (ptr(logits), _vk_dtype(logits.dtype), max(logits.stride(0), V), *hist, *rep, *pres, *freq, bp, bld, *mask,
+                  ptr(allowed_rows))
+
+
+def process_logits(logits, history=None, lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,
+                   allowed_rows=None, out=None, out_dtype=None):
+    """Penalties for repeated tokens, bias and grammar mask on logits [B, V] (bf16 or fp32, unit column stride). For
+    sequence b and token v, c = how often v is among history[b, :lengths[b]] (int64 [B, T <= 65535], int32 [B]):
+      c > 0: z = x / repetition if x > 0 else x * repetition; z -= frequency * c; z -= presence
+      z += bias[v] (fp32 [V] or [B, V]); v not allowed: -inf, whatever was there
+    in fp32, each step rounded in this order, the result rounded once to out_dtype (default: the logits'). repetition (> 0),
+    presence, frequency: floats or fp32 [B]. allowed: int32 [S, ceil(V / 32)] (pack_allowed); allowed_rows int32 [B]: each
+    sequence's mask row, -1 (or any row outside) for none; without it S is 1 or B. out: the caller's buffer, the logits
+    themselves included. The reference's rules are viktor/engine.py:79-116; these have no counterpart there."""
+    B, V, args = _logit_rules("process_logits", logits, history, lengths, repetition, presence, frequency, bias, allowed,
+                              allowed_rows)
+    if out is None:
+        out = torch.empty(B, V, dtype=out_dtype or logits.dtype, device=logits.device)
+    _here("process_logits", out)
+    _require(out.shape == (B, V) and out.dtype in (BF16, torch.float32) and (out_dtype is None or out.dtype == out_dtype)
+             and (out.stride(1) == 1 or V == 1) and (B < 2 or out.stride(0) >= V), "process_logits: out [B, V] bf16 or fp32")
+    call("vk_process_logits", *args, ptr(out), _vk_dtype(out.dtype), max(out.stride(0), V), B, V, stream_handle())
+    return out
+
+
+_MODE_GREEDY, _MODE_GUMBEL, _MODE_CDF = 0, 1, 2
+
+
+def _choose_workspace(B, V, device):
+    nb = ctypes.c_int64(0)
+    call("vk_choose_tokens_workspace", B, V, ctypes.byref(nb))
+    return torch.empty(max(nb.value, 16), dtype=torch.uint8, device=device)
+
+
+def choose_tokens(logits, history=None, lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,
+                  allowed_rows=None, temperature=0.0, uniforms=None, fallback=0):
+    """The token choice over any vocabulary after process_logits' rules, which are applied on the fly (logits stay as they
+    are). z' = z / temperature where it is positive (a float or fp32 [B]); a row with temperature <= 0 is greedy (the first
+    index of the maximum). uniforms in [0, 1): fp32 [B, V] for the Gumbel choice, first argmax of z' - log(-log(max(u, 1e-20)))
+    (viktor/engine.py:80-83's formula), or fp32 [B] for the inverse CDF, the first v with u < sum_{w <= v} softmax(z')_w.
+    Returns (tokens int64 [B], logp fp32 [B]), logp = log softmax(z')[token]. NaN is never chosen and weighs nothing, +inf
+    counts as the largest finite value; a row with nothing left gives `fallback` and -inf."""
+    B, V, args = _logit_rules("choose_tokens", logits, history, lengths, repetition, presence, frequency, bias, allowed,
+                              allowed_rows)
+    _here("choose_tokens", temperature, uniforms)
+    temp = _per_row(temperature, B, "choose_tokens: temperature")
+    mode, up, uld = _MODE_GREEDY, None, 0
+    if uniforms is None:
+        _require(temp[0] is None and temp[1] <= 0, "choose_tokens: a temperature needs uniforms")
+    else:
+        _require(uniforms.dtype == torch.float32 and uniforms.shape in ((B,), (B, V)), "choose_tokens: uniforms fp32 [B] or [B, V]")
+        if uniforms.dim() == 2:
+            _require((uniforms.stride(1) == 1 or V == 1) and (B < 2 or uniforms.stride(0) >= V), "choose_tokens: uniform rows")
+            mode, uld = _MODE_GUMBEL, max(uniforms.stride(0), V)
+        else:
+            _require(uniforms.is_contiguous(), "choose_tokens: contiguous uniforms")
+            mode, uld = _MODE_CDF, 1
+        up = uniforms.data_ptr()
+    token = torch.empty(B, dtype=torch.long, device=logits.device)
+    logp = torch.empty(B, dtype=torch.float32, device=logits.device)
+    ws = _choose_workspace(B, V, logits.device)
+    call("vk_choose_tokens", *args, *temp, mode, up, uld, int(fallback), ptr(token), ptr(logp), B, V, ptr(ws), ws.numel(),
+         stream_handle())
+    return token, logp
+
+
 def _norm_blocks(n):
     b = ctypes.c_int32(0)
     _lib.check(_lib.load().vk_rmsnorm_backward_blocks(n, ctypes.byref(b)), "rmsnorm_backward_blocks")
