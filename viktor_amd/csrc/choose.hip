@@ -77,86 +77,119 @@ __device__ __forceinline__ RowRules row_rules(const Rules &r, int64_t b, int V) 
   return o;
 }
 
-// cnt: 16-bit counts, two a word, of tokens v0 .. v0 + slice - 1 in hist[0 .. len - 1]. Ends with a barrier.
+// cnt: 16-bit counts, two a word, of tokens v0 .. v0 + slice - 1 in hist[0 .. len - 1] (slice % 32 == 0). Ends with a
+// barrier.
 __device__ __forceinline__ void count_history(uint32_t *cnt, const int64_t *hist, int len, int v0, int slice) {
-  for (int i = threadIdx.x; i < (slice + 1) / 2; i += CH_THREADS) cnt[i] = 0;
+  const int64_t first = hist[threadIdx.x < len ? threadIdx.x : 0];  // in flight while the counts are cleared
+  for (int i = threadIdx.x; i < slice / 8; i += CH_THREADS) reinterpret_cast<u32x4 *>(cnt)[i] = u32x4{0u, 0u, 0u, 0u};
   __syncthreads();
   for (int t = threadIdx.x; t < len; t += CH_THREADS) {
-    const int64_t rel = hist[t] - v0;
+    const int64_t rel = (t == static_cast<int>(threadIdx.x) ? first : hist[t]) - v0;
     if (rel >= 0 && rel < slice) atomicAdd(&cnt[rel >> 1], (rel & 1) ? 0x10000u : 1u);
   }
   __syncthreads();
 }
 
-// The rules on N tokens from v (N divides 8 and v: one mask word; `have` of them exist).
-template <int N>
-__device__ __forceinline__ void apply_rules(float (&z)[N], const RowRules &r, const uint32_t *cnt, int rel, int v,
-                                            int have) {
+// N consecutive tokens' logits and what the rules read for them, loaded ahead of their use. A vector that does not fit
+// into the row (its last one, where N does not divide V) is read one by one when it is used; its place here holds the
+// row's last whole vector, so that every load is unconditional and in bounds.
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  u32x4 raw;
+  float bias[N];
+  uint32_t mask;
+
+  __device__ __forceinline__ void load(const T *row, const RowRules &r, int v, int V) {
+    if (V < N) return;
+    const int at = v <= V - N ? v : V - N;
+    raw = load_16(row + at);
+    if (r.bias != nullptr) load_row<N>(r.bias + at, bias);
+    if (r.allowed != nullptr) mask = r.allowed[at >> 5];
+  }
+
+  // z: the logits after the rules, -inf past the row's end. v < V, v % N == 0; cnt: the counts of tokens v, v + 1, ...
+  __device__ __forceinline__ void rules(float (&z)[N], const T *row, const RowRules &r, const uint32_t *cnt, int v, int V) {
 #pragma clang fp contract(off)
-  if (r.len > 0) {
-    uint32_t w[N / 2], any = 0;
+    const bool whole = v <= V - N;
+    if (whole) {
 #pragma unroll
-    for (int k = 0; k < N / 2; ++k) any |= w[k] = cnt[rel / 2 + k];
-    if (any) {
+      for (int k = 0; k < N; ++k)
+        if constexpr (sizeof(T) == 4)
+          z[k] = __uint_as_float(raw[k]);
+        else
+          z[k] = (k & 1) ? hi_bf(raw[k / 2]) : lo_bf(raw[k / 2]);
+    } else {
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int c = (k & 1) ? w[k / 2] >> 16 : w[k / 2] & 0xffff;
-        if (c > 0) {
-          z[k] = z[k] > 0.f ? z[k] / r.rep : z[k] * r.rep;
-          z[k] = z[k] - r.freq * static_cast<float>(c);
-          z[k] = z[k] - r.pres;
+      for (int k = 0; k < N; ++k) z[k] = load_one(row + (v + k < V ? v + k : V - 1));
+      if (r.bias != nullptr)
+#pragma unroll
+        for (int k = 0; k < N; ++k) bias[k] = r.bias[v + k < V ? v + k : V - 1];
+      if (r.allowed != nullptr) mask = r.allowed[v >> 5];
+    }
+    if (r.len > 0) {
+      uint32_t w[N / 2], any = 0;
+#pragma unroll
+      for (int k = 0; k < N / 2; ++k) any |= w[k] = cnt[k];
+      if (any) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int c = (k & 1) ? w[k / 2] >> 16 : w[k / 2] & 0xffff;
+          if (c > 0) {
+            z[k] = z[k] > 0.f ? z[k] / r.rep : z[k] * r.rep;
+            z[k] = z[k] - r.freq * static_cast<float>(c);
+            z[k] = z[k] - r.pres;
+          }
         }
       }
     }
-  }
-  if (r.bias != nullptr) {
-    float bv[N];
-    if (have == N) {
-      load_row<N>(r.bias + v, bv);
-    } else {
-      for (int k = 0; k < N; ++k) bv[k] = k < have ? r.bias[v + k] : 0.f;
+    if (r.bias != nullptr)
+#pragma unroll
+      for (int k = 0; k < N; ++k) z[k] = z[k] + bias[k];
+    if (r.allowed != nullptr) {
+      const uint32_t bits = mask >> (v & 31);
+#pragma unroll
+      for (int k = 0; k < N; ++k) z[k] = (bits >> k) & 1 ? z[k] : -INFINITY;
     }
+    if (!whole)
 #pragma unroll
-    for (int k = 0; k < N; ++k) z[k] = z[k] + bv[k];
+      for (int k = 0; k < N; ++k)
+        if (v + k >= V) z[k] = -INFINITY;
   }
-  if (r.allowed != nullptr) {
-    const uint32_t bits = r.allowed[v >> 5] >> (v & 31);
-#pragma unroll
-    for (int k = 0; k < N; ++k) z[k] = (bits >> k) & 1 ? z[k] : -INFINITY;
-  }
-}
+};
 
-template <int N, typename T>
-__device__ __forceinline__ int load_some(const T *row, int v, int V, float (&z)[N]) {
-  const int have = V - v < N ? V - v : N;
-  if (have == N) {
-    load_row<N>(row + v, z);
-  } else {
-    for (int k = 0; k < N; ++k) z[k] = k < have ? load_one(row + v + k) : -INFINITY;
-  }
-  return have;
-}
+// Vectors that a thread has in flight: 16 elements.
+template <typename T>
+constexpr int kAhead = sizeof(T);
 
 // grid: B x slices workgroups, a sequence's slices side by side. out may be logits.
 template <typename T, typename OT>
 __global__ __launch_bounds__(CH_THREADS) void process_logits_kernel(const T *logits, int64_t ld, Rules rules, int V,
                                                                     int slices, int slice, OT *out, int64_t out_ld) {
-  extern __shared__ uint32_t cnt[];
-  constexpr int N = 16 / sizeof(T);
+  extern __shared__ __attribute__((aligned(16))) uint32_t cnt[];
+  constexpr int N = Vec<T>::N, R = kAhead<T>, STEP = CH_THREADS * N;
   const int64_t b = blockIdx.x / slices;
   const int v0 = static_cast<int>(blockIdx.x % slices) * slice, v1 = V - v0 < slice ? V : v0 + slice;
   const RowRules r = row_rules(rules, b, V);
-  if (r.len > 0) count_history(cnt, r.hist, r.len, v0, slice);
   const T *row = logits + b * ld;
   OT *dst = out + b * out_ld;
-  for (int v = v0 + threadIdx.x * N; v < v1; v += CH_THREADS * N) {
-    float z[N];
-    const int have = load_some<N>(row, v, V, z);
-    apply_rules<N>(z, r, cnt, v - v0, v, have);
-    if (have == N) {
-      store_row<N>(dst + v, z);
-    } else {
-      for (int k = 0; k < have; ++k) store_one(dst + v + k, z[k]);
+  const int mine = v0 + static_cast<int>(threadIdx.x) * N;
+  Vec<T> x[R];
+  for (int w = v0; w < v1; w += R * STEP) {
+#pragma unroll
+    for (int q = 0; q < R; ++q) x[q].load(row, r, w - v0 + mine + q * STEP, V);
+    if (w == v0 && r.len > 0) count_history(cnt, r.hist, r.len, v0, slice);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int v = w - v0 + mine + q * STEP;
+      if (v >= v1) continue;
+      float z[N];
+      x[q].rules(z, row, r, cnt + (v - v0) / 2, v, V);
+      if (v <= V - N) {
+        store_row<N>(dst + v, z);
+      } else {
+        for (int k = 0; k < N && v + k < V; ++k) store_one(dst + v + k, z[k]);
+      }
     }
   }
 }
@@ -165,65 +198,87 @@ __global__ __launch_bounds__(CH_THREADS) void process_logits_kernel(const T *log
 
 enum { CH_GREEDY = 0, CH_GUMBEL = 1, CH_CDF = 2 };
 
-struct Best {
-  float s;    // its score in fp32 (Gumbel: within score_slack of the exact one)
-  float z;    // its logit after the rules, before the temperature
-  float u;    // its uniform
+// Running state of a part of a row: the maximum of z (at least -FLT_MAX), the sum of exp((z - m) / T), and the best token.
+// Gumbel: v is that token, s its score in fp32 (within score_slack of the exact one), z its logit and u its uniform.
+// Else: z is the largest logit (-inf: none) and v the first token, or the first token of the vector, that has it.
+struct Part {
+  float m, sum, s, z, u;
   int32_t v;  // -1: none yet
 };
 
-struct Part {
-  float m, sum;  // max of z' (at least -FLT_MAX) and sum of exp(z' - m)
-  Best best;
-};
+__device__ __forceinline__ Part no_part() { return {-FLT_MAX, 0.f, -INFINITY, -INFINITY, 0.f, -1}; }
 
-// How far the fp32 score of a token can be from the exact one: rounding of z' and of the sum (1.2e-7 of its size each),
-// and of the two logarithms.
+// How far the fp32 score of a token can be from the exact one: the roundings of z' and of the sum (1.2e-7 of its size
+// each), and of the two logarithms.
 __device__ __forceinline__ float score_slack(float s) { return 1e-5f + 1e-6f * fabsf(s); }
 
 // The exact score: z' rounded to fp32, the noise in 64 bits.
-__device__ __forceinline__ double exact_score(const Best &a, float T) {
-  return static_cast<double>(a.z / T) - log(-log(fmax(static_cast<double>(a.u), 1e-20)));
+__device__ __forceinline__ double exact_score(float z, float u, float T) {
+  return static_cast<double>(z / T) - log(-log(fmax(static_cast<double>(u), 1e-20)));
 }
 
-// Whether b comes before a. Gumbel scores that fp32 cannot order are compared in 64 bits.
+// Whether b's token comes before a's. Gumbel scores that fp32 cannot order are compared in 64 bits.
 template <bool GUMBEL>
-__device__ __forceinline__ bool better(const Best &a, const Best &b, float T) {
+__device__ __forceinline__ bool better(const Part &a, const Part &b, float T) {
   if (b.v < 0) return false;
   if (a.v < 0) return true;
   if (GUMBEL && T > 0.f) {
     const float d = b.s - a.s;
     if (fabsf(d) > 2.f * score_slack(fmaxf(fabsf(a.s), fabsf(b.s)))) return d > 0.f;
-    const double ea = exact_score(a, T), eb = exact_score(b, T);
+    const double ea = exact_score(a.z, a.u, T), eb = exact_score(b.z, b.u, T);
     return eb > ea || (eb == ea && b.v < a.v);
   }
-  return b.s > a.s || (b.s == a.s && b.v < a.v);
+  return b.z > a.z || (b.z == a.z && b.v < a.v);
 }
 
-__device__ __forceinline__ void join_sums(float &m, float &sum, float m2, float sum2) {
-  const float M = fmaxf(m, m2);
-  sum = sum * __expf(m - M) + sum2 * __expf(m2 - M);
-  m = M;
+// L: log2(e) / T. Differences first: nothing overflows where all logits are the type's lowest value.
+template <bool GUMBEL>
+__device__ __forceinline__ void join_parts(Part &a, const Part &b, float L, float T) {
+  const float M = fmaxf(a.m, b.m);
+  a.sum = a.sum * __builtin_amdgcn_exp2f((a.m - M) * L) + b.sum * __builtin_amdgcn_exp2f((b.m - M) * L);
+  a.m = M;
+  if (better<GUMBEL>(a, b, T)) {
+    a.s = b.s;
+    a.z = b.z;
+    a.u = b.u;
+    a.v = b.v;
+  }
 }
 
 template <bool GUMBEL>
-__device__ __forceinline__ void join_lanes(Part &p, float T) {
+__device__ __forceinline__ void join_lanes(Part &p, float L, float T) {
 #pragma unroll 1
   for (int o = 32; o > 0; o >>= 1) {
     Part q;
     q.m = __shfl_xor(p.m, o, 64);
     q.sum = __shfl_xor(p.sum, o, 64);
-    q.best.s = __shfl_xor(p.best.s, o, 64);
-    q.best.z = __shfl_xor(p.best.z, o, 64);
-    q.best.u = __shfl_xor(p.best.u, o, 64);
-    q.best.v = __shfl_xor(p.best.v, o, 64);
-    join_sums(p.m, p.sum, q.m, q.sum);
-    if (better<GUMBEL>(p.best, q.best, T)) p.best = q.best;
+    q.s = GUMBEL ? __shfl_xor(p.s, o, 64) : 0.f;
+    q.z = __shfl_xor(p.z, o, 64);
+    q.u = GUMBEL ? __shfl_xor(p.u, o, 64) : 0.f;
+    q.v = __shfl_xor(p.v, o, 64);
+    join_parts<GUMBEL>(p, q, L, T);
   }
 }
 
-// A NaN becomes -inf, +inf the largest finite value.
-__device__ __forceinline__ float tame(float z) { return fminf(fmaxf(z, -INFINITY), FLT_MAX); }
+// A NaN becomes -inf, +inf the largest finite value: v_med3_f32 of a NaN is the smaller of the others. As asm: the
+// compiler's own med3 with -inf is a minimum, which a NaN passes as the other operand.
+__device__ __forceinline__ float tame(float z) {
+  float d;
+  asm("v_med3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(z), "v"(-INFINITY), "v"(FLT_MAX));
+  return d;
+}
+
+struct Scale {
+  float T, inv, L;  // the temperature, 1 / T (1 for a greedy row) kept finite, and log2(e) / T
+};
+
+__device__ __forceinline__ Scale row_scale(const float *temp, float temp0, int64_t b) {
+  Scale c;
+  c.T = temp ? temp[b] : temp0;
+  c.inv = c.T > 0.f ? fminf(1.f / c.T, 0.5f * FLT_MAX) : 1.f;
+  c.L = fminf(c.inv * 1.44269504f, 0.5f * FLT_MAX);
+  return c;
+}
 
 // The uniforms of sequence b are at u + b * ld; in a decode step those of its output column (clamped to the columns there
 // are), a column being 1 uniform (inverse CDF) or V of them (Gumbel).
@@ -239,58 +294,6 @@ __device__ __forceinline__ const float *noise_at(const Noise &n, const Rules &r,
     col = col < 0 ? 0 : (col >= n.cols ? n.cols - 1 : col);
   }
   return n.u + b * n.ld + col * per_column;
-}
-
-template <typename T, bool GUMBEL>
-__global__ __launch_bounds__(CH_THREADS) void choose_slices_kernel(const T *__restrict__ logits, int64_t ld, Rules rules,
-                                                                   const float *__restrict__ temp, float temp0,
-                                                                   Noise noise, int V, int slices, int slice, Part *__restrict__ parts) {
-  extern __shared__ uint32_t cnt[];
-  __shared__ Part red[CH_THREADS / 64];
-  constexpr int N = 16 / sizeof(T);
-  const int64_t b = blockIdx.x / slices;
-  const int v0 = static_cast<int>(blockIdx.x % slices) * slice, v1 = V - v0 < slice ? V : v0 + slice;
-  const RowRules r = row_rules(rules, b, V);
-  const float temperature = temp ? temp[b] : temp0;
-  const float inv = temperature > 0.f ? 1.f / temperature : 1.f;
-  const bool noisy = GUMBEL && temperature > 0.f;
-  if (r.len > 0) count_history(cnt, r.hist, r.len, v0, slice);
-  const T *row = logits + b * ld;
-  const float *urow = noisy ? noise_at(noise, rules, b, V) : nullptr;
-  Part p = {-FLT_MAX, 0.f, {-INFINITY, 0.f, 0.f, -1}};
-  for (int v = v0 + threadIdx.x * N; v < v1; v += CH_THREADS * N) {
-    float z[N], u[N];
-    const int have = load_some<N>(row, v, V, z);
-    if (noisy) load_some<N>(urow, v, V, u);
-    apply_rules<N>(z, r, cnt, v - v0, v, have);
-    float q[N], m = p.m;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      z[k] = tame(z[k]);
-      q[k] = tame(z[k] * inv);
-      m = fmaxf(m, q[k]);
-    }
-    p.sum *= __expf(p.m - m);
-    p.m = m;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      p.sum += __expf(q[k] - m);
-      if (z[k] == -INFINITY) continue;
-      const Best c = {noisy ? q[k] - logf(-logf(fmaxf(u[k], 1e-20f))) : q[k], z[k], noisy ? u[k] : 0.f, v + k};
-      if (better<GUMBEL>(p.best, c, temperature)) p.best = c;
-    }
-  }
-  join_lanes<GUMBEL>(p, temperature);
-  const int lane = threadIdx.x & 63;
-  if (lane == 0) red[threadIdx.x >> 6] = p;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < CH_THREADS / 64; ++w) {
-      join_sums(p.m, p.sum, red[w].m, red[w].sum);
-      if (better<GUMBEL>(p.best, red[w].best, temperature)) p.best = red[w].best;
-    }
-    parts[blockIdx.x] = p;
-  }
 }
 
 struct Choice {
@@ -330,7 +333,114 @@ __device__ __forceinline__ void finish_row(const Choice &c, const Step &st, int6
                 st.rope_off ? st.rope_off[b] : 0, st.s.cache_base ? st.s.cache_base[b] : 0);
 }
 
-// One wavefront per sequence joins its slices in slice order.
+// log softmax(z')[token] of a logit z of the row that p sums.
+__device__ __forceinline__ float logp_of(float z, const Part &p, const Scale &c) {
+  const float d = z - p.m;
+  return (c.T > 0.f ? d / c.T : d) - logf(p.sum);
+}
+
+// One slice of one sequence, or with ONE the whole vocabulary and the step's end.
+template <typename T, bool GUMBEL, bool ONE>
+__global__ __launch_bounds__(CH_THREADS) void choose_slices_kernel(const T *__restrict__ logits, int64_t ld, Rules rules,
+                                                                   const float *__restrict__ temp, float temp0,
+                                                                   Noise noise, int V, int slices, int slice,
+                                                                   Part *__restrict__ parts, Choice choice, Step step) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t cnt[];
+  __shared__ Part red[CH_THREADS / 64];
+  constexpr int N = Vec<T>::N, R = kAhead<T>, STEP = CH_THREADS * N;
+  const int64_t b = ONE ? blockIdx.x : blockIdx.x / slices;
+  const int v0 = ONE ? 0 : static_cast<int>(blockIdx.x % slices) * slice, v1 = V - v0 < slice ? V : v0 + slice;
+  const RowRules r = row_rules(rules, b, V);
+  const Scale c = row_scale(temp, temp0, b);
+  const bool noisy = GUMBEL && c.T > 0.f;
+  const T *row = logits + b * ld;
+  const float *urow = noisy ? noise_at(noise, rules, b, V) : nullptr;
+  const int mine = v0 + static_cast<int>(threadIdx.x) * N;
+  Part p = no_part();
+  Vec<T> x[R];
+  float u[GUMBEL ? R : 1][N];
+  for (int w = v0; w < v1; w += R * STEP) {
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int v = w - v0 + mine + q * STEP;
+      x[q].load(row, r, v, V);
+      if (noisy && V >= N) load_row<N>(urow + (v <= V - N ? v : V - N), u[GUMBEL ? q : 0]);
+    }
+    if (w == v0 && r.len > 0) count_history(cnt, r.hist, r.len, v0, slice);
+    float z[R][N], top = -INFINITY;
+    int topv = -1;
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int v = w - v0 + mine + q * STEP;
+      if (v < v1) {
+        x[q].rules(z[q], row, r, cnt + (v - v0) / 2, v, V);
+        if (noisy && v > V - N)
+#pragma unroll
+          for (int k = 0; k < N; ++k) u[GUMBEL ? q : 0][k] = urow[v + k < V ? v + k : V - 1];
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) z[q][k] = -INFINITY;
+      }
+      float most = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        z[q][k] = tame(z[q][k]);
+        most = vmax2(most, z[q][k]);
+      }
+      if (most > top) {
+        top = most;
+        topv = v;
+      }
+    }
+    const float m = vmax2(p.m, top);
+    p.sum *= __builtin_amdgcn_exp2f((p.m - m) * c.L);
+    p.m = m;
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+      for (int k = 0; k < N; ++k) p.sum += __builtin_amdgcn_exp2f((z[q][k] - m) * c.L);
+    if (!noisy) {
+      if (top > p.z) {
+        p.z = top;
+        p.v = topv;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < R; ++q)
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const float uk = u[GUMBEL ? q : 0][k];
+          Part t = p;
+          t.z = z[q][k];
+          t.u = uk;
+          t.s = fmaf(t.z, c.inv, -logf(-logf(fmaxf(uk, 1e-20f))));
+          t.v = t.z == -INFINITY ? -1 : w - v0 + mine + q * STEP + k;
+          if (better<GUMBEL>(p, t, c.T)) p = t;
+        }
+    }
+  }
+  join_lanes<GUMBEL>(p, c.L, c.T);
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) red[threadIdx.x >> 6] = p;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < CH_THREADS / 64; ++w) join_parts<GUMBEL>(p, red[w], c.L, c.T);
+  if (!noisy && p.v >= 0) {  // the token inside its vector
+    float z[N];
+    x[0].load(row, r, p.v, V);
+    x[0].rules(z, row, r, cnt + (p.v - v0) / 2, p.v, V);
+    int k = 0;
+#pragma unroll
+    for (int e = N - 1; e >= 0; --e) k = tame(z[e]) == p.z ? e : k;
+    p.v += k;
+  }
+  if constexpr (ONE)
+    finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
+  else
+    parts[blockIdx.x] = p;
+}
+
+// One wavefront per sequence joins its slices.
 template <bool GUMBEL>
 __global__ __launch_bounds__(256) void choose_join_kernel(const Part *__restrict__ parts, const float *__restrict__ temp,
                                                           float temp0, int64_t B, int V, int slices, Choice choice,
@@ -338,17 +448,11 @@ __global__ __launch_bounds__(256) void choose_join_kernel(const Part *__restrict
   const int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (b >= B) return;
   const int lane = threadIdx.x & 63;
-  const float temperature = temp ? temp[b] : temp0;
-  Part p = {-FLT_MAX, 0.f, {-INFINITY, 0.f, 0.f, -1}};
-  for (int s = lane; s < slices; s += 64) {
-    const Part q = parts[b * slices + s];
-    join_sums(p.m, p.sum, q.m, q.sum);
-    if (better<GUMBEL>(p.best, q.best, temperature)) p.best = q.best;
-  }
-  join_lanes<GUMBEL>(p, temperature);
-  if (lane != 0) return;
-  const float zt = temperature > 0.f ? tame(p.best.z / temperature) : p.best.z;
-  finish_row(choice, step, b, V, p.best.v, (zt - p.m) - logf(p.sum));
+  const Scale c = row_scale(temp, temp0, b);
+  Part p = no_part();
+  for (int s = lane; s < slices; s += 64) join_parts<GUMBEL>(p, parts[b * slices + s], c.L, c.T);
+  join_lanes<GUMBEL>(p, c.L, c.T);
+  if (lane == 0) finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
 }
 
 // Inverse CDF: one workgroup per sequence finds the slice that u falls into from the slices' sums (64 bits), then walks
@@ -359,110 +463,102 @@ __global__ __launch_bounds__(CH_THREADS) void choose_cdf_kernel(const T *__restr
                                                                 Noise noise, int V, int slices, int slice,
                                                                 const Part *__restrict__ parts,
                                                                 Choice choice, Step step) {
-  extern __shared__ uint32_t cnt[];
+  extern __shared__ __attribute__((aligned(16))) uint32_t cnt[];
   __shared__ double wave_total[CH_THREADS / 64];
   __shared__ int found, last;
-  constexpr int N = 16 / sizeof(T);
+  constexpr int N = Vec<T>::N;
   const int64_t b = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const float temperature = temp ? temp[b] : temp0;
-  const float inv = temperature > 0.f ? 1.f / temperature : 1.f;
+  const Scale c = row_scale(temp, temp0, b);
   const Part *mine = parts + b * slices;
   // every thread joins the slices the same way
-  float M = -FLT_MAX;
-  Best best = {-INFINITY, 0.f, 0.f, -1};
-  for (int s = 0; s < slices; ++s) {
-    M = fmaxf(M, mine[s].m);
-    if (better<false>(best, mine[s].best, 0.f)) best = mine[s].best;
+  Part p = no_part();
+  for (int s = 0; s < slices; ++s) join_parts<false>(p, mine[s], c.L, c.T);
+  if (p.v < 0 || !(c.T > 0.f)) {
+    if (tid == 0) finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
+    return;
   }
+  auto weight = [&](int s) { return static_cast<double>(mine[s].sum * __builtin_amdgcn_exp2f((mine[s].m - p.m) * c.L)); };
   double total = 0.;
-  for (int s = 0; s < slices; ++s) total += static_cast<double>(mine[s].sum * __expf(mine[s].m - M));
-  int pick = best.v;
-  if (best.v >= 0 && temperature > 0.f) {
-    const double target = static_cast<double>(*noise_at(noise, rules, b, 1)) * total;
-    double before = 0.;
-    int at = -1, filled = 0;
-    double base = 0.;
-    for (int s = 0; s < slices; ++s) {
-      const double w = static_cast<double>(mine[s].sum * __expf(mine[s].m - M));
-      if (at < 0 && w > 0.) {
-        filled = s;
-        base = before;
-        if (target < before + w) at = s;
-      }
-      before += w;
+  for (int s = 0; s < slices; ++s) total += weight(s);
+  const double target = static_cast<double>(*noise_at(noise, rules, b, 1)) * total;
+  // the slice: the first whose running sum passes the target (rounding, or a uniform of 1: the last with any weight)
+  int at = -1, filled = 0;
+  double before = 0., run = 0.;
+  for (int s = 0; s < slices && at < 0; ++s) {
+    const double w = weight(s);
+    if (w > 0.) {
+      filled = s;
+      run = before;
+      if (target < before + w) at = s;
     }
-    if (at < 0) at = filled;  // rounding, or a uniform of 1: the last slice with any weight
-    const RowRules r = row_rules(rules, b, V);
-    const int v0 = at * slice, v1 = V - v0 < slice ? V : v0 + slice;
-    if (tid == 0) {
-      found = 0x7fffffff;
-      last = -1;
-    }
-    __syncthreads();
-    if (r.len > 0) count_history(cnt, r.hist, r.len, v0, slice);
-    const T *row = logits + b * ld;
-    double run = base;
-    for (int w0 = v0; w0 < v1; w0 += CH_THREADS * N) {
-      const int v = w0 + tid * N;
-      double e[N], sum = 0.;
-      int top = -1;
+    before += w;
+  }
+  if (at < 0) at = filled;
+  const RowRules r = row_rules(rules, b, V);
+  const int v0 = at * slice, v1 = V - v0 < slice ? V : v0 + slice;
+  if (tid == 0) {
+    found = 0x7fffffff;
+    last = -1;
+  }
+  __syncthreads();
+  if (r.len > 0) count_history(cnt, r.hist, r.len, v0, slice);
+  const T *row = logits + b * ld;
+  Vec<T> x;
+  float z[N];
+  for (int w0 = v0; w0 < v1; w0 += CH_THREADS * N) {
+    const int v = w0 + tid * N;
+    double e[N], sum = 0.;
+    int top = -1;
 #pragma unroll
-      for (int k = 0; k < N; ++k) e[k] = 0.;
-      if (v < v1) {
-        float z[N];
-        const int have = load_some<N>(row, v, V, z);
-        apply_rules<N>(z, r, cnt, v - v0, v, have);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          e[k] = static_cast<double>(__expf(tame(tame(z[k]) * inv) - M));
-          if (e[k] > 0.) top = v + k;
-          sum += e[k];
-        }
-      }
-      double inc = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += up;
-      }
-      if (lane == 63) wave_total[wid] = inc;
-      __syncthreads();
-      double left = run;
-      for (int w = 0; w < CH_THREADS / 64; ++w) {
-        if (w < wid) left += wave_total[w];
-        run += wave_total[w];
-      }
-      left += inc - sum;
-      double cdf = left;
-      int hit = 0x7fffffff;
+    for (int k = 0; k < N; ++k) e[k] = 0.;
+    if (v < v1) {
+      x.load(row, r, v, V);
+      x.rules(z, row, r, cnt + (v - v0) / 2, v, V);
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        cdf += e[k];
-        if (hit == 0x7fffffff && e[k] > 0. && target < cdf) hit = v + k;
+        e[k] = static_cast<double>(__builtin_amdgcn_exp2f((tame(z[k]) - p.m) * c.L));
+        if (e[k] > 0.) top = v + k;
+        sum += e[k];
       }
-      if (hit != 0x7fffffff) atomicMin(&found, hit);
-      if (top >= 0) atomicMax(&last, top);
-      __syncthreads();
-      if (found != 0x7fffffff) break;
     }
-    pick = found != 0x7fffffff ? found : last;
+    double inc = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double up = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 63) wave_total[wid] = inc;
+    __syncthreads();
+    double cdf = run;
+    for (int w = 0; w < CH_THREADS / 64; ++w) {
+      if (w < wid) cdf += wave_total[w];
+      run += wave_total[w];
+    }
+    cdf += inc - sum;
+    int hit = 0x7fffffff;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      cdf += e[k];
+      if (hit == 0x7fffffff && e[k] > 0. && target < cdf) hit = v + k;
+    }
+    if (hit != 0x7fffffff) atomicMin(&found, hit);
+    if (top >= 0) atomicMax(&last, top);
+    __syncthreads();
+    if (found != 0x7fffffff) break;
   }
   if (tid != 0) return;
-  float logp = -INFINITY;
-  if (pick >= 0) {  // the choice's own logit again
-    const RowRules r = row_rules(rules, b, V);
-    const int v = pick & ~(N - 1);
-    float z[N];
-    const int have = load_some<N>(logits + b * ld, v, V, z);
-    if (best.v >= 0 && temperature > 0.f) {
-      apply_rules<N>(z, r, cnt, v % slice, v, have);  // (slices start at multiples of the slice)
-      logp = (tame(tame(z[pick - v]) / temperature) - M) - logf(static_cast<float>(total));
-    } else {
-      logp = (best.z - M) - logf(static_cast<float>(total));
-    }
+  const int pick = found != 0x7fffffff ? found : last, v = pick & ~(N - 1);
+  if (pick < 0) {  // (a slice with weight holds a token with weight)
+    finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
+    return;
   }
-  finish_row(choice, step, b, V, pick, logp);
+  x.load(row, r, v, V);  // the choice's own logit again
+  x.rules(z, row, r, cnt + (v - v0) / 2, v, V);
+  float zt = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) zt = v + k == pick ? tame(z[k]) : zt;
+  finish_row(choice, step, b, V, pick, logp_of(zt, p, c));
 }
 
 // Slices per sequence: about two workgroups per CU in all, of 2048 to 16384 tokens each.
@@ -507,17 +603,26 @@ static int launch_choose(const void *logits, int64_t ld, const Rules &r, const f
   const T *x = static_cast<const T *>(logits);
   const size_t lds = r.hist ? static_cast<size_t>(slice) * 2 : 0;
   const unsigned grid = static_cast<unsigned>(B * slices), join = static_cast<unsigned>((B + 3) / 4);
-  if (mode == CH_GUMBEL) {
-    choose_slices_kernel<T, true><<<grid, CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, slices, slice, parts);
+#define VK_SLICES(GUMBEL, ONE)                                                                                          \
+  choose_slices_kernel<T, GUMBEL, ONE><<<grid, CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, slices, slice, parts, \
+                                                                     choice, step)
+  if (mode == CH_CDF) {
+    VK_SLICES(false, false);
+    choose_cdf_kernel<T><<<static_cast<unsigned>(B), CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, slices, slice,
+                                                                       parts, choice, step);
+  } else if (slices == 1) {
+    if (mode == CH_GUMBEL)
+      VK_SLICES(true, true);
+    else
+      VK_SLICES(false, true);
+  } else if (mode == CH_GUMBEL) {
+    VK_SLICES(true, false);
     choose_join_kernel<true><<<join, 256, 0, s>>>(parts, temp, temp0, B, V, slices, choice, step);
   } else {
-    choose_slices_kernel<T, false><<<grid, CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, slices, slice, parts);
-    if (mode == CH_CDF)
-      choose_cdf_kernel<T><<<static_cast<unsigned>(B), CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, slices, slice,
-                                                                         parts, choice, step);
-    else
-      choose_join_kernel<false><<<join, 256, 0, s>>>(parts, temp, temp0, B, V, slices, choice, step);
+    VK_SLICES(false, false);
+    choose_join_kernel<false><<<join, 256, 0, s>>>(parts, temp, temp0, B, V, slices, choice, step);
   }
+#undef VK_SLICES
   return launch_status("choose_tokens");
 }
 

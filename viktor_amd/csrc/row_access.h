@@ -9,6 +9,12 @@ namespace vk {
 typedef float f32x4_e __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t u16x4_e __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint16_t u16x8_e __attribute__((ext_vector_type(8), aligned(2)));
+typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// 16 bytes of a row as they are.
+__device__ __forceinline__ u32x4 load_16(const bf16_t *p) { return *reinterpret_cast<const u32x4_at2 *>(p); }
+__device__ __forceinline__ u32x4 load_16(const float *p) { return *reinterpret_cast<const u32x4_at4 *>(p); }
 
 template <int N>
 __device__ __forceinline__ void load_row(const float *p, float (&v)[N]) {

@@ -37,11 +37,14 @@ class DecodeEngine:
     # (264 KiB) instead of 512 KiB + 256 B and 256 KiB
     PREFIX_PAD_ROWS = 95
     OWN_PAD_ROWS = 32
+    FUSED_HEAD_VOCAB = 512  # largest vocabulary of select_update, whose LM head and choice are one launch
 
     def __init__(self, model, batch_size: int, max_new_tokens: int, max_frames: int, backend: str = "auto",
                  cuda_graph: bool = True, prefill_batch: int = 128, check_every: int = 32,
                  attention_backend: str = "auto", temperature: float = 0.0, max_homopolymer=64, group_size: int = 1,
-                 logprobs: bool = False, force_eos_last: bool = False, sampling: str = "inverse_cdf"):
+                 logprobs: bool = False, force_eos_last: bool = False, sampling: str = "inverse_cdf",
+                 repetition_penalty: float = 1.0, presence_penalty: float = 0.0, frequency_penalty: float = 0.0,
+                 grammar=None):
         self.model, self.dec = model, model.decoder
         self.temperature = float(temperature)
         # force_eos_last: the last output column (max_new_tokens - 1) is EOS for every sequence still running when
@@ -108,6 +111,21 @@ class DecodeEngine:
         u_shape = (batch_size, max_new_tokens) + ((tk.vocab_size,) if self.gumbel else ())
         self.uniforms = torch.zeros(u_shape, dtype=torch.float32, device=dev)
         self._uniforms_set = False
+        # the rules on logits beyond the bias, over what each sequence has produced (see _choose). grammar = (allowed bool
+        # [S, V], rows int [V]): after token t only the tokens that allowed[rows[t]] names may follow (rows[t] < 0: any)
+        if not repetition_penalty > 0:
+            raise ValueError(f"repetition_penalty must be positive (got {repetition_penalty})")
+        self.penalties = (float(repetition_penalty), float(presence_penalty), float(frequency_penalty))
+        self.allowed = self.token_rows = None
+        if grammar is not None:
+            mask, rows = (torch.as_tensor(t) for t in grammar)
+            if mask.dtype != torch.bool or mask.dim() != 2 or mask.shape[1] != tk.vocab_size or rows.shape != (tk.vocab_size,) \
+                    or rows.dtype not in (torch.int32, torch.int64) or int(rows.max()) >= mask.shape[0]:
+                raise ValueError("grammar: (allowed bool [S, V], rows int [V] with values below S)")
+            self.allowed = ops.pack_allowed(mask.to(dev))
+            self.token_rows = rows.to(dev, torch.int32).contiguous()
+        self._fused_head = (tk.vocab_size <= self.FUSED_HEAD_VOCAB and self.penalties == (1.0, 0.0, 0.0)
+                            and grammar is None)
         # logprobs=True: logp[b, j] = log-probability of output token j under the distribution it was chosen
         # from (log softmax of (logits + bias) / T, or of logits + bias when greedy), before the grammar rules
         self.logp = torch.zeros(batch_size, max_new_tokens, dtype=torch.float32, device=dev) if logprobs else None
@@ -130,11 +148,26 @@ class DecodeEngine:
             x = self.fast.decode_residual(self.pos32, self.rows, self.seqlens, self.cache, rope_pos=self.rpos32,
                                           tok=self.tok, prefix=(self.prefix_cache, self.prefix_len32, self.G,
                                                                 self.grouped_workspace))
-        ops.select_update(self.bias, self.is_tail, self.is_homo, self.homo_stop, self.tok, self.run, self.pos,
-                          self.plen, self.rope_off, self.out, self.pos32, self.seqlens, self.rpos32, EOS, PAD,
-                          h=x, norm_w=self.dec.norm.weight, eps=self.dec.cfg.norm_eps, w_head=self.dec.lm_head.weight,
-                          round_bf16=self.temperature > 0, temperature=self.temperature, uniforms=self.uniforms, gumbel=self.gumbel,
-                          cache_base=None if self.G == 1 else self.cache_base, logp_out=self.logp)
+        self._choose(x, self.dec.norm.weight, self.temperature > 0)
+
+    def _choose(self, h, norm_w, round_bf16):
+        """Token choice and state update from the residual stream h and the final norm's weight, or from the final-normed
+        hidden state (norm_w None). Up to FUSED_HEAD_VOCAB tokens without penalties and grammar the LM head is part of the
+        choice; else it is a product of its own, whose logits choose_update reads once."""
+        state = (self.bias, self.is_tail, self.is_homo, self.homo_stop, self.tok, self.run, self.pos, self.plen,
+                 self.rope_off, self.out, self.pos32, self.seqlens, self.rpos32, EOS, PAD)
+        opts = dict(temperature=self.temperature, uniforms=self.uniforms, gumbel=self.gumbel,
+                    cache_base=None if self.G == 1 else self.cache_base, logp_out=self.logp)
+        if self._fused_head:
+            ops.select_update(*state, h=h, norm_w=norm_w, eps=self.dec.cfg.norm_eps, w_head=self.dec.lm_head.weight,
+                              round_bf16=round_bf16, **opts)
+            return
+        if norm_w is not None:
+            h = ops.add_rmsnorm(h, norm_w, self.dec.cfg.norm_eps)
+        logits = ops.linear(h, self.dec.lm_head.weight, out_dtype=torch.bfloat16 if round_bf16 else torch.float32)
+        rep, pres, freq = self.penalties
+        ops.choose_update(logits, *state, **opts, repetition=rep, presence=pres, frequency=freq, allowed=self.allowed,
+                          token_rows=self.token_rows)
 
     def _reset_state(self):
         self.pos.fill_(1)
@@ -269,11 +302,7 @@ class DecodeEngine:
         if G > 1:
             self.cache_base.copy_(self.plen + 1)  # the first sampled token goes to own-token row 0
         self.rope_off.copy_(self.plen * (self.pos_scale - 1))
-        ops.select_update(self.bias, self.is_tail, self.is_homo, self.homo_stop, self.tok, self.run, self.pos,
-                          self.plen, self.rope_off, self.out, self.pos32, self.seqlens, self.rpos32, EOS, PAD,
-                          h=h.contiguous(), w_head=self.dec.lm_head.weight, round_bf16=True,
-                          temperature=self.temperature, uniforms=self.uniforms, gumbel=self.gumbel,
-                          cache_base=None if G == 1 else self.cache_base, logp_out=self.logp)
+        self._choose(h.contiguous(), None, True)
         self.step_idx.fill_(1)
 
     def _check_groups(self, frames, frame_lens, offs):

@@ -15,6 +15,7 @@ status other than OK raises HipLibraryError.
 """
 
 import ctypes
+import functools
 
 import numpy as np
 
@@ -856,16 +857,33 @@ def embed_grad(d_rows, tokens, vocab):
     return out
 
 
+def _refuse(what, msg):
+    raise AssertionError(f"{what}: {msg}")
+
+
 def _here(what, *ts):
     """Every tensor on the current device: launches go to its current stream."""
+    dev = None
     for t in ts:
-        if torch.is_tensor(t):
-            require_device(t, what)
-            _require(t.get_device() == torch.cuda.current_device(), f"{what}: tensors on the current device")
+        if isinstance(t, torch.Tensor):
+            if not t.is_cuda:
+                require_device(t, what)
+            if dev is None:
+                dev = torch._C._cuda_getDevice()
+            if t.get_device() != dev:
+                _refuse(what, "tensors on the current device")
 
 
 def _vk_dtype(t):
     return VK_DTYPE_F32 if t == torch.float32 else VK_DTYPE_BF16
+
+
+def _rows_ok(t):
+    """[n, d] bf16 or fp32 whose rows are contiguous and do not overlap."""
+    if t.dim() != 2 or t.dtype not in (BF16, torch.float32):
+        return False
+    n, d = t.shape
+    return d > 0 and (t.is_contiguous() or ((t.stride(1) == 1 or d == 1) and (n < 2 or t.stride(0) >= d)))
 
 
 def embed_lookup(weight, tokens, scale=1.0, out_dtype=None):
@@ -873,15 +891,24 @@ def embed_lookup(weight, tokens, scale=1.0, out_dtype=None):
     (bf16 or fp32; default: the weight's). The product is fp32, rounded once. Ids outside [0, V) give zero rows.
     Reference: nn.Embedding's gather, viktor/model.py:77."""
     _here("embed_lookup", weight, tokens)
-    odt = out_dtype or weight.dtype
-    _require(weight.dim() == 2 and weight.dtype in (BF16, torch.float32) and odt in (BF16, torch.float32)
-             and weight.shape[0] > 0 and weight.shape[1] > 0, "embed_lookup: weight [V, d] and out bf16 or fp32")
-    _require(tokens.dtype == torch.long and _contig(weight, tokens), "embed_lookup: contiguous weight and int64 tokens")
+    wdt = weight.dtype
+    odt = out_dtype or wdt
+    if weight.dim() != 2 or wdt not in (BF16, torch.float32) or odt not in (BF16, torch.float32) or weight.numel() == 0:
+        _refuse("embed_lookup", "weight [V, d] and out bf16 or fp32")
+    if tokens.dtype != torch.long or not (weight.is_contiguous() and tokens.is_contiguous()):
+        _refuse("embed_lookup", "contiguous weight and int64 tokens")
     V, d = weight.shape
-    out = torch.empty(*tokens.shape, d, dtype=odt, device=weight.device)
-    call("vk_embed_lookup", ptr(weight), _vk_dtype(weight.dtype), ptr(tokens), tokens.numel(), V, d, float(scale), ptr(out),
-         _vk_dtype(odt), stream_handle())
+    out = torch.empty((*tokens.shape, d), dtype=odt, device=weight.device)
+    call("vk_embed_lookup", weight.data_ptr(), _vk_dtype(wdt), tokens.data_ptr(), tokens.numel(), V, d, float(scale),
+         out.data_ptr(), _vk_dtype(odt), stream_handle())
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _sorted_workspace(n, V, d):
+    nb = ctypes.c_int64(0)
+    call("vk_embed_grad_sorted_workspace", n, V, d, ctypes.byref(nb))
+    return nb.value
 
 
 def embed_grad_sorted(d_rows, tokens, vocab, scale=1.0, pad=None, out=None, accumulate=False):
@@ -890,23 +917,24 @@ def embed_grad_sorted(d_rows, tokens, vocab, scale=1.0, pad=None, out=None, accu
     n, vocab and the ids alone decide. Rows of ids outside [0, vocab) and of the id `pad` add nothing. out: the caller's
     contiguous fp32 [vocab, d]; accumulate: added to what it holds. Reference: the backward of nn.Embedding,
     viktor/decoder.py:127, as viktor/model.py:77 gathers it."""
-    _here("embed_grad_sorted", d_rows, tokens, out)
-    _require(d_rows.dim() == 2 and d_rows.dtype in (BF16, torch.float32) and d_rows.shape[1] > 0
-             and (d_rows.stride(1) == 1 or d_rows.shape[1] == 1) and (d_rows.shape[0] < 2 or d_rows.stride(0) >= d_rows.shape[1]),
-             "embed_grad_sorted: d_rows [n, d] bf16 or fp32, rows side by side")
-    _require(tokens.shape == (d_rows.shape[0],) and tokens.dtype == torch.long and tokens.is_contiguous(),
-             "embed_grad_sorted: tokens [n] int64")
-    _require(vocab > 0 and (out is not None or not accumulate), "embed_grad_sorted: vocab > 0, accumulate into out")
+    what = "embed_grad_sorted"
+    _here(what, d_rows, tokens, out)
+    if not _rows_ok(d_rows):
+        _refuse(what, "d_rows [n, d] bf16 or fp32, rows side by side")
     n, d = d_rows.shape
-    _require(out is None or (out.dtype == torch.float32 and out.shape == (vocab, d) and out.is_contiguous()),
-             "embed_grad_sorted: out fp32 [vocab, d]")
-    nb = ctypes.c_int64(0)
-    call("vk_embed_grad_sorted_workspace", n, vocab, d, ctypes.byref(nb))
-    ws = torch.empty(nb.value, dtype=torch.uint8, device=d_rows.device)
+    if tokens.shape != (n,) or tokens.dtype != torch.long or not tokens.is_contiguous():
+        _refuse(what, "tokens [n] int64")
+    if vocab <= 0 or (accumulate and out is None):
+        _refuse(what, "vocab > 0, accumulate into out")
     if out is None:
-        out = torch.empty(vocab, d, dtype=torch.float32, device=d_rows.device)
-    call("vk_embed_grad_sorted", ptr(d_rows), _vk_dtype(d_rows.dtype), max(d_rows.stride(0), d), ptr(tokens), n, vocab, d,
-         float(scale), -1 if pad is None else int(pad), ptr(out), int(bool(accumulate)), ptr(ws), nb.value, stream_handle())
+        out = torch.empty((vocab, d), dtype=torch.float32, device=d_rows.device)
+    elif out.dtype != torch.float32 or out.shape != (vocab, d) or not out.is_contiguous():
+        _refuse(what, "out fp32 [vocab, d]")
+    nb = _sorted_workspace(n, vocab, d)
+    ws = torch.empty(nb, dtype=torch.uint8, device=d_rows.device)
+    call("vk_embed_grad_sorted", d_rows.data_ptr(), _vk_dtype(d_rows.dtype), max(d_rows.stride(0), d), tokens.data_ptr(), n,
+         vocab, d, float(scale), -1 if pad is None else int(pad), out.data_ptr(), int(bool(accumulate)), ws.data_ptr(), nb,
+         stream_handle())
     return out
 
 
@@ -922,56 +950,66 @@ def pack_allowed(mask):
     return torch.where(w >= 2 ** 31, w - 2 ** 32, w).to(torch.int32)
 
 
-def _per_row(x, B, what):
+def _per_row(x, B, what, name):
     """A float, or fp32 [B] on the device -> (pointer or None, the float)."""
-    if not torch.is_tensor(x):
+    if not isinstance(x, torch.Tensor):
         return None, float(x)
-    _require(x.dtype == torch.float32 and x.shape == (B,) and x.is_contiguous(), f"{what}: a float or fp32 [B]")
+    if x.dtype != torch.float32 or x.shape != (B,) or not x.is_contiguous():
+        _refuse(what, f"{name}: a float or fp32 [B]")
     return x.data_ptr(), 0.0
 
 
 def _mask_args(allowed, V, what):
     if allowed is None:
         return None, 0, 0
-    _require(allowed.dim() == 2 and allowed.dtype == torch.int32 and allowed.shape[0] > 0
-             and allowed.shape[1] >= -(-V // 32) and allowed.is_contiguous(), f"{what}: allowed int32 [S, ceil(V / 32)]")
-    return allowed.data_ptr(), allowed.shape[1], allowed.shape[0]
+    if allowed.dim() != 2 or allowed.dtype != torch.int32 or not allowed.is_contiguous():
+        _refuse(what, "allowed int32 [S, ceil(V / 32)]")
+    S, words = allowed.shape
+    if S == 0 or words < (V + 31) // 32:
+        _refuse(what, "allowed int32 [S, ceil(V / 32)]")
+    return allowed.data_ptr(), words, S
 
 
 def _logit_rules(what, logits, history, lengths, repetition, presence, frequency, bias, allowed, allowed_rows):
-    """The checked arguments of the rules, in the C entry points' order."""
+    """B, V and the checked arguments of the rules, in the C entry points' order."""
     _here(what, logits, history, lengths, repetition, presence, frequency, bias, allowed, allowed_rows)
-    _require(logits.dim() == 2 and logits.dtype in (BF16, torch.float32) and logits.shape[1] > 0
-             and (logits.stride(1) == 1 or logits.shape[1] == 1)
-             and (logits.shape[0] < 2 or logits.stride(0) >= logits.shape[1]), f"{what}: logits [B, V] bf16 or fp32, rows side by side")
+    if not _rows_ok(logits):
+        _refuse(what, "logits [B, V] bf16 or fp32, rows side by side")
     B, V = logits.shape
-    rep, pres, freq = (_per_row(x, B, f"{what}: {name}") for x, name in
-                       ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")))
-    _require(rep[0] is not None or rep[1] > 0, f"{what}: the repetition penalty must be positive")
+    rep = _per_row(repetition, B, what, "repetition")
+    pres = _per_row(presence, B, what, "presence")
+    freq = _per_row(frequency, B, what, "frequency")
+    if rep[0] is None and not rep[1] > 0:
+        _refuse(what, "the repetition penalty must be positive")
     hist = (None, 0, 0, None)
     if history is None:
-        _require(lengths is None and rep == (None, 1.0) and pres == (None, 0.0) and freq == (None, 0.0),
-                 f"{what}: penalties need the history and its lengths")
+        if lengths is not None or rep != (None, 1.0) or pres != (None, 0.0) or freq != (None, 0.0):
+            _refuse(what, "penalties need the history and its lengths")
     else:
-        _require(history.dim() == 2 and history.shape[0] == B and history.dtype == torch.long
-                 and (history.stride(1) == 1 or history.shape[1] < 2)
-                 and (B < 2 or history.stride(0) >= history.shape[1]), f"{what}: history int64 [B, T], rows side by side")
-        _require(lengths is not None and lengths.shape == (B,) and lengths.dtype == torch.int32 and lengths.is_contiguous(),
-                 f"{what}: lengths int32 [B]")
-        if history.shape[1] > 0:
-            hist = (history.data_ptr(), max(history.stride(0), history.shape[1]), history.shape[1], lengths.data_ptr())
+        if history.dim() != 2 or history.dtype != torch.long or history.shape[0] != B:
+            _refuse(what, "history int64 [B, T]")
+        T = history.shape[1]
+        if not history.is_contiguous() and ((T > 1 and history.stride(1) != 1) or (B > 1 and history.stride(0) < T)):
+            _refuse(what, "history rows side by side")
+        if lengths is None or lengths.shape != (B,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+            _refuse(what, "lengths int32 [B]")
+        if T > 0:
+            hist = (history.data_ptr(), max(history.stride(0), T), T, lengths.data_ptr())
     bp, bld = None, 0
     if bias is not None:
-        _require(bias.dtype == torch.float32 and bias.shape in ((V,), (B, V)) and (bias.stride(-1) == 1 or V == 1)
-                 and (bias.dim() == 1 or B < 2 or bias.stride(0) >= V), f"{what}: bias fp32 [V] or [B, V]")
+        if bias.dtype != torch.float32 or bias.shape not in ((V,), (B, V)):
+            _refuse(what, "bias fp32 [V] or [B, V]")
+        if not bias.is_contiguous() and ((V > 1 and bias.stride(-1) != 1) or (bias.dim() == 2 and B > 1 and bias.stride(0) < V)):
+            _refuse(what, "bias rows side by side")
         bp, bld = bias.data_ptr(), 0 if bias.dim() == 1 else max(bias.stride(0), V)
-    mask = _mask_args(allowed, V, what)
-    _require(allowed_rows is None or (allowed is not None and allowed_rows.shape == (B,) and allowed_rows.dtype == torch.int32
-                                      and allowed_rows.is_contiguous()), f"{what}: allowed_rows int32 [B], with allowed")
-    _require(allowed is None or allowed_rows is not None or allowed.shape[0] in (1, B),
-             f"{what}: allowed without allowed_rows has 1 row or one per sequence")
-    return B, V, (ptr(logits), _vk_dtype(logits.dtype), max(logits.stride(0), V), *hist, *rep, *pres, *freq, bp, bld, *mask,
-                  ptr(allowed_rows))
+    ap, words, S = _mask_args(allowed, V, what)
+    if allowed_rows is not None:
+        if allowed is None or allowed_rows.shape != (B,) or allowed_rows.dtype != torch.int32 or not allowed_rows.is_contiguous():
+            _refuse(what, "allowed_rows int32 [B], with allowed")
+    elif allowed is not None and S not in (1, B):
+        _refuse(what, "allowed without allowed_rows has 1 row or one per sequence")
+    return B, V, (logits.data_ptr(), _vk_dtype(logits.dtype), max(logits.stride(0), V), *hist, *rep, *pres, *freq, bp, bld,
+                  ap, words, S, ptr(allowed_rows))
 
 
 def process_logits(logits, history=None, lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,
@@ -987,21 +1025,26 @@ def process_logits(logits, history=None, lengths=None, repetition=1.0, presence=
     B, V, args = _logit_rules("process_logits", logits, history, lengths, repetition, presence, frequency, bias, allowed,
                               allowed_rows)
     if out is None:
-        out = torch.empty(B, V, dtype=out_dtype or logits.dtype, device=logits.device)
-    _here("process_logits", out)
-    _require(out.shape == (B, V) and out.dtype in (BF16, torch.float32) and (out_dtype is None or out.dtype == out_dtype)
-             and (out.stride(1) == 1 or V == 1) and (B < 2 or out.stride(0) >= V), "process_logits: out [B, V] bf16 or fp32")
-    call("vk_process_logits", *args, ptr(out), _vk_dtype(out.dtype), max(out.stride(0), V), B, V, stream_handle())
+        odt = out_dtype or logits.dtype
+        if odt not in (BF16, torch.float32):
+            _refuse("process_logits", "out bf16 or fp32")
+        out = torch.empty((B, V), dtype=odt, device=logits.device)
+    else:
+        _here("process_logits", out)
+        if out.shape != (B, V) or not _rows_ok(out) or (out_dtype is not None and out.dtype != out_dtype):
+            _refuse("process_logits", "out [B, V] bf16 or fp32, rows side by side")
+    call("vk_process_logits", *args, out.data_ptr(), _vk_dtype(out.dtype), max(out.stride(0), V), B, V, stream_handle())
     return out
 
 
 _MODE_GREEDY, _MODE_GUMBEL, _MODE_CDF = 0, 1, 2
 
 
-def _choose_workspace(B, V, device):
+@functools.lru_cache(maxsize=256)
+def _choose_workspace(B, V):
     nb = ctypes.c_int64(0)
     call("vk_choose_tokens_workspace", B, V, ctypes.byref(nb))
-    return torch.empty(max(nb.value, 16), dtype=torch.uint8, device=device)
+    return max(nb.value, 16)
 
 
 def choose_tokens(logits, history=None, lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,
@@ -1015,25 +1058,85 @@ def choose_tokens(logits, history=None, lengths=None, repetition=1.0, presence=0
     B, V, args = _logit_rules("choose_tokens", logits, history, lengths, repetition, presence, frequency, bias, allowed,
                               allowed_rows)
     _here("choose_tokens", temperature, uniforms)
-    temp = _per_row(temperature, B, "choose_tokens: temperature")
+    temp = _per_row(temperature, B, "choose_tokens", "temperature")
     mode, up, uld = _MODE_GREEDY, None, 0
     if uniforms is None:
-        _require(temp[0] is None and temp[1] <= 0, "choose_tokens: a temperature needs uniforms")
+        if temp[0] is not None or temp[1] > 0:
+            _refuse("choose_tokens", "a temperature needs uniforms")
     else:
-        _require(uniforms.dtype == torch.float32 and uniforms.shape in ((B,), (B, V)), "choose_tokens: uniforms fp32 [B] or [B, V]")
+        if uniforms.dtype != torch.float32 or uniforms.shape not in ((B,), (B, V)):
+            _refuse("choose_tokens", "uniforms fp32 [B] or [B, V]")
         if uniforms.dim() == 2:
-            _require((uniforms.stride(1) == 1 or V == 1) and (B < 2 or uniforms.stride(0) >= V), "choose_tokens: uniform rows")
+            if not _rows_ok(uniforms):
+                _refuse("choose_tokens", "uniform rows side by side")
             mode, uld = _MODE_GUMBEL, max(uniforms.stride(0), V)
         else:
-            _require(uniforms.is_contiguous(), "choose_tokens: contiguous uniforms")
+            if not uniforms.is_contiguous():
+                _refuse("choose_tokens", "contiguous uniforms")
             mode, uld = _MODE_CDF, 1
         up = uniforms.data_ptr()
-    token = torch.empty(B, dtype=torch.long, device=logits.device)
-    logp = torch.empty(B, dtype=torch.float32, device=logits.device)
-    ws = _choose_workspace(B, V, logits.device)
-    call("vk_choose_tokens", *args, *temp, mode, up, uld, int(fallback), ptr(token), ptr(logp), B, V, ptr(ws), ws.numel(),
-         stream_handle())
+    dev = logits.device
+    token = torch.empty(B, dtype=torch.long, device=dev)
+    logp = torch.empty(B, dtype=torch.float32, device=dev)
+    nb = _choose_workspace(B, V)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    call("vk_choose_tokens", *args, *temp, mode, up, uld, int(fallback), token.data_ptr(), logp.data_ptr(), B, V,
+         ws.data_ptr(), nb, stream_handle())
     return token, logp
+
+
+def choose_update(logits, bias, is_tail, is_homo, homo_stop, tok, run, pos, plen, rope_off, out, pos32, seqlens, rpos32,
+                  eos, pad, temperature=0.0, uniforms=None, gumbel=False, logp_out=None, cache_base=None, repetition=1.0,
+                  presence=0.0, frequency=0.0, allowed=None, token_rows=None):
+    """select_update from logits [B, V] (bf16 or fp32) at any vocabulary, after process_logits' rules: the penalties
+    (floats) count what each sequence has produced, out[b, :pos[b] - plen[b]]; bias fp32 [V]; allowed int32
+    [S, ceil(V / 32)] with token_rows int32 [V], the mask row that follows each previous token (-1: no mask). uniforms
+    [B, T], or [B, T, V] with gumbel, read at the output column. The bookkeeping and the other arguments are
+    select_update's; a sequence with nothing left takes pad."""
+    what = "choose_update"
+    _here(what, logits, bias, is_tail, is_homo, tok, run, pos, plen, rope_off, out, pos32, seqlens, rpos32, uniforms,
+          logp_out, cache_base, allowed, token_rows)
+    if not _rows_ok(logits):
+        _refuse(what, "logits [B, V] bf16 or fp32, rows side by side")
+    B, V = logits.shape
+    if bias.shape != (V,) or bias.dtype != torch.float32 or not bias.is_contiguous():
+        _refuse(what, "bias fp32 [V]")
+    for t, dt in ((tok, torch.long), (pos, torch.long), (run, torch.long), (plen, torch.long), (rope_off, torch.long),
+                  (cache_base, torch.long), (pos32, torch.int32), (seqlens, torch.int32), (rpos32, torch.int32)):
+        if t is not None and (t.dtype != dt or t.shape != (B,) or not t.is_contiguous()):
+            _refuse(what, "state tensors [B]")
+    if out.dim() != 2 or out.shape[0] != B or out.dtype != torch.long or out.stride(1) != 1 or out.stride(0) < out.shape[1]:
+        _refuse(what, "out int64 [B, T]")
+    for m in (is_tail, is_homo):
+        if m.dtype not in (torch.bool, torch.uint8) or m.shape != (V,) or not m.is_contiguous():
+            _refuse(what, "masks [V]")
+    mode, us, uc = _MODE_GREEDY, 0, 0
+    if temperature > 0:
+        mode = _MODE_GUMBEL if gumbel else _MODE_CDF
+        tail = (V,) if gumbel else ()
+        if (uniforms is None or uniforms.dtype != torch.float32 or uniforms.dim() != 2 + len(tail)
+                or uniforms.shape[0] != B or uniforms.shape[2:] != tail or not uniforms.is_contiguous()):
+            _refuse(what, "uniforms fp32 [B, T], or [B, T, V] with gumbel")
+        us, uc = uniforms.stride(0), uniforms.shape[1]
+    lp_stride = 0
+    if logp_out is not None:
+        if logp_out.dtype != torch.float32 or logp_out.dim() not in (1, 2) or logp_out.shape[0] != B or logp_out.stride(-1) != 1:
+            _refuse(what, "logp_out [B] or [B, T] fp32")
+        if logp_out.dim() == 2:
+            if logp_out.shape[1] < out.shape[1]:
+                _refuse(what, "logp_out columns")
+            lp_stride = logp_out.stride(0)
+    mask = _mask_args(allowed, V, what)
+    if (allowed is None) != (token_rows is None) or (token_rows is not None and (
+            token_rows.dtype != torch.int32 or token_rows.shape != (V,) or not token_rows.is_contiguous())):
+        _refuse(what, "allowed goes with token_rows int32 [V]")
+    nb = _choose_workspace(B, V)
+    ws = torch.empty(nb, dtype=torch.uint8, device=logits.device)
+    call("vk_choose_update", logits.data_ptr(), _vk_dtype(logits.dtype), max(logits.stride(0), V), float(repetition),
+         float(presence), float(frequency), bias.data_ptr(), *mask, ptr(token_rows), is_tail.data_ptr(), is_homo.data_ptr(),
+         int(homo_stop), float(temperature), mode, ptr(uniforms) if mode else None, us, uc, tok.data_ptr(), ptr(run),
+         pos.data_ptr(), ptr(plen), ptr(rope_off), ptr(cache_base), out.data_ptr(), out.stride(0), out.shape[1], ptr(pos32),
+         ptr(seqlens), ptr(rpos32), ptr(logp_out), lp_stride, B, V, int(eos), int(pad), ws.data_ptr(), nb, stream_handle())
 
 
 def _norm_blocks(n):

@@ -32,6 +32,7 @@ from . import hip_ops as ops
 from .gspo import sequence_ratio_loss
 
 BF16 = torch.bfloat16
+SORTED_GRAD_VOCAB = 343
 _LAYER_PARAMS = ("attn_norm.weight", "attn.qkv_proj.weight", "attn.q_norm.weight", "attn.k_norm.weight",
                  "attn.o_proj.weight", "mlp_norm.weight", "gate_up.weight", "down.weight")
 
@@ -53,21 +54,33 @@ def _residual_norm(x, a, w, norm_w, eps):
 
 
 class _TokenEmbed(torch.autograd.Function):
-    """emb[tokens] in fp32 (the gather of viktor/model.py:77, 81-84: nn.Embedding of fp32 weights, which autocast
-    leaves in fp32) with the table's gradient as the fp32 sum of the gradient rows of each token id (vk_embed_grad:
-    deterministic, no atomics)."""
+    """scale * emb[tokens] in fp32 (at scale 1 the gather of viktor/model.py:77, 81-84: nn.Embedding of fp32 weights, which
+    autocast leaves in fp32) with the table's gradient as scale times the fp32 sum of the gradient rows of each token id,
+    rows of the id `pad` left out (deterministic, no atomics)."""
 
     @staticmethod
-    def forward(ctx, weight, tokens):
+    def forward(ctx, weight, tokens, scale=1.0, pad=None):
         ctx.save_for_backward(tokens)
-        ctx.vocab = weight.shape[0]
-        return weight.detach().float()[tokens]
+        ctx.vocab, ctx.scale, ctx.pad, ctx.dtype = weight.shape[0], scale, pad, weight.dtype
+        return ops.embed_lookup(weight.detach().contiguous(), tokens.contiguous(), scale=scale, out_dtype=torch.float32)
 
     @staticmethod
     def backward(ctx, d_rows):
         (tokens,) = ctx.saved_tensors
         d = d_rows.reshape(-1, d_rows.shape[-1]).float().contiguous()
-        return ops.embed_grad(d, tokens.reshape(-1).contiguous(), ctx.vocab), None
+        t = tokens.reshape(-1).contiguous()
+        if ctx.vocab <= SORTED_GRAD_VOCAB and ctx.scale == 1.0 and ctx.pad is None and d.shape[1] % 8 == 0:
+            g = ops.embed_grad(d, t, ctx.vocab)
+        else:
+            g = ops.embed_grad_sorted(d, t, ctx.vocab, scale=ctx.scale, pad=ctx.pad)
+        return g.to(ctx.dtype), None, None, None
+
+
+def token_embedding(weight, tokens, scale=1.0, pad=None):
+    """Differentiable scaled token embedding: scale * weight[tokens] in fp32, weight [V, d] fp32 or bf16, tokens int64 of any
+    shape. The gradient of weight sums the rows of each id (by sorted tokens past SORTED_GRAD_VOCAB ids), without those
+    of the id `pad` (nn.Embedding's padding_idx). What train_logits runs, at scale 1; reference: viktor/model.py:77."""
+    return _TokenEmbed.apply(weight, tokens, float(scale), pad)
 
 
 def _pad_cols(t, width):
@@ -307,7 +320,7 @@ def train_logits(model, frames, tokens_in, plens=None, group_size=1):
     proj = model.projector
     prefix = _Projector.apply(frames.reshape(B * P, -1).to(BF16).contiguous(), proj[0].weight, proj[0].bias,
                               proj[2].weight, proj[2].bias)                            # [B P, d] bf16
-    emb = _TokenEmbed.apply(dec.embed.weight, tokens_in.to(dev).reshape(-1))          # [B T, d] fp32
+    emb = token_embedding(dec.embed.weight, tokens_in.to(dev, torch.long).reshape(-1))  # [B T, d] fp32
     # packed layout, window b: its plens[b] real prefix rows, then its T token rows; row indices on the host
     s = model.pos_scale
 
@@ -347,7 +360,7 @@ def _train_logits_shared(model, frames, tokens_in, plens_h, G):
     proj = model.projector
     prefix = _Projector.apply(frames[::G].reshape(ng * P, -1).to(BF16).contiguous(), proj[0].weight, proj[0].bias,
                               proj[2].weight, proj[2].bias)                            # [B / G P, d] bf16
-    emb = _TokenEmbed.apply(dec.embed.weight, tokens_in.to(dev).reshape(-1))          # [B T, d] fp32
+    emb = token_embedding(dec.embed.weight, tokens_in.to(dev, torch.long).reshape(-1))  # [B T, d] fp32
     s = model.pos_scale
 
     def build():
