@@ -224,7 +224,7 @@ def _dev(*ts):
     return [t.to(DEV) for t in ts]
 
 
-SIZES = [(1, 1, 1), (3, 7, 5), (2, 343, 40), (5, 1367, 100), (4, 5463, 300), (2, 2049, 2049), (600, 33, 9), (3, 40001, 500)]
+SIZES = [(1, 1, 1), (3, 7, 5), (2, 343, 40), (5, 1367, 100), (4, 5463, 300), (2, 2049, 2049), (600, 33, 9), (512, 9001, 20), (3, 40001, 500)]
 
 
 @pytest.mark.parametrize("B,V,T", SIZES)

@@ -9,9 +9,15 @@
 // never chosen and weighs nothing; +inf counts as the largest finite value. log-probability: z' of the choice minus
 // log sum exp z'. A row with nothing left takes the fallback token, log-probability -inf.
 //
-// A workgroup takes one slice of one sequence's vocabulary and counts the history's tokens of that slice in LDS (16 bits
-// each), so no count per (sequence, token) exists in memory. Slices give (max, sum of exponentials at it, best); one
-// wavefront per sequence joins them.
+// A workgroup takes one slice of one sequence's vocabulary. The history's tokens of the slice are gathered in LDS (Seen),
+// so no count per (sequence, token) exists in memory and the streaming pass over the logits knows of the history only that
+// a token is left out: a distinct token of it is computed once, by one thread. The pass is bound by memory while it runs;
+// what keeps it from the rate of a plain copy is the gathering (two barriers, a dependent load) that every slice begins
+// with, and the bias, which is read through the same in-order path as the logits. Slices of 4096 to 8192 tokens: 512 x
+// 87383 bf16 logits take 35 us without rules (5.1 TB/s, a copy of that size 31 to 36 us), 42 us with a bias, 46 us with a
+// history of 256, 52 us with all; slices of 16384 took 58 us, of 4096 58 us. The choice from fp32 logits gives (max, sum of
+// exponentials at it, best) per slice, joined by one wavefront per sequence, or takes a whole row per workgroup of 512
+// threads: 43 us against 54 us in slices at 512 x 87383.
 #include <float.h>
 #include <math.h>
 
@@ -21,9 +27,11 @@
 namespace vk {
 
 constexpr int CH_THREADS = 256;
-constexpr int CH_SLICE = 16384;   // tokens of a slice at most: 32 KB of LDS counts
-constexpr int CH_SLICE_MIN = 2048;
-constexpr int CH_HIST_MAX = 65535;  // a count has 16 bits
+constexpr int CH_THREADS_ONE = 512;  // of a workgroup that takes a whole row
+constexpr int CH_WHOLE = 1 << 17;    // tokens of such a row at most, where it has more than one slice: 16 KB of LDS bits
+constexpr int CH_SLICE = 8192;       // tokens of a slice at most
+constexpr int CH_HASH_MAX = 2048;    // history columns at most whose counts are hashed: 32 KB of LDS either way
+constexpr int CH_HIST_MAX = 65535;
 
 struct Rules {
   const int64_t *hist;  // [B, hist_cols], row stride hist_ld; null: no penalties
@@ -41,6 +49,12 @@ struct Rules {
   const int64_t *tok;
 };
 
+// How a call is cut: slices of `slice` tokens per sequence, and the history's table (Seen).
+struct Plan {
+  int slices, slice, slots;
+  bool hashed, one;
+};
+
 struct RowRules {
   const int64_t *hist;
   int len;  // 0: no penalties
@@ -49,13 +63,24 @@ struct RowRules {
   const uint32_t *allowed;
 };
 
+// What a pointer that is not given is read from instead, so that a row's scalars are loaded side by side.
+__device__ const int64_t kNothing[1] = {0};
+
+template <typename P>
+__device__ __forceinline__ P at_or_zero(const P *p, int64_t i) {
+  return *(p != nullptr ? p + i : reinterpret_cast<const P *>(kNothing));
+}
+
 __device__ __forceinline__ RowRules row_rules(const Rules &r, int64_t b, int V) {
+  const float rep = at_or_zero(r.rep, b), pres = at_or_zero(r.pres, b), freq = at_or_zero(r.freq, b);
+  const int32_t len = at_or_zero(r.len, b), arow = at_or_zero(r.arow, b);
+  const int64_t pos = at_or_zero(r.pos, b), plen = at_or_zero(r.plen, b), tok = at_or_zero(r.tok, b);
   RowRules o = {};
   if (r.hist != nullptr) {
-    o.rep = r.rep ? r.rep[b] : r.rep0;
-    o.pres = r.pres ? r.pres[b] : r.pres0;
-    o.freq = r.freq ? r.freq[b] : r.freq0;
-    int64_t n = r.len ? r.len[b] : r.pos[b] - (r.plen ? r.plen[b] : 0);
+    o.rep = r.rep ? rep : r.rep0;
+    o.pres = r.pres ? pres : r.pres0;
+    o.freq = r.freq ? freq : r.freq0;
+    int64_t n = r.len ? len : pos - plen;
     n = n < 0 ? 0 : (n > r.hist_cols ? r.hist_cols : n);
     o.hist = r.hist + b * r.hist_ld;
     // repetition 1 divides and multiplies by one, and the others subtract zero: nothing to count
@@ -64,133 +89,210 @@ __device__ __forceinline__ RowRules row_rules(const Rules &r, int64_t b, int V) 
   o.bias = r.bias ? r.bias + b * r.bias_ld : nullptr;
   if (r.allowed != nullptr) {
     int64_t a = b;
-    if (r.token_row != nullptr) {
-      const int64_t t = r.tok[b];
-      a = t >= 0 && t < V ? r.token_row[t] : -1;
-    } else if (r.arow != nullptr) {
-      a = r.arow[b];
-    } else if (r.n_allowed == 1) {
+    if (r.token_row != nullptr)
+      a = tok >= 0 && tok < V ? r.token_row[tok] : -1;
+    else if (r.arow != nullptr)
+      a = arow;
+    else if (r.n_allowed == 1)
       a = 0;
-    }
     if (a >= 0 && a < r.n_allowed) o.allowed = r.allowed + a * r.allowed_ld;
   }
   return o;
 }
 
-// cnt: 16-bit counts, two a word, of tokens v0 .. v0 + slice - 1 in hist[0 .. len - 1] (slice % 32 == 0). Ends with a
-// barrier.
-__device__ __forceinline__ void count_history(uint32_t *cnt, const int64_t *hist, int len, int v0, int slice) {
-  const int64_t first = hist[threadIdx.x < len ? threadIdx.x : 0];  // in flight while the counts are cleared
-  for (int i = threadIdx.x; i < slice / 8; i += CH_THREADS) reinterpret_cast<u32x4 *>(cnt)[i] = u32x4{0u, 0u, 0u, 0u};
-  __syncthreads();
-  for (int t = threadIdx.x; t < len; t += CH_THREADS) {
-    const int64_t rel = (t == static_cast<int>(threadIdx.x) ? first : hist[t]) - v0;
-    if (rel >= 0 && rel < slice) atomicAdd(&cnt[rel >> 1], (rel & 1) ? 0x10000u : 1u);
+// The history's tokens of a slice, in dynamic LDS: a bit per token of the slice, and how often each occurs, in a hash
+// table of `slots` (a power of two, at least twice the history's columns) or, for long histories, by token (slots = slice).
+// Every distinct token is then one slot, whose logit one thread computes; the streaming pass leaves tokens with a bit out.
+template <int THREADS>
+struct Seen {
+  uint32_t *bits, *count, *key;  // key: null by token
+  int slots, shift;
+  static constexpr uint32_t kEmpty = 0xffffffffu;
+
+  __device__ __forceinline__ Seen(uint32_t *lds, int slice, int slots_, bool hashed)
+      : bits(lds), count(lds + slice / 32), key(hashed ? lds + slice / 32 + slots_ : nullptr), slots(slots_),
+        shift(__clz(slots_) + 1) {}
+  __device__ __forceinline__ bool has(int rel) const { return (bits[rel >> 5] >> (rel & 31)) & 1; }
+  // The slot of a token of the slice; of one that is not there, a new one (at most half of them get used).
+  __device__ __forceinline__ int slot(uint32_t rel) const {
+    if (key == nullptr) return static_cast<int>(rel);
+    uint32_t h = (rel * 0x9E3779B1u) >> shift;
+    while (true) {
+      const uint32_t old = atomicCAS(&key[h], kEmpty, rel);
+      if (old == kEmpty || old == rel) return static_cast<int>(h);
+      h = (h + 1) & (slots - 1);
+    }
   }
-  __syncthreads();
+  // Of tokens v0 .. v1 - 1. Ends with a barrier.
+  __device__ __forceinline__ void fill(const int64_t *hist, int len, int v0, int v1, int slice) const {
+    const int tid = threadIdx.x;
+    const int64_t first = hist[tid < len ? tid : 0];  // in flight while the table is cleared
+    for (int i = tid; i < (slice / 32 + slots) / 4; i += THREADS) reinterpret_cast<u32x4 *>(bits)[i] = u32x4{0u, 0u, 0u, 0u};
+    if (key != nullptr)
+      for (int i = tid; i < slots / 4; i += THREADS)
+        reinterpret_cast<u32x4 *>(key)[i] = u32x4{kEmpty, kEmpty, kEmpty, kEmpty};
+    __syncthreads();
+    for (int t = tid; t < len; t += THREADS) {
+      const int64_t rel = (t == tid ? first : hist[t]) - v0;
+      if (rel >= 0 && rel < v1 - v0) {
+        atomicAdd(&count[slot(static_cast<uint32_t>(rel))], 1u);
+        atomicOr(&bits[rel >> 5], 1u << (rel & 31));
+      }
+    }
+    __syncthreads();
+  }
+  // This thread's distinct tokens, as f(token of the slice, its count's place).
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int i = threadIdx.x; i < slots; i += THREADS) {
+      if (key != nullptr ? key[i] != kEmpty : has(i)) f(static_cast<int>(key != nullptr ? key[i] : i), count[i]);
+    }
+  }
+};
+
+// One token's logit after the rules; count: its occurrences in the history.
+template <typename T>
+__device__ __forceinline__ float one_logit(const T *row, const RowRules &r, int v, uint32_t count) {
+#pragma clang fp contract(off)
+  float z = load_one(row + v);
+  const float bias = r.bias != nullptr ? r.bias[v] : 0.f;
+  const bool allowed = r.allowed == nullptr || ((r.allowed[v >> 5] >> (v & 31)) & 1);
+  if (count > 0) {
+    z = z > 0.f ? z / r.rep : z * r.rep;
+    z = z - r.freq * static_cast<float>(count);
+    z = z - r.pres;
+  }
+  if (r.bias != nullptr) z = z + bias;
+  return allowed ? z : -INFINITY;
 }
 
-// N consecutive tokens' logits and what the rules read for them, loaded ahead of their use. A vector that does not fit
-// into the row (its last one, where N does not divide V) is read one by one when it is used; its place here holds the
-// row's last whole vector, so that every load is unconditional and in bounds.
-template <typename T>
-struct Vec {
-  static constexpr int N = 16 / sizeof(T);
-  u32x4 raw;
-  float bias[N];
-  uint32_t mask;
+template <typename T, int THREADS>
+__device__ __forceinline__ float one_logit(const T *row, const RowRules &r, const Seen<THREADS> &s, int v0, int v) {
+  return one_logit(row, r, v, r.len > 0 && s.has(v - v0) ? s.count[s.slot(v - v0)] : 0);
+}
 
-  __device__ __forceinline__ void load(const T *row, const RowRules &r, int v, int V) {
-    if (V < N) return;
-    const int at = v <= V - N ? v : V - N;
-    raw = load_16(row + at);
-    if (r.bias != nullptr) load_row<N>(r.bias + at, bias);
-    if (r.allowed != nullptr) mask = r.allowed[at >> 5];
+// What a thread takes of a workgroup's next 16 THREADS tokens: R vectors of N tokens, vector q at token
+// first + q * THREADS * N + threadIdx.x * N. CUT: the row ends inside the batch; one that is cut (N does not divide V) is
+// read token by token.
+template <typename T, int THREADS>
+struct Batch {
+  static constexpr int N = 16 / sizeof(T), R = sizeof(T), STEP = THREADS * N, TOKENS = R * STEP;
+  u32x4 raw[R];
+
+  static __device__ __forceinline__ int token(int first, int q) {
+    return first + q * STEP + static_cast<int>(threadIdx.x) * N;
+  }
+  // Where vector q is loaded from (V >= N): past the row's end, its last whole vector. So all loads are unconditional and
+  // in bounds, and a wait for older loads can leave them in flight.
+  static __device__ __forceinline__ int from(int first, int q, int V) { return min(token(first, q), V - N); }
+
+  // (V >= N)
+  __device__ __forceinline__ void load(const T *row, int first, int V) {
+#pragma unroll
+    for (int q = 0; q < R; ++q) raw[q] = stream_16(row + from(first, q, V));
   }
 
-  // z: the logits after the rules, -inf past the row's end. v < V, v % N == 0; cnt: the counts of tokens v, v + 1, ...
-  __device__ __forceinline__ void rules(float (&z)[N], const T *row, const RowRules &r, const uint32_t *cnt, int v, int V) {
+  // z: the batch's logits after bias and mask (-inf past the row's end). MORE: the next batch's logits are loaded as soon
+  // as these are taken, behind this one's bias and mask.
+  template <bool CUT, bool MORE>
+  __device__ __forceinline__ void rules(float (&z)[R][N], const T *row, const RowRules &r, int first, int V) {
 #pragma clang fp contract(off)
-    const bool whole = v <= V - N;
-    if (whole) {
+#pragma unroll
+    for (int q = 0; q < R; ++q)
 #pragma unroll
       for (int k = 0; k < N; ++k)
         if constexpr (sizeof(T) == 4)
-          z[k] = __uint_as_float(raw[k]);
+          z[q][k] = __uint_as_float(raw[q][k]);
         else
-          z[k] = (k & 1) ? hi_bf(raw[k / 2]) : lo_bf(raw[k / 2]);
-    } else {
+          z[q][k] = (k & 1) ? hi_bf(raw[q][k / 2]) : lo_bf(raw[q][k / 2]);
+    float bias[R][N];
+    uint32_t mask[R];
+    if (r.bias != nullptr && !(CUT && V < N))
 #pragma unroll
-      for (int k = 0; k < N; ++k) z[k] = load_one(row + (v + k < V ? v + k : V - 1));
-      if (r.bias != nullptr)
+      for (int q = 0; q < R; ++q) load_row<N>(r.bias + (CUT ? from(first, q, V) : token(first, q)), bias[q]);
+    if (r.allowed != nullptr)
 #pragma unroll
-        for (int k = 0; k < N; ++k) bias[k] = r.bias[v + k < V ? v + k : V - 1];
-      if (r.allowed != nullptr) mask = r.allowed[v >> 5];
-    }
-    if (r.len > 0) {
-      uint32_t w[N / 2], any = 0;
+      for (int q = 0; q < R; ++q) mask[q] = r.allowed[(CUT ? min(token(first, q), V - 1) : token(first, q)) >> 5];
+    if (MORE) load(row, first + TOKENS, V);
+    if (CUT) {
 #pragma unroll
-      for (int k = 0; k < N / 2; ++k) any |= w[k] = cnt[k];
-      if (any) {
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const int c = (k & 1) ? w[k / 2] >> 16 : w[k / 2] & 0xffff;
-          if (c > 0) {
-            z[k] = z[k] > 0.f ? z[k] / r.rep : z[k] * r.rep;
-            z[k] = z[k] - r.freq * static_cast<float>(c);
-            z[k] = z[k] - r.pres;
+      for (int q = 0; q < R; ++q) {
+        const int v = token(first, q);
+        if (v < V && v > V - N)
+          for (int k = 0; k < N; ++k) {
+            const int at = v + k < V ? v + k : V - 1;
+            z[q][k] = load_one(row + at);
+            if (r.bias != nullptr) bias[q][k] = r.bias[at];
           }
-        }
       }
     }
     if (r.bias != nullptr)
 #pragma unroll
-      for (int k = 0; k < N; ++k) z[k] = z[k] + bias[k];
-    if (r.allowed != nullptr) {
-      const uint32_t bits = mask >> (v & 31);
+      for (int q = 0; q < R; ++q)
 #pragma unroll
-      for (int k = 0; k < N; ++k) z[k] = (bits >> k) & 1 ? z[k] : -INFINITY;
-    }
-    if (!whole)
+        for (int k = 0; k < N; ++k) z[q][k] = z[q][k] + bias[q][k];
+    const int lane_bit = (threadIdx.x * N) & 31;  // (first and STEP are multiples of 32)
+    if (r.allowed != nullptr)
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (v + k >= V) z[k] = -INFINITY;
+      for (int q = 0; q < R; ++q) {
+        const uint32_t bits = mask[q] >> lane_bit;
+#pragma unroll
+        for (int k = 0; k < N; ++k) z[q][k] = (bits >> k) & 1 ? z[q][k] : -INFINITY;
+      }
+    if (CUT)
+#pragma unroll
+      for (int q = 0; q < R; ++q)
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (token(first, q) + k >= V) z[q][k] = -INFINITY;
   }
 };
 
-// Vectors that a thread has in flight: 16 elements.
-template <typename T>
-constexpr int kAhead = sizeof(T);
+template <typename T, typename OT, bool CUT, bool MORE>
+__device__ __forceinline__ void process_batch(Batch<T, CH_THREADS> &x, const T *row, OT *dst, const RowRules &r, int w, int V) {
+  using X = Batch<T, CH_THREADS>;
+  float z[X::R][X::N];
+  x.template rules<CUT, MORE>(z, row, r, w, V);
+#pragma unroll
+  for (int q = 0; q < X::R; ++q) {
+    const int v = X::token(w, q);
+    if (!CUT || v <= V - X::N)
+      store_row<X::N>(dst + v, z[q]);
+    else
+      for (int k = 0; k < X::N && v + k < V; ++k) store_one(dst + v + k, z[q][k]);
+  }
+}
 
-// grid: B x slices workgroups, a sequence's slices side by side. out may be logits.
+// grid: B x slices workgroups, a sequence's slices side by side. The logits of the history's tokens are computed from what
+// was there before any store (out may be logits), and stored over what the streaming pass, which knows of no history, has
+// put there.
 template <typename T, typename OT>
-__global__ __launch_bounds__(CH_THREADS) void process_logits_kernel(const T *logits, int64_t ld, Rules rules, int V,
-                                                                    int slices, int slice, OT *out, int64_t out_ld) {
-  extern __shared__ __attribute__((aligned(16))) uint32_t cnt[];
-  constexpr int N = Vec<T>::N, R = kAhead<T>, STEP = CH_THREADS * N;
-  const int64_t b = blockIdx.x / slices;
-  const int v0 = static_cast<int>(blockIdx.x % slices) * slice, v1 = V - v0 < slice ? V : v0 + slice;
-  const RowRules r = row_rules(rules, b, V);
+__global__ __launch_bounds__(CH_THREADS) void process_logits_kernel(const T *logits, int64_t ld, Rules rules, int V, Plan plan,
+                                                                    OT *out, int64_t out_ld) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+  using X = Batch<T, CH_THREADS>;
+  const int64_t b = blockIdx.x / plan.slices;
+  const int v0 = static_cast<int>(blockIdx.x % plan.slices) * plan.slice, v1 = V - v0 < plan.slice ? V : v0 + plan.slice;
+  const Seen<CH_THREADS> seen(lds, plan.slice, plan.slots, plan.hashed);
   const T *row = logits + b * ld;
   OT *dst = out + b * out_ld;
-  const int mine = v0 + static_cast<int>(threadIdx.x) * N;
-  Vec<T> x[R];
-  for (int w = v0; w < v1; w += R * STEP) {
-#pragma unroll
-    for (int q = 0; q < R; ++q) x[q].load(row, r, w - v0 + mine + q * STEP, V);
-    if (w == v0 && r.len > 0) count_history(cnt, r.hist, r.len, v0, slice);
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const int v = w - v0 + mine + q * STEP;
-      if (v >= v1) continue;
-      float z[N];
-      x[q].rules(z, row, r, cnt + (v - v0) / 2, v, V);
-      if (v <= V - N) {
-        store_row<N>(dst + v, z);
-      } else {
-        for (int k = 0; k < N && v + k < V; ++k) store_one(dst + v + k, z[k]);
-      }
-    }
+  X x;
+  if (V >= X::N) x.load(row, v0, V);
+  const RowRules r = row_rules(rules, b, V);
+  if (r.len > 0) {
+    seen.fill(r.hist, r.len, v0, v1, plan.slice);
+    seen.each([&](int rel, uint32_t &count) { count = __float_as_uint(one_logit(row, r, v0 + rel, count)); });
+    __syncthreads();
+  }
+  int w = v0;
+  for (; w + X::TOKENS < v1; w += X::TOKENS) process_batch<T, OT, false, true>(x, row, dst, r, w, V);
+  if (w + X::TOKENS <= V)
+    process_batch<T, OT, false, false>(x, row, dst, r, w, V);
+  else
+    process_batch<T, OT, true, false>(x, row, dst, r, w, V);
+  if (r.len > 0) {
+    __syncthreads();
+    seen.each([&](int rel, uint32_t z) { store_one(dst + v0 + rel, __uint_as_float(z)); });
   }
 }
 
@@ -198,12 +300,11 @@ __global__ __launch_bounds__(CH_THREADS) void process_logits_kernel(const T *log
 
 enum { CH_GREEDY = 0, CH_GUMBEL = 1, CH_CDF = 2 };
 
-// Running state of a part of a row: the maximum of z (at least -FLT_MAX), the sum of exp((z - m) / T), and the best token.
-// Gumbel: v is that token, s its score in fp32 (within score_slack of the exact one), z its logit and u its uniform.
-// Else: z is the largest logit (-inf: none) and v the first token, or the first token of the vector, that has it.
+// A slice's result: the maximum of z (at least -FLT_MAX), the sum of exp((z - m) / T), and the best token v (-1: none).
+// Its z is its logit after the rules; Gumbel: s its score in fp32 (within score_slack of the exact one), u its uniform.
 struct Part {
   float m, sum, s, z, u;
-  int32_t v;  // -1: none yet
+  int32_t v;
 };
 
 __device__ __forceinline__ Part no_part() { return {-FLT_MAX, 0.f, -INFINITY, -INFINITY, 0.f, -1}; }
@@ -215,6 +316,24 @@ __device__ __forceinline__ float score_slack(float s) { return 1e-5f + 1e-6f * f
 // The exact score: z' rounded to fp32, the noise in 64 bits.
 __device__ __forceinline__ double exact_score(float z, float u, float T) {
   return static_cast<double>(z / T) - log(-log(fmax(static_cast<double>(u), 1e-20)));
+}
+
+struct Scale {
+  float T, inv, L;  // the temperature, 1 / T (1 for a greedy row) kept finite, and log2(e) / T
+};
+
+__device__ __forceinline__ Scale row_scale(const float *temp, float temp0, int64_t b) {
+  Scale c;
+  c.T = temp ? temp[b] : temp0;
+  c.inv = c.T > 0.f ? fminf(1.f / c.T, 0.5f * FLT_MAX) : 1.f;
+  c.L = fminf(c.inv * 1.44269504f, 0.5f * FLT_MAX);
+  return c;
+}
+
+// The score in fp32, from the hardware's base-2 logarithms. -inf for -inf.
+__device__ __forceinline__ float gumbel_score(float z, float u, const Scale &c) {
+  const float w = -0.693147181f * __builtin_amdgcn_logf(fmaxf(u, 1e-20f));
+  return fmaf(z, c.inv, -0.693147181f * __builtin_amdgcn_logf(w));
 }
 
 // Whether b's token comes before a's. Gumbel scores that fp32 cannot order are compared in 64 bits.
@@ -266,18 +385,6 @@ __device__ __forceinline__ float tame(float z) {
   float d;
   asm("v_med3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(z), "v"(-INFINITY), "v"(FLT_MAX));
   return d;
-}
-
-struct Scale {
-  float T, inv, L;  // the temperature, 1 / T (1 for a greedy row) kept finite, and log2(e) / T
-};
-
-__device__ __forceinline__ Scale row_scale(const float *temp, float temp0, int64_t b) {
-  Scale c;
-  c.T = temp ? temp[b] : temp0;
-  c.inv = c.T > 0.f ? fminf(1.f / c.T, 0.5f * FLT_MAX) : 1.f;
-  c.L = fminf(c.inv * 1.44269504f, 0.5f * FLT_MAX);
-  return c;
 }
 
 // The uniforms of sequence b are at u + b * ld; in a decode step those of its output column (clamped to the columns there
@@ -339,101 +446,215 @@ __device__ __forceinline__ float logp_of(float z, const Part &p, const Scale &c)
   return (c.T > 0.f ? d / c.T : d) - logf(p.sum);
 }
 
-// One slice of one sequence, or with ONE the whole vocabulary and the step's end.
-template <typename T, bool GUMBEL, bool ONE>
-__global__ __launch_bounds__(CH_THREADS) void choose_slices_kernel(const T *__restrict__ logits, int64_t ld, Rules rules,
-                                                                   const float *__restrict__ temp, float temp0,
-                                                                   Noise noise, int V, int slices, int slice,
-                                                                   Part *__restrict__ parts, Choice choice, Step step) {
-  extern __shared__ __attribute__((aligned(16))) uint32_t cnt[];
-  __shared__ Part red[CH_THREADS / 64];
-  constexpr int N = Vec<T>::N, R = kAhead<T>, STEP = CH_THREADS * N;
-  const int64_t b = ONE ? blockIdx.x : blockIdx.x / slices;
-  const int v0 = ONE ? 0 : static_cast<int>(blockIdx.x % slices) * slice, v1 = V - v0 < slice ? V : v0 + slice;
-  const RowRules r = row_rules(rules, b, V);
-  const Scale c = row_scale(temp, temp0, b);
+__device__ __forceinline__ float wave_max_of(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = vmax2(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// What a thread knows of its tokens: the maximum of z (at least -FLT_MAX), the sum of exponentials at it, the best logit
+// or score with its first token, and the second best score.
+struct Mine {
+  float m = -FLT_MAX, sum = 0.f, best = -INFINITY, second = -INFINITY;
+  int v = -1;
+};
+
+// The uniforms of the batch to come (Gumbel; a greedy row's are loaded too, so that the loads are unconditional).
+template <typename T, int THREADS, bool GUMBEL>
+struct Uniforms {
+  using X = Batch<T, THREADS>;
+  float next[GUMBEL ? X::R : 1][X::N];
+  __device__ __forceinline__ void load(const float *urow, int first, int V) {
+    if constexpr (GUMBEL) {
+#pragma unroll
+      for (int q = 0; q < X::R; ++q) stream_row<X::N>(urow + X::from(first, q, V), next[q]);
+    }
+  }
+  __device__ __forceinline__ void take(float (&u)[GUMBEL ? X::R : 1][X::N]) const {
+    if constexpr (GUMBEL)
+#pragma unroll
+      for (int q = 0; q < X::R; ++q)
+#pragma unroll
+        for (int k = 0; k < X::N; ++k) u[q][k] = next[q][k];
+  }
+};
+
+template <typename T, int THREADS, bool GUMBEL, bool CUT, bool MORE>
+__device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, THREADS, GUMBEL> &un, Mine &t, const T *row, const float *urow, const RowRules &r,
+                                             const Scale &c, const Seen<THREADS> &s, int v0, int w, int V) {
+  using X = Batch<T, THREADS>;
   const bool noisy = GUMBEL && c.T > 0.f;
-  const T *row = logits + b * ld;
-  const float *urow = noisy ? noise_at(noise, rules, b, V) : nullptr;
-  const int mine = v0 + static_cast<int>(threadIdx.x) * N;
-  Part p = no_part();
-  Vec<T> x[R];
-  float u[GUMBEL ? R : 1][N];
-  for (int w = v0; w < v1; w += R * STEP) {
+  float z[X::R][X::N], u[GUMBEL ? X::R : 1][X::N];
+  un.take(u);
+  x.template rules<CUT, MORE>(z, row, r, w, V);
+  if (MORE) un.load(urow, w + X::TOKENS, V);
+  if (r.len > 0)  // the history's tokens are none of these
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const int v = w - v0 + mine + q * STEP;
-      x[q].load(row, r, v, V);
-      if (noisy && V >= N) load_row<N>(urow + (v <= V - N ? v : V - N), u[GUMBEL ? q : 0]);
+    for (int q = 0; q < X::R; ++q) {
+      const uint32_t left = s.bits[(X::token(w, q) - v0) >> 5] >> ((threadIdx.x * X::N) & 31);
+      if (left & ((1u << X::N) - 1))
+#pragma unroll
+        for (int k = 0; k < X::N; ++k) z[q][k] = (left >> k) & 1 ? -INFINITY : z[q][k];
     }
-    if (w == v0 && r.len > 0) count_history(cnt, r.hist, r.len, v0, slice);
-    float z[R][N], top = -INFINITY;
-    int topv = -1;
+  float top = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const int v = w - v0 + mine + q * STEP;
-      if (v < v1) {
-        x[q].rules(z[q], row, r, cnt + (v - v0) / 2, v, V);
-        if (noisy && v > V - N)
+  for (int q = 0; q < X::R; ++q)
 #pragma unroll
-          for (int k = 0; k < N; ++k) u[GUMBEL ? q : 0][k] = urow[v + k < V ? v + k : V - 1];
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) z[q][k] = -INFINITY;
-      }
-      float most = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        z[q][k] = tame(z[q][k]);
-        most = vmax2(most, z[q][k]);
-      }
-      if (most > top) {
-        top = most;
-        topv = v;
-      }
+    for (int k = 0; k < X::N; k += 2) {
+      z[q][k] = tame(z[q][k]);
+      z[q][k + 1] = tame(z[q][k + 1]);
+      top = vmax3(top, z[q][k], z[q][k + 1]);
     }
-    const float m = vmax2(p.m, top);
-    p.sum *= __builtin_amdgcn_exp2f((p.m - m) * c.L);
-    p.m = m;
+  const float m = vmax2(t.m, top);
+  t.sum *= __builtin_amdgcn_exp2f((t.m - m) * c.L);
+  t.m = m;
 #pragma unroll
-    for (int q = 0; q < R; ++q)
+  for (int q = 0; q < X::R; ++q)
 #pragma unroll
-      for (int k = 0; k < N; ++k) p.sum += __builtin_amdgcn_exp2f((z[q][k] - m) * c.L);
-    if (!noisy) {
-      if (top > p.z) {
-        p.z = top;
-        p.v = topv;
-      }
-    } else {
+    for (int k = 0; k < X::N; ++k) t.sum += __builtin_amdgcn_exp2f((z[q][k] - m) * c.L);
+  if (noisy) {
+    if constexpr (GUMBEL) {
+      if (CUT)
 #pragma unroll
-      for (int q = 0; q < R; ++q)
+        for (int q = 0; q < X::R; ++q) {
+          const int v = X::token(w, q);
+          if (v < V && v > V - X::N)
+            for (int k = 0; k < X::N; ++k) u[q][k] = urow[v + k < V ? v + k : V - 1];
+        }
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const float uk = u[GUMBEL ? q : 0][k];
-          Part t = p;
-          t.z = z[q][k];
-          t.u = uk;
-          t.s = fmaf(t.z, c.inv, -logf(-logf(fmaxf(uk, 1e-20f))));
-          t.v = t.z == -INFINITY ? -1 : w - v0 + mine + q * STEP + k;
-          if (better<GUMBEL>(p, t, c.T)) p = t;
+      for (int q = 0; q < X::R; ++q)
+#pragma unroll
+        for (int k = 0; k < X::N; ++k) {
+          const float sc = gumbel_score(z[q][k], u[q][k], c);
+          t.second = fmaxf(t.second, fminf(t.best, sc));
+          if (sc > t.best) {
+            t.best = sc;
+            t.v = X::token(w, q) + k;
+          }
         }
     }
-  }
-  join_lanes<GUMBEL>(p, c.L, c.T);
-  const int lane = threadIdx.x & 63;
-  if (lane == 0) red[threadIdx.x >> 6] = p;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int w = 1; w < CH_THREADS / 64; ++w) join_parts<GUMBEL>(p, red[w], c.L, c.T);
-  if (!noisy && p.v >= 0) {  // the token inside its vector
-    float z[N];
-    x[0].load(row, r, p.v, V);
-    x[0].rules(z, row, r, cnt + (p.v - v0) / 2, p.v, V);
-    int k = 0;
+  } else if (top > t.best || (top == t.best && top > -INFINITY)) {  // (a token of the history may be behind these)
+    t.v = top > t.best ? 0x7fffffff : t.v;
+    t.best = top;
 #pragma unroll
-    for (int e = N - 1; e >= 0; --e) k = tame(z[e]) == p.z ? e : k;
-    p.v += k;
+    for (int q = X::R - 1; q >= 0; --q)
+#pragma unroll
+      for (int k = X::N - 1; k >= 0; --k) t.v = z[q][k] == top ? min(t.v, X::token(w, q) + k) : t.v;
   }
+}
+
+// One slice of one sequence, or with ONE the whole vocabulary and the step's end. The workgroup's best logit or score
+// tells who can have the best token: the lowest token of the largest logit, or the threads within the scores' slack of
+// the largest score. These read their token again and are compared exactly; one whose second score is as near goes
+// through all of its tokens. The sum is taken at the workgroup's maximum.
+template <typename T, int THREADS, bool GUMBEL, bool ONE>
+__global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restrict__ logits, int64_t ld, Rules rules,
+                                                                   const float *__restrict__ temp, float temp0,
+                                                                   Noise noise, int V, Plan plan,
+                                                                   Part *__restrict__ parts, Choice choice, Step step) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+  constexpr int WAVES = THREADS / 64;
+  __shared__ float red_m[WAVES], red_s[WAVES], red_sum[WAVES];
+  __shared__ int first_best, contenders;
+  __shared__ Part contender[GUMBEL ? THREADS : 1];
+  using X = Batch<T, THREADS>;
+  const int64_t b = ONE ? blockIdx.x : blockIdx.x / plan.slices;
+  const int v0 = ONE ? 0 : static_cast<int>(blockIdx.x % plan.slices) * plan.slice;
+  const int v1 = V - v0 < plan.slice ? V : v0 + plan.slice;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const Seen<THREADS> seen(lds, plan.slice, plan.slots, plan.hashed);
+  const T *row = logits + b * ld;
+  X x;
+  if (V >= X::N) x.load(row, v0, V);
+  const Scale c = row_scale(temp, temp0, b);
+  const RowRules r = row_rules(rules, b, V);
+
+  const bool noisy = GUMBEL && c.T > 0.f;
+  const float *urow = GUMBEL ? noise_at(noise, rules, b, V) : nullptr;
+  Uniforms<T, THREADS, GUMBEL> un;
+  if (V >= X::N) un.load(urow, v0, V);
+  if (tid == 0) {
+    first_best = 0x7fffffff;
+    contenders = 0;
+  }
+  Mine t;
+  if (r.len > 0) {
+    seen.fill(r.hist, r.len, v0, v1, plan.slice);
+    seen.each([&](int rel, uint32_t count) {
+      const int v = v0 + rel;
+      const float z = tame(one_logit(row, r, v, count));
+      const float m = vmax2(t.m, z);
+      t.sum = t.sum * __builtin_amdgcn_exp2f((t.m - m) * c.L) + __builtin_amdgcn_exp2f((z - m) * c.L);
+      t.m = m;
+      const float sc = noisy ? gumbel_score(z, urow[v], c) : z;
+      t.second = fmaxf(t.second, fminf(t.best, sc));
+      if (sc > t.best || (sc == t.best && sc > -INFINITY && v < t.v)) {
+        t.best = sc;
+        t.v = v;
+      }
+    });
+  }
+  int w = v0;
+  for (; w + X::TOKENS < v1; w += X::TOKENS)
+    choose_batch<T, THREADS, GUMBEL, false, true>(x, un, t, row, urow, r, c, seen, v0, w, V);
+  if (w + X::TOKENS <= V)
+    choose_batch<T, THREADS, GUMBEL, false, false>(x, un, t, row, urow, r, c, seen, v0, w, V);
+  else
+    choose_batch<T, THREADS, GUMBEL, true, false>(x, un, t, row, urow, r, c, seen, v0, w, V);
+  const float wm = wave_max_of(t.m), wb = wave_max_of(t.best);
+  if (lane == 0) {
+    red_m[wid] = wm;
+    red_s[wid] = wb;
+  }
+  __syncthreads();
+  float M = red_m[0], most = red_s[0];
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i) {
+    M = vmax2(M, red_m[i]);
+    most = vmax2(most, red_s[i]);
+  }
+  const float ws = wave_sum(t.sum * __builtin_amdgcn_exp2f((t.m - M) * c.L));
+  if (lane == 0) red_sum[wid] = ws;
+  if (most > -INFINITY) {
+    if (!noisy) {
+      if (t.best == most) atomicMin(&first_best, t.v);
+    } else if (t.best > -INFINITY && (t.best == most || most - t.best <= 2.5f * score_slack(most))) {
+      Part p = no_part();
+      auto offer = [&](int v) {
+        Part e = no_part();
+        e.z = tame(one_logit(row, r, seen, v0, v));
+        e.u = urow[v];
+        e.s = gumbel_score(e.z, e.u, c);
+        e.v = e.z == -INFINITY ? -1 : v;
+        if (better<true>(p, e, c.T)) p = e;
+      };
+      if (t.second == most || most - t.second <= 2.5f * score_slack(most)) {
+        for (int i = v0; i < v1; i += X::STEP)
+          for (int k = 0; k < X::N; ++k) {
+            const int v = i + tid * X::N + k;
+            if (v < v1 && !(r.len > 0 && seen.has(v - v0))) offer(v);
+          }
+        if (r.len > 0) seen.each([&](int rel, uint32_t) { offer(v0 + rel); });
+      } else {
+        offer(t.v);
+      }
+      contender[atomicAdd(&contenders, 1)] = p;
+    }
+  }
+  __syncthreads();
+  if (tid != 0) return;
+  Part p = no_part();
+  if (noisy) {
+    for (int i = 0; i < contenders; ++i)
+      if (better<true>(p, contender[i], c.T)) p = contender[i];
+  } else if (most > -INFINITY) {
+    p.z = most;
+    p.v = first_best;
+  }
+  p.m = M;
+  p.sum = red_sum[0];
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i) p.sum += red_sum[i];
   if constexpr (ONE)
     finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
   else
@@ -460,16 +681,18 @@ __global__ __launch_bounds__(256) void choose_join_kernel(const Part *__restrict
 template <typename T>
 __global__ __launch_bounds__(CH_THREADS) void choose_cdf_kernel(const T *__restrict__ logits, int64_t ld, Rules rules,
                                                                 const float *__restrict__ temp, float temp0,
-                                                                Noise noise, int V, int slices, int slice,
+                                                                Noise noise, int V, Plan plan,
                                                                 const Part *__restrict__ parts,
                                                                 Choice choice, Step step) {
-  extern __shared__ __attribute__((aligned(16))) uint32_t cnt[];
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
   __shared__ double wave_total[CH_THREADS / 64];
   __shared__ int found, last;
-  constexpr int N = Vec<T>::N;
+  using X = Batch<T, CH_THREADS>;
+  constexpr int N = X::N;
   const int64_t b = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const Scale c = row_scale(temp, temp0, b);
+  const int slices = plan.slices, slice = plan.slice;
   const Part *mine = parts + b * slices;
   // every thread joins the slices the same way
   Part p = no_part();
@@ -502,25 +725,26 @@ __global__ __launch_bounds__(CH_THREADS) void choose_cdf_kernel(const T *__restr
     last = -1;
   }
   __syncthreads();
-  if (r.len > 0) count_history(cnt, r.hist, r.len, v0, slice);
+  const Seen<CH_THREADS> seen(lds, slice, plan.slots, plan.hashed);
   const T *row = logits + b * ld;
-  Vec<T> x;
-  float z[N];
-  for (int w0 = v0; w0 < v1; w0 += CH_THREADS * N) {
+  if (r.len > 0) seen.fill(r.hist, r.len, v0, v1, slice);
+  for (int w0 = v0; w0 < v1; w0 += X::STEP) {
     const int v = w0 + tid * N;
     double e[N], sum = 0.;
     int top = -1;
 #pragma unroll
     for (int k = 0; k < N; ++k) e[k] = 0.;
     if (v < v1) {
-      x.load(row, r, v, V);
-      x.rules(z, row, r, cnt + (v - v0) / 2, v, V);
+      float z[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        e[k] = static_cast<double>(__builtin_amdgcn_exp2f((tame(z[k]) - p.m) * c.L));
-        if (e[k] > 0.) top = v + k;
-        sum += e[k];
-      }
+      for (int k = 0; k < N; ++k) z[k] = one_logit(row, r, seen, v0, v + k < V ? v + k : V - 1);
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (v + k < V) {
+          e[k] = static_cast<double>(__builtin_amdgcn_exp2f((tame(z[k]) - p.m) * c.L));
+          if (e[k] > 0.) top = v + k;
+          sum += e[k];
+        }
     }
     double inc = sum;
 #pragma unroll
@@ -548,29 +772,43 @@ __global__ __launch_bounds__(CH_THREADS) void choose_cdf_kernel(const T *__restr
     if (found != 0x7fffffff) break;
   }
   if (tid != 0) return;
-  const int pick = found != 0x7fffffff ? found : last, v = pick & ~(N - 1);
-  if (pick < 0) {  // (a slice with weight holds a token with weight)
+  const int pick = found != 0x7fffffff ? found : last;
+  if (pick < 0)  // (a slice with weight holds a token with weight)
     finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
-    return;
-  }
-  x.load(row, r, v, V);  // the choice's own logit again
-  x.rules(z, row, r, cnt + (v - v0) / 2, v, V);
-  float zt = 0.f;
-#pragma unroll
-  for (int k = 0; k < N; ++k) zt = v + k == pick ? tame(z[k]) : zt;
-  finish_row(choice, step, b, V, pick, logp_of(zt, p, c));
+  else
+    finish_row(choice, step, b, V, pick, logp_of(tame(one_logit(row, r, seen, v0, pick)), p, c));
 }
 
-// Slices per sequence: about two workgroups per CU in all, of 2048 to 16384 tokens each.
-static void slice_plan(int64_t B, int V, int *slices, int *slice) {
-  const int64_t want = (2 * device_cus_cached() + B - 1) / B;
-  int64_t s = (V + CH_SLICE_MIN - 1) / CH_SLICE_MIN;
-  if (s > want) s = want;
-  const int64_t least = (V + CH_SLICE - 1) / CH_SLICE;
+// How B rows of V tokens are cut: about two workgroups per CU in all, of 4096 tokens (one batch) to CH_SLICE. `whole`: one
+// workgroup of CH_THREADS_ONE may take a sequence's whole vocabulary, where that spares the slices' joining and leaves the
+// CUs evenly loaded. hist_cols: 0 without a history.
+static Plan make_plan(int64_t B, int V, int64_t hist_cols, bool whole) {
+  constexpr int UNIT = Batch<float, CH_THREADS>::TOKENS;
+  static_assert(UNIT == Batch<bf16_t, CH_THREADS>::TOKENS && CH_SLICE % UNIT == 0, "slices are whole batches");
+  Plan p = {};
+  p.hashed = hist_cols <= CH_HASH_MAX;
+  const int64_t cus = device_cus_cached(), units = (static_cast<int64_t>(V) + UNIT - 1) / UNIT;
+  const int64_t want = (2 * cus + B - 1) / B, least = (V + CH_SLICE - 1) / CH_SLICE;
+  int64_t s = units < want ? units : want;
   if (s < least) s = least;
-  const int64_t len = ((V + s - 1) / s + 31) / 32 * 32;
-  *slice = static_cast<int>(len);
-  *slices = static_cast<int>((V + len - 1) / len);
+  int64_t len = (units + s - 1) / s * UNIT;
+  p.slices = static_cast<int>((V + len - 1) / len);
+  const int64_t rounds = (B + cus - 1) / cus;  // workgroups of the busiest CU, one a sequence
+  if (whole && (p.slices == 1 || (p.hashed && V <= CH_WHOLE && B >= 2 * cus && 20 * B >= 17 * rounds * cus))) {
+    constexpr int ONE_UNIT = Batch<float, CH_THREADS_ONE>::TOKENS;
+    p.one = true;
+    p.slices = 1;
+    len = (static_cast<int64_t>(V) + ONE_UNIT - 1) / ONE_UNIT * ONE_UNIT;
+  }
+  p.slice = static_cast<int>(len);
+  p.slots = p.slice;
+  if (p.hashed)
+    for (p.slots = 64; p.slots < 2 * hist_cols;) p.slots *= 2;
+  return p;
+}
+
+static size_t plan_lds(const Plan &p, bool hist) {
+  return hist ? static_cast<size_t>(p.slice) / 8 + static_cast<size_t>(p.slots) * (p.hashed ? 8 : 4) : 0;
 }
 
 static int check_rules(const Rules &r, int64_t B, int V, const char *what) {
@@ -598,29 +836,28 @@ template <typename T>
 static int launch_choose(const void *logits, int64_t ld, const Rules &r, const float *temp, float temp0, int mode,
                          const Noise &noise, int64_t B, int V, Part *parts, const Choice &choice, const Step &step,
                          hipStream_t s) {
-  int slices, slice;
-  slice_plan(B, V, &slices, &slice);
+  const Plan plan = make_plan(B, V, r.hist ? r.hist_cols : 0, mode != CH_CDF);
   const T *x = static_cast<const T *>(logits);
-  const size_t lds = r.hist ? static_cast<size_t>(slice) * 2 : 0;
-  const unsigned grid = static_cast<unsigned>(B * slices), join = static_cast<unsigned>((B + 3) / 4);
-#define VK_SLICES(GUMBEL, ONE)                                                                                          \
-  choose_slices_kernel<T, GUMBEL, ONE><<<grid, CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, slices, slice, parts, \
-                                                                     choice, step)
+  const size_t lds = plan_lds(plan, r.hist != nullptr);
+  const unsigned grid = static_cast<unsigned>(B * plan.slices), join = static_cast<unsigned>((B + 3) / 4);
+#define VK_SLICES(THREADS, GUMBEL, ONE)                                                                                 \
+  choose_slices_kernel<T, THREADS, GUMBEL, ONE><<<grid, THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, plan, parts, \
+                                                                           choice, step)
   if (mode == CH_CDF) {
-    VK_SLICES(false, false);
-    choose_cdf_kernel<T><<<static_cast<unsigned>(B), CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, slices, slice,
-                                                                       parts, choice, step);
-  } else if (slices == 1) {
+    VK_SLICES(CH_THREADS, false, false);
+    choose_cdf_kernel<T><<<static_cast<unsigned>(B), CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, plan, parts, choice,
+                                                                       step);
+  } else if (plan.one) {
     if (mode == CH_GUMBEL)
-      VK_SLICES(true, true);
+      VK_SLICES(CH_THREADS_ONE, true, true);
     else
-      VK_SLICES(false, true);
+      VK_SLICES(CH_THREADS_ONE, false, true);
   } else if (mode == CH_GUMBEL) {
-    VK_SLICES(true, false);
-    choose_join_kernel<true><<<join, 256, 0, s>>>(parts, temp, temp0, B, V, slices, choice, step);
+    VK_SLICES(CH_THREADS, true, false);
+    choose_join_kernel<true><<<join, 256, 0, s>>>(parts, temp, temp0, B, V, plan.slices, choice, step);
   } else {
-    VK_SLICES(false, false);
-    choose_join_kernel<false><<<join, 256, 0, s>>>(parts, temp, temp0, B, V, slices, choice, step);
+    VK_SLICES(CH_THREADS, false, false);
+    choose_join_kernel<false><<<join, 256, 0, s>>>(parts, temp, temp0, B, V, plan.slices, choice, step);
   }
 #undef VK_SLICES
   return launch_status("choose_tokens");
@@ -646,14 +883,13 @@ extern "C" int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, 
                    bias_ld, allowed, allowed_ld, n_allowed, allowed_rows, nullptr, nullptr};
   rc = check_rules(r, B, V, "process_logits");
   if (rc != VK_OK || B == 0) return rc;
-  int slices, slice;
-  slice_plan(B, V, &slices, &slice);
-  const size_t lds = hist ? static_cast<size_t>(slice) * 2 : 0;
-  const unsigned grid = static_cast<unsigned>(B * slices);
+  const Plan plan = make_plan(B, V, hist ? hist_cols : 0, false);
+  const size_t lds = plan_lds(plan, hist != nullptr);
+  const unsigned grid = static_cast<unsigned>(B * plan.slices);
   hipStream_t s = VK_STREAM(stream);
   const bool lf = dtype == VK_DTYPE_F32, of = out_dtype == VK_DTYPE_F32;
 #define VK_PROCESS(T, OT)                                                                                              \
-  process_logits_kernel<T, OT><<<grid, CH_THREADS, lds, s>>>(static_cast<const T *>(logits), ld, r, V, slices, slice,  \
+  process_logits_kernel<T, OT><<<grid, CH_THREADS, lds, s>>>(static_cast<const T *>(logits), ld, r, V, plan,            \
                                                              static_cast<OT *>(out), out_ld)
   if (lf && of)
     VK_PROCESS(float, float);
@@ -669,9 +905,7 @@ extern "C" int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, 
 
 extern "C" int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t *bytes) {
   VK_CHECK_ARG(bytes && B >= 0 && V > 0, "choose_tokens_workspace: bad arguments");
-  int slices = 0, slice = 0;
-  if (B > 0) slice_plan(B, V, &slices, &slice);
-  *bytes = B * slices * static_cast<int64_t>(sizeof(Part));
+  *bytes = B == 0 ? 0 : B * make_plan(B, V, 0, false).slices * static_cast<int64_t>(sizeof(Part));
   return VK_OK;
 }
 

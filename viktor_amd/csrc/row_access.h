@@ -12,9 +12,14 @@ typedef uint16_t u16x8_e __attribute__((ext_vector_type(8), aligned(2)));
 typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// 16 bytes of a row as they are.
-__device__ __forceinline__ u32x4 load_16(const bf16_t *p) { return *reinterpret_cast<const u32x4_at2 *>(p); }
-__device__ __forceinline__ u32x4 load_16(const float *p) { return *reinterpret_cast<const u32x4_at4 *>(p); }
+// 16 bytes of a row as they are, of data that is read once (past the caches' other contents: a plain read of 179 MB takes
+// 29 us, this one 26.5).
+__device__ __forceinline__ u32x4 stream_16(const bf16_t *p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4_at2 *>(p));
+}
+__device__ __forceinline__ u32x4 stream_16(const float *p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4_at4 *>(p));
+}
 
 template <int N>
 __device__ __forceinline__ void load_row(const float *p, float (&v)[N]) {
@@ -49,6 +54,15 @@ __device__ __forceinline__ void store_row(bf16_t *p, const float (&v)[N]) {
 #pragma unroll
   for (int k = 0; k < N / 2; ++k) o[k] = pack_bf(v[2 * k], v[2 * k + 1]);
   *reinterpret_cast<words_e *>(p) = o;
+}
+template <int N>
+__device__ __forceinline__ void stream_row(const float *p, float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const u32x4 a = stream_16(p + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[i + k] = __uint_as_float(a[k]);
+  }
 }
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
 __device__ __forceinline__ float load_one(const bf16_t *p) { return bf2f(*p); }
