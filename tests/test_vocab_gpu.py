@@ -58,14 +58,14 @@ def test_embed_lookup_shapes():
 # ---- gradient --------------------------------------------------------------------------------------------------------------
 
 def _grad_ref(rows, tok, V, scale, pad=None):
-    """(fp64 gradient, what an element may be off by, in units of U): a run's sum is at most 64 additions in a chunk, the
-    chunks' partials over 16 groups, the groups, the lanes' shares, one product."""
+    """(fp64 gradient, what an element may be off by, in units of U): a run's sum is at most 127 additions in a chunk and the
+    next; a longer one's 64 in each chunk, its chunks' sums over 32 groups, and the groups; then one product."""
     keep = (tok >= 0) & (tok < V) & (tok != (-1 if pad is None else pad))
     out = torch.zeros(V, rows.shape[1], dtype=torch.float64)
     mag = torch.zeros_like(out)
     out.index_add_(0, tok[keep], rows[keep].double())
     mag.index_add_(0, tok[keep], rows[keep].double().abs())
-    adds = 64 + 4 + len(tok) / (64 * 16) + 1 + 16 + 2
+    adds = 127 + len(tok) / (64 * 32) + 1 + 32 + 2
     return out * scale, adds * U * mag * abs(scale)
 
 
@@ -86,7 +86,7 @@ def _ids(kind, n, V, g):
     return torch.randint(0, V, (n,), generator=g)
 
 
-@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 129, 1003, 4095, 4096, 4097, 6144, 20001])
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 127, 128, 129, 193, 1003, 4095, 4096, 4097, 8192, 8193, 20001])
 @pytest.mark.parametrize("kind", ["flat", "skew", "one", "padded"])
 def test_embed_grad_sorted(n, kind):
     """Both sorts, chunk and tile borders, and tokens that a large part of the rows share."""
@@ -146,6 +146,33 @@ def test_embed_grad_sorted_ignores_and_accumulates(n):
     used = torch.zeros(V, dtype=torch.bool)
     used[tok[(tok >= 0) & (tok < V) & (tok != 5)]] = True
     assert torch.equal(table.cpu()[~used], old[~used])
+
+
+@pytest.mark.parametrize("lens", [(64, 64, 64), (63, 65, 64), (1, 64, 127, 1), (1, 128, 63), (64, 128, 64), (65, 63, 200, 5),
+                                  (130, 1, 1, 190), (10, 54, 64, 64, 64, 10), (63, 129, 63, 129, 1), (500,), (32, 300, 40, 300)])
+@pytest.mark.parametrize("ignored", [0, 70])
+def test_embed_grad_sorted_run_lengths(lens, ignored):
+    """Runs of given lengths against the chunks of 64 positions: ending and starting at borders, one past them, holding a
+    whole chunk or two, with ignored rows behind the last; shuffled, by both sorts."""
+    for more in (0, 5000):  # (past the counting sort: one more long run at the end)
+        V = 20
+        tok = torch.cat([torch.full((m,), 2 * i, dtype=torch.long) for i, m in enumerate((*lens, more))])
+        tok = torch.cat([tok, torch.full((ignored,), -1, dtype=torch.long)])
+        tok = torch.cat([tok, torch.full((ignored,), V + 5, dtype=torch.long)]) if more else tok
+        g = _gen(sum(lens) + more)
+        tok = tok[torch.randperm(len(tok), generator=g)]
+        rows = torch.randn(len(tok), 260, generator=g)
+        _check_grad(ops.embed_grad_sorted(rows.to(DEV), tok.to(DEV), V), _grad_ref(rows, tok, V, 1.0), more)
+
+
+def test_embed_grad_sorted_many_tiles():
+    """More tiles than a scatter sums itself (524288 rows): the scan in its own launch; a run of a third of the rows."""
+    n, V, d = 524288 + 8193, 5463, 8
+    g = _gen(9)
+    tok = _ids("skew", n, V, g)
+    tok[torch.rand(n, generator=g) < 0.33] = 17
+    rows = torch.randn(n, d, generator=g)
+    _check_grad(ops.embed_grad_sorted(rows.to(DEV), tok.to(DEV), V), _grad_ref(rows, tok, V, 1.0))
 
 
 def test_embed_grad_sorted_of_nothing():

@@ -4,17 +4,18 @@
 //
 // Gradient: g[v, :] = scale * sum over t_r = v of dY[r, :], fp32, without atomics on floats. Rows are brought into token
 // order first (a stable sort of the ids, row numbers as its payload), so that every vocabulary row is one run of
-// consecutive sorted positions in ascending row order; its sum then reads each gradient row once, in an order that only
+// consecutive sorted positions in ascending row order; the sum then reads each gradient row once, in an order that only
 // n, V and the ids decide. Ids outside [0, V), and `pad`, get the key V: they sort behind every row and no sum reads
 // them. The sort:
 //   n <= ES_RANK_MAX: the position of a row is a count, pos = #{key_j < key_i} + #{j < i: key_j = key_i}, taken over all
-//     n keys in LDS; the same loop gives the run's length, so one launch sorts and finds the runs;
-//   larger n: radix passes over digits of at most 9 bits (2 for the vocabularies of k = 6 .. 8), each a histogram per
-//     tile, a scan per digit over the tiles, and a stable scatter.
-// A run of up to ES_CHUNK rows is summed by one group of lanes. A longer one is cut at multiples of ES_CHUNK sorted
-// positions, so that a token that most rows share (padding, a homopolymer) spreads over the chip: each chunk writes the
-// partial sum of its first run and of its last run (no more than these two can be longer than a chunk), and the join
-// adds a run's partials in chunk order.
+//     n keys in LDS, in one launch;
+//   larger n: radix passes over digits of at most 9 bits (2 for the vocabularies of k = 5 .. 8), each a histogram per tile
+//     of 4096 keys and a stable scatter.
+// The sum goes by chunks of 64 sorted positions, one wavefront per 512 columns of each, which keeps loads of 4 to 8
+// gradient rows in flight whatever runs they belong to: it writes the runs that start in its chunk, up to 64 positions past it.
+// A longer run (padding, a homopolymer: tokens that a large part of the rows share) is cut at the chunks' borders, so that
+// it spreads over the chip; the join adds its partial sums in chunk order. Rows without a run are zeroed by wavefronts of
+// their own.
 #include "row_access.h"
 
 namespace vk {
@@ -69,77 +70,71 @@ __global__ __launch_bounds__(256) void embed_lookup_kernel(const WT *__restrict_
 
 constexpr int ES_RANK_MAX = 4096;  // rows that the counting sort takes
 constexpr int ES_RANK_ROWS = 16;   // rows per workgroup of it
-constexpr int ES_TILE = 2048;      // keys per workgroup of a radix pass: 8 per thread
+constexpr int ES_TILE = 4096;      // keys per workgroup of a radix pass: 4 per thread
 constexpr int ES_BITS = 9;         // digit bits at most
-constexpr int ES_CHUNK = 64;       // sorted positions per chunk
+constexpr int ES_FUSED = 128;      // tiles up to which a scatter sums the earlier tiles' counts itself
+constexpr int ES_FEW = 16384;      // rows up to which chunks are short
 
-struct Run {
-  int32_t start, end;
+constexpr uint32_t ES_NONE = 0xffffffffu;  // a key that is none: ignored, or past the last
+
+struct Pair {
+  uint32_t key, row;
 };
 
 __device__ __forceinline__ uint32_t sort_key(int64_t t, int32_t V, int64_t pad) {
   return t >= 0 && t < V && t != pad ? static_cast<uint32_t>(t) : static_cast<uint32_t>(V);
 }
 
-__global__ __launch_bounds__(256) void embed_runs_clear_kernel(Run *__restrict__ runs, int32_t V) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i < V) runs[i] = Run{0, 0};
-}
-
-// 16 rows per workgroup, 16 threads each over a sixteenth of the keys.
+// 16 rows per workgroup, 16 threads each over a sixteenth of the keys, four at a time.
 __global__ __launch_bounds__(256) void embed_rank_kernel(const int64_t *__restrict__ tokens, int32_t n, int32_t V,
-                                                         int64_t pad, uint32_t *__restrict__ keys,
-                                                         int32_t *__restrict__ rows, Run *__restrict__ runs) {
-  __shared__ uint32_t key[ES_RANK_MAX];
-  for (int j = threadIdx.x; j < n; j += 256) key[j] = sort_key(tokens[j], V, pad);
+                                                         int64_t pad, Pair *__restrict__ sorted,
+                                                         int32_t *__restrict__ owners) {
+  __shared__ __attribute__((aligned(16))) uint32_t key[ES_RANK_MAX];
+  if (blockIdx.x == 0 && threadIdx.x == 0) owners[0] = 0;
+  const int up = (n + 3) & ~3;
+  for (int j = threadIdx.x; j < up; j += 256) key[j] = j < n ? sort_key(tokens[j], V, pad) : ES_NONE;
   __syncthreads();
   const int part = threadIdx.x & 15;
   const int i = blockIdx.x * ES_RANK_ROWS + (threadIdx.x >> 4);
   const bool live = i < n;
   const uint32_t mine = key[live ? i : 0];
-  int less = 0, same = 0, before = 0;
-  for (int j = part; j < n; j += 16) {
-    const uint32_t k = key[j];
-    less += k < mine;
-    same += k == mine;
-    before += k == mine && j < i;
+  int pos = 0;
+#pragma unroll 4
+  for (int j = 4 * part; j < up; j += 64) {
+    const u32x4 k = *reinterpret_cast<const u32x4 *>(key + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pos += k[e] < mine + (j + e < i ? 1u : 0u);  // smaller, or equal and earlier
   }
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    less += __shfl_xor(less, o, 64);
-    same += __shfl_xor(same, o, 64);
-    before += __shfl_xor(before, o, 64);
-  }
-  if (live && part == 0) {
-    keys[less + before] = mine;
-    rows[less + before] = i;
-    if (before == 0 && mine < static_cast<uint32_t>(V)) runs[mine] = Run{less, less + same};
-  }
+  for (int o = 8; o > 0; o >>= 1) pos += __shfl_xor(pos, o, 64);
+  if (live && part == 0) sorted[pos] = Pair{mine, static_cast<uint32_t>(i)};
 }
 
-// counts [bins, tiles]: keys of each digit in each tile. The first pass takes the ids themselves and clears the runs.
+// counts [tiles, bins]: keys of each digit in each tile. The first pass takes the ids themselves, and empties the list of
+// long runs.
 template <bool FIRST>
-__global__ __launch_bounds__(256) void embed_hist_kernel(const int64_t *__restrict__ tokens,
-                                                         const uint32_t *__restrict__ keys, int64_t n, int32_t V,
-                                                         int64_t pad, int shift, int bins, uint32_t *__restrict__ counts,
-                                                         Run *__restrict__ runs) {
-  __shared__ uint32_t h[1 << ES_BITS];
-  for (int b = threadIdx.x; b < bins; b += 256) h[b] = 0;
-  if (FIRST)
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < V; i += static_cast<int64_t>(gridDim.x) * 256)
-      runs[i] = Run{0, 0};
-  __syncthreads();
+__global__ __launch_bounds__(1024) void embed_hist_kernel(const int64_t *__restrict__ tokens, const Pair *__restrict__ pairs,
+                                                          int64_t n, int32_t V, int64_t pad, int shift, int bins,
+                                                          uint32_t *__restrict__ counts, int32_t *__restrict__ owners) {
+  if (FIRST && blockIdx.x == 0 && threadIdx.x == 0) owners[0] = 0;
+  // four counters a digit, by lane: a digit that many keys share is not added to one place by a whole wavefront
+  __shared__ u32x4 h[1 << ES_BITS];
+  for (int b = threadIdx.x; b < bins; b += 1024) h[b] = u32x4{0u, 0u, 0u, 0u};
   const int64_t base = static_cast<int64_t>(blockIdx.x) * ES_TILE;
+  uint32_t k[ES_TILE / 1024];
 #pragma unroll
-  for (int u = 0; u < ES_TILE / 256; ++u) {
-    const int64_t i = base + u * 256 + threadIdx.x;
-    if (i < n) {
-      const uint32_t k = FIRST ? sort_key(tokens[i], V, pad) : keys[i];
-      atomicAdd(&h[(k >> shift) & (bins - 1)], 1u);
-    }
+  for (int u = 0; u < ES_TILE / 1024; ++u) {
+    const int64_t i = base + u * 1024 + threadIdx.x, at = i < n ? i : n - 1;
+    k[u] = FIRST ? sort_key(tokens[at], V, pad) : pairs[at].key;
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += 256) counts[static_cast<int64_t>(b) * gridDim.x + blockIdx.x] = h[b];
+#pragma unroll
+  for (int u = 0; u < ES_TILE / 1024; ++u)
+    if (base + u * 1024 + threadIdx.x < n)
+      atomicAdd(reinterpret_cast<uint32_t *>(h) + 4 * ((k[u] >> shift) & (bins - 1)) + (threadIdx.x & 3), 1u);
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += 1024)
+    counts[static_cast<int64_t>(blockIdx.x) * bins + b] = (h[b][0] + h[b][1]) + (h[b][2] + h[b][3]);
 }
 
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {  // inclusive
@@ -151,256 +146,337 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {  // inclus
   return v;
 }
 
-// One wavefront per digit: counts[b, :] becomes its exclusive prefix over the tiles, totals[b] its sum.
-__global__ __launch_bounds__(64) void embed_scan_kernel(uint32_t *__restrict__ counts, int tiles,
+// More than ES_FUSED tiles: one wavefront per digit; its column of counts becomes its exclusive prefix over the tiles,
+// totals[digit] its sum.
+__global__ __launch_bounds__(64) void embed_scan_kernel(uint32_t *__restrict__ counts, int64_t tiles, int bins,
                                                         uint32_t *__restrict__ totals) {
-  uint32_t *row = counts + static_cast<int64_t>(blockIdx.x) * tiles;
+  uint32_t *col = counts + blockIdx.x;
   const int lane = threadIdx.x;
   uint32_t run = 0;
-  for (int t0 = 0; t0 < tiles; t0 += 64) {
-    const uint32_t v = t0 + lane < tiles ? row[t0 + lane] : 0;
+  for (int64_t t0 = 0; t0 < tiles; t0 += 64) {
+    const uint32_t v = t0 + lane < tiles ? col[(t0 + lane) * bins] : 0;
     const uint32_t inc = wave_scan(v, lane);
-    if (t0 + lane < tiles) row[t0 + lane] = run + inc - v;
+    if (t0 + lane < tiles) col[(t0 + lane) * bins] = run + inc - v;
     run += __shfl(inc, 63, 64);
   }
   if (lane == 0) totals[blockIdx.x] = run;
 }
 
-// A stable scatter: wavefront w of a tile owns its keys 512 w .. 512 w + 511 in 8 rounds of 64, so (w, round, lane) is
+// A stable scatter: wavefront w of a tile owns its keys 256 w .. 256 w + 255 in 4 rounds of 64, so (w, round, lane) is
 // the keys' order. In a round the lanes of one digit find each other by a ballot per digit bit; a key's rank is the
-// digit's count in this wavefront's earlier rounds plus its lanes below.
-template <bool FIRST>
-__global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t *__restrict__ tokens,
-                                                            const uint32_t *__restrict__ keys_in,
-                                                            const int32_t *__restrict__ rows_in, int64_t n, int32_t V,
-                                                            int64_t pad, int shift, int bits,
-                                                            const uint32_t *__restrict__ counts,
-                                                            const uint32_t *__restrict__ totals,
-                                                            uint32_t *__restrict__ keys_out,
-                                                            int32_t *__restrict__ rows_out) {
-  constexpr int BINS = 1 << ES_BITS, ROUNDS = ES_TILE / 256;
-  __shared__ uint32_t wcount[4][BINS];
-  __shared__ uint32_t wsum[4];
-  const int bins = 1 << bits;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  for (int b = tid; b < 4 * BINS; b += 256) (&wcount[0][0])[b] = 0;
-  __syncthreads();
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * ES_TILE + wid * (ES_TILE / 4);
-  uint32_t key[ROUNDS];
-  int32_t row[ROUNDS], rank[ROUNDS];
+// digit's count in this wavefront's earlier rounds plus its lanes below. FUSED: the tile's offsets are summed here from
+// the counts of all (at most ES_FUSED) tiles, two threads per digit.
+template <bool FIRST, bool FUSED>
+__global__ __launch_bounds__(1024) void embed_scatter_kernel(const int64_t *__restrict__ tokens,
+                                                             const Pair *__restrict__ in, int64_t n, int32_t V, int64_t pad,
+                                                             int shift, int bits, const uint32_t *__restrict__ counts,
+                                                             const uint32_t *__restrict__ totals,
+                                                             Pair *__restrict__ out) {
+  constexpr int BINS = 1 << ES_BITS, ROUNDS = ES_TILE / 1024, WAVES = 16;
+  __shared__ uint32_t wcount[WAVES][BINS];
+  __shared__ uint32_t half[2][BINS], wsum[WAVES];
+  const int bins = 1 << bits, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * ES_TILE + wid * (ES_TILE / WAVES);
+  Pair x[ROUNDS];
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
-    const int64_t i = base + r * 64 + lane;
-    const bool in = i < n;
-    key[r] = in ? (FIRST ? sort_key(tokens[i], V, pad) : keys_in[i]) : 0;
-    row[r] = FIRST ? static_cast<int32_t>(i) : (in ? rows_in[i] : 0);
+    const int64_t i = base + r * 64 + lane, at = i < n ? i : n - 1;
+    x[r] = FIRST ? Pair{sort_key(tokens[at], V, pad), static_cast<uint32_t>(i)} : in[at];
   }
+  // this digit's keys in earlier tiles, and in all
+  uint32_t before = 0, total = 0;
+  const int bin = tid & (BINS - 1), side = tid / BINS;
+  if (bin < bins) {
+    if (FUSED) {
+      const int tiles = static_cast<int>(gridDim.x), me = static_cast<int>(blockIdx.x);
+      for (int t0 = side; t0 < tiles; t0 += 32) {
+        uint32_t c[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) c[u] = counts[min(t0 + 2 * u, tiles - 1) * bins + bin];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          total += t0 + 2 * u < tiles ? c[u] : 0;
+          before += t0 + 2 * u < me ? c[u] : 0;
+        }
+      }
+    } else if (side == 0) {
+      before = counts[static_cast<int64_t>(blockIdx.x) * bins + bin];
+      total = totals[bin];
+    }
+  }
+  for (int b = tid; b < WAVES * BINS; b += 1024) (&wcount[0][0])[b] = 0;
+  if (side == 1) {
+    half[0][bin] = before;
+    half[1][bin] = total;
+  }
+  __syncthreads();
+  if (FUSED && side == 0) {
+    before += half[0][bin];
+    total += half[1][bin];
+  }
+  int rank[ROUNDS];
   volatile uint32_t *mine = wcount[wid];
   const uint64_t below_mask = (uint64_t(1) << lane) - 1;
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
-    const bool in = base + r * 64 + lane < n;
-    const uint32_t dig = (key[r] >> shift) & (bins - 1);
-    uint64_t peers = __ballot(in);
-    for (int b = 0; b < bits; ++b) {
+    const bool live = base + r * 64 + lane < n;
+    const uint32_t dig = (x[r].key >> shift) & (bins - 1);
+    uint64_t peers = __ballot(live);
+#pragma unroll
+    for (int b = 0; b < ES_BITS; ++b) {
       const bool bit = (dig >> b) & 1;
       const uint64_t m = __ballot(bit);
-      peers &= bit ? m : ~m;
+      if (b < bits) peers &= bit ? m : ~m;
     }
     const int below = __popcll(peers & below_mask);
     const uint32_t old = mine[dig];  // every lane reads before a digit's first lane writes (one wavefront, in order)
-    rank[r] = static_cast<int32_t>(old) + below;
-    if (in && below == 0) mine[dig] = old + static_cast<uint32_t>(__popcll(peers));
+    rank[r] = static_cast<int>(old) + below;
+    if (live && below == 0) mine[dig] = old + static_cast<uint32_t>(__popcll(peers));
   }
-  __syncthreads();
-  // wcount[w][b]: first position of wavefront w's keys of digit b = keys of smaller digits + of this digit in earlier
-  // tiles + in this tile's earlier wavefronts. Thread t scans digits 2 t and 2 t + 1
-  const uint32_t t0 = 2 * tid < bins ? totals[2 * tid] : 0, t1 = 2 * tid + 1 < bins ? totals[2 * tid + 1] : 0;
-  const uint32_t inc = wave_scan(t0 + t1, lane);
+  // digits' first positions: a scan of the totals over threads 0 .. 511
+  const uint32_t inc = wave_scan(side == 0 ? total : 0, lane);
   if (lane == 63) wsum[wid] = inc;
   __syncthreads();
-  uint32_t first = inc - t0 - t1;
-  for (int w = 0; w < wid; ++w) first += wsum[w];
+  if (side == 0 && bin < bins) {
+    uint32_t at = inc - total + before;
+    for (int w = 0; w < wid; ++w) at += wsum[w];
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int b = 2 * tid + q;
-    if (b < bins) {
-      uint32_t at = first + (q ? t0 : 0) + counts[static_cast<int64_t>(b) * gridDim.x + blockIdx.x];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t c = wcount[w][b];
-        wcount[w][b] = at;
-        at += c;
-      }
+    for (int w = 0; w < WAVES; ++w) {
+      const uint32_t c = wcount[w][bin];
+      wcount[w][bin] = at;
+      at += c;
     }
   }
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r)
-    if (base + r * 64 + lane < n) {
-      const uint32_t at = wcount[wid][(key[r] >> shift) & (bins - 1)] + rank[r];
-      keys_out[at] = key[r];
-      rows_out[at] = row[r];
-    }
-}
-
-__global__ __launch_bounds__(256) void embed_runs_kernel(const uint32_t *__restrict__ keys, int64_t n, int32_t V,
-                                                         Run *__restrict__ runs) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n) return;
-  const uint32_t k = keys[i];
-  if (k >= static_cast<uint32_t>(V)) return;
-  if (i == 0 || keys[i - 1] != k) runs[k].start = static_cast<int32_t>(i);
-  if (i == n - 1 || keys[i + 1] != k) runs[k].end = static_cast<int32_t>(i + 1);
+    if (base + r * 64 + lane < n) out[wcount[wid][(x[r].key >> shift) & (bins - 1)] + rank[r]] = x[r];
 }
 
 // ---- the sums ----------------------------------------------------------------------------------------------------------
 
-// Sum over sorted positions [p0, p1) of the gradient rows, for this lane's NCH groups of 4 columns (c, c + 4 LPR, ...):
-// SIDE = 64 / LPR groups of lanes take every SIDE-th position and are added in a fixed order at the end, so every lane of
-// a column has the sum. U positions' loads are in flight together.
-template <typename T, int LPR, int NCH>
-__device__ __forceinline__ void sum_rows(const T *__restrict__ drows, int64_t ld, const int32_t *__restrict__ rows,
-                                         int p0, int p1, int c, int cols, float (&acc)[NCH][4]) {
-  constexpr int SIDE = 64 / LPR, U = 8 / NCH < 2 ? 2 : 8 / NCH;
-  const int sub = (threadIdx.x & 63) / LPR;
+// The columns of a lane in the sum: NQ groups of N, 64 N apart, one sum each. A group that the row's end cuts is moved back
+// to stay inside the row, so that all accesses are 16 bytes wide (columns that two lanes hold get the same sum); `own` is
+// where its own columns begin. PLAIN: sums are stored; else they may be added to what is there, and rows may be narrower
+// than a group, column by column.
+template <typename T, int NQ, bool PLAIN>
+struct Cols {
+  static constexpr int N = 16 / sizeof(T), SPAN = 64 * N * NQ, U = 8 / NQ;
+  int own[NQ], c[NQ], d;
+  float v[NQ][N];
+
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-  for (int q = 0; q < NCH; ++q)
+    for (int q = 0; q < NQ; ++q)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[q][k] = 0.f;
-  for (int p = p0 + sub; p < p1; p += U * SIDE) {
-    float v[U][NCH][4];
+      for (int k = 0; k < N; ++k) v[q][k] = 0.f;
+  }
+  __device__ __forceinline__ void init(int block, int lane, int d_) {
+    d = d_;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int pu = p + u * SIDE;
-      const bool in = pu < p1;
-      const T *src = drows + static_cast<int64_t>(rows[in ? pu : p]) * ld + c;
+    for (int q = 0; q < NQ; ++q) {
+      own[q] = block * SPAN + N * (64 * q + lane);
+      c[q] = own[q] + N <= d || (!PLAIN && d < N) ? own[q] : d - N;
+    }
+    zero();
+  }
+  __device__ __forceinline__ u32x4 load(const T *row, int q) const {
+    if (PLAIN || d >= N) return stream_16(row + c[q]);
+    u32x4 w;
 #pragma unroll
-      for (int q = 0; q < NCH; ++q) {
-        const int cq = c + q * 4 * LPR;
-        if (in && cq + 4 <= cols) {
-          load_row<4>(src + q * 4 * LPR, v[u][q]);
+    for (int k = 0; k < 4; ++k)
+      if constexpr (sizeof(T) == 4)
+        w[k] = __float_as_uint(own[q] + k < d ? load_one(row + own[q] + k) : 0.f);
+      else
+        w[k] = pack_bf(own[q] + 2 * k < d ? load_one(row + own[q] + 2 * k) : 0.f,
+                       own[q] + 2 * k + 1 < d ? load_one(row + own[q] + 2 * k + 1) : 0.f);
+    return w;
+  }
+  __device__ __forceinline__ void add(const u32x4 &w, int q) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if constexpr (sizeof(T) == 4)
+        v[q][k] += __uint_as_float(w[k]);
+      else
+        v[q][k] += (k & 1) ? hi_bf(w[k / 2]) : lo_bf(w[k / 2]);
+  }
+  // scale * the sums into a row (`onto`: added to it); the sums start over.
+  __device__ __forceinline__ void put(float *row, float scale, bool onto) {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      if (own[q] < d) {
+        if (PLAIN || (!onto && d >= N)) {
+          float o[N];
+#pragma unroll
+          for (int k = 0; k < N; ++k) o[k] = v[q][k] * scale;
+          store_row<N>(row + c[q], o);
         } else {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[u][q][k] = in && cq + k < cols ? load_one(src + q * 4 * LPR + k) : 0.f;
+          for (int k = 0; k < N; ++k)
+            if (c[q] + k >= own[q] && c[q] + k < d)
+              row[c[q] + k] = onto ? row[c[q] + k] + v[q][k] * scale : v[q][k] * scale;
         }
       }
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int q = 0; q < NCH; ++q)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[q][k] += v[u][q][k];
+    zero();
   }
+  // Adds positions [a, b) of 64, whose gradient rows' numbers are in the lanes of `rows`: U rows' loads in flight. RUNS:
+  // where `heads` has a bit, the run before that position ends; it goes to the row of `out` that its key names.
+  template <bool RUNS>
+  __device__ __forceinline__ void walk(const T *drows, int64_t ld, uint32_t rows, int a, int b, uint64_t heads, uint32_t keys,
+                                       float *out, float scale, bool onto) {
+    for (int p = a; p < b; p += U) {
+      u32x4 w[U][NQ];
 #pragma unroll
-  for (int o = LPR; o < 64; o <<= 1)
+      for (int u = 0; u < U; ++u) {
+        const int at = p + u < b ? p + u : b - 1;
+        const T *row = drows + static_cast<int64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(rows, at))) * ld;
 #pragma unroll
-    for (int q = 0; q < NCH; ++q)
+        for (int q = 0; q < NQ; ++q) w[u][q] = load(row, q);
+      }
+      const uint32_t h = RUNS ? static_cast<uint32_t>(heads >> p) : 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[q][k] += __shfl_xor(acc[q][k], o, 64);
-}
-
-__device__ __forceinline__ void put4(float *dst, int c, int cols, const float (&v)[4], float scale, bool add) {
-  if (c + 4 <= cols) {
-    f32x4_e o = {v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale};
-    if (add) o += *reinterpret_cast<const f32x4_e *>(dst);
-    *reinterpret_cast<f32x4_e *>(dst) = o;
-  } else {
-    for (int k = 0; k < 4 && c + k < cols; ++k) dst[k] = add ? dst[k] + v[k] * scale : v[k] * scale;
-  }
-}
-
-// Wavefronts 0 .. chunks - 1: one chunk's partial sums of the long runs in it (slot 0: the run at its first position,
-// slot 1: the run at its last, where that is another one). The others: one vocabulary row each, unless its run is long;
-// a row without a run is zero (accumulate: left as it is). grid.y: blocks of 4 LPR NCH columns.
-template <typename T, int LPR, int NCH>
-__global__ __launch_bounds__(256) void embed_sum_kernel(const T *__restrict__ drows, int64_t ld, int32_t n, int32_t V,
-                                                        int d, const uint32_t *__restrict__ keys,
-                                                        const int32_t *__restrict__ rows, const Run *__restrict__ runs,
-                                                        int32_t chunks, float scale, int accumulate,
-                                                        float *__restrict__ part, float *__restrict__ out) {
-  const int lane = threadIdx.x & 63;
-  const int cb = blockIdx.y * 4 * LPR * NCH;
-  const int c = 4 * (lane % LPR), cols = d - cb;  // columns of this block, from cb
-  const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const bool writer = lane < LPR;
-  float acc[NCH][4];
-  const T *base = drows + cb;
-  if (wave < chunks) {
-    const int p0 = static_cast<int>(wave) * ES_CHUNK, p1 = n - p0 < ES_CHUNK ? n : p0 + ES_CHUNK;
-    const uint32_t k0 = keys[p0], k1 = keys[p1 - 1];
-#pragma unroll 1
-    for (int slot = 0; slot < 2; ++slot) {
-      const uint32_t k = slot ? k1 : k0;
-      if (k >= static_cast<uint32_t>(V) || (slot && k1 == k0)) continue;
-      const Run run = runs[k];
-      if (run.end - run.start <= ES_CHUNK) continue;
-      const int a = run.start > p0 ? run.start : p0, b = run.end < p1 ? run.end : p1;
-      sum_rows<T, LPR, NCH>(base, ld, rows, a, b, c, cols, acc);
-      float *dst = part + (2 * wave + slot) * d + cb + c;
+      for (int u = 0; u < U; ++u) {
+        if (p + u < b) {
+          if (RUNS && ((h >> u) & 1)) put(out + static_cast<int64_t>(__builtin_amdgcn_readlane(keys, p + u - 1)) * d, scale, onto);
 #pragma unroll
-      for (int q = 0; q < NCH; ++q)
-        if (writer) put4(dst + q * 4 * LPR, c + q * 4 * LPR, cols, acc[q], 1.f, false);
+          for (int q = 0; q < NQ; ++q) add(w[u][q], q);
+        }
+      }
     }
+  }
+};
+
+// Wavefronts 0 .. chunks - 1: the runs of a chunk of sorted positions, for the columns of block blockIdx.y. A run is long
+// if it starts in a chunk and holds the last position of the next one: then its part in each chunk is a partial sum
+// (slot 1: the one that starts there; slot 0: the one that comes in from the chunk before), and its first chunk goes on
+// `owners`, in any order. The other wavefronts zero 64 vocabulary rows each, those without a run.
+template <typename T, int NQ, bool PLAIN, int CHUNK>
+__global__ __launch_bounds__(256) void embed_sum_kernel(const T *__restrict__ drows, int64_t ld, int32_t n, int32_t V,
+                                                        int d, const Pair *__restrict__ sorted, int32_t chunks, float scale,
+                                                        int accumulate, float *__restrict__ part, int32_t *__restrict__ owners,
+                                                        float *__restrict__ out) {
+  const int lane = threadIdx.x & 63;
+  const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t uV = static_cast<uint32_t>(V);
+  Cols<T, NQ, PLAIN> x;
+  x.init(blockIdx.y, lane, d);
+  if (wave >= chunks) {
+    const int64_t v0 = (wave - chunks) * 64, v = v0 + lane;
+    if (v0 >= V || accumulate) return;
+    int lo = 0, hi = n;  // first sorted position whose key is not below v
+    while (lo < hi) {
+      const int mid = lo + (hi - lo) / 2;
+      if (sorted[mid].key < static_cast<uint32_t>(v))
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    const bool absent = v < V && !(lo < n && sorted[lo].key == static_cast<uint32_t>(v));
+    for (uint64_t left = __ballot(absent); left != 0; left &= left - 1) x.put(out + (v0 + __builtin_ctzll(left)) * d, 1.f, false);
     return;
   }
-  const int64_t v = wave - chunks;
-  if (v >= V) return;
-  const Run run = runs[v];
-  if (run.end - run.start > ES_CHUNK || (accumulate && run.end == run.start)) return;
-  sum_rows<T, LPR, NCH>(base, ld, rows, run.start, run.end, c, cols, acc);
-  float *dst = out + v * d + cb + c;
-#pragma unroll
-  for (int q = 0; q < NCH; ++q)
-    if (writer) put4(dst + q * 4 * LPR, c + q * 4 * LPR, cols, acc[q], scale, accumulate != 0);
+  const int p0 = static_cast<int>(wave) * CHUNK;
+  auto at = [&](int p) {
+    const Pair x = sorted[p < n ? p : n - 1];
+    return Pair{p < n && x.key < uV ? x.key : ES_NONE, x.row};
+  };
+  constexpr uint64_t LANES = CHUNK == 64 ? ~uint64_t(0) : (uint64_t(1) << (CHUNK & 63)) - 1;
+  const Pair lo = at(p0 + lane), hi = at(p0 + CHUNK + lane);
+  const Pair before = at(p0 > 0 ? p0 - 1 : 0), before2 = at(p0 > CHUNK ? p0 - CHUNK - 1 : 0);
+  const uint32_t prev = p0 > 0 ? before.key : ES_NONE, prev2 = p0 > CHUNK ? before2.key : ES_NONE;
+  const int valid = __popcll(__ballot(lo.key != ES_NONE) & LANES);
+  const uint32_t first = __builtin_amdgcn_readlane(lo.key, 0), last = __builtin_amdgcn_readlane(lo.key, CHUNK - 1);
+  if (first == ES_NONE) return;
+  uint32_t left_lo = __shfl_up(lo.key, 1, 64), left_hi = __shfl_up(hi.key, 1, 64);
+  if (lane == 0) {
+    left_lo = prev;
+    left_hi = last;
+  }
+  const uint64_t heads = __ballot(lo.key != left_lo) & LANES, heads_hi = __ballot(hi.key != left_hi) & LANES;
+  // [0, start): the run that comes in; [start, stop): this chunk's runs, of which the last goes on for `ahead` positions
+  // of the next chunk; or [stop, CHUNK) is a long one
+  const int start = heads != 0 ? __builtin_ctzll(heads) : CHUNK;
+  const bool long_in = start > 0 && (prev2 == first || start == CHUNK);
+  int ahead = last == ES_NONE || start == CHUNK ? 0 : (heads_hi != 0 ? __builtin_ctzll(heads_hi) : CHUNK);
+  const bool long_out = ahead == CHUNK;
+  const int stop = long_out ? 63 - __builtin_clzll(heads) : valid;
+  const bool onto = accumulate != 0;
+  if (long_in) {
+    x.template walk<false>(drows, ld, lo.row, 0, start < valid ? start : valid, 0, 0, nullptr, 0.f, false);
+    x.put(part + 2 * wave * d, 1.f, false);
+  }
+  if (start < stop) {
+    x.template walk<true>(drows, ld, lo.row, start, stop, heads & ~(uint64_t(1) << start), lo.key, out, scale, onto);
+    if (!long_out) x.template walk<false>(drows, ld, hi.row, 0, ahead, 0, 0, nullptr, 0.f, false);
+    x.put(out + static_cast<int64_t>(__builtin_amdgcn_readlane(lo.key, stop - 1)) * d, scale, onto);
+  }
+  if (long_out) {
+    x.template walk<false>(drows, ld, lo.row, stop, CHUNK, 0, 0, nullptr, 0.f, false);
+    x.put(part + (2 * wave + 1) * d, 1.f, false);
+    if (lane == 0 && blockIdx.y == 0) owners[1 + atomicAdd(owners, 1)] = static_cast<int32_t>(wave);
+  }
 }
 
-// Long runs: workgroup (chunk, column block of 64) owns the run that starts in its chunk and leaves it, if there is one
-// (it holds the chunk's last position), and adds the run's partials in chunk order: 16 groups of 16 lanes take every
-// 16th partial, then the groups are added in order.
-__global__ __launch_bounds__(256) void embed_join_kernel(const uint32_t *__restrict__ keys, const Run *__restrict__ runs,
-                                                         int32_t n, int32_t V, int d, const float *__restrict__ part,
+constexpr int EJ_GROUPS = 32;
+
+// Long runs: workgroups take (a run's first chunk, 64 columns) and add the run's partials in chunk order: 32 groups of 16
+// lanes take every 32nd, then the groups are added in order.
+__global__ __launch_bounds__(512) void embed_join_kernel(const Pair *__restrict__ sorted, int d, int chunk, int32_t chunks,
+                                                         const float *__restrict__ part, const int32_t *__restrict__ owners,
                                                          float scale, int accumulate, float *__restrict__ out) {
-  __shared__ float red[16][64];
-  const int64_t p0 = static_cast<int64_t>(blockIdx.x) * ES_CHUNK;
-  const int64_t p1 = p0 + ES_CHUNK < n ? p0 + ES_CHUNK : n;
-  const uint32_t k = keys[p1 - 1];
-  if (k >= static_cast<uint32_t>(V)) return;
-  const Run run = runs[k];
-  if (run.end - run.start <= ES_CHUNK || run.start < p0) return;
-  const int64_t first = blockIdx.x, count = (run.end - 1) / ES_CHUNK - first + 1;
-  const int64_t lead = 2 * first + (run.start == p0 ? 0 : 1);
-  const int g = threadIdx.x >> 4, c = blockIdx.y * 64 + 4 * (threadIdx.x & 15);
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t j = g; j < count; j += 16) {
-    const float *src = part + (j == 0 ? lead : 2 * (first + j)) * d + c;
-    if (c + 4 <= d) {
-      float v[4];
-      load_row<4>(src, v);
+  constexpr int U = 4;
+  __shared__ float red[EJ_GROUPS][64];
+  const int tid = threadIdx.x, g = tid >> 4, e0 = 4 * (tid & 15);
+  const int blocks = (d + 63) / 64;
+  const int64_t units = static_cast<int64_t>(owners[0]) * blocks;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int j = owners[1 + unit / blocks], c = static_cast<int>(unit % blocks) * 64 + e0;
+    const uint32_t key = sorted[static_cast<int64_t>(j) * chunk + chunk - 1].key;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    bool more = true;
+    for (int64_t i = j + g; more; i += U * EJ_GROUPS) {
+      uint32_t k[U];
+      float v[U][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += v[e];
-    } else {
-      for (int e = 0; e < 4 && c + e < d; ++e) acc[e] += src[e];
+      for (int u = 0; u < U; ++u) {
+        const int64_t iu = i + u * EJ_GROUPS, in = iu < chunks ? iu : chunks - 1;
+        k[u] = iu < chunks ? (iu == j ? key : sorted[in * chunk].key) : ES_NONE;
+        const float *src = part + (2 * in + (iu == j ? 1 : 0)) * d;
+        if (c + 4 <= d) {
+          load_row<4>(src + c, v[u]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[u][e] = src[min(c + e, d - 1)];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        more = more && k[u] == key;  // (sorted: no later chunk begins with it then)
+        if (more)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += v[u][e];
+      }
     }
-  }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) red[g][4 * (threadIdx.x & 15) + e] = acc[e];
-  __syncthreads();
-  if (threadIdx.x < 16) {
-    float t[4];
+    for (int e = 0; e < 4; ++e) red[g][e0 + e] = acc[e];
+    __syncthreads();
+    const int col = static_cast<int>(unit % blocks) * 64 + tid;
+    if (tid < 64 && col < d) {
+      float t = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      t[e] = 0.f;
-      for (int q = 0; q < 16; ++q) t[e] += red[q][4 * threadIdx.x + e];
+      for (int w = 0; w < EJ_GROUPS; ++w) t += red[w][tid];
+      float *dst = out + static_cast<int64_t>(key) * d + col;
+      *dst = accumulate ? *dst + t * scale : t * scale;
     }
-    if (c < d) put4(out + static_cast<int64_t>(k) * d + c, c, d, t, scale, accumulate != 0);
+    __syncthreads();  // red has been read
   }
 }
 
 struct SortPlan {
-  int64_t keys[2], rows[2], runs, counts, totals, part, bytes;  // offsets in the workspace
-  int passes, bits, tiles, chunks;
+  int64_t pairs[2], counts, totals, part, owners, bytes;  // offsets in the workspace
+  int64_t tiles;
+  int passes, bits, chunk, chunks;
 };
 
 static SortPlan sort_plan(int64_t n, int32_t V, int32_t d) {
@@ -411,46 +487,34 @@ static SortPlan sort_plan(int64_t n, int32_t V, int32_t d) {
     at += (b + 255) / 256 * 256;
     return o;
   };
-  const bool rank = n <= ES_RANK_MAX;
   int need = 0;
   while ((static_cast<int64_t>(V) >> need) != 0) ++need;  // bits of the largest key, V
-  p.passes = rank ? 0 : (need + ES_BITS - 1) / ES_BITS;
-  p.bits = rank ? 0 : (need + p.passes - 1) / p.passes;
-  p.tiles = static_cast<int>((n + ES_TILE - 1) / ES_TILE);
-  p.chunks = n > ES_CHUNK ? static_cast<int>((n + ES_CHUNK - 1) / ES_CHUNK) : 0;  // no run of n <= 64 rows is long
-  p.keys[0] = take(4 * n);
-  p.rows[0] = take(4 * n);
-  p.keys[1] = rank ? 0 : take(4 * n);
-  p.rows[1] = rank ? 0 : take(4 * n);
-  p.runs = take(static_cast<int64_t>(sizeof(Run)) * V);
-  p.counts = rank ? 0 : take(static_cast<int64_t>(4) * p.tiles << p.bits);
-  p.totals = rank ? 0 : take(int64_t(4) << p.bits);
-  p.part = take(static_cast<int64_t>(8) * p.chunks * d);
-  p.bytes = at;
+  p.passes = n <= ES_RANK_MAX ? 0 : (need + ES_BITS - 1) / ES_BITS;
+  p.bits = p.passes == 0 ? 0 : (need + p.passes - 1) / p.passes;
+  p.tiles = (n + ES_TILE - 1) / ES_TILE;
+  p.chunk = n <= ES_FEW ? 16 : 64;
+  p.chunks = static_cast<int>((n + p.chunk - 1) / p.chunk);
+  p.pairs[0] = take(8 * n);
+  p.pairs[1] = p.passes == 0 ? 0 : take(8 * n);
+  p.counts = p.passes == 0 ? 0 : take((4 * p.tiles) << p.bits);
+  p.totals = p.tiles <= ES_FUSED ? 0 : take(int64_t(4) << p.bits);
+  p.part = n < 2 * p.chunk ? 0 : take(static_cast<int64_t>(8) * p.chunks * d);  // (no run is long in fewer)
+  p.owners = take(4 * (p.chunks + 1));
+  p.bytes = at < 16 ? 16 : at;
   return p;
 }
 
-template <typename T>
-static void launch_sum(const SortPlan &p, const T *drows, int64_t ld, int32_t n, int32_t V, int d, const uint32_t *keys,
-                       const int32_t *rows, const Run *runs, float scale, int accumulate, float *part, float *out,
-                       hipStream_t s) {
-  const unsigned gx = static_cast<unsigned>((static_cast<int64_t>(p.chunks) + V + 3) / 4);
-#define VK_EMBED_SUM(LPR, NCH)                                                                                          \
-  embed_sum_kernel<T, LPR, NCH><<<dim3(gx, static_cast<unsigned>((d + 4 * LPR * NCH - 1) / (4 * LPR * NCH))), 256, 0, s>>>( \
-      drows, ld, n, V, d, keys, rows, runs, p.chunks, scale, accumulate, part, out)
-  if (d <= 64)
-    VK_EMBED_SUM(16, 1);
-  else if (d <= 128)
-    VK_EMBED_SUM(32, 1);
-  else if (d <= 256)
-    VK_EMBED_SUM(64, 1);
-  else if (d <= 512)
-    VK_EMBED_SUM(64, 2);
-  else if (d <= 768)
-    VK_EMBED_SUM(64, 3);
-  else
-    VK_EMBED_SUM(64, 4);
-#undef VK_EMBED_SUM
+template <bool FIRST>
+static void launch_pass(const SortPlan &p, const int64_t *tokens, const Pair *in, Pair *out, int64_t n, int32_t V, int64_t pad,
+                        int shift, uint32_t *counts, uint32_t *totals, int32_t *owners, hipStream_t s) {
+  const unsigned tiles = static_cast<unsigned>(p.tiles), bins = 1u << p.bits;
+  embed_hist_kernel<FIRST><<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, bins, counts, owners);
+  if (p.tiles <= ES_FUSED) {
+    embed_scatter_kernel<FIRST, true><<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, p.bits, counts, nullptr, out);
+  } else {
+    embed_scan_kernel<<<bins, 64, 0, s>>>(counts, p.tiles, bins, totals);
+    embed_scatter_kernel<FIRST, false><<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, p.bits, counts, totals, out);
+  }
 }
 
 }  // namespace vk
@@ -509,47 +573,61 @@ extern "C" int vk_embed_grad_sorted(const void *d_rows, int32_t d_dtype, int64_t
                static_cast<long long>(p.bytes));
   hipStream_t s = VK_STREAM(stream);
   char *ws = static_cast<char *>(workspace);
-  auto keys = [&](int i) { return reinterpret_cast<uint32_t *>(ws + p.keys[i]); };
-  auto rows = [&](int i) { return reinterpret_cast<int32_t *>(ws + p.rows[i]); };
-  Run *runs = reinterpret_cast<Run *>(ws + p.runs);
-  int at = 0;  // which of the two key / row buffers holds the sorted ones
-  if (p.passes == 0) {
-    embed_runs_clear_kernel<<<static_cast<unsigned>((static_cast<int64_t>(V) + 255) / 256), 256, 0, s>>>(runs, V);
-    if (n > 0)
-      embed_rank_kernel<<<static_cast<unsigned>((n + ES_RANK_ROWS - 1) / ES_RANK_ROWS), 256, 0, s>>>(
-          tokens, static_cast<int32_t>(n), V, pad, keys(0), rows(0), runs);
-  } else {
+  auto pairs = [&](int i) { return reinterpret_cast<Pair *>(ws + p.pairs[i]); };
+  int32_t *owners = reinterpret_cast<int32_t *>(ws + p.owners);
+  int at = 0;  // which of the two buffers holds the sorted pairs
+  if (n > 0 && p.passes == 0) {
+    embed_rank_kernel<<<static_cast<unsigned>((n + ES_RANK_ROWS - 1) / ES_RANK_ROWS), 256, 0, s>>>(
+        tokens, static_cast<int32_t>(n), V, pad, pairs(0), owners);
+  } else if (n > 0) {
     uint32_t *counts = reinterpret_cast<uint32_t *>(ws + p.counts), *totals = reinterpret_cast<uint32_t *>(ws + p.totals);
-    const unsigned tiles = static_cast<unsigned>(p.tiles), bins = 1u << p.bits;
-    for (int q = 0; q < p.passes; ++q) {
-      const int shift = q * p.bits, to = q & 1;
-      if (q == 0)
-        embed_hist_kernel<true><<<tiles, 256, 0, s>>>(tokens, nullptr, n, V, pad, shift, bins, counts, runs);
-      else
-        embed_hist_kernel<false><<<tiles, 256, 0, s>>>(nullptr, keys(at), n, V, pad, shift, bins, counts, nullptr);
-      embed_scan_kernel<<<bins, 64, 0, s>>>(counts, p.tiles, totals);
-      if (q == 0)
-        embed_scatter_kernel<true><<<tiles, 256, 0, s>>>(tokens, nullptr, nullptr, n, V, pad, shift, p.bits, counts,
-                                                         totals, keys(to), rows(to));
-      else
-        embed_scatter_kernel<false><<<tiles, 256, 0, s>>>(nullptr, keys(at), rows(at), n, V, pad, shift, p.bits, counts,
-                                                          totals, keys(to), rows(to));
-      at = to;
+    launch_pass<true>(p, tokens, nullptr, pairs(0), n, V, pad, 0, counts, totals, owners, s);
+    for (int q = 1; q < p.passes; ++q) {
+      launch_pass<false>(p, nullptr, pairs(at), pairs(1 - at), n, V, pad, q * p.bits, counts, totals, owners, s);
+      at = 1 - at;
     }
-    embed_runs_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(keys(at), n, V, runs);
   }
   int rc = launch_status("embed_grad_sorted sort");
   if (rc != VK_OK) return rc;
   float *part = reinterpret_cast<float *>(ws + p.part);
-  if (d_dtype == VK_DTYPE_F32)
-    launch_sum(p, static_cast<const float *>(d_rows), ld, static_cast<int32_t>(n), V, d, keys(at), rows(at), runs, scale,
-               accumulate, part, out, s);
-  else
-    launch_sum(p, static_cast<const bf16_t *>(d_rows), ld, static_cast<int32_t>(n), V, d, keys(at), rows(at), runs, scale,
-               accumulate, part, out, s);
+  const int64_t waves = p.chunks + (accumulate ? 0 : (static_cast<int64_t>(V) + 63) / 64);
+  if (waves == 0) return VK_OK;
+  const unsigned gx = static_cast<unsigned>((waves + 3) / 4);
+#define VK_EMBED_SUM(T, NQ, PLAIN, CHUNK)                                                                               \
+  embed_sum_kernel<T, NQ, PLAIN, CHUNK>                                                                                 \
+      <<<dim3(gx, static_cast<unsigned>((d + Cols<T, NQ, PLAIN>::SPAN - 1) / Cols<T, NQ, PLAIN>::SPAN)), 256, 0, s>>>(  \
+          static_cast<const T *>(d_rows), ld, static_cast<int32_t>(n), V, d, pairs(at), p.chunks, scale, accumulate,   \
+          part, owners, out)
+#define VK_EMBED_SUM_CHUNK(T, NQ, PLAIN) \
+  do {                                   \
+    if (p.chunk == 16)                   \
+      VK_EMBED_SUM(T, 1, PLAIN, 16);     \
+    else                                 \
+      VK_EMBED_SUM(T, NQ, PLAIN, 64);    \
+  } while (0)
+  const bool plain = !accumulate && d >= 8;
+  if (d_dtype == VK_DTYPE_BF16) {
+    if (plain)
+      VK_EMBED_SUM_CHUNK(bf16_t, 1, true);
+    else
+      VK_EMBED_SUM_CHUNK(bf16_t, 1, false);
+  } else if (d > Cols<float, 1, true>::SPAN) {
+    if (plain)
+      VK_EMBED_SUM_CHUNK(float, 2, true);
+    else
+      VK_EMBED_SUM_CHUNK(float, 2, false);
+  } else {
+    if (plain)
+      VK_EMBED_SUM_CHUNK(float, 1, true);
+    else
+      VK_EMBED_SUM_CHUNK(float, 1, false);
+  }
+#undef VK_EMBED_SUM_CHUNK
+#undef VK_EMBED_SUM
   rc = launch_status("embed_grad_sorted sum");
-  if (rc != VK_OK || p.chunks == 0) return rc;
-  embed_join_kernel<<<dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>((d + 63) / 64)), 256, 0, s>>>(
-      keys(at), runs, static_cast<int32_t>(n), V, d, part, scale, accumulate, out);
+  if (rc != VK_OK || n < 2 * p.chunk) return rc;
+  const int64_t most = (n / (p.chunk + 1) + 1) * ((d + 63) / 64), cap = 4 * device_cus_cached();  // (a long run: chunk + 1 rows)
+  embed_join_kernel<<<static_cast<unsigned>(most < cap ? most : cap), 512, 0, s>>>(pairs(at), d, p.chunk, p.chunks, part, owners, scale,
+                                                                               accumulate, out);
   return launch_status("embed_grad_sorted join");
 }

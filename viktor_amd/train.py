@@ -32,6 +32,9 @@ from . import hip_ops as ops
 from .gspo import sequence_ratio_loss
 
 BF16 = torch.bfloat16
+# The embedding's gradient goes by sorted tokens past this vocabulary. Sorted is the faster way for the 343 ids too (16384
+# rows of 512: 29 against 105 us; 4096 rows of 7 ids: 18 against 19.5 us), but sums in another order: the vocabularies that
+# the slices' sums served before keep them, and with them the bits of their updates.
 SORTED_GRAD_VOCAB = 343
 _LAYER_PARAMS = ("attn_norm.weight", "attn.qkv_proj.weight", "attn.q_norm.weight", "attn.k_norm.weight",
                  "attn.o_proj.weight", "mlp_norm.weight", "gate_up.weight", "down.weight")
