@@ -308,9 +308,10 @@ int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, const int64
  *   mode 2: the first v with u < sum_{w <= v} softmax(z')_w, u = uniforms[b * u_ld] (sums over slices in fp64).
  * token[b] (int64) and logp[b] = log softmax(z')[token] (NULL: not written). NaN is never chosen and weighs nothing, +inf
  * counts as the largest finite value; a row whose mask and bias leave nothing gives `fallback` and -inf.
- * workspace: vk_choose_tokens_workspace() bytes, 16-byte aligned.
+ * workspace: vk_choose_tokens_workspace() bytes for these B, V, hist_cols (0 without a history) and mode, 16-byte aligned;
+ * NULL where that is 0.
  */
-int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t *bytes);
+int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t hist_cols, int32_t mode, int64_t *bytes);
 int vk_choose_tokens(const void *logits, int32_t dtype, int64_t ld, const int64_t *hist, int64_t hist_ld,
                      int64_t hist_cols, const int32_t *hist_len, const float *rep, float rep0, const float *pres,
                      float pres0, const float *freq, float freq0, const float *bias, int64_t bias_ld,
@@ -324,7 +325,9 @@ int vk_choose_tokens(const void *logits, int32_t dtype, int64_t ld, const int64_
  * (vk_choose_tokens) and bookkeeping (vk_select_update's: tail and homopolymer rules, PAD, output column, state). The
  * history is what the sequence has produced, out[b, 0 .. pos[b] - plen[b] - 1]; the mask row is token_rows[tok[b]]
  * ([V] int32, by the previous token). uniforms [B, u_cols] (mode 2) or [B, u_cols, V] (mode 1), row stride u_ld, read at
- * the output column. A row with nothing left takes pad. Other arguments as vk_select_update's and vk_choose_tokens'.
+ * the output column. A row with nothing left takes pad. workspace: vk_choose_tokens_workspace() bytes, hist_cols being
+ * out_cols with penalties (a repetition penalty other than 1, or the others other than 0) and 0 without. Other arguments
+ * as vk_select_update's and vk_choose_tokens'.
  */
 int vk_choose_update(const void *logits, int32_t dtype, int64_t ld, float rep0, float pres0, float freq0,
                      const float *bias, const uint32_t *allowed, int64_t allowed_ld, int64_t n_allowed,

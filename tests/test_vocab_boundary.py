@@ -42,12 +42,14 @@ def test_embedding_workspace_covers_what_the_passes_write():
         assert lib.vk_embed_grad_sorted_workspace(n, V, d, ctypes.byref(b)) == 0
         return b.value
 
-    assert need(0, 7, 1) >= 8 * 7
-    for n in (1, 64, 65, 4096, 4097, 524288):
-        chunks = -(-n // 64) if n > 64 else 0
+    assert need(0, 7, 1) >= 16
+    for n in (1, 31, 32, 64, 65, 4096, 4097, 16384, 16385, 524288, 600000):
+        chunk = 16 if n <= 16384 else 64
+        partials = 8 * -(-n // chunk) if n >= 2 * chunk else 0  # fp32 rows: two slots a chunk
         for V in (1, 343, 87383, 300000):
             for d in (1, 512):
-                assert need(n, V, d) >= (8 if n <= 4096 else 16) * n + 8 * V + 8 * chunks * d
+                # sorted pairs of 8 bytes (two buffers past the counting sort), partial sums, the list of long runs
+                assert need(n, V, d) >= (8 if n <= 4096 else 16) * n + partials * d + 4 * (-(-n // chunk) + 1)
 
 
 def _process(lib, p, **kw):
@@ -83,14 +85,19 @@ def _choose(lib, p, **kw):
 def test_choose_tokens_refuses():
     lib = _lib.load()
     p, _ = _p()
+    big = {"V": 87383, "ld": 87383}  # (needs a workspace)
     for kw, word in (({"token": None}, b"null"), ({"mode": 3}, b"mode"), ({"mode": 1}, b"uniforms"),
                      ({"mode": 1, "uniforms": p, "u_ld": 39}, b"uniforms"), ({"mode": 2, "uniforms": p, "u_ld": 0}, b"uniforms"),
-                     ({"ws": None}, b"workspace"), ({"ws_bytes": 16}, b"workspace"), ({"ws": ctypes.c_void_p(p.value + 4)}, b"workspace")):
+                     ({**big, "ws": None}, b"workspace"), ({**big, "ws_bytes": 16}, b"workspace"),
+                     ({**big, "ws": ctypes.c_void_p(p.value + 4)}, b"workspace")):
         _err(_choose(lib, p, **kw), word)
     assert _choose(lib, p, B=0) == 0
     need = ctypes.c_int64(0)
-    assert lib.vk_choose_tokens_workspace(0, 40, ctypes.byref(need)) == 0 and need.value == 0
-    _err(lib.vk_choose_tokens_workspace(-1, 40, ctypes.byref(need)), b"arguments")
+    assert lib.vk_choose_tokens_workspace(0, 40, 0, 0, ctypes.byref(need)) == 0 and need.value == 0
+    assert lib.vk_choose_tokens_workspace(3, 40, 5, 0, ctypes.byref(need)) == 0 and need.value == 0  # one launch
+    assert lib.vk_choose_tokens_workspace(3, 40, 5, 2, ctypes.byref(need)) == 0 and need.value > 0
+    assert lib.vk_choose_tokens_workspace(3, 87383, 5, 0, ctypes.byref(need)) == 0 and need.value > 0
+    _err(lib.vk_choose_tokens_workspace(-1, 40, 0, 0, ctypes.byref(need)), b"arguments")
 
 
 def test_choose_update_refuses():

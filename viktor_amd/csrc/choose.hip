@@ -29,6 +29,7 @@ namespace vk {
 constexpr int CH_THREADS = 256;
 constexpr int CH_THREADS_ONE = 512;  // of a workgroup that takes a whole row
 constexpr int CH_WHOLE = 1 << 17;    // tokens of such a row at most, where it has more than one slice: 16 KB of LDS bits
+constexpr int CH_SMALL = 32768;      // tokens of a row that one workgroup takes at any batch
 constexpr int CH_SLICE = 8192;       // tokens of a slice at most
 constexpr int CH_HASH_MAX = 2048;    // history columns at most whose counts are hashed: 32 KB of LDS either way
 constexpr int CH_HIST_MAX = 65535;
@@ -794,7 +795,8 @@ static Plan make_plan(int64_t B, int V, int64_t hist_cols, bool whole) {
   int64_t len = (units + s - 1) / s * UNIT;
   p.slices = static_cast<int>((V + len - 1) / len);
   const int64_t rounds = (B + cus - 1) / cus;  // workgroups of the busiest CU, one a sequence
-  if (whole && (p.slices == 1 || (p.hashed && V <= CH_WHOLE && B >= 2 * cus && 20 * B >= 17 * rounds * cus))) {
+  const bool even = V <= CH_WHOLE && B >= 2 * cus && 20 * B >= 17 * rounds * cus;
+  if (whole && (p.slices == 1 || (p.hashed && (V <= CH_SMALL || even)))) {
     constexpr int ONE_UNIT = Batch<float, CH_THREADS_ONE>::TOKENS;
     p.one = true;
     p.slices = 1;
@@ -903,9 +905,12 @@ extern "C" int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, 
   return launch_status("process_logits");
 }
 
-extern "C" int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t *bytes) {
-  VK_CHECK_ARG(bytes && B >= 0 && V > 0, "choose_tokens_workspace: bad arguments");
-  *bytes = B == 0 ? 0 : B * make_plan(B, V, 0, false).slices * static_cast<int64_t>(sizeof(Part));
+// Whether a call of this mode joins slices, or reads them again (inverse CDF), and so needs their results kept.
+static int64_t parts_bytes(const Plan &p, int64_t B) { return p.one ? 0 : B * p.slices * static_cast<int64_t>(sizeof(Part)); }
+
+extern "C" int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t hist_cols, int32_t mode, int64_t *bytes) {
+  VK_CHECK_ARG(bytes && B >= 0 && V > 0 && hist_cols >= 0, "choose_tokens_workspace: bad arguments");
+  *bytes = B == 0 ? 0 : parts_bytes(make_plan(B, V, hist_cols, mode != CH_CDF), B);
   return VK_OK;
 }
 
@@ -922,10 +927,8 @@ static int choose(const void *logits, int32_t dtype, int64_t ld, const Rules &r,
   VK_CHECK_ARG(mode == CH_GREEDY || (noise.u != nullptr && noise.cols > 0 && noise.ld >= noise.cols * per),
                "%s: sampling needs uniforms, rows of columns x %lld", what, static_cast<long long>(per));
   if (B == 0) return VK_OK;
-  int64_t need = 0;
-  rc = vk_choose_tokens_workspace(B, V, &need);
-  if (rc != VK_OK) return rc;
-  VK_CHECK_ARG(workspace && vk_aligned16(workspace) && workspace_bytes >= need,
+  const int64_t need = parts_bytes(make_plan(B, V, r.hist ? r.hist_cols : 0, mode != CH_CDF), B);
+  VK_CHECK_ARG(need == 0 || (workspace && vk_aligned16(workspace) && workspace_bytes >= need),
                "%s: a 16-byte aligned workspace of %lld bytes needed", what, static_cast<long long>(need));
   Part *parts = static_cast<Part *>(workspace);
   return dtype == VK_DTYPE_F32 ? launch_choose<float>(logits, ld, r, temp, temp0, mode, noise, B, V, parts, choice, step,

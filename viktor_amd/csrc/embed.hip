@@ -20,49 +20,51 @@
 
 namespace vk {
 
-constexpr int EL_ROWS = 4;  // rows whose loads a lane has in flight
+constexpr int EL_ROWS = 1;    // rows whose loads a lane has in flight,
+constexpr int EL_GROUPS = 2;  // and groups of columns of each
 
 // LPR lanes share a row (64 / LPR rows per wavefront side by side), N elements each: 16-byte accesses of the narrower
-// type where both are bf16, of the fp32 side otherwise.
+// type where both are bf16, of the fp32 side otherwise. A group of columns that the row's end cuts is moved back to stay
+// inside the row (columns that two lanes hold get the same value); rows narrower than a group go column by column. The
+// rows written are not read again here: past the caches, which keep the table.
 template <typename WT, typename OT, int LPR>
 __global__ __launch_bounds__(256) void embed_lookup_kernel(const WT *__restrict__ w, const int64_t *__restrict__ tokens,
                                                            int64_t n, int64_t V, int d, float scale,
                                                            OT *__restrict__ out) {
-  constexpr int N = sizeof(WT) + sizeof(OT) == 4 ? 8 : 4;
+  constexpr int N = sizeof(WT) + sizeof(OT) == 4 ? 8 : 4, SIDE = 64 / LPR;
   const int lane = threadIdx.x & 63, sub = lane / LPR, c0 = (lane % LPR) * N;
-  constexpr int SIDE = 64 / LPR;
-  const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int64_t r0 = wave * (EL_ROWS * SIDE) + sub;
-  int64_t t[EL_ROWS];
+  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * (EL_ROWS * SIDE) + sub;
+  bool in[EL_ROWS];
+  const WT *src[EL_ROWS];
 #pragma unroll
-  for (int u = 0; u < EL_ROWS; ++u) t[u] = r0 + u * SIDE < n ? tokens[r0 + u * SIDE] : -1;
-  for (int c = c0; c < d; c += LPR * N) {
-    const bool whole = c + N <= d;
-    float v[EL_ROWS][N];
+  for (int u = 0; u < EL_ROWS; ++u) {
+    const int64_t r = r0 + u * SIDE, t = tokens[r < n ? r : n - 1];
+    in[u] = t >= 0 && t < V;
+    src[u] = w + (in[u] ? t : 0) * d;
+  }
+  if (d < N) {
 #pragma unroll
-    for (int u = 0; u < EL_ROWS; ++u) {
-      const bool in = t[u] >= 0 && t[u] < V;
-      const WT *src = w + (in ? t[u] : 0) * d + c;
-      if (whole) {
-        load_row<N>(src, v[u]);
-      } else {
+    for (int u = 0; u < EL_ROWS; ++u)
+      for (int k = c0; k < d && k < c0 + N; ++k)
+        if (r0 + u * SIDE < n) store_one(out + (r0 + u * SIDE) * d + k, in[u] ? load_one(src[u] + k) * scale : 0.f);
+    return;
+  }
+  for (int own = c0; own < d; own += EL_GROUPS * LPR * N) {
+    float v[EL_ROWS][EL_GROUPS][N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[u][k] = c + k < d ? load_one(src + k) : 0.f;
+    for (int u = 0; u < EL_ROWS; ++u)
+#pragma unroll
+      for (int q = 0; q < EL_GROUPS; ++q) load_row<N>(src[u] + min(own + q * LPR * N, d - N), v[u][q]);
+#pragma unroll
+    for (int u = 0; u < EL_ROWS; ++u)
+#pragma unroll
+      for (int q = 0; q < EL_GROUPS; ++q) {
+        const int64_t r = r0 + u * SIDE;
+        if (r >= n || own + q * LPR * N >= d) continue;
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[u][q][k] = in[u] ? v[u][q][k] * scale : 0.f;
+        stream_out<N>(out + r * d + min(own + q * LPR * N, d - N), v[u][q]);
       }
-#pragma unroll
-      for (int k = 0; k < N; ++k) v[u][k] = in ? v[u][k] * scale : 0.f;
-    }
-#pragma unroll
-    for (int u = 0; u < EL_ROWS; ++u) {
-      const int64_t r = r0 + u * SIDE;
-      if (r >= n) continue;
-      OT *dst = out + r * d + c;
-      if (whole) {
-        store_row<N>(dst, v[u]);
-      } else {
-        for (int k = 0; k < N && c + k < d; ++k) store_one(dst + k, v[u][k]);
-      }
-    }
   }
 }
 

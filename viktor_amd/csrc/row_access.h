@@ -64,6 +64,21 @@ __device__ __forceinline__ void stream_row(const float *p, float (&v)[N]) {
     for (int k = 0; k < 4; ++k) v[i + k] = __uint_as_float(a[k]);
   }
 }
+// store_row of data that is not read again soon.
+template <int N>
+__device__ __forceinline__ void stream_out(float *p, const float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4)
+    __builtin_nontemporal_store(f32x4_e{v[i], v[i + 1], v[i + 2], v[i + 3]}, reinterpret_cast<f32x4_e *>(p + i));
+}
+template <int N>
+__device__ __forceinline__ void stream_out(bf16_t *p, const float (&v)[N]) {
+  typedef uint32_t words_e __attribute__((ext_vector_type(N / 2), aligned(2)));
+  words_e o;
+#pragma unroll
+  for (int k = 0; k < N / 2; ++k) o[k] = pack_bf(v[2 * k], v[2 * k + 1]);
+  __builtin_nontemporal_store(o, reinterpret_cast<words_e *>(p));
+}
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
 __device__ __forceinline__ float load_one(const bf16_t *p) { return bf2f(*p); }
 __device__ __forceinline__ void store_one(float *p, float v) { *p = v; }

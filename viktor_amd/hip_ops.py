@@ -861,28 +861,32 @@ def _refuse(what, msg):
     raise AssertionError(f"{what}: {msg}")
 
 
-def _here(what, *ts):
-    """Every tensor on the current device: launches go to its current stream."""
+_Tensor = torch.Tensor
+
+
+def _here(what, ts):
+    """Every tensor among ts on the current device: launches go to its current stream."""
     dev = None
     for t in ts:
-        if isinstance(t, torch.Tensor):
-            if not t.is_cuda:
-                require_device(t, what)
-            if dev is None:
-                dev = torch._C._cuda_getDevice()
-            if t.get_device() != dev:
-                _refuse(what, "tensors on the current device")
+        if isinstance(t, _Tensor):
+            at = t.get_device()
+            if at != dev:
+                if at < 0:
+                    require_device(t, what)
+                if dev is not None or at != torch._C._cuda_getDevice():
+                    _refuse(what, "tensors on the current device")
+                dev = at
 
 
 def _vk_dtype(t):
-    return VK_DTYPE_F32 if t == torch.float32 else VK_DTYPE_BF16
+    return VK_DTYPE_F32 if t is torch.float32 else VK_DTYPE_BF16
 
 
 def _rows_ok(t):
     """[n, d] bf16 or fp32 whose rows are contiguous and do not overlap."""
-    if t.dim() != 2 or t.dtype not in (BF16, torch.float32):
+    if t.dim() != 2 or not (t.dtype is BF16 or t.dtype is torch.float32):
         return False
-    n, d = t.shape
+    n, d = t.size(0), t.size(1)
     return d > 0 and (t.is_contiguous() or ((t.stride(1) == 1 or d == 1) and (n < 2 or t.stride(0) >= d)))
 
 
@@ -890,7 +894,7 @@ def embed_lookup(weight, tokens, scale=1.0, out_dtype=None):
     """scale * weight[tokens]: weight [V, d] bf16 or fp32, tokens int64 of any shape -> [*tokens.shape, d] of out_dtype
     (bf16 or fp32; default: the weight's). The product is fp32, rounded once. Ids outside [0, V) give zero rows.
     Reference: nn.Embedding's gather, viktor/model.py:77."""
-    _here("embed_lookup", weight, tokens)
+    _here("embed_lookup", (weight, tokens))
     wdt = weight.dtype
     odt = out_dtype or wdt
     if weight.dim() != 2 or wdt not in (BF16, torch.float32) or odt not in (BF16, torch.float32) or weight.numel() == 0:
@@ -918,7 +922,7 @@ def embed_grad_sorted(d_rows, tokens, vocab, scale=1.0, pad=None, out=None, accu
     contiguous fp32 [vocab, d]; accumulate: added to what it holds. Reference: the backward of nn.Embedding,
     viktor/decoder.py:127, as viktor/model.py:77 gathers it."""
     what = "embed_grad_sorted"
-    _here(what, d_rows, tokens, out)
+    _here(what, (d_rows, tokens, out))
     if not _rows_ok(d_rows):
         _refuse(what, "d_rows [n, d] bf16 or fp32, rows side by side")
     n, d = d_rows.shape
@@ -950,21 +954,26 @@ def pack_allowed(mask):
     return torch.where(w >= 2 ** 31, w - 2 ** 32, w).to(torch.int32)
 
 
+def _vector(t, n, dtype):
+    """A contiguous [n] of dtype."""
+    return t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()
+
+
 def _per_row(x, B, what, name):
     """A float, or fp32 [B] on the device -> (pointer or None, the float)."""
-    if not isinstance(x, torch.Tensor):
-        return None, float(x)
-    if x.dtype != torch.float32 or x.shape != (B,) or not x.is_contiguous():
-        _refuse(what, f"{name}: a float or fp32 [B]")
-    return x.data_ptr(), 0.0
+    if isinstance(x, _Tensor):
+        if x.dtype is not torch.float32 or x.dim() != 1 or x.numel() != B or not x.is_contiguous():
+            _refuse(what, f"{name}: a float or fp32 [B]")
+        return x.data_ptr(), 0.0
+    return None, float(x)
 
 
 def _mask_args(allowed, V, what):
     if allowed is None:
         return None, 0, 0
-    if allowed.dim() != 2 or allowed.dtype != torch.int32 or not allowed.is_contiguous():
+    if allowed.dim() != 2 or allowed.dtype is not torch.int32 or not allowed.is_contiguous():
         _refuse(what, "allowed int32 [S, ceil(V / 32)]")
-    S, words = allowed.shape
+    S, words = allowed.size(0), allowed.size(1)
     if S == 0 or words < (V + 31) // 32:
         _refuse(what, "allowed int32 [S, ceil(V / 32)]")
     return allowed.data_ptr(), words, S
@@ -972,10 +981,10 @@ def _mask_args(allowed, V, what):
 
 def _logit_rules(what, logits, history, lengths, repetition, presence, frequency, bias, allowed, allowed_rows):
     """B, V and the checked arguments of the rules, in the C entry points' order."""
-    _here(what, logits, history, lengths, repetition, presence, frequency, bias, allowed, allowed_rows)
+    _here(what, (logits, history, lengths, repetition, presence, frequency, bias, allowed, allowed_rows))
     if not _rows_ok(logits):
         _refuse(what, "logits [B, V] bf16 or fp32, rows side by side")
-    B, V = logits.shape
+    B, V = logits.size(0), logits.size(1)
     rep = _per_row(repetition, B, what, "repetition")
     pres = _per_row(presence, B, what, "presence")
     freq = _per_row(frequency, B, what, "frequency")
@@ -986,25 +995,27 @@ def _logit_rules(what, logits, history, lengths, repetition, presence, frequency
         if lengths is not None or rep != (None, 1.0) or pres != (None, 0.0) or freq != (None, 0.0):
             _refuse(what, "penalties need the history and its lengths")
     else:
-        if history.dim() != 2 or history.dtype != torch.long or history.shape[0] != B:
+        if history.dim() != 2 or history.dtype is not torch.long or history.size(0) != B:
             _refuse(what, "history int64 [B, T]")
-        T = history.shape[1]
+        T = history.size(1)
         if not history.is_contiguous() and ((T > 1 and history.stride(1) != 1) or (B > 1 and history.stride(0) < T)):
             _refuse(what, "history rows side by side")
-        if lengths is None or lengths.shape != (B,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+        if lengths is None or not _vector(lengths, B, torch.int32):
             _refuse(what, "lengths int32 [B]")
         if T > 0:
             hist = (history.data_ptr(), max(history.stride(0), T), T, lengths.data_ptr())
     bp, bld = None, 0
     if bias is not None:
-        if bias.dtype != torch.float32 or bias.shape not in ((V,), (B, V)):
-            _refuse(what, "bias fp32 [V] or [B, V]")
-        if not bias.is_contiguous() and ((V > 1 and bias.stride(-1) != 1) or (bias.dim() == 2 and B > 1 and bias.stride(0) < V)):
-            _refuse(what, "bias rows side by side")
-        bp, bld = bias.data_ptr(), 0 if bias.dim() == 1 else max(bias.stride(0), V)
+        if not _vector(bias, V, torch.float32):
+            if bias.dtype is not torch.float32 or bias.shape not in ((V,), (B, V)):
+                _refuse(what, "bias fp32 [V] or [B, V]")
+            if (V > 1 and bias.stride(-1) != 1) or (bias.dim() == 2 and B > 1 and bias.stride(0) < V):
+                _refuse(what, "bias rows side by side")
+            bld = 0 if bias.dim() == 1 else max(bias.stride(0), V)
+        bp = bias.data_ptr()
     ap, words, S = _mask_args(allowed, V, what)
     if allowed_rows is not None:
-        if allowed is None or allowed_rows.shape != (B,) or allowed_rows.dtype != torch.int32 or not allowed_rows.is_contiguous():
+        if allowed is None or not _vector(allowed_rows, B, torch.int32):
             _refuse(what, "allowed_rows int32 [B], with allowed")
     elif allowed is not None and S not in (1, B):
         _refuse(what, "allowed without allowed_rows has 1 row or one per sequence")
@@ -1030,7 +1041,7 @@ def process_logits(logits, history=None, lengths=None, repetition=1.0, presence=
             _refuse("process_logits", "out bf16 or fp32")
         out = torch.empty((B, V), dtype=odt, device=logits.device)
     else:
-        _here("process_logits", out)
+        _here("process_logits", (out,))
         if out.shape != (B, V) or not _rows_ok(out) or (out_dtype is not None and out.dtype != out_dtype):
             _refuse("process_logits", "out [B, V] bf16 or fp32, rows side by side")
     call("vk_process_logits", *args, out.data_ptr(), _vk_dtype(out.dtype), max(out.stride(0), V), B, V, stream_handle())
@@ -1041,10 +1052,10 @@ _MODE_GREEDY, _MODE_GUMBEL, _MODE_CDF = 0, 1, 2
 
 
 @functools.lru_cache(maxsize=256)
-def _choose_workspace(B, V):
+def _choose_workspace(B, V, hist_cols, mode):
     nb = ctypes.c_int64(0)
-    call("vk_choose_tokens_workspace", B, V, ctypes.byref(nb))
-    return max(nb.value, 16)
+    call("vk_choose_tokens_workspace", B, V, hist_cols, mode, ctypes.byref(nb))
+    return nb.value
 
 
 def choose_tokens(logits, history=None, lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,
@@ -1057,31 +1068,29 @@ def choose_tokens(logits, history=None, lengths=None, repetition=1.0, presence=0
     counts as the largest finite value; a row with nothing left gives `fallback` and -inf."""
     B, V, args = _logit_rules("choose_tokens", logits, history, lengths, repetition, presence, frequency, bias, allowed,
                               allowed_rows)
-    _here("choose_tokens", temperature, uniforms)
+    _here("choose_tokens", (temperature, uniforms))
     temp = _per_row(temperature, B, "choose_tokens", "temperature")
     mode, up, uld = _MODE_GREEDY, None, 0
     if uniforms is None:
         if temp[0] is not None or temp[1] > 0:
             _refuse("choose_tokens", "a temperature needs uniforms")
     else:
-        if uniforms.dtype != torch.float32 or uniforms.shape not in ((B,), (B, V)):
-            _refuse("choose_tokens", "uniforms fp32 [B] or [B, V]")
         if uniforms.dim() == 2:
-            if not _rows_ok(uniforms):
-                _refuse("choose_tokens", "uniform rows side by side")
+            if uniforms.dtype is not torch.float32 or not _rows_ok(uniforms) or uniforms.shape != (B, V):
+                _refuse("choose_tokens", "uniforms fp32 [B] or [B, V], rows side by side")
             mode, uld = _MODE_GUMBEL, max(uniforms.stride(0), V)
         else:
-            if not uniforms.is_contiguous():
-                _refuse("choose_tokens", "contiguous uniforms")
+            if not _vector(uniforms, B, torch.float32):
+                _refuse("choose_tokens", "uniforms fp32 [B] or [B, V], rows side by side")
             mode, uld = _MODE_CDF, 1
         up = uniforms.data_ptr()
     dev = logits.device
     token = torch.empty(B, dtype=torch.long, device=dev)
     logp = torch.empty(B, dtype=torch.float32, device=dev)
-    nb = _choose_workspace(B, V)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    call("vk_choose_tokens", *args, *temp, mode, up, uld, int(fallback), token.data_ptr(), logp.data_ptr(), B, V,
-         ws.data_ptr(), nb, stream_handle())
+    nb = _choose_workspace(B, V, args[5], mode)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    call("vk_choose_tokens", *args, *temp, mode, up, uld, int(fallback), token.data_ptr(), logp.data_ptr(), B, V, ptr(ws), nb,
+         stream_handle())
     return token, logp
 
 
@@ -1094,8 +1103,8 @@ def choose_update(logits, bias, is_tail, is_homo, homo_stop, tok, run, pos, plen
     [B, T], or [B, T, V] with gumbel, read at the output column. The bookkeeping and the other arguments are
     select_update's; a sequence with nothing left takes pad."""
     what = "choose_update"
-    _here(what, logits, bias, is_tail, is_homo, tok, run, pos, plen, rope_off, out, pos32, seqlens, rpos32, uniforms,
-          logp_out, cache_base, allowed, token_rows)
+    _here(what, (logits, bias, is_tail, is_homo, tok, run, pos, plen, rope_off, out, pos32, seqlens, rpos32, uniforms,
+                 logp_out, cache_base, allowed, token_rows))
     if not _rows_ok(logits):
         _refuse(what, "logits [B, V] bf16 or fp32, rows side by side")
     B, V = logits.shape
@@ -1130,13 +1139,14 @@ def choose_update(logits, bias, is_tail, is_homo, homo_stop, tok, run, pos, plen
     if (allowed is None) != (token_rows is None) or (token_rows is not None and (
             token_rows.dtype != torch.int32 or token_rows.shape != (V,) or not token_rows.is_contiguous())):
         _refuse(what, "allowed goes with token_rows int32 [V]")
-    nb = _choose_workspace(B, V)
-    ws = torch.empty(nb, dtype=torch.uint8, device=logits.device)
+    cols = out.shape[1] if (repetition, presence, frequency) != (1.0, 0.0, 0.0) else 0
+    nb = _choose_workspace(B, V, cols, mode)
+    ws = torch.empty(nb, dtype=torch.uint8, device=logits.device) if nb else None
     call("vk_choose_update", logits.data_ptr(), _vk_dtype(logits.dtype), max(logits.stride(0), V), float(repetition),
          float(presence), float(frequency), bias.data_ptr(), *mask, ptr(token_rows), is_tail.data_ptr(), is_homo.data_ptr(),
          int(homo_stop), float(temperature), mode, ptr(uniforms) if mode else None, us, uc, tok.data_ptr(), ptr(run),
          pos.data_ptr(), ptr(plen), ptr(rope_off), ptr(cache_base), out.data_ptr(), out.stride(0), out.shape[1], ptr(pos32),
-         ptr(seqlens), ptr(rpos32), ptr(logp_out), lp_stride, B, V, int(eos), int(pad), ws.data_ptr(), nb, stream_handle())
+         ptr(seqlens), ptr(rpos32), ptr(logp_out), lp_stride, B, V, int(eos), int(pad), ptr(ws), nb, stream_handle())
 
 
 def _norm_blocks(n):
