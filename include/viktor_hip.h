@@ -301,10 +301,11 @@ int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, const int64
 
 /*
  * The token choice over a vocabulary of any size after the rules of vk_process_logits (z, in fp32; nothing of it is
- * written). temp [B] fp32, or NULL for temp0; z' = z / T where T > 0, else z' = z and the choice is greedy.
+ * written). temp [B] fp32, or NULL for temp0; z' = z / T where T > 0 (an infinite T
+ * is the largest finite one), else z' = z and the choice is greedy.
  *   mode 0: the first index of max z';
  *   mode 1: the first index of max z'_v - log(-log(max(u_v, 1e-20))), u_v = uniforms[b * u_ld + v] (scores closer than
- *           fp32 can tell are compared in fp64);
+ *           fp32 can tell, and those past its range, are compared in fp64);
  *   mode 2: the first v with u < sum_{w <= v} softmax(z')_w, u = uniforms[b * u_ld] (sums over slices in fp64).
  * token[b] (int64) and logp[b] = log softmax(z')[token] (NULL: not written). NaN is never chosen and weighs nothing, +inf
  * counts as the largest finite value; a row whose mask and bias leave nothing gives `fallback` and -inf.
@@ -504,7 +505,7 @@ int vk_embed_grad(const void *d_rows, int32_t d_dtype, int64_t ld, const int64_t
 
 /*
  * out[r, :] = scale * w[tokens[r], :] (product in fp32, one rounding; w [V, d] and out [n, d] bf16 or fp32, contiguous,
- * any width). Ids outside [0, V) give zero rows. The lookup of nn.Embedding (viktor/decoder.py:127, viktor/model.py:77).
+ * any width up to 2^20). Ids outside [0, V) give zero rows. The lookup of nn.Embedding (viktor/decoder.py:127, viktor/model.py:77).
  */
 int vk_embed_lookup(const void *w, int32_t w_dtype, const int64_t *tokens, int64_t n, int64_t V, int32_t d, float scale,
                     void *out, int32_t out_dtype, void *stream);
@@ -513,7 +514,7 @@ int vk_embed_lookup(const void *w, int32_t w_dtype, const int64_t *tokens, int64
  * vk_embed_grad for large vocabularies, by sorted tokens: out[v, :] = scale * sum over tokens[r] == v of d_rows[r, :]
  * (+ the old out[v, :] with accumulate != 0), fp32 sums in an order that n, V and the ids alone decide. d_rows [n, d] bf16
  * or fp32, row stride ld, any width; ids outside [0, V) and rows of the id `pad` (negative: none) add nothing; a row
- * without ids is zero (accumulate: left as it is). n < 2^31 - 2048; workspace: vk_embed_grad_sorted_workspace() bytes,
+ * without ids is zero (accumulate: left as it is). n < 2^31 - 4096, d <= 2^20; workspace: vk_embed_grad_sorted_workspace() bytes,
  * 16-byte aligned.
  */
 int vk_embed_grad_sorted_workspace(int64_t n, int32_t V, int32_t d, int64_t *bytes);

@@ -22,10 +22,12 @@ def test_embedding_entry_points_refuse():
     lib = _lib.load()
     p, _ = _p()
     _err(lib.vk_embed_lookup(p, 0, p, 4, 0, 8, 1.0, p, 0, None), b"sizes")
+    _err(lib.vk_embed_lookup(p, 0, p, 4, 9, 2 ** 20 + 1, 1.0, p, 0, None), b"sizes")
     _err(lib.vk_embed_lookup(None, 0, p, 4, 9, 8, 1.0, p, 0, None), b"null")
     _err(lib.vk_embed_lookup(p, 2, p, 4, 9, 8, 1.0, p, 0, None), b"dtype")
     need = ctypes.c_int64(0)
     _err(lib.vk_embed_grad_sorted_workspace(2 ** 31, 9, 8, ctypes.byref(need)), b"rows")
+    _err(lib.vk_embed_grad_sorted_workspace(4, 9, 2 ** 20 + 1, ctypes.byref(need)), b"arguments")
     assert lib.vk_embed_grad_sorted_workspace(10000, 5463, 64, ctypes.byref(need)) == 0
     _err(lib.vk_embed_grad_sorted(p, 1, 64, p, 10000, 5463, 64, 1.0, -1, p, 0, p, need.value - 1, None), b"workspace")
     _err(lib.vk_embed_grad_sorted(p, 1, 63, p, 10000, 5463, 64, 1.0, -1, p, 0, p, need.value, None), b"sizes")
@@ -43,8 +45,8 @@ def test_embedding_workspace_covers_what_the_passes_write():
         return b.value
 
     assert need(0, 7, 1) >= 16
-    for n in (1, 31, 32, 64, 65, 4096, 4097, 16384, 16385, 524288, 600000):
-        chunk = 16 if n <= 16384 else 64
+    for n in (1, 31, 32, 64, 65, 4096, 4097, 16384, 16385, 131072, 131073, 524288, 600000):
+        chunk = 16 if n <= 16384 else 32 if n <= 131072 else 64
         partials = 8 * -(-n // chunk) if n >= 2 * chunk else 0  # fp32 rows: two slots a chunk
         for V in (1, 343, 87383, 300000):
             for d in (1, 512):
@@ -69,7 +71,8 @@ def test_process_logits_refuses():
                      ({"hist_len": None}, b"lengths"), ({"hist_cols": 65536, "hist_ld": 65536}, b"65535"), ({"hist_ld": 4}, b"65535"),
                      ({"rep0": 0.0}, b"positive"), ({"rep0": float("nan")}, b"positive"), ({"bias": q, "bias_ld": 7}, b"bias"),
                      ({"allowed": q, "allowed_ld": 1, "n_allowed": 1}, b"words"), ({"allowed": q, "allowed_ld": 2, "n_allowed": 0}, b"words"),
-                     ({"allowed": q, "allowed_ld": 2, "n_allowed": 2}, b"row numbers"), ({"B": 2 ** 20}, b"sequences")):
+                     ({"allowed": q, "allowed_ld": 2, "n_allowed": 2}, b"row numbers"), ({"B": 2 ** 20}, b"sequences"), ({"V": 2 ** 30 + 1, "ld": 2 ** 31}, b"sizes"),
+                     ({"B": 2 ** 19, "V": 2 ** 20, "ld": 2 ** 20, "out_ld": 2 ** 20}, b"too many")):
         _err(_process(lib, p, **kw), word)
     assert _process(lib, p, B=0) == 0
 
@@ -88,6 +91,7 @@ def test_choose_tokens_refuses():
     big = {"V": 87383, "ld": 87383}  # (needs a workspace)
     for kw, word in (({"token": None}, b"null"), ({"mode": 3}, b"mode"), ({"mode": 1}, b"uniforms"),
                      ({"mode": 1, "uniforms": p, "u_ld": 39}, b"uniforms"), ({"mode": 2, "uniforms": p, "u_ld": 0}, b"uniforms"),
+                     ({"B": 2 ** 19, "V": 2 ** 20, "ld": 2 ** 20}, b"too many"), ({"V": 2 ** 30 + 1, "ld": 2 ** 31}, b"sizes"),
                      ({**big, "ws": None}, b"workspace"), ({**big, "ws_bytes": 16}, b"workspace"),
                      ({**big, "ws": ctypes.c_void_p(p.value + 4)}, b"workspace")):
         _err(_choose(lib, p, **kw), word)
@@ -98,6 +102,7 @@ def test_choose_tokens_refuses():
     assert lib.vk_choose_tokens_workspace(3, 40, 5, 2, ctypes.byref(need)) == 0 and need.value > 0
     assert lib.vk_choose_tokens_workspace(3, 87383, 5, 0, ctypes.byref(need)) == 0 and need.value > 0
     _err(lib.vk_choose_tokens_workspace(-1, 40, 0, 0, ctypes.byref(need)), b"arguments")
+    _err(lib.vk_choose_tokens_workspace(1, 2 ** 31 - 1, 0, 0, ctypes.byref(need)), b"arguments")
 
 
 def test_choose_update_refuses():

@@ -55,11 +55,24 @@ def test_embed_lookup_shapes():
     assert ops.embed_lookup(w.to(DEV), tok[:0].to(DEV)).shape == (0, 5, 512)
 
 
+def test_embed_lookup_of_more_rows_than_a_launch():
+    """2^24 workgroups of 16 rows and some: the rows behind the first launch, and those around its end."""
+    n, V = 2 ** 28 + 37, 343
+    w = torch.randn(V, 1, generator=_gen(1)).to(BF).to(DEV)
+    tok = torch.arange(n, device=DEV) % (V + 1)  # (one id past the table)
+    got = ops.embed_lookup(w, tok).view(-1)
+    for a in range(0, n, 2 ** 26):
+        t = tok[a:a + 2 ** 26]
+        assert torch.equal(got[a:a + 2 ** 26], torch.where(t < V, w[:, 0][t.clamp(max=V - 1)], 0.0)), a
+
+
 # ---- gradient --------------------------------------------------------------------------------------------------------------
 
 def _grad_ref(rows, tok, V, scale, pad=None):
-    """(fp64 gradient, what an element may be off by, in units of U): a run's sum is at most 127 additions in a chunk and the
-    next; a longer one's 64 in each chunk, its chunks' sums over 32 groups, and the groups; then one product."""
+    """(fp64 gradient, what an element may be off by, in units of U): a run's sum is at most 127 additions in a chunk (of up
+    to 64 positions) and the next; a longer one's 64 in each chunk, its chunks' sums over 32 groups, and the groups; then one
+    product. Chunks of 16 (n <= 16384) and 32 (n <= 131072) have fewer additions each and no more in all:
+    16 + 16384 / 512 + 32 and 32 + 131072 / 1024 + 32 are below 127 and 127 + 131072 / 2048."""
     keep = (tok >= 0) & (tok < V) & (tok != (-1 if pad is None else pad))
     out = torch.zeros(V, rows.shape[1], dtype=torch.float64)
     mag = torch.zeros_like(out)
@@ -163,6 +176,27 @@ def test_embed_grad_sorted_run_lengths(lens, ignored):
         tok = tok[torch.randperm(len(tok), generator=g)]
         rows = torch.randn(len(tok), 260, generator=g)
         _check_grad(ops.embed_grad_sorted(rows.to(DEV), tok.to(DEV), V), _grad_ref(rows, tok, V, 1.0), more)
+
+
+@pytest.mark.parametrize("chunk,n", [(16, 2000), (16, 16384), (32, 16385), (32, 131072), (64, 131073)])
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_embed_grad_sorted_run_borders(chunk, n, dt):
+    """Runs that end and start at, before and behind the borders of chunks of each size, among runs of a few rows, the last
+    chunk's included; added to a table too."""
+    c = chunk
+    g = _gen(n)
+    V, d = 3 * n // 4, 12
+    for lens in ((c, c, c), (c - 1, c + 1, c), (1, c, 2 * c - 1, 1), (c, 2 * c, c), (c + 1, c - 1, 3 * c + 8, 5), (2 * c + 2, 1, 1, 3 * c - 2),
+                 (c - 1, 2 * c + 1, c - 1, 2 * c + 1, 1), (40 * c + 3,), (c // 2, 5 * c, c // 2, 5 * c)):
+        ends = torch.cat([torch.full((m,), i, dtype=torch.long) for i, m in enumerate(lens)])
+        tok = torch.cat([ends, V - 1 - ends, torch.randint(20, V - 20, (n - 2 * len(ends),), generator=g)])
+        tok = tok[torch.randperm(n, generator=g)]
+        rows = torch.randn(n, d, generator=g).to(dt)
+        ref = _grad_ref(rows, tok, V, 2.0)
+        _check_grad(ops.embed_grad_sorted(rows.to(DEV), tok.to(DEV), V, scale=2.0), ref, lens)
+        table = torch.ones(V, d, device=DEV)
+        ops.embed_grad_sorted(rows.to(DEV), tok.to(DEV), V, scale=2.0, out=table, accumulate=True)
+        _check_grad(table, (ref[0] + 1, ref[1] + 2 * U * (ref[0].abs() + 1)), lens)
 
 
 def test_embed_grad_sorted_many_tiles():
@@ -473,6 +507,64 @@ def test_choose_tokens_odd_values():
     assert torch.equal(got.cpu()[[0, 2, 3, 4, 5]], tok[[0, 2, 3, 4, 5]]) and got[1] in (17, 4321)
 
 
+def test_choose_tokens_lowest_values_and_extreme_temperatures():
+    """A row of the type's lowest value everywhere, where z / T leaves fp32's range: its tokens are alike, and the first
+    allowed one is taken (noise below fp64's resolution there); the inverse CDF takes any. Tiny temperatures order by z,
+    an infinite one by the noise alone. In one launch, in slices, and with a history among the tokens."""
+    for V in (40, 5000, 40001):
+        low = torch.full((3, V), torch.finfo(F32).min)
+        mask = torch.ones(3, V, dtype=torch.bool)
+        mask[1, :7] = False
+        mask[2] = False
+        u = torch.rand(3, V, generator=_gen(V))
+        hist, n = torch.full((3, 2), 20), torch.full((3,), 2, dtype=torch.int32)
+        logv = np.log([V, V - 7])
+        packed = ops.pack_allowed(mask).to(DEV)
+        for T in (0.5, 1e-30):
+            got, lp = ops.choose_tokens(low.to(DEV), *_dev(hist, n), frequency=1.0, allowed=packed, temperature=T,
+                                        uniforms=u.to(DEV), fallback=-1)
+            assert got.tolist() == [0, 7, -1], (V, T)
+            _check_logp(lp, torch.tensor([-logv[0], -logv[1], -np.inf]), torch.zeros(3))
+            got, lp = ops.choose_tokens(low.to(DEV), allowed=packed, temperature=T, uniforms=u[:, 0].contiguous().to(DEV), fallback=-1)
+            assert 0 <= got[0] and 7 <= got[1] < V and got[2] == -1
+            _check_logp(lp, torch.tensor([-logv[0], -logv[1], -np.inf]), torch.zeros(3))
+        x = torch.randn(3, V, generator=_gen(V + 1))
+        for z in (x, x - 100):  # scores past the range on either side
+            for T in (1e-38, 1e-44):
+                got, lp = ops.choose_tokens(z.to(DEV), allowed=packed, temperature=T, uniforms=u.to(DEV), fallback=-1)
+                want = torch.where(mask, z, torch.tensor(-np.inf)).max(1).indices
+                want[2] = -1
+                assert torch.equal(got.cpu(), want), (V, T)
+                assert lp[:2].tolist() == [0, 0]
+        got, lp = ops.choose_tokens(x.to(DEV), allowed=packed, temperature=float("inf"), uniforms=u.to(DEV), fallback=-1)
+        want = torch.where(mask, u, torch.tensor(-1.0)).max(1).indices
+        want[2] = -1
+        assert torch.equal(got.cpu(), want)
+        _check_logp(lp, torch.tensor([-logv[0], -logv[1], -np.inf]), torch.zeros(3))
+        temps = torch.full((3,), float("inf")).to(DEV)
+        got, lp = ops.choose_tokens(x.to(DEV), allowed=packed, temperature=temps, uniforms=u[:, 0].contiguous().to(DEV), fallback=-1)
+        assert 0 <= got[0] < V and 7 <= got[1] < V and got[2] == -1
+        _check_logp(lp, torch.tensor([-logv[0], -logv[1], -np.inf]), torch.zeros(3))
+
+
+def test_choose_tokens_of_the_widest_whole_rows():
+    """512 rows of 2^17 tokens with the longest hashed history, the largest shared memory of one launch: six rows checked."""
+    B, V, T = 512, 2 ** 17, 2048
+    g = torch.Generator(DEV).manual_seed(1)
+    x = (3 * torch.randn(B, V, generator=g, device=DEV)).to(BF)
+    hist = (torch.rand(B, T, generator=g, device=DEV).pow(3) * V).long().clamp(max=V - 1)
+    lens = torch.full((B,), T, dtype=torch.int32, device=DEV)
+    u = torch.rand(B, V, generator=g, device=DEV)
+    rows = [0, 1, 255, 256, 300, 511]
+    z = _rules_ref(x[rows].cpu(), hist[rows].cpu(), lens[rows].cpu(), 1.25, 0.5, 0.25)
+    for temp in (0.0, 0.75):
+        t = torch.full((B,), temp, device=DEV)
+        tok, lp, big = _choice_ref(z, t[rows].cpu(), u[rows].cpu())
+        got, glp = ops.choose_tokens(x, hist, lens, 1.25, 0.5, 0.25, temperature=t if temp else 0.0, uniforms=u if temp else None)
+        assert torch.equal(got[rows].cpu(), tok)
+        _check_logp(glp[rows], lp, big)
+
+
 # ---- streams, graphs, refusals -----------------------------------------------------------------------------------------------
 
 def test_vocabulary_ops_in_a_graph():
@@ -518,6 +610,56 @@ def test_vocabulary_ops_in_a_graph():
                 assert torch.equal(a, b)
 
 
+def test_vocabulary_ops_side_by_side():
+    """Calls of two streams at once, each with workspaces of its own."""
+    V, d, n, B = 21847, 64, 30000, 40
+    g = torch.Generator(DEV).manual_seed(3)
+    sets = []
+    for _ in range(2):
+        sets.append((torch.randint(0, V, (n,), generator=g, device=DEV), torch.randn(n, d, generator=g, device=DEV),
+                     torch.randn(B, V, generator=g, device=DEV), torch.rand(B, V, generator=g, device=DEV)))
+
+    def call(tok, rows, z, u):
+        return (ops.embed_grad_sorted(rows, tok, V), *ops.choose_tokens(z), *ops.choose_tokens(z, temperature=0.9, uniforms=u),
+                *ops.choose_tokens(z, temperature=0.9, uniforms=u[:, 0].contiguous()))
+
+    want = [call(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(call(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            for a, b in zip(out, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_process_logits_out_beside_logits():
+    """Columns of one buffer as logits and out; views that share elements are refused."""
+    B, V = 5, 1367
+    buf = torch.randn(B, 2 * V + 3, generator=_gen(1)).to(DEV)
+    want = buf[:, :V] + 1
+    bias = torch.ones(V, device=DEV)
+    ops.process_logits(buf[:, :V], bias=bias, out=buf[:, V + 3:])
+    assert torch.equal(buf[:, V + 3:], want)
+    flat = torch.zeros(2 * B * V, device=DEV)
+    z = flat[:B * V].view(B, V)
+    ops.process_logits(z, bias=bias, out=flat[B * V:].view(B, V))
+    assert bool((flat[B * V:] == 1).all()) and not bool(flat[:B * V].any())
+    for out in (buf[:, 1:1 + V], buf[:, V - 1:2 * V - 1]):
+        with pytest.raises(AssertionError):
+            ops.process_logits(buf[:, :V], out=out)
+    for out in (flat[4:4 + B * V].view(B, V), flat[V:V + B * V].view(B, V), flat.view(BF)[2:2 + B * V].view(B, V)):
+        with pytest.raises(AssertionError):
+            ops.process_logits(z, out=out)
+    with pytest.raises(ops._lib.HipLibraryError):
+        ops.process_logits(z, out=flat.view(BF)[:B * V].view(B, V))
+
+
 def test_vocabulary_ops_refuse():
     z = torch.zeros(3, 40, device=DEV)
     h, n = torch.zeros(3, 5, dtype=torch.long, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
@@ -528,7 +670,7 @@ def test_vocabulary_ops_refuse():
         lambda: ops.embed_lookup(w.half(), tok), lambda: ops.embed_lookup(w, tok.int()), lambda: ops.embed_lookup(w.t(), tok),
         lambda: ops.embed_lookup(w, tok, out_dtype=torch.float16),
         lambda: ops.embed_grad_sorted(rows, tok[:5], 40), lambda: ops.embed_grad_sorted(rows.t(), tok, 40),
-        lambda: ops.embed_grad_sorted(rows, tok, 0), lambda: ops.embed_grad_sorted(rows, tok, 40, accumulate=True),
+        lambda: ops.embed_grad_sorted(rows, tok, 0), lambda: ops.embed_grad_sorted(rows, tok, 2 ** 32 + 40), lambda: ops.embed_grad_sorted(rows, tok, 40, accumulate=True),
         lambda: ops.embed_grad_sorted(rows, tok, 40, out=torch.zeros(40, 9, device=DEV)),
         lambda: ops.embed_grad_sorted(rows[:1].expand(6, 8), tok, 40),
         lambda: ops.process_logits(z.half()), lambda: ops.process_logits(z, repetition=1.1),
@@ -538,6 +680,7 @@ def test_vocabulary_ops_refuse():
         lambda: ops.process_logits(z, allowed=m[:, :1]), lambda: ops.process_logits(z, allowed_rows=n),
         lambda: ops.process_logits(z, out=torch.zeros(3, 40, dtype=torch.float16, device=DEV)),
         lambda: ops.process_logits(z[:1].expand(3, 40)),
+        lambda: ops.choose_tokens(torch.empty(1, 2 ** 30 + 1, dtype=BF, device=DEV)),
         lambda: ops.choose_tokens(z, temperature=0.5), lambda: ops.choose_tokens(z, temperature=torch.ones(3, device=DEV)),
         lambda: ops.choose_tokens(z, uniforms=torch.zeros(3, 39, device=DEV)),
         lambda: ops.choose_tokens(z, uniforms=torch.zeros(3, 40, dtype=BF, device=DEV)),

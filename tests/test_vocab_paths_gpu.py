@@ -151,7 +151,8 @@ def test_engine_refuses_bad_rules():
             DecodeEngine(m, 2, 8, 16, cuda_graph=False, **kw)
 
 
-@pytest.mark.parametrize("V,d,wt", [(343, 512, torch.float32), (1367, 512, torch.float32), (5463, 64, torch.bfloat16), (50, 30, torch.float32)])
+@pytest.mark.parametrize("V,d,wt", [(343, 512, torch.float32), (1367, 512, torch.float32), (5463, 64, torch.bfloat16), (50, 30, torch.float32),
+                                    (1367, 24, torch.float16)])
 @pytest.mark.parametrize("scale,pad", [(1.0, None), (22.627417, 0)])
 def test_token_embedding(V, d, wt, scale, pad):
     """Forward exact; the gradient within the roundings of fp32 sums (an id's rows in sequence at most, the product, and the

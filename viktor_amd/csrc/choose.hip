@@ -33,6 +33,7 @@ constexpr int CH_SMALL = 32768;      // tokens of a row that one workgroup takes
 constexpr int CH_SLICE = 8192;       // tokens of a slice at most
 constexpr int CH_HASH_MAX = 2048;    // history columns at most whose counts are hashed: 32 KB of LDS either way
 constexpr int CH_HIST_MAX = 65535;
+constexpr int32_t CH_V_MAX = 1 << 30;
 
 struct Rules {
   const int64_t *hist;  // [B, hist_cols], row stride hist_ld; null: no penalties
@@ -52,7 +53,7 @@ struct Rules {
 
 // How a call is cut: slices of `slice` tokens per sequence, and the history's table (Seen).
 struct Plan {
-  int slices, slice, slots;
+  int slices, slice, slots, listed;
   bool hashed, one;
 };
 
@@ -103,16 +104,20 @@ __device__ __forceinline__ RowRules row_rules(const Rules &r, int64_t b, int V) 
 
 // The history's tokens of a slice, in dynamic LDS: a bit per token of the slice, and how often each occurs, in a hash
 // table of `slots` (a power of two, at least twice the history's columns) or, for long histories, by token (slots = slice).
-// Every distinct token is then one slot, whose logit one thread computes; the streaming pass leaves tokens with a bit out.
+// Every distinct token is then one slot, on a list (of at most `listed`, in any order), whose logit one thread computes;
+// the streaming pass leaves tokens with a bit out. Without the list the threads went through all slots, a wait for a
+// logit at nearly every step: 119 us for 512 x 87383 bf16 logits with histories of 2048, and 55 with 256.
 template <int THREADS>
 struct Seen {
-  uint32_t *bits, *count, *key;  // key: null by token
+  uint32_t *bits, *count, *key, *distinct;  // key: null by token
+  uint16_t *list;
   int slots, shift;
   static constexpr uint32_t kEmpty = 0xffffffffu;
 
-  __device__ __forceinline__ Seen(uint32_t *lds, int slice, int slots_, bool hashed)
-      : bits(lds), count(lds + slice / 32), key(hashed ? lds + slice / 32 + slots_ : nullptr), slots(slots_),
-        shift(__clz(slots_) + 1) {}
+  __device__ __forceinline__ Seen(uint32_t *lds, const Plan &p)
+      : bits(lds), count(lds + p.slice / 32), key(p.hashed ? count + p.slots : nullptr),
+        distinct(count + (p.hashed ? 2 : 1) * p.slots), list(reinterpret_cast<uint16_t *>(distinct + 4)), slots(p.slots),
+        shift(__clz(p.slots) + 1) {}
   __device__ __forceinline__ bool has(int rel) const { return (bits[rel >> 5] >> (rel & 31)) & 1; }
   // The slot of a token of the slice; of one that is not there, a new one (at most half of them get used).
   __device__ __forceinline__ int slot(uint32_t rel) const {
@@ -126,18 +131,31 @@ struct Seen {
   }
   // Of tokens v0 .. v1 - 1. Ends with a barrier.
   __device__ __forceinline__ void fill(const int64_t *hist, int len, int v0, int v1, int slice) const {
+    constexpr int U = 4;  // of a thread's tokens in flight, the first ones while the table is cleared
     const int tid = threadIdx.x;
-    const int64_t first = hist[tid < len ? tid : 0];  // in flight while the table is cleared
+    int64_t h[U];
+    auto load = [&](int t0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) h[u] = hist[min(t0 + u * THREADS, len - 1)];
+    };
+    load(tid);
+    if (tid == 0) *distinct = 0;
     for (int i = tid; i < (slice / 32 + slots) / 4; i += THREADS) reinterpret_cast<u32x4 *>(bits)[i] = u32x4{0u, 0u, 0u, 0u};
     if (key != nullptr)
       for (int i = tid; i < slots / 4; i += THREADS)
         reinterpret_cast<u32x4 *>(key)[i] = u32x4{kEmpty, kEmpty, kEmpty, kEmpty};
     __syncthreads();
-    for (int t = tid; t < len; t += THREADS) {
-      const int64_t rel = (t == tid ? first : hist[t]) - v0;
-      if (rel >= 0 && rel < v1 - v0) {
-        atomicAdd(&count[slot(static_cast<uint32_t>(rel))], 1u);
-        atomicOr(&bits[rel >> 5], 1u << (rel & 31));
+    for (int t0 = tid; t0 < len; t0 += U * THREADS) {
+      if (t0 != tid) load(t0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint64_t far = static_cast<uint64_t>(h[u]) - static_cast<uint64_t>(v0);
+        if (t0 + u * THREADS < len && far < static_cast<uint64_t>(v1 - v0)) {
+          const uint32_t rel = static_cast<uint32_t>(far), bit = 1u << (rel & 31);
+          const int at = slot(rel);
+          atomicAdd(&count[at], 1u);
+          if ((atomicOr(&bits[rel >> 5], bit) & bit) == 0) list[atomicAdd(distinct, 1u)] = static_cast<uint16_t>(at);
+        }
       }
     }
     __syncthreads();
@@ -145,8 +163,9 @@ struct Seen {
   // This thread's distinct tokens, as f(token of the slice, its count's place).
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    for (int i = threadIdx.x; i < slots; i += THREADS) {
-      if (key != nullptr ? key[i] != kEmpty : has(i)) f(static_cast<int>(key != nullptr ? key[i] : i), count[i]);
+    for (uint32_t i = threadIdx.x; i < *distinct; i += THREADS) {
+      const int at = list[i];
+      f(static_cast<int>(key != nullptr ? key[at] : at), count[at]);
     }
   }
 };
@@ -274,7 +293,7 @@ __global__ __launch_bounds__(CH_THREADS) void process_logits_kernel(const T *log
   using X = Batch<T, CH_THREADS>;
   const int64_t b = blockIdx.x / plan.slices;
   const int v0 = static_cast<int>(blockIdx.x % plan.slices) * plan.slice, v1 = V - v0 < plan.slice ? V : v0 + plan.slice;
-  const Seen<CH_THREADS> seen(lds, plan.slice, plan.slots, plan.hashed);
+  const Seen<CH_THREADS> seen(lds, plan);
   const T *row = logits + b * ld;
   OT *dst = out + b * out_ld;
   X x;
@@ -308,24 +327,32 @@ struct Part {
   int32_t v;
 };
 
+// A thread's offer for the workgroup's best token.
+struct Best {
+  float s, z, u;
+  int32_t v;
+};
+
 __device__ __forceinline__ Part no_part() { return {-FLT_MAX, 0.f, -INFINITY, -INFINITY, 0.f, -1}; }
 
 // How far the fp32 score of a token can be from the exact one: the roundings of z' and of the sum (1.2e-7 of its size
 // each), and of the two logarithms.
 __device__ __forceinline__ float score_slack(float s) { return 1e-5f + 1e-6f * fabsf(s); }
 
-// The exact score: z' rounded to fp32, the noise in 64 bits.
+// The exact score: z' rounded to fp32 unless that overflows, the noise in 64 bits.
 __device__ __forceinline__ double exact_score(float z, float u, float T) {
-  return static_cast<double>(z / T) - log(-log(fmax(static_cast<double>(u), 1e-20)));
+  const float q = z / T;
+  return (fabsf(q) <= FLT_MAX ? static_cast<double>(q) : static_cast<double>(z) / T) - log(-log(fmax(static_cast<double>(u), 1e-20)));
 }
 
 struct Scale {
-  float T, inv, L;  // the temperature, 1 / T (1 for a greedy row) kept finite, and log2(e) / T
+  float T, inv, L;  // the temperature, 1 / T (1 for a greedy row) and log2(e) / T, all kept finite
 };
 
 __device__ __forceinline__ Scale row_scale(const float *temp, float temp0, int64_t b) {
   Scale c;
   c.T = temp ? temp[b] : temp0;
+  if (c.T > FLT_MAX) c.T = FLT_MAX;  // (an infinite one: -inf would become a NaN)
   c.inv = c.T > 0.f ? fminf(1.f / c.T, 0.5f * FLT_MAX) : 1.f;
   c.L = fminf(c.inv * 1.44269504f, 0.5f * FLT_MAX);
   return c;
@@ -481,8 +508,9 @@ struct Uniforms {
 };
 
 template <typename T, int THREADS, bool GUMBEL, bool CUT, bool MORE>
-__device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, THREADS, GUMBEL> &un, Mine &t, const T *row, const float *urow, const RowRules &r,
-                                             const Scale &c, const Seen<THREADS> &s, int v0, int w, int V) {
+__device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, THREADS, GUMBEL> &un, Mine &t, const T *row,
+                                             const float *urow, const RowRules &r, const Scale &c, const Seen<THREADS> &s,
+                                             int v0, int w, int V) {
   using X = Batch<T, THREADS>;
   const bool noisy = GUMBEL && c.T > 0.f;
   float z[X::R][X::N], u[GUMBEL ? X::R : 1][X::N];
@@ -547,7 +575,7 @@ __device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, T
 // One slice of one sequence, or with ONE the whole vocabulary and the step's end. The workgroup's best logit or score
 // tells who can have the best token: the lowest token of the largest logit, or the threads within the scores' slack of
 // the largest score. These read their token again and are compared exactly; one whose second score is as near goes
-// through all of its tokens. The sum is taken at the workgroup's maximum.
+// through all of its tokens, and so does every thread where all scores are below fp32's range. The sum is taken at the workgroup's maximum.
 template <typename T, int THREADS, bool GUMBEL, bool ONE>
 __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restrict__ logits, int64_t ld, Rules rules,
                                                                    const float *__restrict__ temp, float temp0,
@@ -557,13 +585,13 @@ __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restr
   constexpr int WAVES = THREADS / 64;
   __shared__ float red_m[WAVES], red_s[WAVES], red_sum[WAVES];
   __shared__ int first_best, contenders;
-  __shared__ Part contender[GUMBEL ? THREADS : 1];
+  __shared__ Best contender[GUMBEL ? THREADS : 1];
   using X = Batch<T, THREADS>;
   const int64_t b = ONE ? blockIdx.x : blockIdx.x / plan.slices;
   const int v0 = ONE ? 0 : static_cast<int>(blockIdx.x % plan.slices) * plan.slice;
   const int v1 = V - v0 < plan.slice ? V : v0 + plan.slice;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const Seen<THREADS> seen(lds, plan.slice, plan.slots, plan.hashed);
+  const Seen<THREADS> seen(lds, plan);
   const T *row = logits + b * ld;
   X x;
   if (V >= X::N) x.load(row, v0, V);
@@ -616,10 +644,11 @@ __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restr
   }
   const float ws = wave_sum(t.sum * __builtin_amdgcn_exp2f((t.m - M) * c.L));
   if (lane == 0) red_sum[wid] = ws;
-  if (most > -INFINITY) {
-    if (!noisy) {
-      if (t.best == most) atomicMin(&first_best, t.v);
-    } else if (t.best > -INFINITY && (t.best == most || most - t.best <= 2.5f * score_slack(most))) {
+  if (!noisy) {
+    if (most > -INFINITY && t.best == most) atomicMin(&first_best, t.v);
+  } else {
+    const bool below = most == -INFINITY;  // (t.sum > 0: some logit is finite)
+    if (below ? t.sum > 0.f : t.best > -INFINITY && (t.best == most || most - t.best <= 2.5f * score_slack(most))) {
       Part p = no_part();
       auto offer = [&](int v) {
         Part e = no_part();
@@ -629,7 +658,7 @@ __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restr
         e.v = e.z == -INFINITY ? -1 : v;
         if (better<true>(p, e, c.T)) p = e;
       };
-      if (t.second == most || most - t.second <= 2.5f * score_slack(most)) {
+      if (below || t.second == most || most - t.second <= 2.5f * score_slack(most)) {
         for (int i = v0; i < v1; i += X::STEP)
           for (int k = 0; k < X::N; ++k) {
             const int v = i + tid * X::N + k;
@@ -639,15 +668,18 @@ __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restr
       } else {
         offer(t.v);
       }
-      contender[atomicAdd(&contenders, 1)] = p;
+      contender[atomicAdd(&contenders, 1)] = Best{p.s, p.z, p.u, p.v};
     }
   }
   __syncthreads();
   if (tid != 0) return;
   Part p = no_part();
   if (noisy) {
-    for (int i = 0; i < contenders; ++i)
-      if (better<true>(p, contender[i], c.T)) p = contender[i];
+    for (int i = 0; i < contenders; ++i) {
+      const Best e = contender[i];
+      const Part q = {-FLT_MAX, 0.f, e.s, e.z, e.u, e.v};
+      if (better<true>(p, q, c.T)) p = q;
+    }
   } else if (most > -INFINITY) {
     p.z = most;
     p.v = first_best;
@@ -726,7 +758,7 @@ __global__ __launch_bounds__(CH_THREADS) void choose_cdf_kernel(const T *__restr
     last = -1;
   }
   __syncthreads();
-  const Seen<CH_THREADS> seen(lds, slice, plan.slots, plan.hashed);
+  const Seen<CH_THREADS> seen(lds, plan);
   const T *row = logits + b * ld;
   if (r.len > 0) seen.fill(r.hist, r.len, v0, v1, slice);
   for (int w0 = v0; w0 < v1; w0 += X::STEP) {
@@ -795,7 +827,7 @@ static Plan make_plan(int64_t B, int V, int64_t hist_cols, bool whole) {
   int64_t len = (units + s - 1) / s * UNIT;
   p.slices = static_cast<int>((V + len - 1) / len);
   const int64_t rounds = (B + cus - 1) / cus;  // workgroups of the busiest CU, one a sequence
-  const bool even = V <= CH_WHOLE && B >= 2 * cus && 20 * B >= 17 * rounds * cus;
+  const bool even = V <= CH_WHOLE && 4 * B >= 3 * rounds * cus;
   if (whole && (p.slices == 1 || (p.hashed && (V <= CH_SMALL || even)))) {
     constexpr int ONE_UNIT = Batch<float, CH_THREADS_ONE>::TOKENS;
     p.one = true;
@@ -806,11 +838,20 @@ static Plan make_plan(int64_t B, int V, int64_t hist_cols, bool whole) {
   p.slots = p.slice;
   if (p.hashed)
     for (p.slots = 64; p.slots < 2 * hist_cols;) p.slots *= 2;
+  p.listed = (static_cast<int>(hist_cols < p.slice ? hist_cols : p.slice) + 7) & ~7;
   return p;
 }
 
 static size_t plan_lds(const Plan &p, bool hist) {
-  return hist ? static_cast<size_t>(p.slice) / 8 + static_cast<size_t>(p.slots) * (p.hashed ? 8 : 4) : 0;
+  return hist ? static_cast<size_t>(p.slice) / 8 + static_cast<size_t>(p.slots) * (p.hashed ? 8 : 4) + 16 + 2 * p.listed : 0;
+}
+
+// Workgroups of 256 threads that one launch may have (2^32 threads in all).
+constexpr int64_t CH_GRID_MAX = int64_t(1) << 24;
+
+static int check_grid(const Plan &p, int64_t B, const char *what) {
+  VK_CHECK_ARG(B * p.slices < CH_GRID_MAX, "%s: too many logits for one call", what);
+  return VK_OK;
 }
 
 static int check_rules(const Rules &r, int64_t B, int V, const char *what) {
@@ -827,7 +868,7 @@ static int check_rules(const Rules &r, int64_t B, int V, const char *what) {
 }
 
 static int check_logits(const void *logits, int32_t dtype, int64_t ld, int64_t B, int32_t V, const char *what) {
-  VK_CHECK_ARG(B >= 0 && V > 0 && V <= (int32_t(1) << 30) && ld >= V, "%s: bad sizes", what);
+  VK_CHECK_ARG(B >= 0 && V > 0 && V <= CH_V_MAX && ld >= V, "%s: bad sizes", what);
   VK_CHECK_ARG(B < (int64_t(1) << 20), "%s: at most 2^20 - 1 sequences", what);
   VK_CHECK_ARG(dtype == VK_DTYPE_BF16 || dtype == VK_DTYPE_F32, "%s: logits bf16 or fp32", what);
   VK_CHECK_ARG(B == 0 || logits != nullptr, "%s: null pointer", what);
@@ -836,9 +877,8 @@ static int check_logits(const void *logits, int32_t dtype, int64_t ld, int64_t B
 
 template <typename T>
 static int launch_choose(const void *logits, int64_t ld, const Rules &r, const float *temp, float temp0, int mode,
-                         const Noise &noise, int64_t B, int V, Part *parts, const Choice &choice, const Step &step,
-                         hipStream_t s) {
-  const Plan plan = make_plan(B, V, r.hist ? r.hist_cols : 0, mode != CH_CDF);
+                         const Noise &noise, int64_t B, int V, const Plan &plan, Part *parts, const Choice &choice,
+                         const Step &step, hipStream_t s) {
   const T *x = static_cast<const T *>(logits);
   const size_t lds = plan_lds(plan, r.hist != nullptr);
   const unsigned grid = static_cast<unsigned>(B * plan.slices), join = static_cast<unsigned>((B + 3) / 4);
@@ -886,6 +926,8 @@ extern "C" int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, 
   rc = check_rules(r, B, V, "process_logits");
   if (rc != VK_OK || B == 0) return rc;
   const Plan plan = make_plan(B, V, hist ? hist_cols : 0, false);
+  rc = check_grid(plan, B, "process_logits");
+  if (rc != VK_OK) return rc;
   const size_t lds = plan_lds(plan, hist != nullptr);
   const unsigned grid = static_cast<unsigned>(B * plan.slices);
   hipStream_t s = VK_STREAM(stream);
@@ -909,7 +951,7 @@ extern "C" int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, 
 static int64_t parts_bytes(const Plan &p, int64_t B) { return p.one ? 0 : B * p.slices * static_cast<int64_t>(sizeof(Part)); }
 
 extern "C" int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t hist_cols, int32_t mode, int64_t *bytes) {
-  VK_CHECK_ARG(bytes && B >= 0 && V > 0 && hist_cols >= 0, "choose_tokens_workspace: bad arguments");
+  VK_CHECK_ARG(bytes && B >= 0 && V > 0 && V <= CH_V_MAX && hist_cols >= 0, "choose_tokens_workspace: bad arguments");
   *bytes = B == 0 ? 0 : parts_bytes(make_plan(B, V, hist_cols, mode != CH_CDF), B);
   return VK_OK;
 }
@@ -927,14 +969,17 @@ static int choose(const void *logits, int32_t dtype, int64_t ld, const Rules &r,
   VK_CHECK_ARG(mode == CH_GREEDY || (noise.u != nullptr && noise.cols > 0 && noise.ld >= noise.cols * per),
                "%s: sampling needs uniforms, rows of columns x %lld", what, static_cast<long long>(per));
   if (B == 0) return VK_OK;
-  const int64_t need = parts_bytes(make_plan(B, V, r.hist ? r.hist_cols : 0, mode != CH_CDF), B);
+  const Plan plan = make_plan(B, V, r.hist ? r.hist_cols : 0, mode != CH_CDF);
+  rc = check_grid(plan, B, what);
+  if (rc != VK_OK) return rc;
+  const int64_t need = parts_bytes(plan, B);
   VK_CHECK_ARG(need == 0 || (workspace && vk_aligned16(workspace) && workspace_bytes >= need),
                "%s: a 16-byte aligned workspace of %lld bytes needed", what, static_cast<long long>(need));
   Part *parts = static_cast<Part *>(workspace);
-  return dtype == VK_DTYPE_F32 ? launch_choose<float>(logits, ld, r, temp, temp0, mode, noise, B, V, parts, choice, step,
-                                                      VK_STREAM(stream))
-                               : launch_choose<bf16_t>(logits, ld, r, temp, temp0, mode, noise, B, V, parts, choice, step,
-                                                       VK_STREAM(stream));
+  return dtype == VK_DTYPE_F32 ? launch_choose<float>(logits, ld, r, temp, temp0, mode, noise, B, V, plan, parts, choice,
+                                                      step, VK_STREAM(stream))
+                               : launch_choose<bf16_t>(logits, ld, r, temp, temp0, mode, noise, B, V, plan, parts, choice,
+                                                       step, VK_STREAM(stream));
 }
 
 extern "C" int vk_choose_tokens(const void *logits, int32_t dtype, int64_t ld, const int64_t *hist, int64_t hist_ld,

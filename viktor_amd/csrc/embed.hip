@@ -20,8 +20,8 @@
 
 namespace vk {
 
-constexpr int EL_ROWS = 1;    // rows whose loads a lane has in flight,
-constexpr int EL_GROUPS = 2;  // and groups of columns of each
+constexpr int EL_WIDTH_MAX = 1 << 20;                // elements of a row
+constexpr int64_t EL_GRID_MAX = int64_t(1) << 24;  // workgroups of 256 threads: a launch has fewer than 2^32 threads
 
 // LPR lanes share a row (64 / LPR rows per wavefront side by side), N elements each: 16-byte accesses of the narrower
 // type where both are bf16, of the fp32 side otherwise. A group of columns that the row's end cuts is moved back to stay
@@ -32,39 +32,24 @@ __global__ __launch_bounds__(256) void embed_lookup_kernel(const WT *__restrict_
                                                            int64_t n, int64_t V, int d, float scale,
                                                            OT *__restrict__ out) {
   constexpr int N = sizeof(WT) + sizeof(OT) == 4 ? 8 : 4, SIDE = 64 / LPR;
-  const int lane = threadIdx.x & 63, sub = lane / LPR, c0 = (lane % LPR) * N;
-  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * (EL_ROWS * SIDE) + sub;
-  bool in[EL_ROWS];
-  const WT *src[EL_ROWS];
-#pragma unroll
-  for (int u = 0; u < EL_ROWS; ++u) {
-    const int64_t r = r0 + u * SIDE, t = tokens[r < n ? r : n - 1];
-    in[u] = t >= 0 && t < V;
-    src[u] = w + (in[u] ? t : 0) * d;
-  }
+  const int lane = threadIdx.x & 63, c0 = (lane % LPR) * N;
+  const int64_t r = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * SIDE + lane / LPR;
+  if (r >= n) return;
+  const int64_t t = tokens[r];
+  const bool in = t >= 0 && t < V;
+  const WT *src = w + (in ? t : 0) * d;
+  OT *dst = out + r * d;
   if (d < N) {
-#pragma unroll
-    for (int u = 0; u < EL_ROWS; ++u)
-      for (int k = c0; k < d && k < c0 + N; ++k)
-        if (r0 + u * SIDE < n) store_one(out + (r0 + u * SIDE) * d + k, in[u] ? load_one(src[u] + k) * scale : 0.f);
+    for (int k = c0; k < d && k < c0 + N; ++k) store_one(dst + k, in ? load_one(src + k) * scale : 0.f);
     return;
   }
-  for (int own = c0; own < d; own += EL_GROUPS * LPR * N) {
-    float v[EL_ROWS][EL_GROUPS][N];
+  for (int own = c0; own < d; own += LPR * N) {
+    const int c = min(own, d - N);
+    float v[N];
+    load_row<N>(src + c, v);
 #pragma unroll
-    for (int u = 0; u < EL_ROWS; ++u)
-#pragma unroll
-      for (int q = 0; q < EL_GROUPS; ++q) load_row<N>(src[u] + min(own + q * LPR * N, d - N), v[u][q]);
-#pragma unroll
-    for (int u = 0; u < EL_ROWS; ++u)
-#pragma unroll
-      for (int q = 0; q < EL_GROUPS; ++q) {
-        const int64_t r = r0 + u * SIDE;
-        if (r >= n || own + q * LPR * N >= d) continue;
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[u][q][k] = in[u] ? v[u][q][k] * scale : 0.f;
-        stream_out<N>(out + r * d + min(own + q * LPR * N, d - N), v[u][q]);
-      }
+    for (int k = 0; k < N; ++k) v[k] = in ? v[k] * scale : 0.f;
+    stream_out<N>(dst + c, v);
   }
 }
 
@@ -72,11 +57,13 @@ __global__ __launch_bounds__(256) void embed_lookup_kernel(const WT *__restrict_
 
 constexpr int ES_RANK_MAX = 4096;  // rows that the counting sort takes
 constexpr int ES_RANK_ROWS = 16;   // rows per workgroup of it
-constexpr int ES_TILE = 4096;      // keys per workgroup of a radix pass: 4 per thread
+constexpr int ES_SMALL = 131072;   // rows up to which a workgroup of a radix pass takes 1024 keys; more: 2048
 constexpr int ES_BITS = 9;         // digit bits at most
 constexpr int ES_FUSED = 128;      // tiles up to which a scatter sums the earlier tiles' counts itself
-constexpr int ES_FEW = 16384;      // rows up to which chunks are short
+constexpr int ES_SHORT = 16384;    // rows up to which chunks are of 16 positions,
+constexpr int ES_MEDIUM = 131072;  // and of 32
 
+constexpr int64_t ES_ROWS_MAX = (int64_t(1) << 31) - 4096;  // (32-bit positions, a tile or chunk past the last included)
 constexpr uint32_t ES_NONE = 0xffffffffu;  // a key that is none: ignored, or past the last
 
 struct Pair {
@@ -112,9 +99,9 @@ __global__ __launch_bounds__(256) void embed_rank_kernel(const int64_t *__restri
   if (live && part == 0) sorted[pos] = Pair{mine, static_cast<uint32_t>(i)};
 }
 
-// counts [tiles, bins]: keys of each digit in each tile. The first pass takes the ids themselves, and empties the list of
+// counts [tiles, bins]: keys of each digit in each tile of KEYS x 1024. The first pass takes the ids themselves, and empties the list of
 // long runs.
-template <bool FIRST>
+template <int KEYS, bool FIRST>
 __global__ __launch_bounds__(1024) void embed_hist_kernel(const int64_t *__restrict__ tokens, const Pair *__restrict__ pairs,
                                                           int64_t n, int32_t V, int64_t pad, int shift, int bins,
                                                           uint32_t *__restrict__ counts, int32_t *__restrict__ owners) {
@@ -122,16 +109,16 @@ __global__ __launch_bounds__(1024) void embed_hist_kernel(const int64_t *__restr
   // four counters a digit, by lane: a digit that many keys share is not added to one place by a whole wavefront
   __shared__ u32x4 h[1 << ES_BITS];
   for (int b = threadIdx.x; b < bins; b += 1024) h[b] = u32x4{0u, 0u, 0u, 0u};
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * ES_TILE;
-  uint32_t k[ES_TILE / 1024];
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * KEYS * 1024;
+  uint32_t k[KEYS];
 #pragma unroll
-  for (int u = 0; u < ES_TILE / 1024; ++u) {
+  for (int u = 0; u < KEYS; ++u) {
     const int64_t i = base + u * 1024 + threadIdx.x, at = i < n ? i : n - 1;
     k[u] = FIRST ? sort_key(tokens[at], V, pad) : pairs[at].key;
   }
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < ES_TILE / 1024; ++u)
+  for (int u = 0; u < KEYS; ++u)
     if (base + u * 1024 + threadIdx.x < n)
       atomicAdd(reinterpret_cast<uint32_t *>(h) + 4 * ((k[u] >> shift) & (bins - 1)) + (threadIdx.x & 3), 1u);
   __syncthreads();
@@ -164,24 +151,24 @@ __global__ __launch_bounds__(64) void embed_scan_kernel(uint32_t *__restrict__ c
   if (lane == 0) totals[blockIdx.x] = run;
 }
 
-// A stable scatter: wavefront w of a tile owns its keys 256 w .. 256 w + 255 in 4 rounds of 64, so (w, round, lane) is
+// A stable scatter: wavefront w of a tile owns 64 KEYS keys side by side, in KEYS rounds of 64, so (w, round, lane) is
 // the keys' order. In a round the lanes of one digit find each other by a ballot per digit bit; a key's rank is the
 // digit's count in this wavefront's earlier rounds plus its lanes below. FUSED: the tile's offsets are summed here from
 // the counts of all (at most ES_FUSED) tiles, two threads per digit.
-template <bool FIRST, bool FUSED>
+template <int KEYS, bool FIRST, bool FUSED>
 __global__ __launch_bounds__(1024) void embed_scatter_kernel(const int64_t *__restrict__ tokens,
                                                              const Pair *__restrict__ in, int64_t n, int32_t V, int64_t pad,
                                                              int shift, int bits, const uint32_t *__restrict__ counts,
                                                              const uint32_t *__restrict__ totals,
                                                              Pair *__restrict__ out) {
-  constexpr int BINS = 1 << ES_BITS, ROUNDS = ES_TILE / 1024, WAVES = 16;
+  constexpr int BINS = 1 << ES_BITS, WAVES = 16;
   __shared__ uint32_t wcount[WAVES][BINS];
   __shared__ uint32_t half[2][BINS], wsum[WAVES];
   const int bins = 1 << bits, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * ES_TILE + wid * (ES_TILE / WAVES);
-  Pair x[ROUNDS];
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * KEYS * 1024 + wid * KEYS * 64;
+  Pair x[KEYS];
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
+  for (int r = 0; r < KEYS; ++r) {
     const int64_t i = base + r * 64 + lane, at = i < n ? i : n - 1;
     x[r] = FIRST ? Pair{sort_key(tokens[at], V, pad), static_cast<uint32_t>(i)} : in[at];
   }
@@ -216,11 +203,11 @@ __global__ __launch_bounds__(1024) void embed_scatter_kernel(const int64_t *__re
     before += half[0][bin];
     total += half[1][bin];
   }
-  int rank[ROUNDS];
+  int rank[KEYS];
   volatile uint32_t *mine = wcount[wid];
   const uint64_t below_mask = (uint64_t(1) << lane) - 1;
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
+  for (int r = 0; r < KEYS; ++r) {
     const bool live = base + r * 64 + lane < n;
     const uint32_t dig = (x[r].key >> shift) & (bins - 1);
     uint64_t peers = __ballot(live);
@@ -251,73 +238,63 @@ __global__ __launch_bounds__(1024) void embed_scatter_kernel(const int64_t *__re
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r)
+  for (int r = 0; r < KEYS; ++r)
     if (base + r * 64 + lane < n) out[wcount[wid][(x[r].key >> shift) & (bins - 1)] + rank[r]] = x[r];
 }
 
 // ---- the sums ----------------------------------------------------------------------------------------------------------
 
-// The columns of a lane in the sum: NQ groups of N, 64 N apart, one sum each. A group that the row's end cuts is moved back
-// to stay inside the row, so that all accesses are 16 bytes wide (columns that two lanes hold get the same sum); `own` is
-// where its own columns begin. PLAIN: sums are stored; else they may be added to what is there, and rows may be narrower
-// than a group, column by column.
-template <typename T, int NQ, bool PLAIN>
+// The N columns of a lane in the sum. A group that the row's end cuts is moved back to stay inside the row, so that all
+// accesses are 16 bytes wide (columns that two lanes hold get the same sum); `own` is where its own columns begin. PLAIN:
+// sums are stored; else they may be added to what is there, and rows may be narrower than a group, column by column.
+template <typename T, bool PLAIN>
 struct Cols {
-  static constexpr int N = 16 / sizeof(T), SPAN = 64 * N * NQ, U = 8 / NQ;
-  int own[NQ], c[NQ], d;
-  float v[NQ][N];
+  static constexpr int N = 16 / sizeof(T), SPAN = 64 * N, U = 8;
+  int own, c, d;
+  float v[N];
 
   __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int q = 0; q < NQ; ++q)
-#pragma unroll
-      for (int k = 0; k < N; ++k) v[q][k] = 0.f;
+    for (int k = 0; k < N; ++k) v[k] = 0.f;
   }
   __device__ __forceinline__ void init(int block, int lane, int d_) {
     d = d_;
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      own[q] = block * SPAN + N * (64 * q + lane);
-      c[q] = own[q] + N <= d || (!PLAIN && d < N) ? own[q] : d - N;
-    }
+    own = block * SPAN + N * lane;
+    c = own + N <= d || (!PLAIN && d < N) ? own : d - N;
     zero();
   }
-  __device__ __forceinline__ u32x4 load(const T *row, int q) const {
-    if (PLAIN || d >= N) return stream_16(row + c[q]);
+  __device__ __forceinline__ u32x4 load(const T *row) const {
+    if (PLAIN || d >= N) return stream_16(row + c);
     u32x4 w;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if constexpr (sizeof(T) == 4)
-        w[k] = __float_as_uint(own[q] + k < d ? load_one(row + own[q] + k) : 0.f);
+        w[k] = __float_as_uint(own + k < d ? load_one(row + own + k) : 0.f);
       else
-        w[k] = pack_bf(own[q] + 2 * k < d ? load_one(row + own[q] + 2 * k) : 0.f,
-                       own[q] + 2 * k + 1 < d ? load_one(row + own[q] + 2 * k + 1) : 0.f);
+        w[k] = pack_bf(own + 2 * k < d ? load_one(row + own + 2 * k) : 0.f,
+                       own + 2 * k + 1 < d ? load_one(row + own + 2 * k + 1) : 0.f);
     return w;
   }
-  __device__ __forceinline__ void add(const u32x4 &w, int q) {
+  __device__ __forceinline__ void add(const u32x4 &w) {
 #pragma unroll
     for (int k = 0; k < N; ++k)
       if constexpr (sizeof(T) == 4)
-        v[q][k] += __uint_as_float(w[k]);
+        v[k] += __uint_as_float(w[k]);
       else
-        v[q][k] += (k & 1) ? hi_bf(w[k / 2]) : lo_bf(w[k / 2]);
+        v[k] += (k & 1) ? hi_bf(w[k / 2]) : lo_bf(w[k / 2]);
   }
   // scale * the sums into a row (`onto`: added to it); the sums start over.
   __device__ __forceinline__ void put(float *row, float scale, bool onto) {
+    if (own < d) {
+      if (PLAIN || (!onto && d >= N)) {
+        float o[N];
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      if (own[q] < d) {
-        if (PLAIN || (!onto && d >= N)) {
-          float o[N];
+        for (int k = 0; k < N; ++k) o[k] = v[k] * scale;
+        store_row<N>(row + c, o);
+      } else {
 #pragma unroll
-          for (int k = 0; k < N; ++k) o[k] = v[q][k] * scale;
-          store_row<N>(row + c[q], o);
-        } else {
-#pragma unroll
-          for (int k = 0; k < N; ++k)
-            if (c[q] + k >= own[q] && c[q] + k < d)
-              row[c[q] + k] = onto ? row[c[q] + k] + v[q][k] * scale : v[q][k] * scale;
-        }
+        for (int k = 0; k < N; ++k)
+          if (c + k >= own && c + k < d) row[c + k] = onto ? row[c + k] + v[k] * scale : v[k] * scale;
       }
     }
     zero();
@@ -328,21 +305,18 @@ struct Cols {
   __device__ __forceinline__ void walk(const T *drows, int64_t ld, uint32_t rows, int a, int b, uint64_t heads, uint32_t keys,
                                        float *out, float scale, bool onto) {
     for (int p = a; p < b; p += U) {
-      u32x4 w[U][NQ];
+      u32x4 w[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int at = p + u < b ? p + u : b - 1;
-        const T *row = drows + static_cast<int64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(rows, at))) * ld;
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) w[u][q] = load(row, q);
+        w[u] = load(drows + static_cast<int64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(rows, at))) * ld);
       }
       const uint32_t h = RUNS ? static_cast<uint32_t>(heads >> p) : 0;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (p + u < b) {
           if (RUNS && ((h >> u) & 1)) put(out + static_cast<int64_t>(__builtin_amdgcn_readlane(keys, p + u - 1)) * d, scale, onto);
-#pragma unroll
-          for (int q = 0; q < NQ; ++q) add(w[u][q], q);
+          add(w[u]);
         }
       }
     }
@@ -353,7 +327,7 @@ struct Cols {
 // if it starts in a chunk and holds the last position of the next one: then its part in each chunk is a partial sum
 // (slot 1: the one that starts there; slot 0: the one that comes in from the chunk before), and its first chunk goes on
 // `owners`, in any order. The other wavefronts zero 64 vocabulary rows each, those without a run.
-template <typename T, int NQ, bool PLAIN, int CHUNK>
+template <typename T, bool PLAIN, int CHUNK>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const T *__restrict__ drows, int64_t ld, int32_t n, int32_t V,
                                                         int d, const Pair *__restrict__ sorted, int32_t chunks, float scale,
                                                         int accumulate, float *__restrict__ part, int32_t *__restrict__ owners,
@@ -361,7 +335,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T *__restrict__ dr
   const int lane = threadIdx.x & 63;
   const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t uV = static_cast<uint32_t>(V);
-  Cols<T, NQ, PLAIN> x;
+  Cols<T, PLAIN> x;
   x.init(blockIdx.y, lane, d);
   if (wave >= chunks) {
     const int64_t v0 = (wave - chunks) * 64, v = v0 + lane;
@@ -478,7 +452,7 @@ __global__ __launch_bounds__(512) void embed_join_kernel(const Pair *__restrict_
 struct SortPlan {
   int64_t pairs[2], counts, totals, part, owners, bytes;  // offsets in the workspace
   int64_t tiles;
-  int passes, bits, chunk, chunks;
+  int keys, passes, bits, chunk, chunks;
 };
 
 static SortPlan sort_plan(int64_t n, int32_t V, int32_t d) {
@@ -493,8 +467,9 @@ static SortPlan sort_plan(int64_t n, int32_t V, int32_t d) {
   while ((static_cast<int64_t>(V) >> need) != 0) ++need;  // bits of the largest key, V
   p.passes = n <= ES_RANK_MAX ? 0 : (need + ES_BITS - 1) / ES_BITS;
   p.bits = p.passes == 0 ? 0 : (need + p.passes - 1) / p.passes;
-  p.tiles = (n + ES_TILE - 1) / ES_TILE;
-  p.chunk = n <= ES_FEW ? 16 : 64;
+  p.keys = n <= ES_SMALL ? 1 : 2;
+  p.tiles = (n + p.keys * 1024 - 1) / (p.keys * 1024);
+  p.chunk = n <= ES_SHORT ? 16 : (n <= ES_MEDIUM ? 32 : 64);
   p.chunks = static_cast<int>((n + p.chunk - 1) / p.chunk);
   p.pairs[0] = take(8 * n);
   p.pairs[1] = p.passes == 0 ? 0 : take(8 * n);
@@ -506,17 +481,20 @@ static SortPlan sort_plan(int64_t n, int32_t V, int32_t d) {
   return p;
 }
 
-template <bool FIRST>
+template <int KEYS, bool FIRST>
 static void launch_pass(const SortPlan &p, const int64_t *tokens, const Pair *in, Pair *out, int64_t n, int32_t V, int64_t pad,
                         int shift, uint32_t *counts, uint32_t *totals, int32_t *owners, hipStream_t s) {
   const unsigned tiles = static_cast<unsigned>(p.tiles), bins = 1u << p.bits;
-  embed_hist_kernel<FIRST><<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, bins, counts, owners);
-  if (p.tiles <= ES_FUSED) {
-    embed_scatter_kernel<FIRST, true><<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, p.bits, counts, nullptr, out);
-  } else {
-    embed_scan_kernel<<<bins, 64, 0, s>>>(counts, p.tiles, bins, totals);
-    embed_scatter_kernel<FIRST, false><<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, p.bits, counts, totals, out);
+  embed_hist_kernel<KEYS, FIRST><<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, bins, counts, owners);
+  if constexpr (KEYS == 2) {  // (1024 keys each: ES_SMALL rows are ES_FUSED tiles)
+    if (p.tiles > ES_FUSED) {
+      embed_scan_kernel<<<bins, 64, 0, s>>>(counts, p.tiles, bins, totals);
+      embed_scatter_kernel<2, FIRST, false><<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, p.bits, counts, totals, out);
+      return;
+    }
   }
+  static_assert(ES_SMALL <= 1024 * ES_FUSED, "tiles of 1024 keys have no scan of their own");
+  embed_scatter_kernel<KEYS, FIRST, true><<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, p.bits, counts, nullptr, out);
 }
 
 }  // namespace vk
@@ -525,7 +503,7 @@ using namespace vk;
 
 extern "C" int vk_embed_lookup(const void *w, int32_t w_dtype, const int64_t *tokens, int64_t n, int64_t V, int32_t d,
                                float scale, void *out, int32_t out_dtype, void *stream) {
-  VK_CHECK_ARG(n >= 0 && V > 0 && d > 0, "embed_lookup: bad sizes (V=%lld d=%d)", static_cast<long long>(V), d);
+  VK_CHECK_ARG(n >= 0 && V > 0 && d > 0 && d <= EL_WIDTH_MAX, "embed_lookup: bad sizes (V=%lld d=%d)", static_cast<long long>(V), d);
   VK_CHECK_ARG(n == 0 || (w && tokens && out), "embed_lookup: null pointer");
   VK_CHECK_ARG((w_dtype == VK_DTYPE_BF16 || w_dtype == VK_DTYPE_F32) && (out_dtype == VK_DTYPE_BF16 || out_dtype == VK_DTYPE_F32),
                "embed_lookup: bad dtype");
@@ -533,15 +511,17 @@ extern "C" int vk_embed_lookup(const void *w, int32_t w_dtype, const int64_t *to
   const bool wf = w_dtype == VK_DTYPE_F32, of = out_dtype == VK_DTYPE_F32;
   const int per = !wf && !of ? 8 : 4;  // elements per lane
   const int lpr = d <= 16 * per ? 16 : (d <= 32 * per ? 32 : 64);
-  const int64_t rows_per_block = 4 * EL_ROWS * (64 / lpr), blocks = (n + rows_per_block - 1) / rows_per_block;
-  VK_CHECK_ARG(blocks < (int64_t(1) << 31), "embed_lookup: too many rows");
+  const int64_t rows_per_block = 4 * (64 / lpr), most = rows_per_block * (EL_GRID_MAX - 1);  // rows of a launch
   hipStream_t s = VK_STREAM(stream);
 #define VK_LOOKUP(WT, OT)                                                                                              \
   do {                                                                                                                 \
     auto k = lpr == 16 ? embed_lookup_kernel<WT, OT, 16> : (lpr == 32 ? embed_lookup_kernel<WT, OT, 32>                \
                                                                      : embed_lookup_kernel<WT, OT, 64>);               \
-    k<<<static_cast<unsigned>(blocks), 256, 0, s>>>(static_cast<const WT *>(w), tokens, n, V, d, scale,                \
-                                                    static_cast<OT *>(out));                                           \
+    for (int64_t r = 0; r < n; r += most) {                                                                            \
+      const int64_t rows = n - r < most ? n - r : most;                                                                \
+      k<<<static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block), 256, 0, s>>>(                           \
+          static_cast<const WT *>(w), tokens + r, rows, V, d, scale, static_cast<OT *>(out) + r * d);                  \
+    }                                                                                                                  \
   } while (0)
   if (wf && of)
     VK_LOOKUP(float, float);
@@ -556,8 +536,8 @@ extern "C" int vk_embed_lookup(const void *w, int32_t w_dtype, const int64_t *to
 }
 
 extern "C" int vk_embed_grad_sorted_workspace(int64_t n, int32_t V, int32_t d, int64_t *bytes) {
-  VK_CHECK_ARG(bytes && n >= 0 && V > 0 && d > 0, "embed_grad_sorted_workspace: bad arguments");
-  VK_CHECK_ARG(n < (int64_t(1) << 31) - ES_TILE, "embed_grad_sorted: too many rows");
+  VK_CHECK_ARG(bytes && n >= 0 && V > 0 && d > 0 && d <= EL_WIDTH_MAX, "embed_grad_sorted_workspace: bad arguments");
+  VK_CHECK_ARG(n < ES_ROWS_MAX, "embed_grad_sorted: too many rows");
   *bytes = sort_plan(n, V, d).bytes;
   return VK_OK;
 }
@@ -565,14 +545,15 @@ extern "C" int vk_embed_grad_sorted_workspace(int64_t n, int32_t V, int32_t d, i
 extern "C" int vk_embed_grad_sorted(const void *d_rows, int32_t d_dtype, int64_t ld, const int64_t *tokens, int64_t n,
                                     int32_t V, int32_t d, float scale, int64_t pad, float *out, int32_t accumulate,
                                     void *workspace, int64_t workspace_bytes, void *stream) {
-  VK_CHECK_ARG(n >= 0 && V > 0 && d > 0 && ld >= d, "embed_grad_sorted: bad sizes (V=%d d=%d)", V, d);
-  VK_CHECK_ARG(n < (int64_t(1) << 31) - ES_TILE, "embed_grad_sorted: too many rows");
+  VK_CHECK_ARG(n >= 0 && V > 0 && d > 0 && d <= EL_WIDTH_MAX && ld >= d, "embed_grad_sorted: bad sizes (V=%d d=%d)", V, d);
+  VK_CHECK_ARG(n < ES_ROWS_MAX, "embed_grad_sorted: too many rows");
   VK_CHECK_ARG(out && workspace && (n == 0 || (d_rows && tokens)), "embed_grad_sorted: null pointer");
   VK_CHECK_ARG(d_dtype == VK_DTYPE_BF16 || d_dtype == VK_DTYPE_F32, "embed_grad_sorted: bad row dtype");
   VK_CHECK_ARG(vk_aligned16(workspace), "embed_grad_sorted: workspace must be 16-byte aligned");
   const SortPlan p = sort_plan(n, V, d);
   VK_CHECK_ARG(workspace_bytes >= p.bytes, "embed_grad_sorted: workspace of %lld bytes needed",
                static_cast<long long>(p.bytes));
+  const int64_t waves = p.chunks + (accumulate ? 0 : (static_cast<int64_t>(V) + 63) / 64);
   hipStream_t s = VK_STREAM(stream);
   char *ws = static_cast<char *>(workspace);
   auto pairs = [&](int i) { return reinterpret_cast<Pair *>(ws + p.pairs[i]); };
@@ -583,48 +564,37 @@ extern "C" int vk_embed_grad_sorted(const void *d_rows, int32_t d_dtype, int64_t
         tokens, static_cast<int32_t>(n), V, pad, pairs(0), owners);
   } else if (n > 0) {
     uint32_t *counts = reinterpret_cast<uint32_t *>(ws + p.counts), *totals = reinterpret_cast<uint32_t *>(ws + p.totals);
-    launch_pass<true>(p, tokens, nullptr, pairs(0), n, V, pad, 0, counts, totals, owners, s);
+    auto pass = p.keys == 1 ? launch_pass<1, true> : launch_pass<2, true>;
+    pass(p, tokens, nullptr, pairs(0), n, V, pad, 0, counts, totals, owners, s);
+    pass = p.keys == 1 ? launch_pass<1, false> : launch_pass<2, false>;
     for (int q = 1; q < p.passes; ++q) {
-      launch_pass<false>(p, nullptr, pairs(at), pairs(1 - at), n, V, pad, q * p.bits, counts, totals, owners, s);
+      pass(p, nullptr, pairs(at), pairs(1 - at), n, V, pad, q * p.bits, counts, totals, owners, s);
       at = 1 - at;
     }
   }
   int rc = launch_status("embed_grad_sorted sort");
   if (rc != VK_OK) return rc;
   float *part = reinterpret_cast<float *>(ws + p.part);
-  const int64_t waves = p.chunks + (accumulate ? 0 : (static_cast<int64_t>(V) + 63) / 64);
   if (waves == 0) return VK_OK;
-  const unsigned gx = static_cast<unsigned>((waves + 3) / 4);
-#define VK_EMBED_SUM(T, NQ, PLAIN, CHUNK)                                                                               \
-  embed_sum_kernel<T, NQ, PLAIN, CHUNK>                                                                                 \
-      <<<dim3(gx, static_cast<unsigned>((d + Cols<T, NQ, PLAIN>::SPAN - 1) / Cols<T, NQ, PLAIN>::SPAN)), 256, 0, s>>>(  \
-          static_cast<const T *>(d_rows), ld, static_cast<int32_t>(n), V, d, pairs(at), p.chunks, scale, accumulate,   \
-          part, owners, out)
-#define VK_EMBED_SUM_CHUNK(T, NQ, PLAIN) \
-  do {                                   \
-    if (p.chunk == 16)                   \
-      VK_EMBED_SUM(T, 1, PLAIN, 16);     \
-    else                                 \
-      VK_EMBED_SUM(T, NQ, PLAIN, 64);    \
+  const unsigned gx = static_cast<unsigned>((waves + 3) / 4);  // (below EL_GRID_MAX by the limits of n and V)
+#define VK_EMBED_SUM(T, PLAIN)                                                                                         \
+  do {                                                                                                                 \
+    auto k = p.chunk == 16 ? embed_sum_kernel<T, PLAIN, 16>                                                            \
+                           : (p.chunk == 32 ? embed_sum_kernel<T, PLAIN, 32> : embed_sum_kernel<T, PLAIN, 64>);        \
+    constexpr int span = Cols<T, PLAIN>::SPAN;                                                                         \
+    k<<<dim3(gx, static_cast<unsigned>((d + span - 1) / span)), 256, 0, s>>>(                                          \
+        static_cast<const T *>(d_rows), ld, static_cast<int32_t>(n), V, d, pairs(at), p.chunks, scale, accumulate, part, \
+        owners, out);                                                                                                  \
   } while (0)
   const bool plain = !accumulate && d >= 8;
-  if (d_dtype == VK_DTYPE_BF16) {
-    if (plain)
-      VK_EMBED_SUM_CHUNK(bf16_t, 1, true);
-    else
-      VK_EMBED_SUM_CHUNK(bf16_t, 1, false);
-  } else if (d > Cols<float, 1, true>::SPAN) {
-    if (plain)
-      VK_EMBED_SUM_CHUNK(float, 2, true);
-    else
-      VK_EMBED_SUM_CHUNK(float, 2, false);
-  } else {
-    if (plain)
-      VK_EMBED_SUM_CHUNK(float, 1, true);
-    else
-      VK_EMBED_SUM_CHUNK(float, 1, false);
-  }
-#undef VK_EMBED_SUM_CHUNK
+  if (d_dtype == VK_DTYPE_BF16 && plain)
+    VK_EMBED_SUM(bf16_t, true);
+  else if (d_dtype == VK_DTYPE_BF16)
+    VK_EMBED_SUM(bf16_t, false);
+  else if (plain)
+    VK_EMBED_SUM(float, true);
+  else
+    VK_EMBED_SUM(float, false);
 #undef VK_EMBED_SUM
   rc = launch_status("embed_grad_sorted sum");
   if (rc != VK_OK || n < 2 * p.chunk) return rc;

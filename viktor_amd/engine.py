@@ -120,14 +120,15 @@ class DecodeEngine:
         if grammar is not None:
             mask, rows = (torch.as_tensor(t) for t in grammar)
             if mask.dtype != torch.bool or mask.dim() != 2 or mask.shape[1] != tk.vocab_size or rows.shape != (tk.vocab_size,) \
-                    or rows.dtype not in (torch.int32, torch.int64) or int(rows.max()) >= mask.shape[0]:
+                    or rows.dtype not in (torch.int32, torch.int64) or mask.shape[0] == 0 or int(rows.max()) >= mask.shape[0]:
                 raise ValueError("grammar: (allowed bool [S, V], rows int [V] with values below S)")
             self.allowed = ops.pack_allowed(mask.to(dev))
-            self.token_rows = rows.to(dev, torch.int32).contiguous()
+            self.token_rows = rows.clamp(min=-1).to(dev, torch.int32).contiguous()
         self._fused_head = (tk.vocab_size <= self.FUSED_HEAD_VOCAB and self.penalties == (1.0, 0.0, 0.0)
                             and grammar is None)
         # logprobs=True: logp[b, j] = log-probability of output token j under the distribution it was chosen
-        # from (log softmax of (logits + bias) / T, or of logits + bias when greedy), before the grammar rules
+        # from (log softmax of (logits + bias) / T, or of logits + bias when greedy, after the penalties and the grammar's
+        # masks where there are any), before the rules that force a token
         self.logp = torch.zeros(batch_size, max_new_tokens, dtype=torch.float32, device=dev) if logprobs else None
         self.fast.decode_workspace = ops.decode_attention_workspace(batch_size, self.dec.cfg.n_heads,
                                                                     self.cache.max_len, dev)

@@ -878,6 +878,9 @@ def _here(what, ts):
                 dev = at
 
 
+_WIDEST = 1 << 30  # of a row: the C entry points take 32-bit widths
+
+
 def _vk_dtype(t):
     return VK_DTYPE_F32 if t is torch.float32 else VK_DTYPE_BF16
 
@@ -887,7 +890,7 @@ def _rows_ok(t):
     if t.dim() != 2 or not (t.dtype is BF16 or t.dtype is torch.float32):
         return False
     n, d = t.size(0), t.size(1)
-    return d > 0 and (t.is_contiguous() or ((t.stride(1) == 1 or d == 1) and (n < 2 or t.stride(0) >= d)))
+    return 0 < d <= _WIDEST and (t.is_contiguous() or ((t.stride(1) == 1 or d == 1) and (n < 2 or t.stride(0) >= d)))
 
 
 def embed_lookup(weight, tokens, scale=1.0, out_dtype=None):
@@ -897,7 +900,8 @@ def embed_lookup(weight, tokens, scale=1.0, out_dtype=None):
     _here("embed_lookup", (weight, tokens))
     wdt = weight.dtype
     odt = out_dtype or wdt
-    if weight.dim() != 2 or wdt not in (BF16, torch.float32) or odt not in (BF16, torch.float32) or weight.numel() == 0:
+    if weight.dim() != 2 or wdt not in (BF16, torch.float32) or odt not in (BF16, torch.float32) or weight.numel() == 0 \
+            or weight.size(1) > _WIDEST:
         _refuse("embed_lookup", "weight [V, d] and out bf16 or fp32")
     if tokens.dtype != torch.long or not (weight.is_contiguous() and tokens.is_contiguous()):
         _refuse("embed_lookup", "contiguous weight and int64 tokens")
@@ -928,8 +932,8 @@ def embed_grad_sorted(d_rows, tokens, vocab, scale=1.0, pad=None, out=None, accu
     n, d = d_rows.shape
     if tokens.shape != (n,) or tokens.dtype != torch.long or not tokens.is_contiguous():
         _refuse(what, "tokens [n] int64")
-    if vocab <= 0 or (accumulate and out is None):
-        _refuse(what, "vocab > 0, accumulate into out")
+    if not 0 < vocab < 1 << 31 or (accumulate and out is None):
+        _refuse(what, "0 < vocab < 2^31, accumulate into out")
     if out is None:
         out = torch.empty((vocab, d), dtype=torch.float32, device=d_rows.device)
     elif out.dtype != torch.float32 or out.shape != (vocab, d) or not out.is_contiguous():
@@ -1023,6 +1027,17 @@ def _logit_rules(what, logits, history, lengths, repetition, presence, frequency
                   ap, words, S, ptr(allowed_rows))
 
 
+def _apart(a, b):
+    """Whether matrices a and b [B, V] (rows side by side) share no element: one behind the other, or columns of one
+    buffer."""
+    pa, pb, (B, V) = a.data_ptr(), b.data_ptr(), a.shape
+    ea, eb = a.element_size(), b.element_size()
+    sa, sb = max(a.stride(0), V) * ea, max(b.stride(0), V) * eb
+    if B == 0 or pa + (B - 1) * sa + V * ea <= pb or pb + (B - 1) * sb + V * eb <= pa:
+        return True
+    return sa == sb and V * ea <= (pb - pa) % sa <= sa - V * eb
+
+
 def process_logits(logits, history=None, lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,
                    allowed_rows=None, out=None, out_dtype=None):
     """Penalties for repeated tokens, bias and grammar mask on logits [B, V] (bf16 or fp32, unit column stride). For
@@ -1044,6 +1059,8 @@ def process_logits(logits, history=None, lengths=None, repetition=1.0, presence=
         _here("process_logits", (out,))
         if out.shape != (B, V) or not _rows_ok(out) or (out_dtype is not None and out.dtype != out_dtype):
             _refuse("process_logits", "out [B, V] bf16 or fp32, rows side by side")
+        if out.data_ptr() != logits.data_ptr() and not _apart(logits, out):
+            _refuse("process_logits", "out is the logits themselves, or shares nothing with them")
     call("vk_process_logits", *args, out.data_ptr(), _vk_dtype(out.dtype), max(out.stride(0), V), B, V, stream_handle())
     return out
 
@@ -1062,7 +1079,7 @@ def choose_tokens(logits, history=None, lengths=None, repetition=1.0, presence=0
                   allowed_rows=None, temperature=0.0, uniforms=None, fallback=0):
     """The token choice over any vocabulary after process_logits' rules, which are applied on the fly (logits stay as they
     are). z' = z / temperature where it is positive (a float or fp32 [B]); a row with temperature <= 0 is greedy (the first
-    index of the maximum). uniforms in [0, 1): fp32 [B, V] for the Gumbel choice, first argmax of z' - log(-log(max(u, 1e-20)))
+    index of the maximum), an infinite temperature is the largest finite one. uniforms in [0, 1): fp32 [B, V] for the Gumbel choice, first argmax of z' - log(-log(max(u, 1e-20)))
     (viktor/engine.py:80-83's formula), or fp32 [B] for the inverse CDF, the first v with u < sum_{w <= v} softmax(z')_w.
     Returns (tokens int64 [B], logp fp32 [B]), logp = log softmax(z')[token]. NaN is never chosen and weighs nothing, +inf
     counts as the largest finite value; a row with nothing left gives `fallback` and -inf."""

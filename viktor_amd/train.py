@@ -65,7 +65,9 @@ class _TokenEmbed(torch.autograd.Function):
     def forward(ctx, weight, tokens, scale=1.0, pad=None):
         ctx.save_for_backward(tokens)
         ctx.vocab, ctx.scale, ctx.pad, ctx.dtype = weight.shape[0], scale, pad, weight.dtype
-        return ops.embed_lookup(weight.detach().contiguous(), tokens.contiguous(), scale=scale, out_dtype=torch.float32)
+        w = weight.detach().contiguous()
+        return ops.embed_lookup(w if w.dtype in (torch.float32, BF16) else w.float(), tokens.contiguous(), scale=scale,
+                                out_dtype=torch.float32)
 
     @staticmethod
     def backward(ctx, d_rows):
