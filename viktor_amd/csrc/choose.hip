@@ -213,9 +213,12 @@ struct Batch {
   }
 
   // z: the batch's logits after bias and mask (-inf past the row's end). MORE: the next batch's logits are loaded as soon
-  // as these are taken, behind this one's bias and mask.
+  // as these are taken, behind this one's bias and mask. left_out: a bit per token of the slice from v0, of those that get
+  // -inf too (null: none). All of a token's reasons for -inf are one bit, spread to a word and merged in: 2 instructions a
+  // token.
   template <bool CUT, bool MORE>
-  __device__ __forceinline__ void rules(float (&z)[R][N], const T *row, const RowRules &r, int first, int V) {
+  __device__ __forceinline__ void rules(float (&z)[R][N], const T *row, const RowRules &r, int first, int V,
+                                        const uint32_t *left_out, int v0) {
 #pragma clang fp contract(off)
 #pragma unroll
     for (int q = 0; q < R; ++q)
@@ -252,19 +255,18 @@ struct Batch {
 #pragma unroll
         for (int k = 0; k < N; ++k) z[q][k] = z[q][k] + bias[q][k];
     const int lane_bit = (threadIdx.x * N) & 31;  // (first and STEP are multiples of 32)
-    if (r.allowed != nullptr)
+    if (!CUT && r.allowed == nullptr && left_out == nullptr) return;
 #pragma unroll
-      for (int q = 0; q < R; ++q) {
-        const uint32_t bits = mask[q] >> lane_bit;
+    for (int q = 0; q < R; ++q) {
+      uint32_t keep = r.allowed != nullptr ? mask[q] >> lane_bit : ~0u;
+      if (left_out != nullptr) keep &= ~(left_out[(token(first, q) - v0) >> 5] >> lane_bit);
+      if (CUT) keep &= (1u << max(0, min(N, V - token(first, q)))) - 1;
 #pragma unroll
-        for (int k = 0; k < N; ++k) z[q][k] = (bits >> k) & 1 ? z[q][k] : -INFINITY;
+      for (int k = 0; k < N; ++k) {
+        const uint32_t whole = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(keep), k, 1));
+        z[q][k] = __uint_as_float((__float_as_uint(z[q][k]) & whole) | (0xff800000u & ~whole));
       }
-    if (CUT)
-#pragma unroll
-      for (int q = 0; q < R; ++q)
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-          if (token(first, q) + k >= V) z[q][k] = -INFINITY;
+    }
   }
 };
 
@@ -272,7 +274,7 @@ template <typename T, typename OT, bool CUT, bool MORE>
 __device__ __forceinline__ void process_batch(Batch<T, CH_THREADS> &x, const T *row, OT *dst, const RowRules &r, int w, int V) {
   using X = Batch<T, CH_THREADS>;
   float z[X::R][X::N];
-  x.template rules<CUT, MORE>(z, row, r, w, V);
+  x.template rules<CUT, MORE>(z, row, r, w, V, nullptr, 0);
 #pragma unroll
   for (int q = 0; q < X::R; ++q) {
     const int v = X::token(w, q);
@@ -338,6 +340,9 @@ __device__ __forceinline__ Part no_part() { return {-FLT_MAX, 0.f, -INFINITY, -I
 // How far the fp32 score of a token can be from the exact one: the roundings of z' and of the sum (1.2e-7 of its size
 // each), and of the two logarithms.
 __device__ __forceinline__ float score_slack(float s) { return 1e-5f + 1e-6f * fabsf(s); }
+
+// The least fp32 score that can be the best one where the largest fp32 score is `most` (a NaN for inf: any can).
+__device__ __forceinline__ float contender_from(float most) { return most - 2.5f * score_slack(most); }
 
 // The exact score: z' rounded to fp32 unless that overflows, the noise in 64 bits.
 __device__ __forceinline__ double exact_score(float z, float u, float T) {
@@ -481,9 +486,10 @@ __device__ __forceinline__ float wave_max_of(float v) {
 }
 
 // What a thread knows of its tokens: the maximum of z (at least -FLT_MAX), the sum of exponentials at it, the best logit
-// or score with its first token, and the second best score.
+// or score with its first token, and the second best score. A batch that has nothing near the wavefront's best so far is
+// not looked through for them (a thread's next best comes in most batches, a wavefront's in one of i at the i-th).
 struct Mine {
-  float m = -FLT_MAX, sum = 0.f, best = -INFINITY, second = -INFINITY;
+  float m = -FLT_MAX, sum = 0.f, best = -INFINITY, second = -INFINITY, wave_best = -INFINITY;
   int v = -1;
 };
 
@@ -515,16 +521,8 @@ __device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, T
   const bool noisy = GUMBEL && c.T > 0.f;
   float z[X::R][X::N], u[GUMBEL ? X::R : 1][X::N];
   un.take(u);
-  x.template rules<CUT, MORE>(z, row, r, w, V);
+  x.template rules<CUT, MORE>(z, row, r, w, V, r.len > 0 ? s.bits : nullptr, v0);  // (the history's tokens: each())
   if (MORE) un.load(urow, w + X::TOKENS, V);
-  if (r.len > 0)  // the history's tokens are none of these
-#pragma unroll
-    for (int q = 0; q < X::R; ++q) {
-      const uint32_t left = s.bits[(X::token(w, q) - v0) >> 5] >> ((threadIdx.x * X::N) & 31);
-      if (left & ((1u << X::N) - 1))
-#pragma unroll
-        for (int k = 0; k < X::N; ++k) z[q][k] = (left >> k) & 1 ? -INFINITY : z[q][k];
-    }
   float top = -INFINITY;
 #pragma unroll
   for (int q = 0; q < X::R; ++q)
@@ -550,25 +548,40 @@ __device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, T
           if (v < V && v > V - X::N)
             for (int k = 0; k < X::N; ++k) u[q][k] = urow[v + k < V ? v + k : V - 1];
         }
+      float most = -INFINITY;
 #pragma unroll
       for (int q = 0; q < X::R; ++q)
 #pragma unroll
-        for (int k = 0; k < X::N; ++k) {
-          const float sc = gumbel_score(z[q][k], u[q][k], c);
-          t.second = fmaxf(t.second, fminf(t.best, sc));
-          if (sc > t.best) {
-            t.best = sc;
-            t.v = X::token(w, q) + k;
-          }
+        for (int k = 0; k < X::N; k += 2) {
+          u[q][k] = gumbel_score(z[q][k], u[q][k], c);
+          u[q][k + 1] = gumbel_score(z[q][k + 1], u[q][k + 1], c);
+          most = vmax3(most, u[q][k], u[q][k + 1]);
         }
+      if (__any(!(most < contender_from(t.wave_best)))) {
+#pragma unroll
+        for (int q = 0; q < X::R; ++q)
+#pragma unroll
+          for (int k = 0; k < X::N; ++k) {
+            const float sc = u[q][k];
+            t.second = fmaxf(t.second, fminf(t.best, sc));
+            if (sc > t.best) {
+              t.best = sc;
+              t.v = X::token(w, q) + k;
+            }
+          }
+        t.wave_best = wave_max_of(t.best);
+      }
     }
-  } else if (top > t.best || (top == t.best && top > -INFINITY)) {  // (a token of the history may be behind these)
-    t.v = top > t.best ? 0x7fffffff : t.v;
-    t.best = top;
+  } else if (__any(top >= t.wave_best && top > -INFINITY)) {
+    if (top > t.best || (top == t.best && top > -INFINITY)) {  // (a token of the history may be behind these)
+      t.v = top > t.best ? 0x7fffffff : t.v;
+      t.best = top;
 #pragma unroll
-    for (int q = X::R - 1; q >= 0; --q)
+      for (int q = X::R - 1; q >= 0; --q)
 #pragma unroll
-      for (int k = X::N - 1; k >= 0; --k) t.v = z[q][k] == top ? min(t.v, X::token(w, q) + k) : t.v;
+        for (int k = X::N - 1; k >= 0; --k) t.v = z[q][k] == top ? min(t.v, X::token(w, q) + k) : t.v;
+    }
+    t.wave_best = wave_max_of(t.best);
   }
 }
 
@@ -648,7 +661,7 @@ __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restr
     if (most > -INFINITY && t.best == most) atomicMin(&first_best, t.v);
   } else {
     const bool below = most == -INFINITY;  // (t.sum > 0: some logit is finite)
-    if (below ? t.sum > 0.f : t.best > -INFINITY && (t.best == most || most - t.best <= 2.5f * score_slack(most))) {
+    if (below ? t.sum > 0.f : t.best > -INFINITY && (t.best == most || !(t.best < contender_from(most)))) {
       Part p = no_part();
       auto offer = [&](int v) {
         Part e = no_part();
@@ -658,7 +671,7 @@ __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restr
         e.v = e.z == -INFINITY ? -1 : v;
         if (better<true>(p, e, c.T)) p = e;
       };
-      if (below || t.second == most || most - t.second <= 2.5f * score_slack(most)) {
+      if (below || t.second == most || !(t.second < contender_from(most))) {
         for (int i = v0; i < v1; i += X::STEP)
           for (int k = 0; k < X::N; ++k) {
             const int v = i + tid * X::N + k;
