@@ -45,8 +45,8 @@ def test_embedding_workspace_covers_what_the_passes_write():
         return b.value
 
     assert need(0, 7, 1) >= 16
-    for n in (1, 31, 32, 64, 65, 4096, 4097, 16384, 16385, 131072, 131073, 524288, 600000):
-        chunk = 16 if n <= 16384 else 32 if n <= 131072 else 64
+    for n in (1, 31, 32, 64, 65, 4096, 4097, 16384, 16385, 102400, 102401, 131072, 131073, 524288, 600000):
+        chunk = 16 if n <= 16384 else 32 if n <= 102400 else 64
         partials = 8 * -(-n // chunk) if n >= 2 * chunk else 0  # fp32 rows: two slots a chunk
         for V in (1, 343, 87383, 300000):
             for d in (1, 512):

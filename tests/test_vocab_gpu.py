@@ -71,8 +71,8 @@ def test_embed_lookup_of_more_rows_than_a_launch():
 def _grad_ref(rows, tok, V, scale, pad=None):
     """(fp64 gradient, what an element may be off by, in units of U): a run's sum is at most 127 additions in a chunk (of up
     to 64 positions) and the next; a longer one's 64 in each chunk, its chunks' sums over 32 groups, and the groups; then one
-    product. Chunks of 16 (n <= 16384) and 32 (n <= 131072) have fewer additions each and no more in all:
-    16 + 16384 / 512 + 32 and 32 + 131072 / 1024 + 32 are below 127 and 127 + 131072 / 2048."""
+    product. Chunks of 16 (n <= 16384) and 32 (n <= 102400) have fewer additions each and no more in all:
+    16 + 16384 / 512 + 32 and 32 + 102400 / 1024 + 32 are below 127 and 127 + 102400 / 2048."""
     keep = (tok >= 0) & (tok < V) & (tok != (-1 if pad is None else pad))
     out = torch.zeros(V, rows.shape[1], dtype=torch.float64)
     mag = torch.zeros_like(out)
@@ -178,7 +178,7 @@ def test_embed_grad_sorted_run_lengths(lens, ignored):
         _check_grad(ops.embed_grad_sorted(rows.to(DEV), tok.to(DEV), V), _grad_ref(rows, tok, V, 1.0), more)
 
 
-@pytest.mark.parametrize("chunk,n", [(16, 2000), (16, 16384), (32, 16385), (32, 131072), (64, 131073)])
+@pytest.mark.parametrize("chunk,n", [(16, 2000), (16, 16384), (32, 16385), (32, 102400), (64, 102401), (64, 131073)])
 @pytest.mark.parametrize("dt", [F32, BF])
 def test_embed_grad_sorted_run_borders(chunk, n, dt):
     """Runs that end and start at, before and behind the borders of chunks of each size, among runs of a few rows, the last

@@ -11,13 +11,20 @@
 //
 // A workgroup takes one slice of one sequence's vocabulary. The history's tokens of the slice are gathered in LDS (Seen),
 // so no count per (sequence, token) exists in memory and the streaming pass over the logits knows of the history only that
-// a token is left out: a distinct token of it is computed once, by one thread. The pass is bound by memory while it runs;
-// what keeps it from the rate of a plain copy is the gathering (two barriers, a dependent load) that every slice begins
-// with, and the bias, which is read through the same in-order path as the logits. Slices of 4096 to 8192 tokens: 512 x
-// 87383 bf16 logits take 35 us without rules (5.1 TB/s, a copy of that size 31 to 36 us), 42 us with a bias, 46 us with a
-// history of 256, 52 us with all; slices of 16384 took 58 us, of 4096 58 us. The choice from fp32 logits gives (max, sum of
-// exponentials at it, best) per slice, joined by one wavefront per sequence, or takes a whole row per workgroup of 512
-// threads: 43 us against 54 us in slices at 512 x 87383.
+// a token is left out: a distinct token of it is computed once, by one thread. Logits are loaded a batch ahead of their use.
+// The choice gives (max, sum of exponentials at it, best) per slice, joined by one wavefront per sequence, or takes a whole
+// row per workgroup of 512 threads and finishes it (make_plan).
+//
+// What bounds them: one sequence, the launch and the chain of loads (process 4.8 us at 87383 tokens, choice 8.6 us in two
+// launches); a batch, memory, and before it the gathering and the bias, which is read from the caches as often as there are
+// sequences. 512 x 87383 logits, us (a plain read of the fp32 ones takes 26.5, a copy of the bf16 ones 31 to 36):
+//                 no rules   bias   mask   history of 256   all
+//   process bf16      37      45     38         43           51 (46.8 from logits that are not in a cache)
+//   process fp32      74      78     76         82           83
+//   greedy fp32       31.5    37     33         34           41.5
+//   greedy bf16       23.6    32     27         26           36
+// Measured and not taken: bias and mask loaded a batch ahead (process fp32 -4, all bf16 +2), two sequences a workgroup that
+// share the bias (bf16 -0.6, fp32 +5), 8-byte loads of bf16 (+1 to +2), 1024 threads a row (+5).
 #include <float.h>
 #include <math.h>
 
@@ -29,9 +36,13 @@ namespace vk {
 constexpr int CH_THREADS = 256;
 constexpr int CH_THREADS_ONE = 512;  // of a workgroup that takes a whole row
 constexpr int CH_WHOLE = 1 << 17;    // tokens of such a row at most, where it has more than one slice: 16 KB of LDS bits
-constexpr int CH_SMALL = 32768;      // tokens of a row that one workgroup takes at any batch
-constexpr int CH_SLICE = 8192;       // tokens of a slice at most
-constexpr int CH_HASH_MAX = 2048;    // history columns at most whose counts are hashed: 32 KB of LDS either way
+// Tokens of a row that one workgroup takes at any batch: it spares the join's launch. fp32, greedy, us: 21847 tokens of 1,
+// 77, 200 sequences 8.0, 10.4, 11.1 against 8.3, 10.6, 11.0 in slices; 43000 tokens 11.3, 14.3, 15.7 against 8.2, 12.5, 15.8.
+constexpr int CH_SMALL = 32768;
+constexpr int CH_SLICE = 8192;       // tokens of a slice at most (512 x 87383 bf16, processed: 51 us; of 4096 55, 16384 57)
+// History columns at most whose counts are hashed, 32 KB of LDS at the most. 512 x 87383 bf16, processed, histories of 256:
+// 51 us, counted by token 57 (32 KB to clear and to hold); of 2048: 68 and 66.
+constexpr int CH_HASH_MAX = 2048;
 constexpr int CH_HIST_MAX = 65535;
 constexpr int32_t CH_V_MAX = 1 << 30;
 
@@ -271,7 +282,8 @@ struct Batch {
 };
 
 template <typename T, typename OT, bool CUT, bool MORE>
-__device__ __forceinline__ void process_batch(Batch<T, CH_THREADS> &x, const T *row, OT *dst, const RowRules &r, int w, int V) {
+__device__ __forceinline__ void process_batch(Batch<T, CH_THREADS> &x, const T *row, OT *dst, const RowRules &r, int w,
+                                              int V) {
   using X = Batch<T, CH_THREADS>;
   float z[X::R][X::N];
   x.template rules<CUT, MORE>(z, row, r, w, V, nullptr, 0);
@@ -289,8 +301,8 @@ __device__ __forceinline__ void process_batch(Batch<T, CH_THREADS> &x, const T *
 // was there before any store (out may be logits), and stored over what the streaming pass, which knows of no history, has
 // put there.
 template <typename T, typename OT>
-__global__ __launch_bounds__(CH_THREADS) void process_logits_kernel(const T *logits, int64_t ld, Rules rules, int V, Plan plan,
-                                                                    OT *out, int64_t out_ld) {
+__global__ __launch_bounds__(CH_THREADS) void process_logits_kernel(const T *logits, int64_t ld, Rules rules, int V,
+                                                                    Plan plan, OT *out, int64_t out_ld) {
   extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
   using X = Batch<T, CH_THREADS>;
   const int64_t b = blockIdx.x / plan.slices;
@@ -347,7 +359,8 @@ __device__ __forceinline__ float contender_from(float most) { return most - 2.5f
 // The exact score: z' rounded to fp32 unless that overflows, the noise in 64 bits.
 __device__ __forceinline__ double exact_score(float z, float u, float T) {
   const float q = z / T;
-  return (fabsf(q) <= FLT_MAX ? static_cast<double>(q) : static_cast<double>(z) / T) - log(-log(fmax(static_cast<double>(u), 1e-20)));
+  const double scaled = fabsf(q) <= FLT_MAX ? static_cast<double>(q) : static_cast<double>(z) / T;
+  return scaled - log(-log(fmax(static_cast<double>(u), 1e-20)));
 }
 
 struct Scale {
@@ -588,7 +601,8 @@ __device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, T
 // One slice of one sequence, or with ONE the whole vocabulary and the step's end. The workgroup's best logit or score
 // tells who can have the best token: the lowest token of the largest logit, or the threads within the scores' slack of
 // the largest score. These read their token again and are compared exactly; one whose second score is as near goes
-// through all of its tokens, and so does every thread where all scores are below fp32's range. The sum is taken at the workgroup's maximum.
+// through all of its tokens, and so does every thread where all scores are below fp32's range. The sum is taken at the
+// workgroup's maximum.
 template <typename T, int THREADS, bool GUMBEL, bool ONE>
 __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restrict__ logits, int64_t ld, Rules rules,
                                                                    const float *__restrict__ temp, float temp0,
@@ -826,8 +840,9 @@ __global__ __launch_bounds__(CH_THREADS) void choose_cdf_kernel(const T *__restr
 }
 
 // How B rows of V tokens are cut: about two workgroups per CU in all, of 4096 tokens (one batch) to CH_SLICE. `whole`: one
-// workgroup of CH_THREADS_ONE may take a sequence's whole vocabulary, where that spares the slices' joining and leaves the
-// CUs evenly loaded. hist_cols: 0 without a history.
+// workgroup of CH_THREADS_ONE may take a sequence's whole vocabulary, where that spares the slices' joining (CH_SMALL) or
+// the sequences load the CUs evenly, to three quarters at least. fp32, greedy, 87383 tokens, whole and in slices, us: 130
+// sequences 22.1 and 21.3; 192: 23.0, 26.9; 250: 24.0, 31.2; 300: 37.9, 35.4; 512: 41.5, 50.7. hist_cols: 0 without a history.
 static Plan make_plan(int64_t B, int V, int64_t hist_cols, bool whole) {
   constexpr int UNIT = Batch<float, CH_THREADS>::TOKENS;
   static_assert(UNIT == Batch<bf16_t, CH_THREADS>::TOKENS && CH_SLICE % UNIT == 0, "slices are whole batches");
@@ -900,8 +915,8 @@ static int launch_choose(const void *logits, int64_t ld, const Rules &r, const f
                                                                            choice, step)
   if (mode == CH_CDF) {
     VK_SLICES(CH_THREADS, false, false);
-    choose_cdf_kernel<T><<<static_cast<unsigned>(B), CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, plan, parts, choice,
-                                                                       step);
+    choose_cdf_kernel<T><<<static_cast<unsigned>(B), CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, plan, parts,
+                                                                           choice, step);
   } else if (plan.one) {
     if (mode == CH_GUMBEL)
       VK_SLICES(CH_THREADS_ONE, true, true);
@@ -961,7 +976,9 @@ extern "C" int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, 
 }
 
 // Whether a call of this mode joins slices, or reads them again (inverse CDF), and so needs their results kept.
-static int64_t parts_bytes(const Plan &p, int64_t B) { return p.one ? 0 : B * p.slices * static_cast<int64_t>(sizeof(Part)); }
+static int64_t parts_bytes(const Plan &p, int64_t B) {
+  return p.one ? 0 : B * p.slices * static_cast<int64_t>(sizeof(Part));
+}
 
 extern "C" int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t hist_cols, int32_t mode, int64_t *bytes) {
   VK_CHECK_ARG(bytes && B >= 0 && V > 0 && V <= CH_V_MAX && hist_cols >= 0, "choose_tokens_workspace: bad arguments");
@@ -976,8 +993,8 @@ static int choose(const void *logits, int32_t dtype, int64_t ld, const Rules &r,
   if (rc != VK_OK) return rc;
   rc = check_rules(r, B, V, what);
   if (rc != VK_OK) return rc;
-  VK_CHECK_ARG(mode == CH_GREEDY || mode == CH_GUMBEL || mode == CH_CDF, "%s: mode 0 (greedy), 1 (Gumbel) or 2 (inverse CDF)",
-               what);
+  VK_CHECK_ARG(mode == CH_GREEDY || mode == CH_GUMBEL || mode == CH_CDF,
+               "%s: mode 0 (greedy), 1 (Gumbel) or 2 (inverse CDF)", what);
   const int64_t per = mode == CH_GUMBEL ? V : 1;
   VK_CHECK_ARG(mode == CH_GREEDY || (noise.u != nullptr && noise.cols > 0 && noise.ld >= noise.cols * per),
                "%s: sampling needs uniforms, rows of columns x %lld", what, static_cast<long long>(per));

@@ -1,6 +1,8 @@
 // The token embedding at vocabularies past the 4-mers': the lookup of scaled rows and the table's gradient.
 //
-// Lookup: out[r, :] = round(scale * W[t_r, :]), the product in fp32. Ids outside [0, V) give zero rows.
+// Lookup: out[r, :] = round(scale * W[t_r, :]), the product in fp32. Ids outside [0, V) give zero rows. Bound by the rows
+// written (a frequent token's row is read from a cache): 524288 rows of 512 fp32 take 224 us (4.8 TB/s written), 40961 of
+// 1000 bf16 24 us; with stores that go through the caches 244 and 31.
 //
 // Gradient: g[v, :] = scale * sum over t_r = v of dY[r, :], fp32, without atomics on floats. Rows are brought into token
 // order first (a stable sort of the ids, row numbers as its payload), so that every vocabulary row is one run of
@@ -10,12 +12,15 @@
 //   n <= ES_RANK_MAX: the position of a row is a count, pos = #{key_j < key_i} + #{j < i: key_j = key_i}, taken over all
 //     n keys in LDS, in one launch;
 //   larger n: radix passes over digits of at most 9 bits (2 for the vocabularies of k = 5 .. 8), each a histogram per tile
-//     of 4096 keys and a stable scatter.
-// The sum goes by chunks of 64 sorted positions, one wavefront per 512 columns of each, which keeps loads of 4 to 8
-// gradient rows in flight whatever runs they belong to: it writes the runs that start in its chunk, up to 64 positions past it.
+//     of 1024 or 2048 keys and a stable scatter.
+// The sum goes by chunks of 16 to 64 sorted positions, one wavefront per 16 bytes x 64 columns of each, with the loads of 8
+// gradient rows in flight whatever runs they belong to: it writes the runs that start in its chunk, up to a chunk past it.
 // A longer run (padding, a homopolymer: tokens that a large part of the rows share) is cut at the chunks' borders, so that
 // it spreads over the chip; the join adds its partial sums in chunk order. Rows without a run are zeroed by wavefronts of
 // their own.
+// What bounds it: few rows, the launches in series (1003 x 512 fp32: rank 4.4, sum 6.5, join 3.2 us); many, the sum's bytes
+// (524288 x 512 fp32 into 87383 rows: 194 us for 1035 MB, 5.3 TB/s; the sort 36 us, the join 5.5). 98305 x 768 bf16 into
+// 21847 rows: sort 22, sum 48 (218 MB), join 7.5.
 #include "row_access.h"
 
 namespace vk {
@@ -23,7 +28,8 @@ namespace vk {
 constexpr int EL_WIDTH_MAX = 1 << 20;                // elements of a row
 constexpr int64_t EL_GRID_MAX = int64_t(1) << 24;  // workgroups of 256 threads: a launch has fewer than 2^32 threads
 
-// LPR lanes share a row (64 / LPR rows per wavefront side by side), N elements each: 16-byte accesses of the narrower
+// LPR lanes share a row (64 / LPR rows per wavefront side by side), N elements each, as few as span the row (65536 bf16
+// rows of 64, 128, 256: 4.5, 5.6, 9.1 us with 16, 16, 32 lanes, 10.8, 12.1, 12.7 with 64): 16-byte accesses of the narrower
 // type where both are bf16, of the fp32 side otherwise. A group of columns that the row's end cuts is moved back to stay
 // inside the row (columns that two lanes hold get the same value); rows narrower than a group go column by column. The
 // rows written are not read again here: past the caches, which keep the table.
@@ -55,13 +61,23 @@ __global__ __launch_bounds__(256) void embed_lookup_kernel(const WT *__restrict_
 
 // ---- the sort ----------------------------------------------------------------------------------------------------------
 
-constexpr int ES_RANK_MAX = 4096;  // rows that the counting sort takes
-constexpr int ES_RANK_ROWS = 16;   // rows per workgroup of it
-constexpr int ES_SMALL = 131072;   // rows up to which a workgroup of a radix pass takes 1024 keys; more: 2048
-constexpr int ES_BITS = 9;         // digit bits at most
-constexpr int ES_FUSED = 128;      // tiles up to which a scatter sums the earlier tiles' counts itself
-constexpr int ES_SHORT = 16384;    // rows up to which chunks are of 16 positions,
-constexpr int ES_MEDIUM = 131072;  // and of 32
+// The borders below, in rows, with the whole gradient's time on either side (us, rows of 512 fp32, 5463 ids).
+// The counting sort up to here: its work grows with n^2. 2048 rows: 16.8, radix 23.4; 4096: 22.8, 24.6; 8192: 37.0, 27.1.
+constexpr int ES_RANK_MAX = 4096;
+constexpr int ES_RANK_ROWS = 16;  // rows per workgroup of it
+// Tiles of 1024 keys up to here, which spread a pass over more CUs, then 2048, which make fewer tiles to sum. 32768 rows:
+// 34.4, with 2048 36.8; 131072: 74.2, 74.6; 524288: 223 with 1024, 220.
+constexpr int ES_SMALL = 131072;
+constexpr int ES_BITS = 9;  // digit bits at most
+// Tiles up to which a scatter sums the earlier tiles' counts itself, which spares a launch but reads all counts once per
+// tile. 128 tiles (262144 rows of 64): 48.6, with a scan of its own 48.4; 256: 71.4, 68.8.
+constexpr int ES_FUSED = 128;
+// Chunks of 16 positions up to here: a wavefront's loads are serial, and few rows make few wavefronts. 1003 rows: 13.7, of
+// 32 14.3, of 64 21.5; 16384: 29.0, 30.1, 35.3; 32768: 35.3, 34.2, 37.4.
+constexpr int ES_SHORT = 16384;
+// Chunks of 32 up to here, then 64: a chunk's border costs a long run a partial sum, written and read. 65536 rows: 52 with
+// 16, 46.8 with 32, 48.3 with 64; 98304: 32 64.5, 64 64.1; 131072: 93, 74.5, 70.3; 262144: 190, 131, 117.
+constexpr int ES_MEDIUM = 102400;
 
 constexpr int64_t ES_ROWS_MAX = (int64_t(1) << 31) - 4096;  // (32-bit positions, a tile or chunk past the last included)
 constexpr uint32_t ES_NONE = 0xffffffffu;  // a key that is none: ignored, or past the last
@@ -74,7 +90,8 @@ __device__ __forceinline__ uint32_t sort_key(int64_t t, int32_t V, int64_t pad) 
   return t >= 0 && t < V && t != pad ? static_cast<uint32_t>(t) : static_cast<uint32_t>(V);
 }
 
-// 16 rows per workgroup, 16 threads each over a sixteenth of the keys, four at a time.
+// 16 rows per workgroup, 16 threads each over a sixteenth of the keys, four at a time. Bound by its n^2 / 4 LDS reads of 16
+// bytes: 4.4 us at n = 1003.
 __global__ __launch_bounds__(256) void embed_rank_kernel(const int64_t *__restrict__ tokens, int32_t n, int32_t V,
                                                          int64_t pad, Pair *__restrict__ sorted,
                                                          int32_t *__restrict__ owners) {
@@ -99,8 +116,8 @@ __global__ __launch_bounds__(256) void embed_rank_kernel(const int64_t *__restri
   if (live && part == 0) sorted[pos] = Pair{mine, static_cast<uint32_t>(i)};
 }
 
-// counts [tiles, bins]: keys of each digit in each tile of KEYS x 1024. The first pass takes the ids themselves, and empties the list of
-// long runs.
+// counts [tiles, bins]: keys of each digit in each tile of KEYS x 1024 (4 to 5 us: a launch and one memory round trip).
+// The first pass takes the ids themselves, and empties the list of long runs.
 template <int KEYS, bool FIRST>
 __global__ __launch_bounds__(1024) void embed_hist_kernel(const int64_t *__restrict__ tokens, const Pair *__restrict__ pairs,
                                                           int64_t n, int32_t V, int64_t pad, int shift, int bins,
@@ -154,7 +171,8 @@ __global__ __launch_bounds__(64) void embed_scan_kernel(uint32_t *__restrict__ c
 // A stable scatter: wavefront w of a tile owns 64 KEYS keys side by side, in KEYS rounds of 64, so (w, round, lane) is
 // the keys' order. In a round the lanes of one digit find each other by a ballot per digit bit; a key's rank is the
 // digit's count in this wavefront's earlier rounds plus its lanes below. FUSED: the tile's offsets are summed here from
-// the counts of all (at most ES_FUSED) tiles, two threads per digit.
+// the counts of all (at most ES_FUSED) tiles, two threads per digit. 7 us at 98305 rows, 8 at 524288: the chain of load,
+// ranks, offsets and scattered stores.
 template <int KEYS, bool FIRST, bool FUSED>
 __global__ __launch_bounds__(1024) void embed_scatter_kernel(const int64_t *__restrict__ tokens,
                                                              const Pair *__restrict__ in, int64_t n, int32_t V, int64_t pad,
@@ -302,8 +320,8 @@ struct Cols {
   // Adds positions [a, b) of 64, whose gradient rows' numbers are in the lanes of `rows`: U rows' loads in flight. RUNS:
   // where `heads` has a bit, the run before that position ends; it goes to the row of `out` that its key names.
   template <bool RUNS>
-  __device__ __forceinline__ void walk(const T *drows, int64_t ld, uint32_t rows, int a, int b, uint64_t heads, uint32_t keys,
-                                       float *out, float scale, bool onto) {
+  __device__ __forceinline__ void walk(const T *drows, int64_t ld, uint32_t rows, int a, int b, uint64_t heads,
+                                       uint32_t keys, float *out, float scale, bool onto) {
     for (int p = a; p < b; p += U) {
       u32x4 w[U];
 #pragma unroll
@@ -315,7 +333,8 @@ struct Cols {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (p + u < b) {
-          if (RUNS && ((h >> u) & 1)) put(out + static_cast<int64_t>(__builtin_amdgcn_readlane(keys, p + u - 1)) * d, scale, onto);
+          if (RUNS && ((h >> u) & 1))
+            put(out + static_cast<int64_t>(__builtin_amdgcn_readlane(keys, p + u - 1)) * d, scale, onto);
           add(w[u]);
         }
       }
@@ -330,8 +349,8 @@ struct Cols {
 template <typename T, bool PLAIN, int CHUNK>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const T *__restrict__ drows, int64_t ld, int32_t n, int32_t V,
                                                         int d, const Pair *__restrict__ sorted, int32_t chunks, float scale,
-                                                        int accumulate, float *__restrict__ part, int32_t *__restrict__ owners,
-                                                        float *__restrict__ out) {
+                                                        int accumulate, float *__restrict__ part,
+                                                        int32_t *__restrict__ owners, float *__restrict__ out) {
   const int lane = threadIdx.x & 63;
   const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t uV = static_cast<uint32_t>(V);
@@ -349,7 +368,8 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T *__restrict__ dr
         hi = mid;
     }
     const bool absent = v < V && !(lo < n && sorted[lo].key == static_cast<uint32_t>(v));
-    for (uint64_t left = __ballot(absent); left != 0; left &= left - 1) x.put(out + (v0 + __builtin_ctzll(left)) * d, 1.f, false);
+    for (uint64_t left = __ballot(absent); left != 0; left &= left - 1)
+      x.put(out + (v0 + __builtin_ctzll(left)) * d, 1.f, false);
     return;
   }
   const int p0 = static_cast<int>(wave) * CHUNK;
@@ -397,7 +417,8 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T *__restrict__ dr
 constexpr int EJ_GROUPS = 32;
 
 // Long runs: workgroups take (a run's first chunk, 64 columns) and add the run's partials in chunk order: 32 groups of 16
-// lanes take every 32nd, then the groups are added in order.
+// lanes take every 32nd, then the groups are added in order. 3.2 us for a fifth of 1003 rows, 5.5 for one of 524288; a
+// workgroup per chunk, most of which have nothing to add, took 115 us there.
 __global__ __launch_bounds__(512) void embed_join_kernel(const Pair *__restrict__ sorted, int d, int chunk, int32_t chunks,
                                                          const float *__restrict__ part, const int32_t *__restrict__ owners,
                                                          float scale, int accumulate, float *__restrict__ out) {
@@ -482,14 +503,15 @@ static SortPlan sort_plan(int64_t n, int32_t V, int32_t d) {
 }
 
 template <int KEYS, bool FIRST>
-static void launch_pass(const SortPlan &p, const int64_t *tokens, const Pair *in, Pair *out, int64_t n, int32_t V, int64_t pad,
-                        int shift, uint32_t *counts, uint32_t *totals, int32_t *owners, hipStream_t s) {
+static void launch_pass(const SortPlan &p, const int64_t *tokens, const Pair *in, Pair *out, int64_t n, int32_t V,
+                        int64_t pad, int shift, uint32_t *counts, uint32_t *totals, int32_t *owners, hipStream_t s) {
   const unsigned tiles = static_cast<unsigned>(p.tiles), bins = 1u << p.bits;
   embed_hist_kernel<KEYS, FIRST><<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, bins, counts, owners);
   if constexpr (KEYS == 2) {  // (1024 keys each: ES_SMALL rows are ES_FUSED tiles)
     if (p.tiles > ES_FUSED) {
       embed_scan_kernel<<<bins, 64, 0, s>>>(counts, p.tiles, bins, totals);
-      embed_scatter_kernel<2, FIRST, false><<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, p.bits, counts, totals, out);
+      embed_scatter_kernel<2, FIRST, false>
+          <<<tiles, 1024, 0, s>>>(tokens, in, n, V, pad, shift, p.bits, counts, totals, out);
       return;
     }
   }
@@ -503,9 +525,11 @@ using namespace vk;
 
 extern "C" int vk_embed_lookup(const void *w, int32_t w_dtype, const int64_t *tokens, int64_t n, int64_t V, int32_t d,
                                float scale, void *out, int32_t out_dtype, void *stream) {
-  VK_CHECK_ARG(n >= 0 && V > 0 && d > 0 && d <= EL_WIDTH_MAX, "embed_lookup: bad sizes (V=%lld d=%d)", static_cast<long long>(V), d);
+  VK_CHECK_ARG(n >= 0 && V > 0 && d > 0 && d <= EL_WIDTH_MAX, "embed_lookup: bad sizes (V=%lld d=%d)",
+               static_cast<long long>(V), d);
   VK_CHECK_ARG(n == 0 || (w && tokens && out), "embed_lookup: null pointer");
-  VK_CHECK_ARG((w_dtype == VK_DTYPE_BF16 || w_dtype == VK_DTYPE_F32) && (out_dtype == VK_DTYPE_BF16 || out_dtype == VK_DTYPE_F32),
+  VK_CHECK_ARG((w_dtype == VK_DTYPE_BF16 || w_dtype == VK_DTYPE_F32) &&
+                   (out_dtype == VK_DTYPE_BF16 || out_dtype == VK_DTYPE_F32),
                "embed_lookup: bad dtype");
   if (n == 0) return VK_OK;
   const bool wf = w_dtype == VK_DTYPE_F32, of = out_dtype == VK_DTYPE_F32;
@@ -598,8 +622,9 @@ extern "C" int vk_embed_grad_sorted(const void *d_rows, int32_t d_dtype, int64_t
 #undef VK_EMBED_SUM
   rc = launch_status("embed_grad_sorted sum");
   if (rc != VK_OK || n < 2 * p.chunk) return rc;
-  const int64_t most = (n / (p.chunk + 1) + 1) * ((d + 63) / 64), cap = 4 * device_cus_cached();  // (a long run: chunk + 1 rows)
-  embed_join_kernel<<<static_cast<unsigned>(most < cap ? most : cap), 512, 0, s>>>(pairs(at), d, p.chunk, p.chunks, part, owners, scale,
-                                                                               accumulate, out);
+  const int64_t most = (n / (p.chunk + 1) + 1) * ((d + 63) / 64);  // (a long run: chunk + 1 rows)
+  const int64_t cap = 4 * device_cus_cached();
+  embed_join_kernel<<<static_cast<unsigned>(most < cap ? most : cap), 512, 0, s>>>(
+      pairs(at), d, p.chunk, p.chunks, part, owners, scale, accumulate, out);
   return launch_status("embed_grad_sorted join");
 }

@@ -119,8 +119,9 @@ class DecodeEngine:
         self.allowed = self.token_rows = None
         if grammar is not None:
             mask, rows = (torch.as_tensor(t) for t in grammar)
-            if mask.dtype != torch.bool or mask.dim() != 2 or mask.shape[1] != tk.vocab_size or rows.shape != (tk.vocab_size,) \
-                    or rows.dtype not in (torch.int32, torch.int64) or mask.shape[0] == 0 or int(rows.max()) >= mask.shape[0]:
+            V = tk.vocab_size
+            if mask.dtype != torch.bool or mask.dim() != 2 or mask.shape[1] != V or mask.shape[0] == 0 or rows.shape != (V,) \
+                    or rows.dtype not in (torch.int32, torch.int64) or int(rows.max()) >= mask.shape[0]:
                 raise ValueError("grammar: (allowed bool [S, V], rows int [V] with values below S)")
             self.allowed = ops.pack_allowed(mask.to(dev))
             self.token_rows = rows.clamp(min=-1).to(dev, torch.int32).contiguous()

@@ -6,6 +6,9 @@ fused ops so FastDecoder / DecodeEngine code reads the same:
   varlen_attention  (flash_attn_varlen_func as used at viktor/fast_decoder.py:68-73)
   select_update     (LM head + DecodeEngine._select + step bookkeeping, viktor/engine.py:79-116)
   gspo_score, group_advantage  (scripts/gspo.py:340-353, 446-477)
+  embed_lookup, embed_grad_sorted  (nn.Embedding's gather and its backward at large vocabularies, viktor/model.py:77)
+  process_logits, choose_tokens, choose_update  (penalties, bias and grammar masks on logits, and the token choice, at
+                                                 vocabularies past select_update's 512)
 
 Outputs are allocated with torch.empty on the input's device; documented in-place updates: x in
 add_rmsnorm, the KV cache in qkv_rope_cache, the decode state in greedy_update / select_update.
@@ -1079,7 +1082,8 @@ def choose_tokens(logits, history=None, lengths=None, repetition=1.0, presence=0
                   allowed_rows=None, temperature=0.0, uniforms=None, fallback=0):
     """The token choice over any vocabulary after process_logits' rules, which are applied on the fly (logits stay as they
     are). z' = z / temperature where it is positive (a float or fp32 [B]); a row with temperature <= 0 is greedy (the first
-    index of the maximum), an infinite temperature is the largest finite one. uniforms in [0, 1): fp32 [B, V] for the Gumbel choice, first argmax of z' - log(-log(max(u, 1e-20)))
+    index of the maximum), an infinite temperature is the largest finite one. uniforms in [0, 1): fp32 [B, V] for the
+    Gumbel choice, first argmax of z' - log(-log(max(u, 1e-20)))
     (viktor/engine.py:80-83's formula), or fp32 [B] for the inverse CDF, the first v with u < sum_{w <= v} softmax(z')_w.
     Returns (tokens int64 [B], logp fp32 [B]), logp = log softmax(z')[token]. NaN is never chosen and weighs nothing, +inf
     counts as the largest finite value; a row with nothing left gives `fallback` and -inf."""

@@ -137,7 +137,8 @@ class Basecaller(nn.Module):
             return self._hidden_shared(frames, tokens_in, plens_h, int(group_size))
         prefix = self.project(frames)                                       # [B, P, d] bf16
         fast = self.decoder.fast()
-        emb = ops.embed_lookup(fast.w32(self.decoder.embed.weight), tokens_in.to(dev, torch.long).contiguous())  # [B, T, d] fp32
+        emb = ops.embed_lookup(fast.w32(self.decoder.embed.weight),
+                               tokens_in.to(dev, torch.long).contiguous())                  # [B, T, d] fp32
         s = self.pos_scale
 
         def build():  # the packing plan, the window layout's row indices and each row's (rotary) position
@@ -185,7 +186,8 @@ class Basecaller(nn.Module):
         else:
             x_pre = torch.cat([prefix[g, :p] for g, p in enumerate(pre_lens)]).float()
         fast = self.decoder.fast()
-        x_tok = ops.embed_lookup(fast.w32(self.decoder.embed.weight), tokens_in.to(dev, torch.long).reshape(-1).contiguous())  # [B T, d] fp32
+        x_tok = ops.embed_lookup(fast.w32(self.decoder.embed.weight),
+                                 tokens_in.to(dev, torch.long).reshape(-1).contiguous())     # [B T, d] fp32
         s = self.pos_scale
 
         def build():
