@@ -309,10 +309,10 @@ int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, const int64
  *   mode 2: the first v with u < sum_{w <= v} softmax(z')_w, u = uniforms[b * u_ld] (sums over slices in fp64).
  * token[b] (int64) and logp[b] = log softmax(z')[token] (NULL: not written). NaN is never chosen and weighs nothing, +inf
  * counts as the largest finite value; a row whose mask and bias leave nothing gives `fallback` and -inf.
- * workspace: vk_choose_tokens_workspace() bytes for these B, V, hist_cols (0 without a history) and mode, 16-byte aligned;
+ * workspace: vk_choose_tokens_workspace() bytes for these B, V and hist_cols (0 without a history), 16-byte aligned;
  * NULL where that is 0.
  */
-int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t hist_cols, int32_t mode, int64_t *bytes);
+int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t hist_cols, int64_t *bytes);
 int vk_choose_tokens(const void *logits, int32_t dtype, int64_t ld, const int64_t *hist, int64_t hist_ld,
                      int64_t hist_cols, const int32_t *hist_len, const float *rep, float rep0, const float *pres,
                      float pres0, const float *freq, float freq0, const float *bias, int64_t bias_ld,

@@ -97,12 +97,11 @@ def test_choose_tokens_refuses():
         _err(_choose(lib, p, **kw), word)
     assert _choose(lib, p, B=0) == 0
     need = ctypes.c_int64(0)
-    assert lib.vk_choose_tokens_workspace(0, 40, 0, 0, ctypes.byref(need)) == 0 and need.value == 0
-    assert lib.vk_choose_tokens_workspace(3, 40, 5, 0, ctypes.byref(need)) == 0 and need.value == 0  # one launch
-    assert lib.vk_choose_tokens_workspace(3, 40, 5, 2, ctypes.byref(need)) == 0 and need.value > 0
-    assert lib.vk_choose_tokens_workspace(3, 87383, 5, 0, ctypes.byref(need)) == 0 and need.value > 0
-    _err(lib.vk_choose_tokens_workspace(-1, 40, 0, 0, ctypes.byref(need)), b"arguments")
-    _err(lib.vk_choose_tokens_workspace(1, 2 ** 31 - 1, 0, 0, ctypes.byref(need)), b"arguments")
+    assert lib.vk_choose_tokens_workspace(0, 40, 0, ctypes.byref(need)) == 0 and need.value == 0
+    assert lib.vk_choose_tokens_workspace(3, 40, 5, ctypes.byref(need)) == 0 and need.value == 0  # one launch
+    assert lib.vk_choose_tokens_workspace(3, 87383, 5, ctypes.byref(need)) == 0 and need.value > 0
+    _err(lib.vk_choose_tokens_workspace(-1, 40, 0, ctypes.byref(need)), b"arguments")
+    _err(lib.vk_choose_tokens_workspace(1, 2 ** 31 - 1, 0, ctypes.byref(need)), b"arguments")
 
 
 def test_choose_update_refuses():

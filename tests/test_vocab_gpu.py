@@ -444,6 +444,22 @@ def test_choose_tokens_gumbel_near_ties():
     assert torch.equal(got.cpu(), torch.minimum(a, b))
 
 
+def _check_cdf(z, temp, u, got, glp):
+    B = len(u)
+    greedy, glpref, big = _choice_ref(z, temp)
+    zt = torch.where(temp[:, None] > 0, z / torch.where(temp > 0, temp, torch.ones_like(temp))[:, None], z)
+    for b in range(B):
+        if greedy[b] < 0 or temp[b] <= 0:
+            assert got[b] == greedy[b]
+            continue
+        p = torch.softmax(zt[b].double(), 0)
+        c = p.cumsum(0)
+        t = int(got[b])
+        tol = 2 * U * float(200 + 16 * big[b])
+        assert p[t] > 0 and float(c[t]) + tol > float(u[b]) >= float(c[t] - p[t]) - tol, b
+        _check_logp(glp[b:b + 1], torch.log(p[t:t + 1]), big[b:b + 1])
+
+
 @pytest.mark.parametrize("B,V,T", SIZES)
 @pytest.mark.parametrize("dt", [F32, BF])
 def test_choose_tokens_inverse_cdf(B, V, T, dt):
@@ -461,18 +477,32 @@ def test_choose_tokens_inverse_cdf(B, V, T, dt):
     got, glp = ops.choose_tokens(x.to(DEV), **kw, allowed=ops.pack_allowed(masks).to(DEV), allowed_rows=rows.to(DEV),
                                  temperature=temp.to(DEV), uniforms=u.to(DEV), fallback=-1)
     got, glp = got.cpu(), glp.cpu()
-    greedy, glpref, big = _choice_ref(z, temp)
-    zt = torch.where(temp[:, None] > 0, z / torch.where(temp > 0, temp, torch.ones_like(temp))[:, None], z)
-    for b in range(B):
-        if greedy[b] < 0 or temp[b] <= 0:
-            assert got[b] == greedy[b]
-            continue
-        p = torch.softmax(zt[b].double(), 0)
-        c = p.cumsum(0)
-        t = int(got[b])
-        tol = 2 * U * float(200 + 16 * big[b])
-        assert p[t] > 0 and float(c[t]) + tol > float(u[b]) >= float(c[t] - p[t]) - tol, b
-        _check_logp(glp[b:b + 1], torch.log(p[t:t + 1]), big[b:b + 1])
+    _check_cdf(z, temp, u, got, glp)
+
+
+@pytest.mark.parametrize("B,V,T", [(192, 70001, 300), (250, 20000, 2048), (300, 40000, 64), (2, 600001, 500)])
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_choose_tokens_inverse_cdf_of_long_rows(B, V, T, dt):
+    """Rows of several batches in one workgroup, and of many slices: every target from the first token with weight to the
+    last, most of a row's weight on tokens of its history in some, rows without anything."""
+    x, hist, lens, rep, pres, freq, bias, masks, rows, mask = _case(B, V, T, B + V + 4, dt)
+    g = _gen(V + 2)
+    heavy = torch.arange(0, B, 3)
+    x[heavy[:, None], hist[heavy, :5].clamp(max=V - 1)] = torch.tensor(14.0, dtype=dt)
+    temp = 0.7 + torch.rand(B, generator=g)
+    temp[4::9] = 0
+    u = torch.rand(B, generator=g)
+    u[::5] = 0
+    u[1::5] = 1 - 2.0 ** -24
+    x[7::50] = float("-inf")
+    z = _tame(_rules_ref(x, hist, lens, rep, pres, freq, bias, mask))
+    kw = dict(zip(("history", "lengths", "repetition", "presence", "frequency", "bias"), _dev(hist, lens, rep, pres, freq, bias)))
+    args = dict(**kw, allowed=ops.pack_allowed(masks).to(DEV), allowed_rows=rows.to(DEV), temperature=temp.to(DEV),
+                uniforms=u.to(DEV), fallback=-1)
+    got, glp = ops.choose_tokens(x.to(DEV), **args)
+    _check_cdf(z, temp, u, got.cpu(), glp.cpu())
+    again = ops.choose_tokens(x.to(DEV), **args)
+    assert torch.equal(again[0], got) and torch.equal(again[1], glp)
 
 
 def test_choose_tokens_odd_values():
@@ -563,6 +593,20 @@ def test_choose_tokens_of_the_widest_whole_rows():
         got, glp = ops.choose_tokens(x, hist, lens, 1.25, 0.5, 0.25, temperature=t if temp else 0.0, uniforms=u if temp else None)
         assert torch.equal(got[rows].cpu(), tok)
         _check_logp(glp[rows], lp, big)
+
+
+@pytest.mark.parametrize("B,V,T", [(40, 1367, 2000), (200, 5463, 2048), (9, 21847, 3000), (3, 87383, 2048), (200, 87383, 700)])
+def test_choose_tokens_again_the_same_bits(B, V, T):
+    """Long histories, whose tokens are found in another order each time: tokens and log-probabilities stay."""
+    x, hist, lens, rep, pres, freq, bias, masks, rows, mask = _case(B, V, T, B + V + 5)
+    x, hist, lens, rep, pres, freq, bias, rows = _dev(x, hist, lens, rep, pres, freq, bias, rows)
+    u = torch.rand(B, V, generator=torch.Generator(DEV).manual_seed(6), device=DEV)
+    allowed = ops.pack_allowed(masks).to(DEV)
+    for kw in ({}, {"temperature": 0.9, "uniforms": u}, {"temperature": 0.9, "uniforms": u[:, 0].contiguous()}):
+        first = ops.choose_tokens(x, hist, lens, rep, pres, freq, bias, allowed, rows, **kw)
+        for _ in range(6):
+            again = ops.choose_tokens(x, hist, lens, rep, pres, freq, bias, allowed, rows, **kw)
+            assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1]), list(kw)
 
 
 # ---- streams, graphs, refusals -----------------------------------------------------------------------------------------------

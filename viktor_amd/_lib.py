@@ -72,7 +72,7 @@ SIGNATURES = {
     "vk_embed_grad_sorted": [_P, _I32, _I64, _P, _I64, _I32, _I32, _F, _I64, _P, _I32, _P, _I64, _P],
     "vk_process_logits": [_P, _I32, _I64, _P, _I64, _I64, _P, _P, _F, _P, _F, _P, _F, _P, _I64, _P, _I64, _I64, _P, _P, _I32,
                           _I64, _I64, _I32, _P],
-    "vk_choose_tokens_workspace": [_I64, _I32, _I64, _I32, ctypes.POINTER(_I64)],
+    "vk_choose_tokens_workspace": [_I64, _I32, _I64, ctypes.POINTER(_I64)],
     "vk_choose_tokens": [_P, _I32, _I64, _P, _I64, _I64, _P, _P, _F, _P, _F, _P, _F, _P, _I64, _P, _I64, _I64, _P, _P, _F,
                          _I32, _P, _I64, _I64, _P, _P, _I64, _I32, _P, _I64, _P],
     "vk_choose_update": [_P, _I32, _I64, _F, _F, _F, _P, _P, _I64, _I64, _P, _P, _P, _I32, _F, _I32, _P, _I64, _I64, _P, _P,

@@ -22,11 +22,15 @@
 //   process bf16      37      45     38         43           51 (46.8 from logits that are not in a cache)
 //   process fp32      74      78     76         82           83
 //   greedy fp32       31.5    37     33         34           41.5
-//   greedy bf16       23.6    32     27         26           36
+//   greedy bf16       23.6    32     27         26           37
+// The inverse CDF keeps its sums by batch or slice and reads only the batch or slice that the uniform falls into again: with
+// a bias 49 (fp32) and 42 (bf16), with all rules 56 and 47; 5463 tokens 23 against 10 greedy.
 // Measured and not taken: bias and mask loaded a batch ahead (process fp32 -4, all bf16 +2), two sequences a workgroup that
 // share the bias (bf16 -0.6, fp32 +5), 8-byte loads of bf16 (+1 to +2), 1024 threads a row (+5).
 #include <float.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "decode_state.h"
 #include "row_access.h"
@@ -195,11 +199,6 @@ __device__ __forceinline__ float one_logit(const T *row, const RowRules &r, int 
   }
   if (r.bias != nullptr) z = z + bias;
   return allowed ? z : -INFINITY;
-}
-
-template <typename T, int THREADS>
-__device__ __forceinline__ float one_logit(const T *row, const RowRules &r, const Seen<THREADS> &s, int v0, int v) {
-  return one_logit(row, r, v, r.len > 0 && s.has(v - v0) ? s.count[s.slot(v - v0)] : 0);
 }
 
 // What a thread takes of a workgroup's next 16 THREADS tokens: R vectors of N tokens, vector q at token
@@ -498,7 +497,7 @@ __device__ __forceinline__ float wave_max_of(float v) {
   return v;
 }
 
-// What a thread knows of its tokens: the maximum of z (at least -FLT_MAX), the sum of exponentials at it, the best logit
+// What a thread knows of its tokens (without the history's): the maximum of z (at least -FLT_MAX), the sum of exponentials at it, the best logit
 // or score with its first token, and the second best score. A batch that has nothing near the wavefront's best so far is
 // not looked through for them (a thread's next best comes in most batches, a wavefront's in one of i at the i-th).
 struct Mine {
@@ -526,11 +525,12 @@ struct Uniforms {
   }
 };
 
-template <typename T, int THREADS, bool GUMBEL, bool CUT, bool MORE>
-__device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, THREADS, GUMBEL> &un, Mine &t, const T *row,
-                                             const float *urow, const RowRules &r, const Scale &c, const Seen<THREADS> &s,
+template <typename T, int THREADS, int MODE, bool CUT, bool MORE>
+__device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, THREADS, MODE == CH_GUMBEL> &un,
+                                             Mine &t, const T *row, const float *urow, const RowRules &r, const Scale &c, const Seen<THREADS> &s,
                                              int v0, int w, int V) {
   using X = Batch<T, THREADS>;
+  constexpr bool GUMBEL = MODE == CH_GUMBEL;
   const bool noisy = GUMBEL && c.T > 0.f;
   float z[X::R][X::N], u[GUMBEL ? X::R : 1][X::N];
   un.take(u);
@@ -545,13 +545,15 @@ __device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, T
       z[q][k + 1] = tame(z[q][k + 1]);
       top = vmax3(top, z[q][k], z[q][k + 1]);
     }
-  const float m = vmax2(t.m, top);
-  t.sum *= __builtin_amdgcn_exp2f((t.m - m) * c.L);
-  t.m = m;
+  if constexpr (MODE != CH_CDF) {
+    const float m = vmax2(t.m, top);
+    t.sum *= __builtin_amdgcn_exp2f((t.m - m) * c.L);
+    t.m = m;
 #pragma unroll
-  for (int q = 0; q < X::R; ++q)
+    for (int q = 0; q < X::R; ++q)
 #pragma unroll
-    for (int k = 0; k < X::N; ++k) t.sum += __builtin_amdgcn_exp2f((z[q][k] - m) * c.L);
+      for (int k = 0; k < X::N; ++k) t.sum += __builtin_amdgcn_exp2f((z[q][k] - m) * c.L);
+  }
   if (noisy) {
     if constexpr (GUMBEL) {
       if (CUT)
@@ -585,9 +587,9 @@ __device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, T
         t.wave_best = wave_max_of(t.best);
       }
     }
-  } else if (__any(top >= t.wave_best && top > -INFINITY)) {
-    if (top > t.best || (top == t.best && top > -INFINITY)) {  // (a token of the history may be behind these)
-      t.v = top > t.best ? 0x7fffffff : t.v;
+  } else if (__any(top > t.wave_best)) {  // (a later batch's equal logit is behind the earlier one's)
+    if (top > t.best) {
+      t.v = 0x7fffffff;
       t.best = top;
 #pragma unroll
       for (int q = X::R - 1; q >= 0; --q)
@@ -596,23 +598,189 @@ __device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, T
     }
     t.wave_best = wave_max_of(t.best);
   }
+  if constexpr (MODE == CH_CDF) {  // the wavefront's sum of the batch, at its largest logit so far
+    t.m = vmax2(t.wave_best, -FLT_MAX);
+    t.sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < X::R; ++q)
+#pragma unroll
+      for (int k = 0; k < X::N; ++k) t.sum += __builtin_amdgcn_exp2f((z[q][k] - t.m) * c.L);
+    t.sum = wave_sum(t.sum);
+  }
+}
+
+// ---- the inverse CDF ---------------------------------------------------------------------------------------------------
+
+// The history's logits of a slice, in place of their counts (between barriers).
+template <typename T, int THREADS>
+__device__ __forceinline__ void logits_for_counts(const Seen<THREADS> &s, const T *row, const RowRules &r, int v0) {
+  s.each([&](int rel, uint32_t &count) { count = __float_as_uint(one_logit(row, r, v0 + rel, count)); });
+}
+
+// A weight exp((z - M) / T) of at most 1 in whole steps of 2^-40. The history's tokens are added up in these: which thread
+// finds which of them first is not the same in every run, and the order of additions does not matter where they are exact
+// (a slice's distinct tokens, at most 8192, come to 2^53 steps).
+constexpr double STEPS = 1099511627776.;
+__device__ __forceinline__ double weight_steps(float z, float M, const Scale &c) {
+  return floor(static_cast<double>(__builtin_amdgcn_exp2f((z - M) * c.L)) * STEPS);
+}
+
+// What the workgroup's threads share while they look for the token that the target falls into.
+template <int THREADS>
+struct Walk {
+  double segment[4 * (THREADS / 64)];  // sums of the wavefronts' tokens (R <= 4 times 64 N each), in token order
+  int found, last;                     // the token; the last one with any weight so far
+};
+
+// A batch's weights exp((z - M) / T) in token order, after `run`: the first token whose running sum passes the target. Sums
+// in 64 bits: a thread's N tokens, the wavefront's threads by a scan, and the wavefronts' segments one by one. Counts have
+// been replaced by logits. Ends with a barrier.
+template <typename T, int THREADS>
+__device__ __forceinline__ void walk_batch(Batch<T, THREADS> &x, const T *row, const RowRules &r, const Scale &c,
+                                           const Seen<THREADS> &s, int v0, int w, int V, float M, double target, double &run,
+                                           Walk<THREADS> &shared) {
+  using X = Batch<T, THREADS>;
+  constexpr int WAVES = THREADS / 64;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  float z[X::R][X::N];
+  double own[X::R], upto[X::R];
+  x.template rules<true, false>(z, row, r, w, V, nullptr, 0);
+#pragma unroll
+  for (int q = 0; q < X::R; ++q) {
+    if (r.len > 0) {
+      const int rel = X::token(w, q) - v0;
+      const uint32_t left = (s.bits[rel >> 5] >> (rel & 31)) & ((1u << X::N) - 1);
+      if (left != 0)
+#pragma unroll
+        for (int k = 0; k < X::N; ++k)
+          if ((left >> k) & 1) z[q][k] = __uint_as_float(s.count[s.slot(rel + k)]);
+    }
+    own[q] = 0.;
+#pragma unroll
+    for (int k = 0; k < X::N; ++k) {
+      z[q][k] = __builtin_amdgcn_exp2f((tame(z[q][k]) - M) * c.L);
+      own[q] += static_cast<double>(z[q][k]);
+    }
+    upto[q] = own[q];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double up = __shfl_up(upto[q], o, 64);
+      if (lane >= o) upto[q] += up;
+    }
+    if (lane == 63) shared.segment[q * WAVES + wid] = upto[q];
+  }
+  __syncthreads();
+  int hit = 0x7fffffff, top = -1;
+#pragma unroll
+  for (int q = 0; q < X::R; ++q) {
+    double cdf = run;
+    for (int i = 0; i < WAVES; ++i) {
+      if (i == wid) cdf = run;
+      run += shared.segment[q * WAVES + i];
+    }
+    cdf += upto[q] - own[q];
+#pragma unroll
+    for (int k = 0; k < X::N; ++k) {
+      cdf += static_cast<double>(z[q][k]);
+      if (z[q][k] > 0.f) {
+        top = X::token(w, q) + k;
+        if (hit == 0x7fffffff && target < cdf) hit = top;
+      }
+    }
+  }
+  if (hit != 0x7fffffff) atomicMin(&shared.found, hit);
+  if (top >= 0) atomicMax(&shared.last, top);
+  __syncthreads();
+}
+
+// The end of it, by one thread: the token found, or the last with weight (rounding, or a uniform of 1).
+template <typename T, int THREADS>
+__device__ __forceinline__ void finish_walk(const Walk<THREADS> &shared, const T *row, const RowRules &r, const Scale &c,
+                                            const Seen<THREADS> &s, int v0, int V, const Part &p, const Choice &choice,
+                                            const Step &step, int64_t b) {
+  const int pick = shared.found != 0x7fffffff ? shared.found : shared.last;
+  if (pick < 0) {  // (what has weight holds a token with weight)
+    finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
+  } else {
+    const bool seen = r.len > 0 && s.has(pick - v0);
+    const float z = seen ? __uint_as_float(s.count[s.slot(pick - v0)]) : one_logit(row, r, pick, 0);
+    finish_row(choice, step, b, V, pick, logp_of(tame(z), p, c));
+  }
+}
+
+// The whole row's sums by batch and wavefront, of a workgroup that takes a row.
+template <int THREADS>
+struct BatchSums {
+  static constexpr int MOST = CH_WHOLE / (16 * THREADS);
+  float sum[MOST][THREADS / 64], m[MOST][THREADS / 64];
+  double total[MOST];    // of a batch at the row's maximum
+  double history[MOST];  // of its history's tokens
+  Walk<THREADS> walk;
+};
+
+// The choice from a row's sums by batch (p: its maximum and its first best token): the totals at the maximum, the batch that
+// the target falls into, and the token in it.
+template <typename T, int THREADS>
+__device__ __forceinline__ void choose_from_sums(BatchSums<THREADS> &sums, Batch<T, THREADS> &x, const T *row, const RowRules &r,
+                                                 const Scale &c, const Seen<THREADS> &s, int V, int batches, Part p,
+                                                 const float *uniform, const Choice &choice, const Step &step, int64_t b) {
+  using X = Batch<T, THREADS>;
+  constexpr int WAVES = THREADS / 64;
+  const int tid = threadIdx.x;
+  if (r.len > 0)
+    s.each([&](int rel, uint32_t z) {
+      atomicAdd(&sums.history[rel / X::TOKENS], weight_steps(__uint_as_float(z), p.m, c));
+    });
+  __syncthreads();
+  if (tid < batches) {
+    double total = sums.history[tid] / STEPS;
+    for (int i = 0; i < WAVES; ++i)
+      total += static_cast<double>(sums.sum[tid][i]) * __builtin_amdgcn_exp2f((sums.m[tid][i] - p.m) * c.L);
+    sums.total[tid] = total;
+  }
+  __syncthreads();
+  double total = 0.;
+  for (int i = 0; i < batches; ++i) total += sums.total[i];
+  p.sum = static_cast<float>(total);
+  if (p.v < 0 || !(c.T > 0.f)) {
+    if (tid == 0) finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
+    return;
+  }
+  // (rounding, or a uniform of 1: the last batch with any weight)
+  const double target = static_cast<double>(*uniform) * total;
+  int at = 0;
+  double run = 0., before = 0.;
+  for (int i = 0; i < batches; ++i)
+    if (sums.total[i] > 0.) {
+      at = i;
+      run = before;
+      before += sums.total[i];
+      if (target < before) break;
+    }
+  if (V >= X::N) x.load(row, at * X::TOKENS, V);
+  walk_batch(x, row, r, c, s, 0, at * X::TOKENS, V, p.m, target, run, sums.walk);
+  if (tid == 0) finish_walk(sums.walk, row, r, c, s, 0, V, p, choice, step, b);
 }
 
 // One slice of one sequence, or with ONE the whole vocabulary and the step's end. The workgroup's best logit or score
 // tells who can have the best token: the lowest token of the largest logit, or the threads within the scores' slack of
 // the largest score. These read their token again and are compared exactly; one whose second score is as near goes
-// through all of its tokens, and so does every thread where all scores are below fp32's range. The sum is taken at the
-// workgroup's maximum.
-template <typename T, int THREADS, bool GUMBEL, bool ONE>
+// through all of its tokens, its history's too, and so does every thread where all scores are below fp32's range. The sum is taken at the
+// workgroup's maximum. Inverse CDF (ONE): the sums stay by batch, and the batch that the uniform falls into is walked.
+template <typename T, int THREADS, int MODE, bool ONE>
 __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restrict__ logits, int64_t ld, Rules rules,
                                                                    const float *__restrict__ temp, float temp0,
                                                                    Noise noise, int V, Plan plan,
                                                                    Part *__restrict__ parts, Choice choice, Step step) {
   extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
   constexpr int WAVES = THREADS / 64;
+  constexpr bool GUMBEL = MODE == CH_GUMBEL, CDF = MODE == CH_CDF;
+  static_assert(ONE || !CDF, "slices of the inverse CDF are the greedy choice's");
   __shared__ float red_m[WAVES], red_s[WAVES], red_sum[WAVES];
   __shared__ int first_best, contenders;
+  __shared__ double red_steps[WAVES];
   __shared__ Best contender[GUMBEL ? THREADS : 1];
+  __shared__ typename std::conditional<CDF, BatchSums<THREADS>, int>::type sums;
   using X = Batch<T, THREADS>;
   const int64_t b = ONE ? blockIdx.x : blockIdx.x / plan.slices;
   const int v0 = ONE ? 0 : static_cast<int>(blockIdx.x % plan.slices) * plan.slice;
@@ -633,31 +801,50 @@ __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restr
     first_best = 0x7fffffff;
     contenders = 0;
   }
+  if constexpr (CDF) {
+    if (tid < BatchSums<THREADS>::MOST) sums.history[tid] = 0;
+    if (tid == 0) {
+      sums.walk.found = 0x7fffffff;
+      sums.walk.last = -1;
+    }
+  }
   Mine t;
+  // the history's largest logit and its best logit or score of this thread's, apart from the others': what is summed of those
+  // does not depend on which thread has which of these
+  float hist_m = -FLT_MAX, hist_best = -INFINITY;
+  int hist_v = 0x7fffffff;
   if (r.len > 0) {
     seen.fill(r.hist, r.len, v0, v1, plan.slice);
-    seen.each([&](int rel, uint32_t count) {
+    seen.each([&](int rel, uint32_t &count) {
       const int v = v0 + rel;
       const float z = tame(one_logit(row, r, v, count));
-      const float m = vmax2(t.m, z);
-      t.sum = t.sum * __builtin_amdgcn_exp2f((t.m - m) * c.L) + __builtin_amdgcn_exp2f((z - m) * c.L);
-      t.m = m;
+      count = __float_as_uint(z);  // (from here on the token's logit)
+      hist_m = vmax2(hist_m, z);
       const float sc = noisy ? gumbel_score(z, urow[v], c) : z;
-      t.second = fmaxf(t.second, fminf(t.best, sc));
-      if (sc > t.best || (sc == t.best && sc > -INFINITY && v < t.v)) {
-        t.best = sc;
-        t.v = v;
+      if (sc > hist_best || (sc == hist_best && v < hist_v)) {
+        hist_best = sc;
+        hist_v = v;
       }
     });
   }
   int w = v0;
-  for (; w + X::TOKENS < v1; w += X::TOKENS)
-    choose_batch<T, THREADS, GUMBEL, false, true>(x, un, t, row, urow, r, c, seen, v0, w, V);
+  [[maybe_unused]] auto keep_sums = [&](int first) {
+    if constexpr (CDF)
+      if (lane == 0) {
+        sums.sum[first / X::TOKENS][wid] = t.sum;
+        sums.m[first / X::TOKENS][wid] = t.m;
+      }
+  };
+  for (; w + X::TOKENS < v1; w += X::TOKENS) {
+    choose_batch<T, THREADS, MODE, false, true>(x, un, t, row, urow, r, c, seen, v0, w, V);
+    keep_sums(w);
+  }
   if (w + X::TOKENS <= V)
-    choose_batch<T, THREADS, GUMBEL, false, false>(x, un, t, row, urow, r, c, seen, v0, w, V);
+    choose_batch<T, THREADS, MODE, false, false>(x, un, t, row, urow, r, c, seen, v0, w, V);
   else
-    choose_batch<T, THREADS, GUMBEL, true, false>(x, un, t, row, urow, r, c, seen, v0, w, V);
-  const float wm = wave_max_of(t.m), wb = wave_max_of(t.best);
+    choose_batch<T, THREADS, MODE, true, false>(x, un, t, row, urow, r, c, seen, v0, w, V);
+  keep_sums(w);
+  const float wm = wave_max_of(vmax2(t.m, hist_m)), wb = wave_max_of(vmax2(t.best, hist_best));
   if (lane == 0) {
     red_m[wid] = wm;
     red_s[wid] = wb;
@@ -669,36 +856,59 @@ __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restr
     M = vmax2(M, red_m[i]);
     most = vmax2(most, red_s[i]);
   }
-  const float ws = wave_sum(t.sum * __builtin_amdgcn_exp2f((t.m - M) * c.L));
-  if (lane == 0) red_sum[wid] = ws;
+  if constexpr (!CDF) {
+    const float ws = wave_sum(t.sum * __builtin_amdgcn_exp2f((t.m - M) * c.L));
+    if (lane == 0) red_sum[wid] = ws;
+    double steps = 0.;
+    if (r.len > 0) {
+      seen.each([&](int, uint32_t z) { steps += weight_steps(__uint_as_float(z), M, c); });
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) steps += __shfl_xor(steps, o, 64);
+    }
+    if (lane == 0) red_steps[wid] = steps;
+  }
   if (!noisy) {
     if (most > -INFINITY && t.best == most) atomicMin(&first_best, t.v);
+    if (most > -INFINITY && hist_best == most) atomicMin(&first_best, hist_v);
   } else {
     const bool below = most == -INFINITY;  // (t.sum > 0: some logit is finite)
-    if (below ? t.sum > 0.f : t.best > -INFINITY && (t.best == most || !(t.best < contender_from(most)))) {
+    const auto near = [&](float s) { return s == most || !(s < contender_from(most)); };
+    const bool mine = below ? t.sum > 0.f : t.best > -INFINITY && near(t.best);
+    const bool hist = r.len > 0 && (below || (hist_best > -INFINITY && near(hist_best)));
+    if (mine || hist) {
       Part p = no_part();
-      auto offer = [&](int v) {
+      auto offer = [&](int v, float z) {
         Part e = no_part();
-        e.z = tame(one_logit(row, r, seen, v0, v));
+        e.z = z;
         e.u = urow[v];
         e.s = gumbel_score(e.z, e.u, c);
         e.v = e.z == -INFINITY ? -1 : v;
         if (better<true>(p, e, c.T)) p = e;
       };
-      if (below || t.second == most || !(t.second < contender_from(most))) {
+      if (mine && (below || near(t.second))) {
         for (int i = v0; i < v1; i += X::STEP)
           for (int k = 0; k < X::N; ++k) {
             const int v = i + tid * X::N + k;
-            if (v < v1 && !(r.len > 0 && seen.has(v - v0))) offer(v);
+            if (v < v1 && !(r.len > 0 && seen.has(v - v0))) offer(v, tame(one_logit(row, r, v, 0)));
           }
-        if (r.len > 0) seen.each([&](int rel, uint32_t) { offer(v0 + rel); });
-      } else {
-        offer(t.v);
+      } else if (mine) {
+        offer(t.v, tame(one_logit(row, r, t.v, 0)));
       }
-      contender[atomicAdd(&contenders, 1)] = Best{p.s, p.z, p.u, p.v};
+      if (hist) seen.each([&](int rel, uint32_t z) { offer(v0 + rel, __uint_as_float(z)); });
+      if (p.v >= 0) contender[atomicAdd(&contenders, 1)] = Best{p.s, p.z, p.u, p.v};
     }
   }
   __syncthreads();
+  if constexpr (CDF) {
+    Part p = no_part();
+    p.m = vmax2(most, -FLT_MAX);
+    if (most > -INFINITY) {
+      p.z = most;
+      p.v = first_best;
+    }
+    choose_from_sums(sums, x, row, r, c, seen, V, w / X::TOKENS + 1, p, noise_at(noise, rules, b, 1), choice, step, b);
+    return;
+  }
   if (tid != 0) return;
   Part p = no_part();
   if (noisy) {
@@ -715,6 +925,10 @@ __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restr
   p.sum = red_sum[0];
 #pragma unroll
   for (int i = 1; i < WAVES; ++i) p.sum += red_sum[i];
+  double steps = 0.;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) steps += red_steps[i];
+  p.sum += static_cast<float>(steps / STEPS);
   if constexpr (ONE)
     finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
   else
@@ -736,8 +950,9 @@ __global__ __launch_bounds__(256) void choose_join_kernel(const Part *__restrict
   if (lane == 0) finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
 }
 
-// Inverse CDF: one workgroup per sequence finds the slice that u falls into from the slices' sums (64 bits), then walks
-// that slice in token order, CH_THREADS x N tokens a round. A row with temperature <= 0 takes the greedy choice.
+// Inverse CDF of a row in slices: one workgroup per sequence finds the slice that u falls into from the slices' sums (64
+// bits, every wavefront by itself), then walks that slice in token order. A row with temperature <= 0 takes the greedy
+// choice.
 template <typename T>
 __global__ __launch_bounds__(CH_THREADS) void choose_cdf_kernel(const T *__restrict__ logits, int64_t ld, Rules rules,
                                                                 const float *__restrict__ temp, float temp0,
@@ -745,98 +960,71 @@ __global__ __launch_bounds__(CH_THREADS) void choose_cdf_kernel(const T *__restr
                                                                 const Part *__restrict__ parts,
                                                                 Choice choice, Step step) {
   extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
-  __shared__ double wave_total[CH_THREADS / 64];
-  __shared__ int found, last;
+  __shared__ Walk<CH_THREADS> walk;
   using X = Batch<T, CH_THREADS>;
-  constexpr int N = X::N;
   const int64_t b = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const Scale c = row_scale(temp, temp0, b);
+  const int tid = threadIdx.x, lane = tid & 63;
   const int slices = plan.slices, slice = plan.slice;
   const Part *mine = parts + b * slices;
-  // every thread joins the slices the same way
+  const RowRules r = row_rules(rules, b, V);
+  const Scale c = row_scale(temp, temp0, b);
+  const float uniform = *noise_at(noise, rules, b, 1);
+  if (tid == 0) {
+    walk.found = 0x7fffffff;
+    walk.last = -1;
+  }
+  // every wavefront joins the slices the same way
   Part p = no_part();
-  for (int s = 0; s < slices; ++s) join_parts<false>(p, mine[s], c.L, c.T);
+  for (int s = lane; s < slices; s += 64) join_parts<false>(p, mine[s], c.L, c.T);
+  join_lanes<false>(p, c.L, c.T);
   if (p.v < 0 || !(c.T > 0.f)) {
     if (tid == 0) finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
     return;
   }
-  auto weight = [&](int s) { return static_cast<double>(mine[s].sum * __builtin_amdgcn_exp2f((mine[s].m - p.m) * c.L)); };
-  double total = 0.;
-  for (int s = 0; s < slices; ++s) total += weight(s);
-  const double target = static_cast<double>(*noise_at(noise, rules, b, 1)) * total;
-  // the slice: the first whose running sum passes the target (rounding, or a uniform of 1: the last with any weight)
-  int at = -1, filled = 0;
-  double before = 0., run = 0.;
-  for (int s = 0; s < slices && at < 0; ++s) {
-    const double w = weight(s);
-    if (w > 0.) {
-      filled = s;
-      run = before;
-      if (target < before + w) at = s;
-    }
-    before += w;
-  }
-  if (at < 0) at = filled;
-  const RowRules r = row_rules(rules, b, V);
-  const int v0 = at * slice, v1 = V - v0 < slice ? V : v0 + slice;
-  if (tid == 0) {
-    found = 0x7fffffff;
-    last = -1;
-  }
-  __syncthreads();
-  const Seen<CH_THREADS> seen(lds, plan);
-  const T *row = logits + b * ld;
-  if (r.len > 0) seen.fill(r.hist, r.len, v0, v1, slice);
-  for (int w0 = v0; w0 < v1; w0 += X::STEP) {
-    const int v = w0 + tid * N;
-    double e[N], sum = 0.;
-    int top = -1;
-#pragma unroll
-    for (int k = 0; k < N; ++k) e[k] = 0.;
-    if (v < v1) {
-      float z[N];
-#pragma unroll
-      for (int k = 0; k < N; ++k) z[k] = one_logit(row, r, seen, v0, v + k < V ? v + k : V - 1);
-#pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (v + k < V) {
-          e[k] = static_cast<double>(__builtin_amdgcn_exp2f((tame(z[k]) - p.m) * c.L));
-          if (e[k] > 0.) top = v + k;
-          sum += e[k];
-        }
-    }
-    double inc = sum;
+  auto weight = [&](int s) {
+    return s < slices ? static_cast<double>(mine[s].sum * __builtin_amdgcn_exp2f((mine[s].m - p.m) * c.L)) : 0.;
+  };
+  auto scan = [&](double v) {  // inclusive
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const double up = __shfl_up(inc, o, 64);
-      if (lane >= o) inc += up;
+      const double up = __shfl_up(v, o, 64);
+      if (lane >= o) v += up;
     }
-    if (lane == 63) wave_total[wid] = inc;
-    __syncthreads();
-    double cdf = run;
-    for (int w = 0; w < CH_THREADS / 64; ++w) {
-      if (w < wid) cdf += wave_total[w];
-      run += wave_total[w];
+    return v;
+  };
+  double total = 0.;
+  for (int s0 = 0; s0 < slices; s0 += 64) total += __shfl(scan(weight(s0 + lane)), 63, 64);
+  const double target = static_cast<double>(uniform) * total;
+  // the slice: the first whose running sum passes the target (rounding, or a uniform of 1: the last with any weight)
+  int at = 0;
+  double before = 0., run = 0.;
+  for (int s0 = 0; s0 < slices; s0 += 64) {
+    const double v = weight(s0 + lane), upto = scan(v);
+    const uint64_t filled = __ballot(v > 0.), past = __ballot(v > 0. && target < before + upto);
+    const int l = past != 0 ? __builtin_ctzll(past) : 63 - __builtin_clzll(filled | 1);
+    if (filled != 0) {
+      at = s0 + l;
+      run = before + __shfl(upto - v, l, 64);
     }
-    cdf += inc - sum;
-    int hit = 0x7fffffff;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      cdf += e[k];
-      if (hit == 0x7fffffff && e[k] > 0. && target < cdf) hit = v + k;
-    }
-    if (hit != 0x7fffffff) atomicMin(&found, hit);
-    if (top >= 0) atomicMax(&last, top);
-    __syncthreads();
-    if (found != 0x7fffffff) break;
+    if (past != 0) break;
+    before += __shfl(upto, 63, 64);
   }
-  if (tid != 0) return;
-  const int pick = found != 0x7fffffff ? found : last;
-  if (pick < 0)  // (a slice with weight holds a token with weight)
-    finish_row(choice, step, b, V, p.v, logp_of(p.z, p, c));
-  else
-    finish_row(choice, step, b, V, pick, logp_of(tame(one_logit(row, r, seen, v0, pick)), p, c));
+  const int v0 = at * slice, v1 = V - v0 < slice ? V : v0 + slice;
+  const Seen<CH_THREADS> seen(lds, plan);
+  const T *row = logits + b * ld;
+  X x;
+  if (V >= X::N) x.load(row, v0, V);
+  if (r.len > 0) {
+    seen.fill(r.hist, r.len, v0, v1, slice);
+    logits_for_counts(seen, row, r, v0);
+  }
+  __syncthreads();
+  for (int w = v0; w < v1; w += X::TOKENS) {
+    if (w > v0 && V >= X::N) x.load(row, w, V);
+    walk_batch(x, row, r, c, seen, v0, w, V, p.m, target, run, walk);
+    if (walk.found != 0x7fffffff) break;
+  }
+  if (tid == 0) finish_walk(walk, row, r, c, seen, v0, V, p, choice, step, b);
 }
 
 // How B rows of V tokens are cut: about two workgroups per CU in all, of 4096 tokens (one batch) to CH_SLICE. `whole`: one
@@ -910,24 +1098,26 @@ static int launch_choose(const void *logits, int64_t ld, const Rules &r, const f
   const T *x = static_cast<const T *>(logits);
   const size_t lds = plan_lds(plan, r.hist != nullptr);
   const unsigned grid = static_cast<unsigned>(B * plan.slices), join = static_cast<unsigned>((B + 3) / 4);
-#define VK_SLICES(THREADS, GUMBEL, ONE)                                                                                 \
-  choose_slices_kernel<T, THREADS, GUMBEL, ONE><<<grid, THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, plan, parts, \
+#define VK_SLICES(THREADS, MODE, ONE)                                                                                   \
+  choose_slices_kernel<T, THREADS, MODE, ONE><<<grid, THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, plan, parts, \
                                                                            choice, step)
-  if (mode == CH_CDF) {
-    VK_SLICES(CH_THREADS, false, false);
-    choose_cdf_kernel<T><<<static_cast<unsigned>(B), CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, plan, parts,
-                                                                           choice, step);
-  } else if (plan.one) {
+  if (plan.one) {
     if (mode == CH_GUMBEL)
-      VK_SLICES(CH_THREADS_ONE, true, true);
+      VK_SLICES(CH_THREADS_ONE, CH_GUMBEL, true);
+    else if (mode == CH_CDF)
+      VK_SLICES(CH_THREADS_ONE, CH_CDF, true);
     else
-      VK_SLICES(CH_THREADS_ONE, false, true);
+      VK_SLICES(CH_THREADS_ONE, CH_GREEDY, true);
   } else if (mode == CH_GUMBEL) {
-    VK_SLICES(CH_THREADS, true, false);
+    VK_SLICES(CH_THREADS, CH_GUMBEL, false);
     choose_join_kernel<true><<<join, 256, 0, s>>>(parts, temp, temp0, B, V, plan.slices, choice, step);
   } else {
-    VK_SLICES(CH_THREADS, false, false);
-    choose_join_kernel<false><<<join, 256, 0, s>>>(parts, temp, temp0, B, V, plan.slices, choice, step);
+    VK_SLICES(CH_THREADS, CH_GREEDY, false);
+    if (mode == CH_CDF)
+      choose_cdf_kernel<T><<<static_cast<unsigned>(B), CH_THREADS, lds, s>>>(x, ld, r, temp, temp0, noise, V, plan, parts,
+                                                                             choice, step);
+    else
+      choose_join_kernel<false><<<join, 256, 0, s>>>(parts, temp, temp0, B, V, plan.slices, choice, step);
   }
 #undef VK_SLICES
   return launch_status("choose_tokens");
@@ -975,14 +1165,14 @@ extern "C" int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, 
   return launch_status("process_logits");
 }
 
-// Whether a call of this mode joins slices, or reads them again (inverse CDF), and so needs their results kept.
+// Whether a call joins slices, and so needs their results kept.
 static int64_t parts_bytes(const Plan &p, int64_t B) {
   return p.one ? 0 : B * p.slices * static_cast<int64_t>(sizeof(Part));
 }
 
-extern "C" int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t hist_cols, int32_t mode, int64_t *bytes) {
+extern "C" int vk_choose_tokens_workspace(int64_t B, int32_t V, int64_t hist_cols, int64_t *bytes) {
   VK_CHECK_ARG(bytes && B >= 0 && V > 0 && V <= CH_V_MAX && hist_cols >= 0, "choose_tokens_workspace: bad arguments");
-  *bytes = B == 0 ? 0 : parts_bytes(make_plan(B, V, hist_cols, mode != CH_CDF), B);
+  *bytes = B == 0 ? 0 : parts_bytes(make_plan(B, V, hist_cols, true), B);
   return VK_OK;
 }
 
@@ -999,7 +1189,7 @@ static int choose(const void *logits, int32_t dtype, int64_t ld, const Rules &r,
   VK_CHECK_ARG(mode == CH_GREEDY || (noise.u != nullptr && noise.cols > 0 && noise.ld >= noise.cols * per),
                "%s: sampling needs uniforms, rows of columns x %lld", what, static_cast<long long>(per));
   if (B == 0) return VK_OK;
-  const Plan plan = make_plan(B, V, r.hist ? r.hist_cols : 0, mode != CH_CDF);
+  const Plan plan = make_plan(B, V, r.hist ? r.hist_cols : 0, true);
   rc = check_grid(plan, B, what);
   if (rc != VK_OK) return rc;
   const int64_t need = parts_bytes(plan, B);

@@ -1072,9 +1072,9 @@ _MODE_GREEDY, _MODE_GUMBEL, _MODE_CDF = 0, 1, 2
 
 
 @functools.lru_cache(maxsize=256)
-def _choose_workspace(B, V, hist_cols, mode):
+def _choose_workspace(B, V, hist_cols):
     nb = ctypes.c_int64(0)
-    call("vk_choose_tokens_workspace", B, V, hist_cols, mode, ctypes.byref(nb))
+    call("vk_choose_tokens_workspace", B, V, hist_cols, ctypes.byref(nb))
     return nb.value
 
 
@@ -1108,7 +1108,7 @@ def choose_tokens(logits, history=None, lengths=None, repetition=1.0, presence=0
     dev = logits.device
     token = torch.empty(B, dtype=torch.long, device=dev)
     logp = torch.empty(B, dtype=torch.float32, device=dev)
-    nb = _choose_workspace(B, V, args[5], mode)
+    nb = _choose_workspace(B, V, args[5])
     ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
     call("vk_choose_tokens", *args, *temp, mode, up, uld, int(fallback), token.data_ptr(), logp.data_ptr(), B, V, ptr(ws), nb,
          stream_handle())
@@ -1161,7 +1161,7 @@ def choose_update(logits, bias, is_tail, is_homo, homo_stop, tok, run, pos, plen
             token_rows.dtype != torch.int32 or token_rows.shape != (V,) or not token_rows.is_contiguous())):
         _refuse(what, "allowed goes with token_rows int32 [V]")
     cols = out.shape[1] if (repetition, presence, frequency) != (1.0, 0.0, 0.0) else 0
-    nb = _choose_workspace(B, V, cols, mode)
+    nb = _choose_workspace(B, V, cols)
     ws = torch.empty(nb, dtype=torch.uint8, device=logits.device) if nb else None
     call("vk_choose_update", logits.data_ptr(), _vk_dtype(logits.dtype), max(logits.stride(0), V), float(repetition),
          float(presence), float(frequency), bias.data_ptr(), *mask, ptr(token_rows), is_tail.data_ptr(), is_homo.data_ptr(),
