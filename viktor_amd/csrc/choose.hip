@@ -497,9 +497,10 @@ __device__ __forceinline__ float wave_max_of(float v) {
   return v;
 }
 
-// What a thread knows of its tokens (without the history's): the maximum of z (at least -FLT_MAX), the sum of exponentials at it, the best logit
-// or score with its first token, and the second best score. A batch that has nothing near the wavefront's best so far is
-// not looked through for them (a thread's next best comes in most batches, a wavefront's in one of i at the i-th).
+// What a thread knows of its tokens (without the history's): the maximum of z (at least -FLT_MAX), the sum of exponentials
+// at it, the best logit or score with its first token, and the second best score. A batch that has nothing near the
+// wavefront's best so far is not looked through for them (a thread's next best comes in most batches, a wavefront's in one
+// of i at the i-th).
 struct Mine {
   float m = -FLT_MAX, sum = 0.f, best = -INFINITY, second = -INFINITY, wave_best = -INFINITY;
   int v = -1;
@@ -527,8 +528,8 @@ struct Uniforms {
 
 template <typename T, int THREADS, int MODE, bool CUT, bool MORE>
 __device__ __forceinline__ void choose_batch(Batch<T, THREADS> &x, Uniforms<T, THREADS, MODE == CH_GUMBEL> &un,
-                                             Mine &t, const T *row, const float *urow, const RowRules &r, const Scale &c, const Seen<THREADS> &s,
-                                             int v0, int w, int V) {
+                                             Mine &t, const T *row, const float *urow, const RowRules &r, const Scale &c,
+                                             const Seen<THREADS> &s, int v0, int w, int V) {
   using X = Batch<T, THREADS>;
   constexpr bool GUMBEL = MODE == CH_GUMBEL;
   const bool noisy = GUMBEL && c.T > 0.f;
@@ -721,9 +722,10 @@ struct BatchSums {
 // The choice from a row's sums by batch (p: its maximum and its first best token): the totals at the maximum, the batch that
 // the target falls into, and the token in it.
 template <typename T, int THREADS>
-__device__ __forceinline__ void choose_from_sums(BatchSums<THREADS> &sums, Batch<T, THREADS> &x, const T *row, const RowRules &r,
-                                                 const Scale &c, const Seen<THREADS> &s, int V, int batches, Part p,
-                                                 const float *uniform, const Choice &choice, const Step &step, int64_t b) {
+__device__ __forceinline__ void choose_from_sums(BatchSums<THREADS> &sums, Batch<T, THREADS> &x, const T *row,
+                                                 const RowRules &r, const Scale &c, const Seen<THREADS> &s, int V,
+                                                 int batches, Part p, const float *uniform, const Choice &choice,
+                                                 const Step &step, int64_t b) {
   using X = Batch<T, THREADS>;
   constexpr int WAVES = THREADS / 64;
   const int tid = threadIdx.x;
@@ -765,8 +767,9 @@ __device__ __forceinline__ void choose_from_sums(BatchSums<THREADS> &sums, Batch
 // One slice of one sequence, or with ONE the whole vocabulary and the step's end. The workgroup's best logit or score
 // tells who can have the best token: the lowest token of the largest logit, or the threads within the scores' slack of
 // the largest score. These read their token again and are compared exactly; one whose second score is as near goes
-// through all of its tokens, its history's too, and so does every thread where all scores are below fp32's range. The sum is taken at the
-// workgroup's maximum. Inverse CDF (ONE): the sums stay by batch, and the batch that the uniform falls into is walked.
+// through all of its tokens, its history's too, and so does every thread where all scores are below fp32's range. The sum is
+// taken at the workgroup's maximum. Inverse CDF (ONE): the sums stay by batch, and the batch that the uniform falls into is
+// walked.
 template <typename T, int THREADS, int MODE, bool ONE>
 __global__ __launch_bounds__(THREADS) void choose_slices_kernel(const T *__restrict__ logits, int64_t ld, Rules rules,
                                                                    const float *__restrict__ temp, float temp0,
