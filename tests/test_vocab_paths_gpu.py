@@ -179,6 +179,34 @@ def test_token_embedding(V, d, wt, scale, pad):
     assert torch.allclose(w.grad.cpu().double(), (count * scale)[:, None].expand(V, d), rtol=2 ** -8 if wt != torch.float32 else 2 ** -22, atol=0)
 
 
+@pytest.mark.parametrize("V", [343, 5463])
+def test_token_embedding_in_a_graph(V):
+    """Forward and backward captured together, replayed with other ids and gradients, eager calls in between."""
+    g = torch.Generator().manual_seed(V)
+    w = torch.randn(V, 64, generator=g).to(DEV).requires_grad_()
+    tok, L = torch.zeros(6000, dtype=torch.long, device=DEV), torch.zeros(6000, 64, device=DEV)
+
+    def call():
+        y = TR.token_embedding(w, tok, 2.0, 0)
+        return y.detach(), torch.autograd.grad(y, w, L)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for _ in range(3):
+        tok.copy_(torch.randint(0, V, (6000,), generator=g))
+        L.copy_(torch.randn(6000, 64, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, call()):
+            assert torch.equal(a, b)
+
+
 def test_rollout_scoring_and_update_of_6mers():
     """A model of the 6-mer vocabulary (5463 tokens) through the public path: sampled rollout with penalties, its
     log-probabilities against the scoring forward's, rewards, one update; the embedding's gradient is the one that the
