@@ -26,7 +26,8 @@
 // The inverse CDF keeps its sums by batch or slice and reads only the batch or slice that the uniform falls into again: with
 // a bias 49 (fp32) and 42 (bf16), with all rules 56 and 47; 5463 tokens 23 against 10 greedy.
 // Measured and not taken: bias and mask loaded a batch ahead (process fp32 -4, all bf16 +2), two sequences a workgroup that
-// share the bias (bf16 -0.6, fp32 +5), 8-byte loads of bf16 (+1 to +2), 1024 threads a row (+5).
+// share the bias (bf16 -0.6, fp32 +5), 8-byte loads of bf16 (+1 to +2), 1024 threads a row (+5), two batches ahead (+1 to
+// +2).
 #include <float.h>
 #include <math.h>
 
