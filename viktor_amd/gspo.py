@@ -81,7 +81,7 @@ def token_logprobs(model, frames, plens, seqs, ended, group_size=1):
     prefix runs once (Basecaller.logits); the log-probs are those of the unshared forward."""
     tokens_in, targets, _ = model.batch(seqs, pad_to=128)
     dev = frames.device
-    tokens_in, targets = tokens_in.to(dev), targets.to(dev)
+    targets = targets.to(dev)
     logits = model.logits(frames, tokens_in, plens, group_size=group_size)
     lp = ops.gspo_score(logits.contiguous(), targets.clamp(min=0).contiguous())["lp"]
     mask = sampled_mask(targets, seqs, ended, model.tokenizer.k)

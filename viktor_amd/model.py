@@ -45,6 +45,25 @@ def check_groups(frames, plens_h, G):
     return pre_lens
 
 
+def token_ids(tokens_in, vocab, dev):
+    """tokens_in as the embedding's lookup takes it: contiguous int64 on dev, the ids -vocab .. -1 counted from the
+    vocabulary's end, as an index counts them. IndexError where tokens_in holds no integers, or, in a host tensor, an id
+    past either end; in a device tensor such an id stays as it is (a zero row, no gradient): to see it, the host would wait."""
+    if tokens_in.dtype.is_floating_point or tokens_in.dtype.is_complex or tokens_in.dtype == torch.bool:
+        raise IndexError(f"token ids are integers (got {tokens_in.dtype})")
+    if tokens_in.is_cuda:
+        t = tokens_in.to(dev, torch.long)
+        return t.add(t < 0, alpha=vocab).contiguous()
+    t = tokens_in.to(torch.long)
+    if t.numel() > 0:
+        lo, hi = (int(v) for v in t.aminmax())
+        if lo < -vocab or hi >= vocab:
+            raise IndexError(f"token ids from {lo} to {hi} in a vocabulary of {vocab}")
+        if lo < 0:
+            t = t.add(t < 0, alpha=vocab)
+    return t.contiguous().to(dev)
+
+
 class Basecaller(nn.Module):
     def __init__(self, encoder, tokenizer: KmerTokenizer, cfg: Optional[DecoderConfig] = None, d_enc: int = 512):
         super().__init__()
@@ -116,6 +135,7 @@ class Basecaller(nn.Module):
         projector's bf16 output and the token embeddings gathered into an fp32 residual stream
         (viktor/model.py:81-84; fp32 embedding rows from fp32 weights), the decoder on that fp32 stream
         (FastDecoder.teacher_forced) and the LM head as a bf16 product.
+        tokens_in [B, T]: ids as token_ids takes them.
         group_size = G > 1: consecutive groups of G windows carry the same prefix (a GSPO rollout's repeated
         windows, scripts/gspo.py:444; checked on the device, ValueError otherwise), which then runs once per group
         (see hidden())."""
@@ -133,12 +153,12 @@ class Basecaller(nn.Module):
         dev = frames.device
         plens_h = [P] * B if plens is None else [int(p) for p in plens.tolist()]
         assert all(0 < p <= P for p in plens_h), "plens outside 1..P"
+        ids = token_ids(tokens_in, self.cfg.vocab_size, dev)
         if int(group_size) > 1:
-            return self._hidden_shared(frames, tokens_in, plens_h, int(group_size))
+            return self._hidden_shared(frames, ids, plens_h, int(group_size))
         prefix = self.project(frames)                                       # [B, P, d] bf16
         fast = self.decoder.fast()
-        emb = ops.embed_lookup(fast.w32(self.decoder.embed.weight),
-                               tokens_in.to(dev, torch.long).contiguous())                  # [B, T, d] fp32
+        emb = ops.embed_lookup(fast.w32(self.decoder.embed.weight), ids)    # [B, T, d] fp32
         s = self.pos_scale
 
         def build():  # the packing plan, the window layout's row indices and each row's (rotary) position
@@ -172,11 +192,11 @@ class Basecaller(nn.Module):
             x[tok_dst] = emb.reshape(B * T, -1)
         return fast.teacher_forced(x, pos, plan, rope_pos=rpos)            # [B * T, d] bf16
 
-    def _hidden_shared(self, frames, tokens_in, plens_h, G):
+    def _hidden_shared(self, frames, ids, plens_h, G):
         """hidden() over groups of G windows that share their prefix: each group's frames are projected and run
-        through the decoder once, as its members' common prefix."""
+        through the decoder once, as its members' common prefix. ids: token_ids' [B, T]."""
         B, P = frames.shape[:2]
-        T = tokens_in.shape[1]
+        T = ids.shape[1]
         dev = frames.device
         pre_lens = check_groups(frames, plens_h, G)
         d = self.cfg.d_model
@@ -186,8 +206,7 @@ class Basecaller(nn.Module):
         else:
             x_pre = torch.cat([prefix[g, :p] for g, p in enumerate(pre_lens)]).float()
         fast = self.decoder.fast()
-        x_tok = ops.embed_lookup(fast.w32(self.decoder.embed.weight),
-                                 tokens_in.to(dev, torch.long).reshape(-1).contiguous())     # [B T, d] fp32
+        x_tok = ops.embed_lookup(fast.w32(self.decoder.embed.weight), ids.view(-1))  # [B T, d] fp32
         s = self.pos_scale
 
         def build():

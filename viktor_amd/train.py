@@ -83,8 +83,9 @@ class _TokenEmbed(torch.autograd.Function):
 
 def token_embedding(weight, tokens, scale=1.0, pad=None):
     """Differentiable scaled token embedding: scale * weight[tokens] in fp32, weight [V, d] fp32 or bf16, tokens int64 of any
-    shape. The gradient of weight sums the rows of each id (by sorted tokens past SORTED_GRAD_VOCAB ids), without those
-    of the id `pad` (nn.Embedding's padding_idx). What train_logits runs, at scale 1; reference: viktor/model.py:77."""
+    shape; ids outside [0, V) give zero rows and no gradient. The gradient of weight sums the rows of each id (by sorted
+    tokens past SORTED_GRAD_VOCAB ids), without those of the id `pad` (nn.Embedding's padding_idx). What train_logits runs,
+    at scale 1; reference: viktor/model.py:77."""
     return _TokenEmbed.apply(weight, tokens, float(scale), pad)
 
 
@@ -312,7 +313,8 @@ def train_logits(model, frames, tokens_in, plens=None, group_size=1):
     scripts/gspo.py:444, 459-466; checked, ValueError otherwise). Each group's prefix rows then run the
     projector and the decoder once, its members' token rows attend to them, and the backward sums every
     member's gradient into them: the same logits as the unshared forward, and the same gradients up to the
-    order of the fp32 sums over the members."""
+    order of the fp32 sums over the members. tokens_in [B, T]: ids as model.token_ids takes them."""
+    from .model import token_ids
     dec = model.decoder
     cfg = dec.cfg
     B, P = frames.shape[:2]
@@ -320,12 +322,13 @@ def train_logits(model, frames, tokens_in, plens=None, group_size=1):
     dev = frames.device
     plens_h = [P] * B if plens is None else [int(p) for p in plens.tolist()]
     assert all(0 < p <= P for p in plens_h), "plens outside 1..P"
+    ids = token_ids(tokens_in, dec.embed.weight.shape[0], dev)
     if int(group_size) > 1:
-        return _train_logits_shared(model, frames, tokens_in, plens_h, int(group_size))
+        return _train_logits_shared(model, frames, ids, plens_h, int(group_size))
     proj = model.projector
     prefix = _Projector.apply(frames.reshape(B * P, -1).to(BF16).contiguous(), proj[0].weight, proj[0].bias,
                               proj[2].weight, proj[2].bias)                            # [B P, d] bf16
-    emb = token_embedding(dec.embed.weight, tokens_in.to(dev, torch.long).reshape(-1))  # [B T, d] fp32
+    emb = token_embedding(dec.embed.weight, ids.view(-1))                                 # [B T, d] fp32
     # packed layout, window b: its plens[b] real prefix rows, then its T token rows; row indices on the host
     s = model.pos_scale
 
@@ -351,21 +354,21 @@ def train_logits(model, frames, tokens_in, plens=None, group_size=1):
     return _LMHead.apply(h, dec.lm_head.weight).view(B, T, -1)
 
 
-def _train_logits_shared(model, frames, tokens_in, plens_h, G):
+def _train_logits_shared(model, frames, ids, plens_h, G):
     """train_logits over groups of G windows that share their prefix: packed rows [each group's prefix rows |
-    every member's token rows] (TrainPlan.shared)."""
+    every member's token rows] (TrainPlan.shared). ids: model.token_ids' [B, T]."""
     from .model import check_groups
     dec = model.decoder
     cfg = dec.cfg
     B, P = frames.shape[:2]
-    T = tokens_in.shape[1]
+    T = ids.shape[1]
     dev = frames.device
     pre_lens = check_groups(frames, plens_h, G)
     ng = len(pre_lens)
     proj = model.projector
     prefix = _Projector.apply(frames[::G].reshape(ng * P, -1).to(BF16).contiguous(), proj[0].weight, proj[0].bias,
                               proj[2].weight, proj[2].bias)                            # [B / G P, d] bf16
-    emb = token_embedding(dec.embed.weight, tokens_in.to(dev, torch.long).reshape(-1))  # [B T, d] fp32
+    emb = token_embedding(dec.embed.weight, ids.view(-1))                                 # [B T, d] fp32
     s = model.pos_scale
 
     def build():
@@ -453,7 +456,7 @@ def token_logprobs_train(model, frames, plens, seqs, ended, group_size=1):
     from .gspo import sampled_mask
     tokens_in, targets, _ = model.batch(seqs, pad_to=128)
     dev = frames.device
-    tokens_in, targets = tokens_in.to(dev), targets.to(dev)
+    targets = targets.to(dev)
     logits = train_logits(model, frames, tokens_in, plens, group_size)
     mask = sampled_mask(targets, seqs, ended, model.tokenizer.k)
     return logits, targets, mask
@@ -471,7 +474,8 @@ def frame_loss(model, frames, seqs, weights=None, plens=None):
     GSPO update (Basecaller.frame_loss / weighted_loss / token_metrics, viktor/model.py:153-177, 201-203;
     called at scripts/gspo.py:482-484): sum(ce * w) / sum(w) over the targets (PAD ignored)."""
     dev = frames.device
-    tokens_in, targets, w = (t.to(dev) for t in model.batch(seqs, weights))
+    tokens_in, targets, w = model.batch(seqs, weights)
+    targets, w = targets.to(dev), w.to(dev)
     logits = train_logits(model, frames, tokens_in, plens)
     ce = torch.nn.functional.cross_entropy(logits.flatten(0, 1).float(), targets.flatten(), ignore_index=0,
                                            reduction="none").view_as(targets)
