@@ -291,6 +291,7 @@ int vk_select_update(const float *logits, const void *h, const void *norm_w, flo
  * penalties. bias NULL: none; bias_ld 0: one row for all. allowed [n_allowed, allowed_ld] 32-bit words; allowed_rows [B]
  * int32 names each sequence's mask row, one outside 0 .. n_allowed - 1 meaning no mask; NULL: the one row, or row b of B.
  * allowed NULL: no masks. out [B, V] bf16 or fp32 (row stride out_ld) may be logits itself (same dtype and stride).
+ * B = 0 launches nothing, and what has B rows may be NULL then; so also below.
  * No reference counterpart: the reference's rules are the bias and the k-mer grammar of viktor/engine.py:79-116.
  */
 int vk_process_logits(const void *logits, int32_t dtype, int64_t ld, const int64_t *hist, int64_t hist_ld,

@@ -1082,7 +1082,8 @@ static int check_rules(const Rules &r, int64_t B, int V, const char *what) {
   VK_CHECK_ARG(r.bias == nullptr || r.bias_ld == 0 || r.bias_ld >= V, "%s: bias row stride below V", what);
   VK_CHECK_ARG(r.allowed == nullptr || (r.n_allowed > 0 && r.allowed_ld >= (V + 31) / 32),
                "%s: masks are rows of ceil(V / 32) words", what);
-  VK_CHECK_ARG(r.allowed == nullptr || r.arow != nullptr || r.token_row != nullptr || r.n_allowed == 1 || r.n_allowed == B,
+  VK_CHECK_ARG(r.allowed == nullptr || r.arow != nullptr || r.token_row != nullptr || r.n_allowed == 1 || r.n_allowed == B ||
+                   B == 0,
                "%s: masks without row numbers: 1 row or one per sequence", what);
   return VK_OK;
 }
@@ -1190,7 +1191,7 @@ static int choose(const void *logits, int32_t dtype, int64_t ld, const Rules &r,
   VK_CHECK_ARG(mode == CH_GREEDY || mode == CH_GUMBEL || mode == CH_CDF,
                "%s: mode 0 (greedy), 1 (Gumbel) or 2 (inverse CDF)", what);
   const int64_t per = mode == CH_GUMBEL ? V : 1;
-  VK_CHECK_ARG(mode == CH_GREEDY || (noise.u != nullptr && noise.cols > 0 && noise.ld >= noise.cols * per),
+  VK_CHECK_ARG(mode == CH_GREEDY || ((B == 0 || noise.u != nullptr) && noise.cols > 0 && noise.ld >= noise.cols * per),
                "%s: sampling needs uniforms, rows of columns x %lld", what, static_cast<long long>(per));
   if (B == 0) return VK_OK;
   const Plan plan = make_plan(B, V, r.hist ? r.hist_cols : 0, true);
@@ -1229,8 +1230,8 @@ extern "C" int vk_choose_update(const void *logits, int32_t dtype, int64_t ld, f
                                 int64_t out_cols, int32_t *pos32, int32_t *seqlens, int32_t *rpos32, float *logp,
                                 int64_t logp_stride, int64_t B, int32_t V, int32_t eos, int32_t pad, void *workspace,
                                 int64_t workspace_bytes, void *stream) {
-  VK_CHECK_ARG(bias && is_tail && is_homo && tok && pos && out, "choose_update: null pointer");
-  VK_CHECK_ARG(homo_stop <= 0 || run != nullptr, "choose_update: homopolymer rule needs run");
+  VK_CHECK_ARG(bias && is_tail && is_homo && (B == 0 || (tok && pos && out)), "choose_update: null pointer");
+  VK_CHECK_ARG(homo_stop <= 0 || run != nullptr || B == 0, "choose_update: homopolymer rule needs run");
   VK_CHECK_ARG(out_cols > 0 && out_stride >= out_cols, "choose_update: output rows");
   VK_CHECK_ARG(logp_stride == 0 || logp_stride >= out_cols, "choose_update: logp_stride must be 0 or >= out_cols");
   VK_CHECK_ARG(allowed == nullptr || token_rows != nullptr, "choose_update: masks need the mask row of each token");

@@ -978,13 +978,13 @@ def _per_row(x, B, what, name):
     return None, float(x)
 
 
-def _mask_args(allowed, V, what):
+def _mask_args(allowed, V, what, least=1):
     if allowed is None:
         return None, 0, 0
     if allowed.dim() != 2 or allowed.dtype is not torch.int32 or not allowed.is_contiguous():
         _refuse(what, "allowed int32 [S, ceil(V / 32)]")
     S, words = allowed.shape
-    if S == 0 or words < (V + 31) // 32:
+    if S < least or words < (V + 31) // 32:
         _refuse(what, "allowed int32 [S, ceil(V / 32)]")
     return allowed.data_ptr(), words, S
 
@@ -1023,7 +1023,7 @@ def _logit_rules(what, logits, history, lengths, repetition, presence, frequency
                 _refuse(what, "bias rows side by side")
             bld = 0 if bias.dim() == 1 else max(bias.stride(0), V)
         bp = bias.data_ptr()
-    ap, words, S = _mask_args(allowed, V, what)
+    ap, words, S = _mask_args(allowed, V, what, min(B, 1))
     if allowed_rows is not None:
         if allowed is None or not _vector(allowed_rows, B, torch.int32):
             _refuse(what, "allowed_rows int32 [B], with allowed")
