@@ -15,16 +15,23 @@
 // The choice gives (max, sum of exponentials at it, best) per slice, joined by one wavefront per sequence, or takes a whole
 // row per workgroup of 512 threads and finishes it (make_plan).
 //
-// What bounds them: one sequence, the launch and the chain of loads (process 4.8 us at 87383 tokens, choice 8.6 us in two
-// launches); a batch, memory, and before it the gathering and the bias, which is read from the caches as often as there are
-// sequences. 512 x 87383 logits, us (a plain read of the fp32 ones takes 26.5, a copy of the bf16 ones 31 to 36):
+// What bounds them: one sequence, the launch and the chain of loads (process 4.8 us at 5463 tokens, choice 8.9 us at 87383
+// in two launches; in a graph); a batch, memory, and before it the gathering and the bias, which is read from the L2s as
+// often as there are sequences (of 179 MB of fp32 logits and as many of bias, 192 MB pass the L2s in all). 512 x 87383
+// logits, us (a plain read of the fp32 ones takes 26.5, a copy of the bf16 ones 31 to 36):
 //                 no rules   bias   mask   history of 256   all
-//   process bf16      37      45     38         43           51 (46.8 from logits that are not in a cache)
-//   process fp32      74      78     76         82           83
-//   greedy fp32       31.5    37     33         34           41.5
-//   greedy bf16       23.6    32     27         26           37
+//   process bf16      37      45     38         43           51 (46.4 from logits that are not in a cache)
+//   process fp32      74      79     77         81           84
+//   greedy fp32       31.5    37     33         35           42
+//   greedy bf16       23.7    33     27         27           37
+// Histories of 1, 64, 1024, 2048, 4096 columns take processed bf16 logits 47, 50, 56, 68, 86: each slice of a row reads all
+// of its sequence's history.
 // The inverse CDF keeps its sums by batch or slice and reads only the batch or slice that the uniform falls into again: with
-// a bias 49 (fp32) and 42 (bf16), with all rules 56 and 47; 5463 tokens 23 against 10 greedy.
+// a bias 49 (fp32) and 42 (bf16), with all rules 56 and 47; 5463 tokens 23 against 10 greedy, since a row of one batch is
+// loaded, ruled and scanned a second time.
+// A decode step (choose_update), us, greedy / Gumbel / inverse CDF with a bias, then with penalties and a grammar too, fp32:
+// 1 x 5463 5.2 / 7.1 / 13.8, 7.1 / 9.3 / 16.6; 64 x 5463 5.9 / 7.8 / 14.5, 8.0 / 10.2 / 17.7; 512 x 5463 8.0 / 11.3 / 19.6,
+// 10.8 / 14.7 / 23.3; 64 x 87383 13.1 / 18.8 / 27.0, 16.1 / 21.7 / 33.3; 512 x 87383 39.2 / 63.6 / 51.6, 43.3 / 71.0 / 58.4.
 // Measured and not taken: bias and mask loaded a batch ahead (process fp32 -4, all bf16 +2), two sequences a workgroup that
 // share the bias (bf16 -0.6, fp32 +5), 8-byte loads of bf16 (+1 to +2), 1024 threads a row (+5), two batches ahead (+1 to
 // +2).
@@ -41,8 +48,15 @@ namespace vk {
 constexpr int CH_THREADS = 256;
 constexpr int CH_THREADS_ONE = 512;  // of a workgroup that takes a whole row
 constexpr int CH_WHOLE = 1 << 17;    // tokens of such a row at most, where it has more than one slice: 16 KB of LDS bits
-// Tokens of a row that one workgroup takes at any batch: it spares the join's launch. fp32, greedy, us: 21847 tokens of 1,
-// 77, 200 sequences 8.0, 10.4, 11.1 against 8.3, 10.6, 11.0 in slices; 43000 tokens 11.3, 14.3, 15.7 against 8.2, 12.5, 15.8.
+// Tokens of a row that one workgroup takes at any batch: it spares the join's launch, and the inverse CDF the history's
+// second gathering. All rules, fp32, us in a graph, 1 / 8 / 77 sequences, whole against slices:
+//             greedy                              Gumbel                               inverse CDF
+//    9001  7.5  7.8  8.8 : 8.6 9.3 10.1   10.2 10.5 11.8 : 10.3 11.2 12.2   14.4 18.5 20.2 : 17.3 21.7 22.9
+//   21847  8.4  9.5 10.8 : 8.6 9.4 10.9   12.5 13.3 14.8 : 10.4 11.7 14.2   15.6 19.9 22.1 : 17.2 21.2 23.4
+//   32000  9.9 11.0 12.1 : 8.5 9.5 12.5   14.9 15.9 17.2 : 10.4 11.6 17.1   17.1 21.5 23.4 : 16.7 21.3 31.6
+//   43000 11.4 13.7 14.9 : 8.6 9.4 12.8   18.0 21.2 22.6 : 10.4 11.7 17.6   19.2 24.8 26.6 : 17.2 21.2 31.4
+// One border for all three: the Gumbel choice of a few sequences gains 2 us from slices at 21847 already (it computes more
+// a token), the inverse CDF of 77 loses 5 by them at 43000.
 constexpr int CH_SMALL = 32768;
 constexpr int CH_SLICE = 8192;       // tokens of a slice at most (512 x 87383 bf16, processed: 51 us; of 4096 55, 16384 57)
 // History columns at most whose counts are hashed, 32 KB of LDS at the most. 512 x 87383 bf16, processed, histories of 256:
@@ -1033,8 +1047,10 @@ __global__ __launch_bounds__(CH_THREADS) void choose_cdf_kernel(const T *__restr
 
 // How B rows of V tokens are cut: about two workgroups per CU in all, of 4096 tokens (one batch) to CH_SLICE. `whole`: one
 // workgroup of CH_THREADS_ONE may take a sequence's whole vocabulary, where that spares the slices' joining (CH_SMALL) or
-// the sequences load the CUs evenly, to three quarters at least. fp32, greedy, 87383 tokens, whole and in slices, us: 130
-// sequences 22.1 and 21.3; 192: 23.0, 26.9; 250: 24.0, 31.2; 300: 37.9, 35.4; 512: 41.5, 50.7. hist_cols: 0 without a history.
+// the sequences load the CUs evenly, to three quarters at least. fp32, 87383 tokens, whole and in slices, us, greedy, Gumbel,
+// inverse CDF: 130 sequences 22.1 and 21.4, 36.9 and 34.6, 34.0 and 39.0; 192: 22.8, 27.9; 38.6, 43.6; 34.7, 45.4; 250: 23.8,
+// 32.2; 40.3, 51.0; 35.8, 50.4; 300: 38.0, 37.1; 60.4, 58.9; 51.4, 54.4; 400: 39.8, 44.7; 63.8, 72.9; 53.1, 61.6; 512: 43.4,
+// 52.9; 69.7, 88.3; 55.4, 70.0. hist_cols: 0 without a history.
 static Plan make_plan(int64_t B, int V, int64_t hist_cols, bool whole) {
   constexpr int UNIT = Batch<float, CH_THREADS>::TOKENS;
   static_assert(UNIT == Batch<bf16_t, CH_THREADS>::TOKENS && CH_SLICE % UNIT == 0, "slices are whole batches");

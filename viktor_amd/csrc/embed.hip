@@ -1,8 +1,9 @@
 // The token embedding at vocabularies past the 4-mers': the lookup of scaled rows and the table's gradient.
 //
 // Lookup: out[r, :] = round(scale * W[t_r, :]), the product in fp32. Ids outside [0, V) give zero rows. Bound by the rows
-// written (a frequent token's row is read from a cache): 524288 rows of 512 fp32 take 224 us (4.8 TB/s written), 40961 of
-// 1000 bf16 24 us; with stores that go through the caches 244 and 31.
+// written (a frequent token's row is read from a cache: of 1074 MB gathered from an 11 MB table, 542 pass the L2s): 524288
+// rows of 512 fp32 take 224 us (4.8 TB/s written), 40961 of 1000 bf16 24 us; with stores that go through the caches 244 and
+// 31. The same 40961 from bf16 to fp32 44, fp32 to bf16 37, fp32 to fp32 47.5.
 //
 // Gradient: g[v, :] = scale * sum over t_r = v of dY[r, :], fp32, without atomics on floats. Rows are brought into token
 // order first (a stable sort of the ids, row numbers as its payload), so that every vocabulary row is one run of
@@ -264,7 +265,9 @@ __global__ __launch_bounds__(1024) void embed_scatter_kernel(const int64_t *__re
 
 // The N columns of a lane in the sum. A group that the row's end cuts is moved back to stay inside the row, so that all
 // accesses are 16 bytes wide (columns that two lanes hold get the same sum); `own` is where its own columns begin. PLAIN:
-// sums are stored; else they may be added to what is there, and rows may be narrower than a group, column by column.
+// sums are stored; else they may be added to what is there, and rows may be narrower than a group, column by column (the
+// whole gradient, us, stored and added: 98305 x 768 bf16 into 21847 rows 78 and 134, fp32 105 and 134; 65536 x 512 fp32 into
+// 5463 53 and 66; rows of 7 bf16 70 and 73, of 3 fp32 36.5 and 38).
 template <typename T, bool PLAIN>
 struct Cols {
   static constexpr int N = 16 / sizeof(T), SPAN = 64 * N, U = 8;
