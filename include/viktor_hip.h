@@ -672,6 +672,73 @@ int vk_gemm_rows(const void *x, const void *w, void *y, int64_t M, int32_t N, in
                  void *stream);
 
 /*
+ * Objectives on the decoder's logits, with their gradients. Logits [B, T, V] bf16 or fp32 (dtype), V up to 2^30, element
+ * (b, t, v) at b ld_b + t ld_t + v (rows apart from each other); B T < 2^31; targets int64 and mask uint8 [B, T], contiguous
+ * as every other input and output. A token counts if its mask is set and its target is in [0, V); nothing else of a token
+ * that does not count is read, its outputs and gradients are zero. lp = log softmax(z)[target].
+ * dlogits [B, T, V] of the logits' type, or NULL for the loss alone. upstream: NULL, or one float on the device that the
+ * gradient is multiplied by; unless_one: do nothing where that is 1 (dlogits holds the gradient already). Outputs other than
+ * dlogits may be NULL then (loss included). Every sum runs in a fixed order. Workspace: vk_objective_workspace(B, T, P)
+ * bytes (P = 0 but for the preference loss), 16-byte aligned.
+ */
+#define VK_PER_SEQUENCE 0   /* a token's weight is inv_n over its sequence's tokens that count */
+#define VK_PER_TOKEN 1      /* inv_n */
+#define VK_PER_TOKEN_MEAN 2 /* one over all tokens that count */
+int vk_objective_workspace(int64_t B, int64_t T, int64_t P, int64_t *bytes);
+
+/*
+ * Clipped policy loss per token with a KL term to a reference policy. r = exp(lp - old_lp),
+ * pg = -min(r A, clip(r, 1 - eps_lo, 1 + eps_hi) A), x = ref_lp - lp, kl = exp(x) - x - 1,
+ * loss = sum of w (pg + kl_coef kl) with w by `per`. adv fp32 [B], or [B, T] with adv_per_token; ref_lp may be NULL
+ * (then kl_coef is 0 and kl NULL). The minimum's equal sides share its gradient evenly, as scripts/gspo.py:474-477's
+ * torch.minimum does. Writes loss, pg, kl, lp [B, T], dlogits. Beside vk_gspo_score, whose ratio is per sequence; the
+ * reference has no per-token objective.
+ */
+int vk_policy_score(const void *logits, int32_t dtype, int64_t ld_b, int64_t ld_t, const int64_t *targets,
+                    const uint8_t *mask, const float *old_lp, const float *adv, int32_t adv_per_token, const float *ref_lp,
+                    double eps_lo, double eps_hi, double kl_coef, int32_t per, double inv_n, float *loss, float *pg,
+                    float *kl, float *lp, void *dlogits, const float *upstream, int32_t unless_one, int64_t B, int64_t T,
+                    int32_t V, void *ws, int64_t ws_bytes, void *stream);
+
+/*
+ * Loss of paired log ratios. S_b = sum over b's tokens that count of (lp - ref_lp) / lengths[b] (ref_lp NULL: 0; lengths
+ * fp32 [B], positive, NULL: 1); pair p = (chosen, rejected) = pairs[2 p], pairs[2 p + 1] (int64; NULL: sequences 2 p and
+ * 2 p + 1, B = 2 P): margin_p = beta (S_chosen - S_rejected) - target,
+ * loss = inv_n sum_p (1 - smoothing) softplus(-margin_p) + smoothing softplus(margin_p).
+ * A sequence may be in any number of pairs; a pair with an index outside [0, B) has margin 0 and counts nothing.
+ * parts: 1 = loss, margin [P], lp [B, T]; 2 = dlogits, from what part 1 left in the workspace; 3 = both. No counterpart in
+ * the reference.
+ */
+int vk_preference_score(const void *logits, int32_t dtype, int64_t ld_b, int64_t ld_t, const int64_t *targets,
+                        const uint8_t *mask, const float *ref_lp, const float *lengths, const int64_t *pairs, int64_t P,
+                        double beta, double target, double smoothing, double inv_n, float *loss, float *margin, float *lp,
+                        void *dlogits, const float *upstream, int32_t unless_one, int32_t parts, int64_t B, int64_t T,
+                        int32_t V, void *ws, int64_t ws_bytes, void *stream);
+
+/*
+ * Divergence from a teacher's list of K (1 to 128) logits a token: values [B, T, K] bf16 or fp32, ids [B, T, K] int32 or
+ * int64 (ids_64); entries of value -inf or an id outside [0, V) are none, equal ids add. With p = softmax(z / tau) and
+ * q = softmax(values / tau) over the entries, or exp(values / tau - t_lse) where t_lse fp32 [B, T] is given:
+ * kl = sum q (log q - log p[id]), loss = tau^2 sum of w kl, w = weights (fp32 [B, T], NULL: 1) over their sum (mean) or
+ * times inv_n. Tokens with a weight that is not positive are not read; tokens without an entry count nothing in the sum of
+ * kl. Writes loss, kl [B, T], dlogits. Beside the weighted cross-entropy of viktor/model.py:153-177; the reference has no
+ * distillation.
+ */
+int vk_distill_score(const void *logits, int32_t dtype, int64_t ld_b, int64_t ld_t, const void *values,
+                     int32_t values_dtype, const void *ids, int32_t ids_64, int32_t K, const float *t_lse,
+                     const float *weights, double temperature, int32_t mean, double inv_n, float *loss, float *kl,
+                     void *dlogits, const float *upstream, int32_t unless_one, int64_t B, int64_t T, int32_t V, void *ws,
+                     int64_t ws_bytes, void *stream);
+
+/*
+ * The K (1 to 128, at most V) largest logits of each row in falling order, equal ones the lower id first: values
+ * [B, T, K] of the logits' type, ids int32 [B, T, K], lse fp32 [B, T] = log sum exp(z / temperature). Logits of -inf and NaN
+ * are no entries; a list that runs out ends in value -inf, id -1. Logits as above. No counterpart in the reference.
+ */
+int vk_top_logits(const void *logits, int32_t dtype, int64_t ld_b, int64_t ld_t, int32_t K, double temperature,
+                  void *values, int32_t *ids, float *lse, int64_t B, int64_t T, int32_t V, void *stream);
+
+/*
  * Timing support, no counterpart in the reference (its benchmark times whole replays): vk_timestamp stores the
  * device's constant-rate wall clock, read when its one-thread kernel runs, to stamps[index] (uint64, device
  * memory). Launched on a capturing stream it becomes a graph node, so a pair around another node times that node

@@ -23,6 +23,7 @@ _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
+_D = ctypes.c_double
 
 # name -> argument types (mirrors include/viktor_hip.h)
 SIGNATURES = {
@@ -96,6 +97,14 @@ SIGNATURES = {
     "vk_linear_residual_big": [_P, _P, _P, _I32, _I64, _I32, _I32, _P, _F, _P, _P, _P],
     "vk_rmsnorm_apply_ss": [_P, _I32, _P, _I32, _P, _I32, _P, _I64, _I32, _F, _P],
     "vk_rmsnorm_f32": [_P, _P, _P, _I64, _I32, _F, _P],
+    "vk_objective_workspace": [_I64, _I64, _I64, ctypes.POINTER(_I64)],
+    "vk_policy_score": [_P, _I32, _I64, _I64, _P, _P, _P, _P, _I32, _P, _D, _D, _D, _I32, _D, _P, _P, _P, _P, _P, _P, _I32,
+                        _I64, _I64, _I32, _P, _I64, _P],
+    "vk_preference_score": [_P, _I32, _I64, _I64, _P, _P, _P, _P, _P, _I64, _D, _D, _D, _D, _P, _P, _P, _P, _P, _I32, _I32,
+                            _I64, _I64, _I32, _P, _I64, _P],
+    "vk_distill_score": [_P, _I32, _I64, _I64, _P, _I32, _P, _I32, _I32, _P, _P, _D, _I32, _D, _P, _P, _P, _P, _I32, _I64,
+                         _I64, _I32, _P, _I64, _P],
+    "vk_top_logits": [_P, _I32, _I64, _I64, _I32, _D, _P, _P, _P, _I64, _I64, _I32, _P],
     "vk_timestamp": [_P, _I64, _P],
     "vk_timestamp_rate_khz": [ctypes.POINTER(_I64)],
     "vk_linear_qkv_rope": [_P, _P, _I64, _I32, _P, _P, _I32, _F, _P, _P, _I32, _I64, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64,
