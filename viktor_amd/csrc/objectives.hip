@@ -64,17 +64,6 @@ __device__ __forceinline__ void sum_parts(const double *parts, double *out) {
   __syncthreads();
 }
 
-// exp(x) - 1 - x without cancellation: its series below 1/2 (12 terms: off by 1e-16 of it), exp beyond.
-__device__ __forceinline__ double exp_beyond_line(double x) {
-  if (fabs(x) < 0.5) {
-    double t = 1.0;
-#pragma unroll
-    for (int n = 14; n >= 3; --n) t = fma(t * x, 1.0 / n, 1.0);
-    return 0.5 * x * x * t;
-  }
-  return exp(x) - 1.0 - x;
-}
-
 // Whether a token counts: masked in, with a target of the vocabulary.
 __device__ __forceinline__ bool counts(const uint8_t *mask, const int64_t *targets, int64_t row, int V, int &y) {
   const int64_t t = targets[row];
@@ -181,10 +170,10 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void policy_rows_kernel(Log
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL;
   __shared__ float sh[2][GL > 64 ? GL / 64 : 1];
   __shared__ float coef_sh;
-  __shared__ double total_sh, loss_sh[GROUPS];
+  __shared__ double total_sh, loss_sh[4];
   const float factor = a.up.get();
   if (a.up.done(factor)) return;
-  const int lane = threadIdx.x % GL, group = threadIdx.x / GL;
+  const int lane = lane_of<GL>(), group = group_of<GL>();
   double w_all = a.inv_n;
   if (a.per == VK_PER_TOKEN_MEAN) {
     sum_parts(a.weight_parts, &total_sh);
@@ -212,9 +201,11 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void policy_rows_kernel(Log
     float top = -INFINITY;
     r.values([&](float x) { top = fmaxf(top, x); });
     top = group_max<GL>(top, sh[0]);
+    r.keep();
     float s = 0.f;
     r.values([&](float x) { s += exp_of(x, top, kUnit); });
     s = group_add<GL>(s, sh[1]);
+    r.keep();
     float c = 0.f;
     if (GL <= 64 || threadIdx.x == 0) {
       const double lp = static_cast<double>(zy) - static_cast<double>(top) - log_of(s);
@@ -244,13 +235,8 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void policy_rows_kernel(Log
     if (lane == owner_of<T, GL>(r.s, y)) store_one(d + y, c + exp_of(zy, top, kUnit) * k);
   }
   if (!a.loss_parts) return;
-  if (lane == 0) loss_sh[group] = loss;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double v = 0.0;
-    for (int i = 0; i < GROUPS; ++i) v += loss_sh[i];
-    a.loss_parts[blockIdx.x] = v;
-  }
+  if (GROUPS > 1) loss = block_sum64(loss, loss_sh);
+  if (threadIdx.x == 0) a.loss_parts[blockIdx.x] = loss;
 }
 
 // ---- paired log ratios --------------------------------------------------------------------------------------------------
@@ -273,7 +259,7 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void token_ratio_kernel(Log
   typedef typename Row::type T;
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL;
   __shared__ float sh[2][GL > 64 ? GL / 64 : 1];
-  const int lane = threadIdx.x % GL, group = threadIdx.x / GL;
+  const int lane = lane_of<GL>(), group = group_of<GL>();
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < in.N;
        row += static_cast<int64_t>(gridDim.x) * GROUPS) {
     const uint32_t b = static_cast<uint32_t>(row) / in.T, t = static_cast<uint32_t>(row) % in.T;
@@ -292,9 +278,11 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void token_ratio_kernel(Log
     float top = -INFINITY;
     r.values([&](float x) { top = fmaxf(top, x); });
     top = group_max<GL>(top, sh[0]);
+    r.keep();
     float s = 0.f;
     r.values([&](float x) { s += exp_of(x, top, kUnit); });
     s = group_add<GL>(s, sh[1]);
+    r.keep();
     if (lane == 0) {
       const double lp = static_cast<double>(zy) - static_cast<double>(top) - log_of(s);
       a.lp[row] = static_cast<float>(lp);
@@ -379,7 +367,7 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void softmax_grad_kernel(Lo
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL;
   const float factor = up.get();
   if (up.done(factor)) return;
-  const int lane = threadIdx.x % GL, group = threadIdx.x / GL;
+  const int lane = lane_of<GL>(), group = group_of<GL>();
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < in.N;
        row += static_cast<int64_t>(gridDim.x) * GROUPS) {
     const uint32_t b = static_cast<uint32_t>(row) / in.T, t = static_cast<uint32_t>(row) % in.T;
@@ -440,13 +428,13 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
   constexpr int BITS = GL == 16 ? 1024 : GL == 64 ? 4096 : 65536;  // ids seen, by their low bits
   __shared__ float sh[2][GL > 64 ? GL / 64 : 1];
   __shared__ uint32_t seen[GROUPS * BITS / 32];
-  __shared__ double total_sh, loss_sh[GROUPS];
+  __shared__ double total_sh, loss_sh[4];
   __shared__ float qs[GROUPS][LIST_MAX];
   __shared__ int ids_sh[GROUPS][LIST_MAX];
   __shared__ float mass_sh;
   const float factor = a.up.get();
   if (a.up.done(factor)) return;
-  const int lane = threadIdx.x % GL, group = threadIdx.x / GL;
+  const int lane = lane_of<GL>(), group = group_of<GL>();
   for (int i = threadIdx.x; i < GROUPS * BITS / 32; i += group_threads(GL)) seen[i] = 0;
   double w_all = a.inv_n;
   if (a.mean) {
@@ -531,7 +519,8 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
       mass = static_cast<float>(mass64);
       if (!a.t_lse && mass64 != 0.0) {
         cross /= mass64;
-        lse_q = static_cast<double>(most) * a.inv_tau + log(mass64);
+        const float m32 = static_cast<float>(mass64);
+        lse_q = static_cast<double>(most) * a.inv_tau + log_of(m32) + (mass64 - m32) / mass64;
         const float rs = static_cast<float>(1.0 / mass64);
 #pragma unroll
         for (int i = 0; i < TeacherList<LL>::N; ++i) list.q[i] *= rs;
@@ -553,9 +542,11 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
     float top = -INFINITY;
     r.values([&](float x) { top = fmaxf(top, x); });
     top = group_max<GL>(top, sh[0]);
+    r.keep();
     float s = 0.f;
     r.values([&](float x) { s += exp_of(x, top, scale); });
     s = group_add<GL>(s, sh[1]);
+    r.keep();
     if constexpr (GL > 64) mass = mass_sh;
     const double share = static_cast<double>(w) * w_all * a.tau;
     if (lane == 0) {
@@ -596,13 +587,8 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
     group_sync<GL>();  // before the next row's list
   }
   if (!a.loss_parts) return;
-  if (lane == 0) loss_sh[group] = loss;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double v = 0.0;
-    for (int i = 0; i < GROUPS; ++i) v += loss_sh[i];
-    a.loss_parts[blockIdx.x] = v;
-  }
+  if (GROUPS > 1) loss = block_sum64(loss, loss_sh);
+  if (threadIdx.x == 0) a.loss_parts[blockIdx.x] = loss;
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
@@ -616,16 +602,21 @@ inline unsigned row_blocks(int64_t n, int gl) {
   return static_cast<unsigned>(want < most ? want : most);
 }
 
-template <typename T, typename F>
+template <typename T, bool LANES, typename F>
 int with_form(int V, F f) {
+  if constexpr (LANES) {
+    if (V <= 8) return f(static_cast<RowLane<T, 8> *>(nullptr));
+    if (V <= 16) return f(static_cast<RowLane<T, 16> *>(nullptr));
+  }
   return row_form((V + kVec<T> - 1) / kVec<T>, [&](auto gl, auto nv) {
     typedef typename RowForm<T, decltype(gl)::value, decltype(nv)::value>::type Row;
     return f(static_cast<Row *>(nullptr));
   });
 }
-template <typename F>
+// LANES: rows of up to 16 logits a thread each
+template <bool LANES, typename F>
 int with_row(int dtype, int V, F f) {
-  return dtype == VK_DTYPE_BF16 ? with_form<bf16_t>(V, f) : with_form<float>(V, f);
+  return dtype == VK_DTYPE_BF16 ? with_form<bf16_t, LANES>(V, f) : with_form<float, LANES>(V, f);
 }
 
 }  // namespace vk
@@ -688,7 +679,7 @@ extern "C" int vk_policy_score(const void *logits, int32_t dtype, int64_t ld_b, 
     const LogitRows in{logits, ld_b, ld_t, N, static_cast<uint32_t>(T), V};
     const PolicyArgs a{targets, mask, old_lp, adv, ref_lp, adv_per_token, 1.0 - eps_lo, 1.0 + eps_hi, kl_coef, per, inv_n,
                        counts, weight_parts, pg, kl, lp, dlogits, loss ? loss_parts : nullptr, up};
-    rc = with_row(dtype, V, [&](auto *form) {
+    rc = with_row<true>(dtype, V, [&](auto *form) {
       typedef typename std::remove_pointer<decltype(form)>::type Row;
       blocks = row_blocks(N, Row::GL);
       policy_rows_kernel<Row><<<blocks, group_threads(Row::GL), 0, st>>>(in, a);
@@ -729,7 +720,7 @@ extern "C" int vk_preference_score(const void *logits, int32_t dtype, int64_t ld
   const PairArgs a{targets, mask, ref_lp, lp, token_ratio, stats};
   if (forward) {
     if (N > 0) {
-      rc = with_row(dtype, V, [&](auto *form) {
+      rc = with_row<true>(dtype, V, [&](auto *form) {
         typedef typename std::remove_pointer<decltype(form)>::type Row;
         token_ratio_kernel<Row><<<row_blocks(N, Row::GL), group_threads(Row::GL), 0, st>>>(in, a);
         return launch_status("preference_score log-ratios");
@@ -748,7 +739,7 @@ extern "C" int vk_preference_score(const void *logits, int32_t dtype, int64_t ld
     if (rc != VK_OK) return rc;
   }
   if (!backward || N == 0) return VK_OK;
-  return with_row(dtype, V, [&](auto *form) {
+  return with_row<true>(dtype, V, [&](auto *form) {
     typedef typename std::remove_pointer<decltype(form)>::type Row;
     softmax_grad_kernel<Row><<<row_blocks(N, Row::GL), group_threads(Row::GL), 0, st>>>(in, a, coef, dlogits,
                                                                                        Upstream{upstream, unless_one});
@@ -793,7 +784,7 @@ extern "C" int vk_distill_score(const void *logits, int32_t dtype, int64_t ld_b,
     const LogitRows in{logits, ld_b, ld_t, N, static_cast<uint32_t>(T), V};
     const DistillArgs a{values, values_dtype == VK_DTYPE_BF16, ids, ids_64, K, t_lse, weights, temperature,
                         1.0 / temperature, ExpScale::of(temperature), parts, scale, weight_parts, kl, dlogits, loss ? loss_parts : nullptr, up};
-    rc = with_row(dtype, V, [&](auto *form) {
+    rc = with_row<false>(dtype, V, [&](auto *form) {
       typedef typename std::remove_pointer<decltype(form)>::type Row;
       blocks = row_blocks(N, Row::GL);
       distill_rows_kernel<Row><<<blocks, group_threads(Row::GL), 0, st>>>(in, a);

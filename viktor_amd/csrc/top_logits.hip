@@ -1,12 +1,14 @@
 // The k largest logits of each row with their ids, in falling order (equal values: the lower id first), and the row's
 // log-sum-exp: a teacher's list for distillation.
 //
-// The row stays in registers. A bound that at least k logits reach comes from one value a thread: each wavefront finds the
-// ceil(k / wavefronts)-th largest of its lanes' maxima, bit by bit with ballots, and the least of these bounds the row's
-// k-th logit from below. What reaches it (a little more than k logits of most rows) goes to shared memory, where each
-// candidate counts the ones before it: its place in the list. Rows with more candidates than fit (many equal logits, lists
-// nearly as long as the row) have their k-th logit searched bit by bit over all of it, then the id up to which equal ones
-// are taken. Logits of -inf and NaN are no entries: a list that runs out ends in id -1, value -inf.
+// The row stays in the registers of a wavefront (up to 512 logits, element lane + 64 i with lane `lane`) or of a workgroup.
+// A bound that at least k logits reach comes from one value a thread: each wavefront finds the ceil(k / wavefronts)-th
+// largest of its lanes' maxima, bit by bit with ballots, and the least of these bounds the row's k-th logit from below. What
+// reaches it (a little more than k logits of most rows) goes to shared memory with its id, and one wavefront sorts it in
+// registers. Rows with more candidates than fit (many equal logits, lists nearly as long as the row) have their k-th logit
+// searched bit by bit over all of it, then the id up to which equal ones are taken. Rows of up to 16 logits go one a thread:
+// each logit counts the ones before it.
+// Logits of -inf and NaN are no entries: a list that runs out ends in id -1, value -inf.
 #include "common.h"
 #include "vocab_rows.h"
 
@@ -24,6 +26,50 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
+// A logit and its id as one number, larger ones first in the list: 64 bits, or 32 where the logit is a bf16 and the id
+// fits 16.
+template <typename Entry>
+__device__ __forceinline__ Entry entry_of(float z, int id);
+template <>
+__device__ __forceinline__ uint64_t entry_of(float z, int id) {
+  return (static_cast<uint64_t>(key_of(z)) << 32) | (0xffffffffu - static_cast<uint32_t>(id));
+}
+template <>
+__device__ __forceinline__ uint32_t entry_of(float z, int id) {
+  return (key_of(z) & 0xffff0000u) | (0xffffu - static_cast<uint32_t>(id));
+}
+__device__ __forceinline__ float value_of(uint64_t e) { return of_key(static_cast<uint32_t>(e >> 32)); }
+__device__ __forceinline__ int id_of(uint64_t e) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(e)); }
+// (a negative bf16's key has ones below)
+__device__ __forceinline__ float value_of(uint32_t e) {
+  return of_key(e & 0x80000000u ? e & 0xffff0000u : e | 0xffffu);
+}
+__device__ __forceinline__ int id_of(uint32_t e) { return static_cast<int>(0xffffu - (e & 0xffffu)); }
+
+// Element lane + 64 i with lane `lane`: every lane has its share of a short row.
+template <typename T, int NE>
+struct RowStrided {
+  typedef T type;
+  static constexpr int GL = 64;
+  float z[NE];
+
+  __device__ __forceinline__ void load(const T *p, int V, int lane) {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) z[i] = lane + 64 * i < V ? load_one(p + lane + 64 * i) : -INFINITY;
+  }
+  __device__ __forceinline__ void keep() {}
+  template <typename F>
+  __device__ __forceinline__ void values(F f) const {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) f(z[i]);
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(int lane, F f) const {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) f(lane + 64 * i, z[i]);
+  }
+};
+
 // Sum of an int over the group; callable again at once.
 template <int GL>
 __device__ __forceinline__ int group_count(int v, int *sh) {
@@ -40,30 +86,82 @@ __device__ __forceinline__ int group_count(int v, int *sh) {
   return v;
 }
 
-template <typename Row>
+// Sorts 64 R entries of a wavefront, entry 64 r + lane with e[r], the largest first (bitonic).
+template <typename Entry, int R>
+__device__ __forceinline__ void sort_entries(Entry (&e)[R], int lane) {
+#pragma unroll
+  for (int k = 2; k <= 64 * R; k <<= 1) {
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      if (j >= 64) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int q = r ^ (j >> 6);
+          if (q > r) {
+            const bool falls = ((64 * r + lane) & k) == 0 || k == 64 * R;
+            const Entry hi = e[r] > e[q] ? e[r] : e[q], lo = e[r] > e[q] ? e[q] : e[r];
+            e[r] = falls ? hi : lo;
+            e[q] = falls ? lo : hi;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const bool falls = ((64 * r + lane) & k) == 0 || k == 64 * R, first = (lane & j) == 0;
+          const Entry o = __shfl_xor(e[r], j, kWave);
+          e[r] = (falls == first) == (e[r] > o) ? e[r] : o;
+        }
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void write_entry(T *values, int32_t *ids, int64_t at, float value, int id) {
+  store_one(values + at, value);
+  ids[at] = id;
+}
+
+template <typename T, typename Entry, int R>
+__device__ __forceinline__ void sort_and_write(const Entry *cand, int C, int K, T *values, int32_t *ids, int64_t at, int lane) {
+  Entry e[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) e[r] = 64 * r + lane < C ? cand[64 * r + lane] : 0;
+  sort_entries<Entry, R>(e, lane);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int place = 64 * r + lane;
+    if (place < K) write_entry(values, ids, at + place, e[r] ? value_of(e[r]) : -INFINITY, e[r] ? id_of(e[r]) : -1);
+  }
+  for (int place = 64 * R + lane; place < K; place += 64) write_entry(values, ids, at + place, -INFINITY, -1);
+}
+
+template <typename Row, typename Entry>
 __global__ __launch_bounds__(group_threads(Row::GL)) void top_rows_kernel(const void *logits, int64_t ld_b, int64_t ld_t,
                                                                          int64_t N, uint32_t T_, int V, int K, ExpScale scale,
-                                                                         double inv_tau, void *values, int32_t *ids,
+                                                                         double inv_tau, void *values_, int32_t *ids,
                                                                          float *lse) {
   typedef typename Row::type T;
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL, WAVES = GL / 64;
-  constexpr int CAP = GL == 64 ? 256 : 512;  // candidates
-  __shared__ uint64_t cand[GROUPS][CAP];
+  constexpr int CAP = 512;  // candidates
+  __shared__ Entry cand[GROUPS][CAP];
   __shared__ int taken[GROUPS];
   __shared__ float sh[2][WAVES];
   __shared__ int shc[WAVES];
   __shared__ uint32_t shk[WAVES];
-  const int lane = threadIdx.x % GL, group = threadIdx.x / GL;
+  const int lane = lane_of<GL>(), group = group_of<GL>();
+  T *values = static_cast<T *>(values_);
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < N;
        row += static_cast<int64_t>(gridDim.x) * GROUPS) {
     const uint32_t b = static_cast<uint32_t>(row) / T_, t = static_cast<uint32_t>(row) % T_;
     const T *z = static_cast<const T *>(logits) + b * ld_b + t * ld_t;
     Row r;
     r.load(z, V, lane);
-    if (lane == 0) taken[group] = 0;
+    if (GL > 64 && lane == 0) taken[group] = 0;
     float mine = -INFINITY;
     r.values([&](float x) { mine = fmaxf(mine, x); });
     const float top = group_max<GL>(mine, sh[0]);
+    r.keep();
     // the wavefront's bound
     const int share = (K + WAVES - 1) / WAVES;
     uint32_t bound = 0;
@@ -75,8 +173,7 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void top_rows_kernel(const 
         const uint32_t trial = bound | (1u << bit);
         if (__popcll(__ballot(key >= trial)) >= share) bound = trial;
       }
-      // (a negative bf16's key has ones there)
-      if (LOW && bound && !(bound & 0x80000000u)) bound |= 0xffffu;
+      if (LOW && bound && !(bound & 0x80000000u)) bound |= 0xffffu;  // (a negative bf16's key has ones there)
     }
     if constexpr (GL > 64) {
       if ((threadIdx.x & 63) == 0) shk[threadIdx.x >> 6] = bound;
@@ -84,72 +181,124 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void top_rows_kernel(const 
     float s = 0.f;
     r.values([&](float x) { s += exp_of(x, top, scale); });
     s = group_add<GL>(s, sh[1]);
+    r.keep();
     if constexpr (GL > 64) {
       bound = shk[0];
 #pragma unroll
       for (int w = 1; w < WAVES; ++w) bound = min(bound, shk[w]);
     }
-    group_sync<GL>();
     if (lane == 0) lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (top == -INFINITY ? 0.0 : log_of(s)));
     // candidates
-    const float floor = bound ? of_key(bound) : -INFINITY;
-    int n = 0;
-    r.values([&](float x) { n += (x >= floor && x > -INFINITY) ? 1 : 0; });
-    int at = n ? atomicAdd(&taken[group], n) : 0;
-    group_sync<GL>();
-    int C = taken[group];
-    group_sync<GL>();
-    if (C <= CAP) {
-      if (n)
-        r.each(lane, [&](int i, float x) {
-          if (x >= floor && x > -INFINITY) cand[group][at++] = (static_cast<uint64_t>(key_of(x)) << 32) | (0xffffffffu - i);
-        });
+    const float least = bound ? of_key(bound) : -INFINITY;
+    auto reaches = [&](float x) { return x >= least && x > -INFINITY; };
+    int C = 0;
+    if constexpr (GL == 64) {
+      r.each(lane, [&](int i, float x) {
+        const uint64_t m = __ballot(reaches(x));
+        if (m) {
+          const int at = C + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(m >> 32),
+                                                       __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(m), 0));
+          if (reaches(x) && at < CAP) cand[group][at] = entry_of<Entry>(x, i);
+          C += __popcll(m);
+        }
+      });
     } else {
-      // the k-th key, bit by bit over the row (more than CAP >= K logits are above -inf), then the ids of its equals
+      int n = 0;
+      r.values([&](float x) { n += reaches(x) ? 1 : 0; });
+      r.keep();
+      int at = n ? atomicAdd(&taken[group], n) : 0;
+      if (n && at + n <= CAP)
+        r.each(lane, [&](int i, float x) {
+          if (reaches(x)) cand[group][at++] = entry_of<Entry>(x, i);
+        });
+      __syncthreads();
+      C = taken[group];
+    }
+    if (C > CAP) {
+      // the k-th key, bit by bit over the row (more than CAP >= K logits are above -inf), then the ids of its equals. (Walked in
+      // memory: the registers of a form for this rare case would be every row's.)
+      RowWalk<T, GL> w;
+      w.load(z, V, lane);
       uint32_t kth = 0;
       for (int bit = 31; bit >= 0; --bit) {
         const uint32_t trial = kth | (1u << bit);
         const float f = of_key(trial);
         int c = 0;
-        r.values([&](float x) { c += x >= f ? 1 : 0; });
+        w.values([&](float x) { c += x >= f ? 1 : 0; });
         if (group_count<GL>(c, shc) >= K) kth = trial;
       }
       const float f = of_key(kth);
       int c = 0;
-      r.values([&](float x) { c += x > f ? 1 : 0; });
+      w.values([&](float x) { c += x > f ? 1 : 0; });
       const int want = K - group_count<GL>(c, shc);
       uint32_t last = 0;  // the largest id bound that has fewer than `want` equals below it
       for (int bit = 30; bit >= 0; --bit) {
         const uint32_t trial = last | (1u << bit);
         c = 0;
-        r.each(lane, [&](int i, float x) { c += (x == f && static_cast<uint32_t>(i) < trial) ? 1 : 0; });
+        w.each(lane, [&](int i, float x) { c += (x == f && static_cast<uint32_t>(i) < trial) ? 1 : 0; });
         if (group_count<GL>(c, shc) < want) last = trial;
       }
       if (lane == 0) taken[group] = 0;
       group_sync<GL>();
-      r.each(lane, [&](int i, float x) {
+      w.each(lane, [&](int i, float x) {
         if (x > f || (x == f && static_cast<uint32_t>(i) <= last))
-          cand[group][atomicAdd(&taken[group], 1)] = (static_cast<uint64_t>(key_of(x)) << 32) | (0xffffffffu - i);
+          cand[group][atomicAdd(&taken[group], 1)] = entry_of<Entry>(x, i);
       });
       C = K;
     }
     group_sync<GL>();
-    // each candidate's place
-    for (int i = lane; i < C; i += GL) {
-      const uint64_t me = cand[group][i];
-      int place = 0;
-      for (int j = 0; j < C; ++j) place += cand[group][j] > me ? 1 : 0;
-      if (place < K) {
-        store_one(static_cast<T *>(values) + row * K + place, of_key(static_cast<uint32_t>(me >> 32)));
-        ids[row * K + place] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(me));
+    const int64_t at = row * K;
+    if (C <= 256) {
+      if (lane < 64) {
+        if (C <= 64)
+          sort_and_write<T, Entry, 1>(cand[group], C, K, values, ids, at, lane);
+        else if (C <= 128)
+          sort_and_write<T, Entry, 2>(cand[group], C, K, values, ids, at, lane);
+        else
+          sort_and_write<T, Entry, 4>(cand[group], C, K, values, ids, at, lane);
       }
-    }
-    for (int i = C + lane; i < K; i += GL) {
-      store_one(static_cast<T *>(values) + row * K + i, -INFINITY);
-      ids[row * K + i] = -1;
+    } else {
+      // each candidate's place: how many are before it (C > 256 > K: no places are left over)
+      for (int i = lane; i < C; i += GL) {
+        const Entry me = cand[group][i];
+        int place = 0;
+        for (int j = 0; j < C; ++j) place += cand[group][j] > me ? 1 : 0;
+        if (place < K) write_entry(values, ids, at + place, value_of(me), id_of(me));
+      }
     }
     group_sync<GL>();
   }
+}
+
+// Rows of up to NE logits, one a thread.
+template <typename T, int NE>
+__global__ __launch_bounds__(256) void top_lanes_kernel(const void *logits, int64_t ld_b, int64_t ld_t, int64_t N, uint32_t T_,
+                                                       int V, int K, ExpScale scale, double inv_tau, void *values,
+                                                       int32_t *ids, float *lse) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (row >= N) return;
+  const uint32_t b = static_cast<uint32_t>(row) / T_, t = static_cast<uint32_t>(row) % T_;
+  RowLane<T, NE> r;
+  r.load(static_cast<const T *>(logits) + b * ld_b + t * ld_t, V, 0);
+  float top = -INFINITY, s = 0.f;
+  r.values([&](float x) { top = fmaxf(top, x); });
+  r.values([&](float x) { s += exp_of(x, top, scale); });
+  lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (top == -INFINITY ? 0.0 : log_of(s)));
+  uint32_t key[NE];
+  int entries = 0;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    key[i] = key_of(r.z[i]);
+    entries += key[i] ? 1 : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    int place = 0;
+#pragma unroll
+    for (int j = 0; j < NE; ++j) place += (j < i ? key[j] >= key[i] : key[j] > key[i]) ? 1 : 0;
+    if (key[i] && place < K) write_entry(static_cast<T *>(values), ids, row * K + place, of_key(key[i]), i);
+  }
+  for (int place = entries; place < K; ++place) write_entry(static_cast<T *>(values), ids, row * K + place, -INFINITY, -1);
 }
 
 }  // namespace vk
@@ -169,17 +318,25 @@ extern "C" int vk_top_logits(const void *logits, int32_t dtype, int64_t ld_b, in
   VK_CHECK_ARG(logits && values && ids && lse, "top_logits: null pointer");
   VK_CHECK_ARG((T < 2 || ld_t >= V) && (B < 2 || ld_b >= V) && ld_t >= 0 && ld_b >= 0, "top_logits: rows overlap");
   const ExpScale scale = ExpScale::of(temperature);
+  auto run = [&](auto kernel, int threads, int groups, bool all) {
+    const int64_t want = (N + groups - 1) / groups, most = static_cast<int64_t>(device_cus_cached()) * (2048 / threads);
+    kernel<<<static_cast<unsigned>(all || want < most ? want : most), threads, 0, VK_STREAM(stream)>>>(
+        logits, ld_b, ld_t, N, static_cast<uint32_t>(T), V, K, scale, 1.0 / temperature, values, ids, lse);
+    return launch_status("top_logits");
+  };
   auto launch = [&](auto elem) {
     typedef decltype(elem) E;
+    typedef typename std::conditional<sizeof(E) == 2, uint32_t, uint64_t>::type Short;
+    if (V <= 8) return run(top_lanes_kernel<E, 8>, 256, 256, true);
+    if (V <= 16) return run(top_lanes_kernel<E, 16>, 256, 256, true);
+    if (V <= 256) return run(top_rows_kernel<RowStrided<E, 4>, Short>, 256, 4, false);
+    if (V <= 512) return run(top_rows_kernel<RowStrided<E, 8>, Short>, 256, 4, false);
     return row_form((V + kVec<E> - 1) / kVec<E>, [&](auto gl, auto nv) {
       constexpr int G = decltype(gl)::value < 64 ? 64 : decltype(gl)::value;
-      constexpr int NV = decltype(gl)::value < 64 ? 2 : decltype(nv)::value;  // 16 lanes of 3 or 6 vectors: 64 of 2
+      constexpr int NV = decltype(gl)::value < 64 ? 3 : decltype(nv)::value;
       typedef typename RowForm<E, G, NV>::type Row;
-      constexpr int threads = group_threads(G), groups = threads / G;
-      const int64_t want = (N + groups - 1) / groups, most = static_cast<int64_t>(device_cus_cached()) * (2048 / threads);
-      top_rows_kernel<Row><<<static_cast<unsigned>(want < most ? want : most), threads, 0, VK_STREAM(stream)>>>(
-          logits, ld_b, ld_t, N, static_cast<uint32_t>(T), V, K, scale, 1.0 / temperature, values, ids, lse);
-      return launch_status("top_logits");
+      if (V <= 65536) return run(top_rows_kernel<Row, Short>, group_threads(G), group_threads(G) / G, false);
+      return run(top_rows_kernel<Row, uint64_t>, group_threads(G), group_threads(G) / G, false);
     });
   };
   return dtype == VK_DTYPE_BF16 ? launch(bf16_t{}) : launch(float{});

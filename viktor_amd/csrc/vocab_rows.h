@@ -47,6 +47,7 @@ __device__ __forceinline__ int edge_index(const Span &s, int l) {
 // the thread (of GL) that holds element i
 template <typename T, int GL>
 __device__ __forceinline__ int owner_of(const Span &s, int i) {
+  if constexpr (GL == 1) return 0;
   if (i < s.head) return i;
   const int j = (i - s.head) / kVec<T>;
   return j < s.nv ? j % GL : i - s.nv * kVec<T>;
@@ -112,6 +113,12 @@ struct RowRegs {
     }
     edge = lane < s.edges ? load_one(p + edge_index<T>(s, lane)) : -INFINITY;
   }
+  // Between two walks: the vectors stay as they are. (The compiler keeps every element of the first walk unpacked for the
+  // next ones otherwise, twice the registers.)
+  __device__ __forceinline__ void keep() {
+#pragma unroll
+    for (int c = 0; c < NV; ++c) asm("" : "+v"(v[c]));
+  }
   // f(value) for each element, with -inf for places behind the end
   template <typename F>
   __device__ __forceinline__ void values(F f) const {
@@ -148,6 +155,35 @@ struct RowRegs {
   }
 };
 
+// A row of up to NE elements in one thread. (Its loads and stores are 2 or 4 bytes a lane, a row's length apart; the lines
+// they share stay in the caches: 512 x 1024 rows of 7 bf16 move 4.9 TB/s so.)
+template <typename T, int NE>
+struct RowLane {
+  typedef T type;
+  static constexpr int GL = 1;
+  Span s;
+  float z[NE];
+  int n;
+
+  __device__ __forceinline__ void load(const T *p, int V, int lane) {
+    n = V;
+#pragma unroll
+    for (int k = 0; k < NE; ++k) z[k] = k < V ? load_one(p + k) : -INFINITY;
+  }
+  __device__ __forceinline__ void keep() {}
+  template <typename F>
+  __device__ __forceinline__ void values(F f) const {
+#pragma unroll
+    for (int k = 0; k < NE; ++k) f(z[k]);
+  }
+  template <typename F>
+  __device__ __forceinline__ void write(T *d, int lane, F f) const {
+#pragma unroll
+    for (int k = 0; k < NE; ++k)
+      if (k < n) store_one(d + k, f(z[k]));
+  }
+};
+
 // Of any length: read again by each walk.
 template <typename T, int GL_>
 struct RowWalk {
@@ -164,6 +200,7 @@ struct RowWalk {
     s = span_of(p, V);
     edge = lane < s.edges ? load_one(p + edge_index<T>(s, lane)) : -INFINITY;
   }
+  __device__ __forceinline__ void keep() {}
   template <typename F>
   __device__ __forceinline__ void values(F f) const {
     for (int j = lane; j < s.nv; j += GL) {
@@ -218,7 +255,7 @@ __device__ __forceinline__ void zero_row(T *d, int V, int lane) {
   const Span s = span_of(d, V);
   const float o[kVec<T>] = {};
   for (int j = lane; j < s.nv; j += GL) store_row(d + s.head + static_cast<int64_t>(j) * kVec<T>, o);
-  if (lane < s.edges) store_one(d + edge_index<T>(s, lane), 0.f);
+  for (int l = lane; l < s.edges; l += GL) store_one(d + edge_index<T>(s, l), 0.f);
 }
 
 // log s of a sum of exponentials, off by some 3e-8 whatever its size: the exponent's part in 64 bits, the mantissa's
@@ -233,10 +270,46 @@ __device__ __forceinline__ double log_of(float s) {
   return static_cast<double>(ex) * 0.6931471805599453 + static_cast<double>(log1pf(m - 1.f));
 }
 
-// Threads of a workgroup that holds groups of GL.
-constexpr int group_threads(int GL) { return GL < 256 ? 256 : GL; }
+// exp(x) - 1, off by a few 1e-16 of it (and of x near 0): a series on x halved until it is under 1/2, then
+// expm1(2 y) = expm1(y) (expm1(y) + 2). A dozen registers, where the library's takes thirty from the row.
+__device__ __forceinline__ double series_beyond_line(double x) {  // exp(x) - 1 - x for |x| < 1/2
+  double t = 1.0;
+#pragma unroll
+  for (int n = 14; n >= 3; --n) t = fma(t * x, 1.0 / n, 1.0);
+  return 0.5 * x * x * t;
+}
+__device__ __forceinline__ double expm1_of(double x) {
+  int m;
+  frexp(x, &m);
+  if (!(fabs(x) >= 0.5) || fabs(x) > 800.0) m = -1;
+  const double y = ldexp(fabs(x) > 800.0 ? 0.0 : x, -(m + 1));
+  double e = y + series_beyond_line(y);
+  for (; m >= 0; --m) e *= e + 2.0;
+  if (x > 800.0) e = INFINITY;
+  if (x < -800.0) e = -1.0;
+  return e;
+}
+// exp(x) - 1 - x without cancellation
+__device__ __forceinline__ double exp_beyond_line(double x) {
+  return fabs(x) < 0.5 ? series_beyond_line(x) : expm1_of(x) - x;
+}
 
-// The smallest register form that holds that many vectors: calls f(GL, NV), both as integral constants; NV = 0 for rows
+// Threads of a workgroup that holds groups of GL; a thread's group, known to be the same for a wavefront where it is (row
+// numbers and row addresses are scalars then); its place in the group.
+constexpr int group_threads(int GL) { return GL < 256 ? 256 : GL; }
+template <int GL>
+__device__ __forceinline__ int group_of() {
+  if constexpr (GL >= 256) return 0;
+  if constexpr (GL >= 64) return __builtin_amdgcn_readfirstlane(threadIdx.x / GL);
+  return threadIdx.x / GL;
+}
+template <int GL>
+__device__ __forceinline__ int lane_of() {
+  if constexpr (GL >= 256) return threadIdx.x;
+  return threadIdx.x % GL;
+}
+
+// The smallest register form of at least 16 lanes that holds that many vectors: calls f(GL, NV), both as integral constants; NV = 0 for rows
 // that are walked.
 template <typename F>
 inline int row_form(int64_t vectors, F f) {
@@ -256,6 +329,7 @@ inline int row_form(int64_t vectors, F f) {
   return f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 0>{});
 }
 
+// GL = 1: NV is the number of elements
 template <typename T, int GL, int NV>
 struct RowForm {
   typedef RowRegs<T, GL, NV> type;
@@ -263,6 +337,10 @@ struct RowForm {
 template <typename T, int GL>
 struct RowForm<T, GL, 0> {
   typedef RowWalk<T, GL> type;
+};
+template <typename T, int NE>
+struct RowForm<T, 1, NE> {
+  typedef RowLane<T, NE> type;
 };
 
 }  // namespace vk
