@@ -209,7 +209,7 @@ def check_preference(z, y, mask, ref, scale=1.0, **kw):
     near(got["margin"], want["margin"], mtol, "margin")
     P = max(want["margin"].numel(), 1)
     times = kw["inv_n"] * P if kw.get("inv_n") else 1.0
-    m = float(mtol.max()) if want["margin"].numel() else 0.0
+    m = float(mtol.detach().max()) if want["margin"].numel() else 0.0
     near(got["loss"], want["loss"], times * m + 2.0 ** -23 * (1 + float(want["loss"].detach().abs())), "loss")
     # a sequence's coefficient: the slopes of its pairs (each off by m / 4) with beta / P / length
     check_gradient(got["dlogits"], leaf, want["loss"], z.dtype, 4 * tol + m, "preference")
@@ -480,7 +480,7 @@ def test_same_bits_every_run():
         a = score(z, **kw)
         for _ in range(3):
             b = score(z, **kw)
-            assert all(torch.equal(a[k], b[k]) for k in a if k != "workspace" and a[k] is not None)
+            assert all(torch.equal(a[k], b[k]) for k in a if a[k] is not None)
 
 
 def test_forms_agree():
@@ -552,7 +552,7 @@ def test_side_stream():
         top2 = ops.top_logits(z, 20)
     side.synchronize()
     for a, b in zip(wants, gots):
-        assert all(torch.equal(a[k], b[k]) for k in a if k != "workspace" and a[k] is not None)
+        assert all(torch.equal(a[k], b[k]) for k in a if a[k] is not None)
     assert all(torch.equal(a, b) for a, b in zip(top, top2))
 
 
@@ -564,7 +564,7 @@ def test_captured_and_replayed():
     def program():
         outs = []
         for loss_fn, score, _, kw in calls:
-            outs += [v for k, v in score(leaf.detach(), **kw).items() if k != "workspace" and v is not None]
+            outs += [v for k, v in score(leaf.detach(), **kw).items() if v is not None]
             loss = loss_fn(leaf, **kw)[0]
             outs += [loss.detach(), *torch.autograd.grad(loss * 0.5, leaf)]
             outs += torch.autograd.grad(loss_fn(leaf, **kw)[0], leaf)
@@ -601,15 +601,14 @@ def test_refusals():
                   dict(mask=mask[:1]), dict(old_lp=old.double()), dict(old_lp=old[:1]), dict(old_lp=None), dict(adv=adv[:2]),
                   dict(adv=adv.double()), dict(ref_lp=ref[:, :2]), dict(kl_coef=0.1, ref_lp=None), dict(per="batch"),
                   dict(eps_lo=-0.1), dict(out=torch.empty(4, 6, 33, device=DEV, dtype=BF16)), dict(out=z), dict(out=z[:, :3]),
-                  dict(unless_one=True), dict(upstream=adv), dict(out=torch.empty_like(z), grad=False),
+                  dict(upstream=adv), dict(out=torch.empty_like(z), grad=False),
                   dict(targets=y.cpu()), dict(upstream=torch.ones((), dtype=torch.float64, device=DEV))]
     for kw in bad_policy:
         with pytest.raises((AssertionError, RuntimeError)):
             ops.policy_score(**{**dict(logits=z, targets=y, mask=mask, old_lp=old, adv=adv, ref_lp=ref), **kw})
     for kw in (dict(logits=z[:3], targets=y[:3], mask=mask[:3], ref_lp=ref[:3]), dict(pairs=torch.zeros(2, 2, device=DEV)),
                dict(pairs=torch.zeros(4, dtype=torch.long, device=DEV)), dict(lengths=adv[:1]), dict(smoothing=1.5),
-               dict(smoothing=math.nan), dict(unless_one=True, upstream=adv[:1]),
-               dict(workspace=torch.empty(8, dtype=torch.uint8, device=DEV)), dict(ref_lp=ref.double())):
+               dict(smoothing=math.nan), dict(ref_lp=ref.double())):
         with pytest.raises(AssertionError):
             ops.preference_score(**{**dict(logits=z, targets=y, mask=mask, ref_lp=ref), **kw})
     for kw in (dict(values=val[..., :3]), dict(values=val.double()), dict(ids=ids.short()), dict(values=val[0], ids=ids[0]),

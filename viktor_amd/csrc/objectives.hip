@@ -43,17 +43,21 @@ struct Upstream {
   __device__ __forceinline__ bool done(float f) const { return unless_one && f == 1.f; }
 };
 
-// Sum over a workgroup of 256 threads, in a fixed order; every thread gets it.
+// Sum over a workgroup, in a fixed order; every thread gets it. sh: a number per wavefront.
+template <int THREADS = 256>
 __device__ __forceinline__ double block_sum64(double v, double *sh) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
   __syncthreads();
-  return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+  v = sh[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) v += sh[w];
+  return v;
 }
 
-// Sum of OBJ_PARTS partial sums by the first wavefront of a workgroup, to *out in shared memory (a barrier behind it).
+// Sum of OBJ_PARTS partial sums by the first wavefront of a workgroup, to *out in shared memory (a barrier has to follow).
 __device__ __forceinline__ void sum_parts(const double *parts, double *out) {
   if (threadIdx.x < 64) {
     double v = (parts[threadIdx.x] + parts[threadIdx.x + 64]) + (parts[threadIdx.x + 128] + parts[threadIdx.x + 192]);
@@ -61,7 +65,6 @@ __device__ __forceinline__ void sum_parts(const double *parts, double *out) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
     if (threadIdx.x == 0) *out = v;
   }
-  __syncthreads();
 }
 
 // Whether a token counts: masked in, with a target of the vocabulary.
@@ -69,6 +72,44 @@ __device__ __forceinline__ bool counts(const uint8_t *mask, const int64_t *targe
   const int64_t t = targets[row];
   y = static_cast<int>(t);
   return mask[row] != 0 && t >= 0 && t < V;
+}
+
+// A token's target and mask as loaded, ahead of their use.
+struct Token {
+  int64_t target;
+  uint8_t mask;
+  __device__ __forceinline__ void load(const uint8_t *m, const int64_t *t, int64_t row, int64_t N) {
+    const int64_t at = row < N ? row : N - 1;
+    target = t[at];
+    mask = m[at];
+  }
+  __device__ __forceinline__ bool counts(int V) const { return mask != 0 && target >= 0 && target < V; }
+};
+
+// The same by the rows' own kernels, where that is the cheaper way (count_here below): the tokens of a sequence that count, by
+// a group.
+template <int GL>
+__device__ __forceinline__ int count_sequence(const uint8_t *mask, const int64_t *targets, int64_t b, int64_t T, int V, int lane,
+                                              float *sh) {
+  int n = 0, y;
+  for (int64_t t = lane; t < T; t += GL) n += counts(mask, targets, b * T + t, V, y);
+  return static_cast<int>(group_add<GL>(static_cast<float>(n), sh));  // (below 2^24: exact)
+}
+// All tokens that count or, where weights are given, their sum, by a workgroup; every thread gets it.
+template <int THREADS>
+__device__ __forceinline__ double count_all(const uint8_t *mask, const int64_t *targets, const float *weights, int64_t N, int V,
+                                            double *sh) {
+  double v = 0.0;
+  int y;
+  for (int64_t i = threadIdx.x; i < N; i += THREADS) {
+    if (weights) {
+      const float w = weights[i];
+      if (w > 0.f) v += static_cast<double>(w);
+    } else if (counts(mask, targets, i, V, y)) {
+      v += 1.0;
+    }
+  }
+  return block_sum64<THREADS>(v, sh);
 }
 
 // A wavefront per sequence: how many of its tokens count.
@@ -126,7 +167,7 @@ struct PolicyArgs {
   int per;                 // VK_PER_*
   double inv_n;
   const int32_t *counts;
-  const double *weight_parts;
+  const double *weight_parts;  // NULL: counted here
   float *pg, *kl, *lp;
   void *dlogits;
   double *loss_parts;
@@ -164,29 +205,42 @@ __device__ __forceinline__ PolicyTerms policy_terms(double lp, float old_lp, flo
   return t;
 }
 
-template <typename Row>
-__global__ __launch_bounds__(group_threads(Row::GL)) void policy_rows_kernel(LogitRows in, PolicyArgs a) {
+// COUNTS: each group counts its rows' sequences (per sequence, where no launch did).
+template <typename Row, bool COUNTS>
+__global__ __launch_bounds__(group_threads(Row::GL), Row::WAVES_A_SIMD) void policy_rows_kernel(LogitRows in, PolicyArgs a) {
   typedef typename Row::type T;
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL;
-  __shared__ float sh[2][GL > 64 ? GL / 64 : 1];
+  __shared__ float sh[2][GL > 64 ? GL / 64 : 1], count_sh[COUNTS && GL > 64 ? GL / 64 : 1];
   __shared__ float coef_sh;
-  __shared__ double total_sh, loss_sh[4];
+  __shared__ double total_sh, loss_sh[group_threads(GL) / 64];
   const float factor = a.up.get();
   if (a.up.done(factor)) return;
   const int lane = lane_of<GL>(), group = group_of<GL>();
   double w_all = a.inv_n;
   if (a.per == VK_PER_TOKEN_MEAN) {
-    sum_parts(a.weight_parts, &total_sh);
-    w_all = 1.0 / fmax(total_sh, 1.0);
+    double total;
+    if (a.weight_parts) {
+      sum_parts(a.weight_parts, &total_sh);
+      __syncthreads();
+      total = total_sh;
+    } else {
+      total = count_all<group_threads(GL)>(a.mask, a.targets, nullptr, in.N, in.V, loss_sh);
+    }
+    w_all = 1.0 / fmax(total, 1.0);
   }
   double loss = 0.0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < in.N;
-       row += static_cast<int64_t>(gridDim.x) * GROUPS) {
+  int turn = 0;  // a workgroup's wavefronts do the tokens' 64-bit numbers in turn: they are on one SIMD each
+  const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group;
+  for (; row < in.N; row += step) {
+    Token token;
+    token.load(a.mask, a.targets, row, in.N);
     const uint32_t b = static_cast<uint32_t>(row) / in.T, t = static_cast<uint32_t>(row) % in.T;
     T *d = a.dlogits ? static_cast<T *>(a.dlogits) + row * in.V : nullptr;
-    int y;
-    if (!counts(a.mask, a.targets, row, in.V, y)) {
-      if (d) zero_row<T, GL>(d, in.V, lane);
+    const int lead = GL > 64 ? turn : 0;
+    if (GL > 64) turn = (turn + 64) % GL;
+    if (!token.counts(in.V)) {
+      if (d) Row::zero(d, in.V, lane);
       if (lane == 0) {
         if (a.lp) a.lp[row] = 0.f;
         if (a.pg) a.pg[row] = 0.f;
@@ -195,25 +249,23 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void policy_rows_kernel(Log
       continue;
     }
     const T *z = in.row<T>(b, t);
+    const int y = static_cast<int>(token.target);
+    const float zy = load_one(z + y);
     Row r;
     r.load(z, in.V, lane);
-    const float zy = load_one(z + y);
-    float top = -INFINITY;
-    r.values([&](float x) { top = fmaxf(top, x); });
-    top = group_max<GL>(top, sh[0]);
-    r.keep();
-    float s = 0.f;
-    r.values([&](float x) { s += exp_of(x, top, kUnit); });
-    s = group_add<GL>(s, sh[1]);
-    r.keep();
+    int among = 1;
+    if constexpr (COUNTS) among = count_sequence<GL>(a.mask, a.targets, b, in.T, in.V, lane, count_sh);
+    float top, s;
+    row_stats<GL>(r, kUnit, sh, top, s);
     float c = 0.f;
-    if (GL <= 64 || threadIdx.x == 0) {
+    if (GL <= 64 || lane == lead) {
       const double lp = static_cast<double>(zy) - static_cast<double>(top) - log_of(s);
       const PolicyTerms p = policy_terms(lp, a.old_lp[row], a.adv[a.adv_per_token ? row : b], a.ref_lp != nullptr,
                                          a.ref_lp ? a.ref_lp[row] : 0.f, a.lo, a.hi, a.kl_coef);
-      const double w = a.per == VK_PER_SEQUENCE ? w_all / static_cast<double>(a.counts[b]) : w_all;
+      if (!COUNTS && a.per == VK_PER_SEQUENCE) among = a.counts[b];
+      const double w = w_all / static_cast<double>(among);
       c = static_cast<float>(w * static_cast<double>(p.g) * static_cast<double>(factor));
-      if (lane == 0) {
+      if (lane == lead) {
         loss += w * p.loss;
         if (a.lp) a.lp[row] = static_cast<float>(p.lp);
         if (a.pg) a.pg[row] = static_cast<float>(p.pg);
@@ -230,12 +282,12 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void policy_rows_kernel(Log
       c = coef_sh;
     }
     const float k = -c / s;
-    r.write(d, lane, [&](float x) { return exp_of(x, top, kUnit) * k; });
+    r.write(d, lane, top, kUnit, k);
     // (after this thread's own vector that holds it)
     if (lane == owner_of<T, GL>(r.s, y)) store_one(d + y, c + exp_of(zy, top, kUnit) * k);
   }
   if (!a.loss_parts) return;
-  if (GROUPS > 1) loss = block_sum64(loss, loss_sh);
+  loss = block_sum64<group_threads(GL)>(loss, loss_sh);
   if (threadIdx.x == 0) a.loss_parts[blockIdx.x] = loss;
 }
 
@@ -260,11 +312,15 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void token_ratio_kernel(Log
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL;
   __shared__ float sh[2][GL > 64 ? GL / 64 : 1];
   const int lane = lane_of<GL>(), group = group_of<GL>();
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < in.N;
-       row += static_cast<int64_t>(gridDim.x) * GROUPS) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group;
+  Token next;
+  next.load(a.mask, a.targets, row, in.N);
+  for (; row < in.N; row += step) {
+    const Token token = next;
+    next.load(a.mask, a.targets, row + step, in.N);
     const uint32_t b = static_cast<uint32_t>(row) / in.T, t = static_cast<uint32_t>(row) % in.T;
-    int y;
-    if (!counts(a.mask, a.targets, row, in.V, y)) {
+    if (!token.counts(in.V)) {
       if (lane == 0) {
         a.lp[row] = 0.f;
         a.ratio[row] = 0.f;
@@ -272,22 +328,16 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void token_ratio_kernel(Log
       continue;
     }
     const T *z = in.row<T>(b, t);
+    const float zy = load_one(z + static_cast<int>(token.target)), ref_lp = a.ref_lp ? a.ref_lp[row] : 0.f;
     Row r;
     r.load(z, in.V, lane);
-    const float zy = load_one(z + y);
-    float top = -INFINITY;
-    r.values([&](float x) { top = fmaxf(top, x); });
-    top = group_max<GL>(top, sh[0]);
-    r.keep();
-    float s = 0.f;
-    r.values([&](float x) { s += exp_of(x, top, kUnit); });
-    s = group_add<GL>(s, sh[1]);
-    r.keep();
+    float top, s;
+    row_stats<GL>(r, kUnit, sh, top, s);
     if (lane == 0) {
       const double lp = static_cast<double>(zy) - static_cast<double>(top) - log_of(s);
       a.lp[row] = static_cast<float>(lp);
       // (rounded to 32 bits after the difference: off by 2^-24 of the ratio, not of lp)
-      a.ratio[row] = static_cast<float>(lp - (a.ref_lp ? static_cast<double>(a.ref_lp[row]) : 0.0));
+      a.ratio[row] = static_cast<float>(lp - static_cast<double>(ref_lp));
       if (a.stats) a.stats[row] = RowStats{top, 1.f / s};
     }
   }
@@ -313,49 +363,88 @@ __device__ __forceinline__ double logistic(double x) {
   return (x >= 0.0 ? 1.0 : e) / (1.0 + e);
 }
 
-// One workgroup: every pair's margin, the loss, and the loss's derivative by the margin's log-ratio difference.
+// Pair p's margin, the loss's derivative by its log-ratio difference, and (returned) its share of the loss over inv_n.
+__device__ __forceinline__ double pair_terms(const double *ratio, const int64_t *pairs, int64_t p, int64_t B, double beta,
+                                             double target, double smoothing, double inv_n, float *margin, double *slope) {
+  const int64_t c = pairs ? pairs[2 * p] : 2 * p, r = pairs ? pairs[2 * p + 1] : 2 * p + 1;
+  double h = 0.0, dh = 0.0, loss = 0.0;
+  if (c >= 0 && c < B && r >= 0 && r < B) {
+    h = beta * (ratio[c] - ratio[r]) - target;
+    loss = (1.0 - smoothing) * softplus(-h) + smoothing * softplus(h);
+    // sigma(h) - (1 - smoothing), without cancellation where the margin is far
+    dh = inv_n * beta * (smoothing * logistic(h) - (1.0 - smoothing) * logistic(-h));
+  }
+  margin[p] = static_cast<float>(h);
+  slope[p] = dh;
+  return loss;
+}
+
+// The derivative of the loss by the tokens' log-probabilities of sequence b, from all pairs that name it, by a wavefront.
+__device__ __forceinline__ double sequence_slope(const double *slope, const int64_t *pairs, int64_t b, int64_t P, int lane) {
+  if (!pairs) return b / 2 < P ? ((b & 1) ? -slope[b / 2] : slope[b / 2]) : 0.0;
+  double v = 0.0;
+  for (int64_t p = lane; p < P; p += 64) {
+    const int64_t c = pairs[2 * p], r = pairs[2 * p + 1];
+    const double s = slope[p];
+    if (c == b) v += s;
+    if (r == b) v -= s;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+  return v;
+}
+
+// One workgroup: every pair's margin and slope, and the loss.
 __global__ __launch_bounds__(256) void pair_loss_kernel(const double *__restrict__ ratio, const int64_t *__restrict__ pairs,
                                                        int64_t P, int64_t B, double beta, double target, double smoothing,
                                                        double inv_n, float *__restrict__ margin, double *__restrict__ slope,
                                                        float *__restrict__ loss) {
   __shared__ double sh[4];
   double sum = 0.0;
-  for (int64_t p = threadIdx.x; p < P; p += 256) {
-    const int64_t c = pairs ? pairs[2 * p] : 2 * p, r = pairs ? pairs[2 * p + 1] : 2 * p + 1;
-    double h = 0.0, dh = 0.0;
-    if (c >= 0 && c < B && r >= 0 && r < B) {
-      h = beta * (ratio[c] - ratio[r]) - target;
-      sum += (1.0 - smoothing) * softplus(-h) + smoothing * softplus(h);
-      // sigma(h) - (1 - smoothing), without cancellation where the margin is far
-      dh = inv_n * beta * (smoothing * logistic(h) - (1.0 - smoothing) * logistic(-h));
-    }
-    margin[p] = static_cast<float>(h);
-    slope[p] = dh;
-  }
+  for (int64_t p = threadIdx.x; p < P; p += 256)
+    sum += pair_terms(ratio, pairs, p, B, beta, target, smoothing, inv_n, margin, slope);
   sum = block_sum64(sum, sh);
   if (threadIdx.x == 0) loss[0] = static_cast<float>(sum * inv_n);
 }
 
-// A wavefront per sequence: the derivative of the loss by its tokens' log-probabilities, from all pairs that name it.
+// A wavefront per sequence.
 __global__ __launch_bounds__(256) void sequence_slope_kernel(const double *__restrict__ slope, const int64_t *__restrict__ pairs,
                                                             const float *__restrict__ lengths, int64_t P, int64_t B,
                                                             float *__restrict__ coef) {
   const int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (b >= B) return;
-  double v = 0.0;
-  if (pairs) {
-    for (int64_t p = threadIdx.x & 63; p < P; p += 64) {
-      const int64_t c = pairs[2 * p], r = pairs[2 * p + 1];
-      const double s = slope[p];
-      if (c == b) v += s;
-      if (r == b) v -= s;
-    }
+  const double v = sequence_slope(slope, pairs, b, P, threadIdx.x & 63);
+  if ((threadIdx.x & 63) == 0) coef[b] = static_cast<float>(lengths ? v / static_cast<double>(lengths[b]) : v);
+}
+
+// The three steps above in one workgroup, for calls of few tokens: two launches less. 260 tokens in 2 pairs: 28.1 -> 22.8 us;
+// 16384 tokens and 4096 (sequence, pair) combinations each take it 3 us, as long as the launches do.
+constexpr int64_t PAIRS_AT_ONCE_TOKENS = 8192, PAIRS_AT_ONCE_PAIRS = 1024;
+__global__ __launch_bounds__(1024) void pairs_at_once_kernel(const float *__restrict__ token_ratio,
+                                                             const float *__restrict__ lengths, const int64_t *__restrict__ pairs,
+                                                             int P, int B, int64_t T, double beta, double target,
+                                                             double smoothing, double inv_n, double *ratio, double *slope,
+                                                             float *__restrict__ margin, float *__restrict__ loss,
+                                                             float *__restrict__ coef) {
+  __shared__ double sh[16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int b = wave; b < B; b += 16) {
+    double v = 0.0;
+    for (int64_t t = lane; t < T; t += 64) v += static_cast<double>(token_ratio[b * T + t]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-  } else {
-    v = b / 2 < P ? ((b & 1) ? -slope[b / 2] : slope[b / 2]) : 0.0;
+    if (lane == 0) ratio[b] = lengths ? v / static_cast<double>(lengths[b]) : v;
   }
-  if ((threadIdx.x & 63) == 0) coef[b] = static_cast<float>(lengths ? v / static_cast<double>(lengths[b]) : v);
+  __syncthreads();
+  double sum = 0.0;
+  for (int p = threadIdx.x; p < P; p += 1024)
+    sum += pair_terms(ratio, pairs, p, B, beta, target, smoothing, inv_n, margin, slope);
+  sum = block_sum64<1024>(sum, sh);
+  if (threadIdx.x == 0) loss[0] = static_cast<float>(sum * inv_n);
+  for (int b = wave; b < B; b += 16) {
+    const double v = sequence_slope(slope, pairs, b, P, lane);
+    if (lane == 0) coef[b] = static_cast<float>(lengths ? v / static_cast<double>(lengths[b]) : v);
+  }
 }
 
 // dlogits = c (onehot(y) - softmax) with the rows' maxima and sums known.
@@ -368,23 +457,28 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void softmax_grad_kernel(Lo
   const float factor = up.get();
   if (up.done(factor)) return;
   const int lane = lane_of<GL>(), group = group_of<GL>();
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < in.N;
-       row += static_cast<int64_t>(gridDim.x) * GROUPS) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group;
+  Token next;
+  next.load(a.mask, a.targets, row, in.N);
+  for (; row < in.N; row += step) {
+    const Token token = next;
+    next.load(a.mask, a.targets, row + step, in.N);
     const uint32_t b = static_cast<uint32_t>(row) / in.T, t = static_cast<uint32_t>(row) % in.T;
     T *d = static_cast<T *>(dlogits) + row * in.V;
-    int y;
     const float c = coef[b] * factor;
-    if (!counts(a.mask, a.targets, row, in.V, y) || c == 0.f) {
-      zero_row<T, GL>(d, in.V, lane);
+    if (!token.counts(in.V) || c == 0.f) {
+      Row::zero(d, in.V, lane);
       continue;
     }
     const T *z = in.row<T>(b, t);
-    Row r;
-    r.load(z, in.V, lane);
+    const int y = static_cast<int>(token.target);
     const float zy = load_one(z + y);
     const RowStats st = a.stats[row];
+    Row r;
+    r.load(z, in.V, lane);
     const float k = -c * st.rs;
-    r.write(d, lane, [&](float x) { return exp_of(x, st.top, kUnit) * k; });
+    r.write_fresh(d, lane, st.top, kUnit, k);
     if (lane == owner_of<T, GL>(r.s, y)) store_one(d + y, c + exp_of(zy, st.top, kUnit) * k);
   }
 }
@@ -404,14 +498,14 @@ struct DistillArgs {
   ExpScale scale;
   int mean;  // the weights over their sum (weight_parts), else times inv_n
   double inv_n;
-  const double *weight_parts;
+  const double *weight_parts;  // NULL: summed here
   float *kl;
   void *dlogits;
   double *loss_parts;
   Upstream up;
 };
 
-// What the lanes of a list's wavefront (or of a group of 16) hold of it: entry i with lane i % LL.
+// What the lanes of the list's wavefront (or of a group of 16) hold of it: entry i with lane i % LL.
 template <int LL>
 struct TeacherList {
   static constexpr int N = LIST_MAX / LL;
@@ -424,11 +518,11 @@ template <typename Row>
 __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(LogitRows in, DistillArgs a) {
   typedef typename Row::type T;
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL;
-  constexpr int LL = GL < 64 ? GL : 64;                       // lanes that hold the list: the group's first wavefront
+  constexpr int LL = GL < 64 ? GL : 64;                       // lanes that hold the list
   constexpr int BITS = GL == 16 ? 1024 : GL == 64 ? 4096 : 65536;  // ids seen, by their low bits
   __shared__ float sh[2][GL > 64 ? GL / 64 : 1];
   __shared__ uint32_t seen[GROUPS * BITS / 32];
-  __shared__ double total_sh, loss_sh[4];
+  __shared__ double total_sh, loss_sh[group_threads(GL) / 64];
   __shared__ float qs[GROUPS][LIST_MAX];
   __shared__ int ids_sh[GROUPS][LIST_MAX];
   __shared__ float mass_sh;
@@ -438,20 +532,31 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
   for (int i = threadIdx.x; i < GROUPS * BITS / 32; i += group_threads(GL)) seen[i] = 0;
   double w_all = a.inv_n;
   if (a.mean) {
-    sum_parts(a.weight_parts, &total_sh);
-    w_all = total_sh > 0.0 ? 1.0 / total_sh : 0.0;
+    double total;
+    if (a.weight_parts) {
+      sum_parts(a.weight_parts, &total_sh);
+      __syncthreads();
+      total = total_sh;
+    } else {
+      total = count_all<group_threads(GL)>(nullptr, nullptr, a.weights, in.N, in.V, loss_sh);
+    }
+    w_all = total > 0.0 ? 1.0 / total : 0.0;
   }
-  __syncthreads();
+  __syncthreads();  // (what was seen: nothing)
   uint32_t *bits = seen + group * (BITS / 32);
   const ExpScale scale = a.scale;
   double loss = 0.0;
+  int turn = 0;  // a workgroup's wavefronts hold the list and do the token's numbers in turn
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < in.N;
        row += static_cast<int64_t>(gridDim.x) * GROUPS) {
     const uint32_t b = static_cast<uint32_t>(row) / in.T, t = static_cast<uint32_t>(row) % in.T;
     T *d = a.dlogits ? static_cast<T *>(a.dlogits) + row * in.V : nullptr;
     const float w = a.weights ? a.weights[row] : 1.f;
+    const int ll = GL > 64 ? static_cast<int>(threadIdx.x) - turn : lane;  // the list's lanes: 0 .. LL - 1
+    const bool holds = ll >= 0 && ll < LL;
+    if (GL > 64) turn = (turn + 64) % GL;
     if (!(w > 0.f)) {
-      if (d) zero_row<T, GL>(d, in.V, lane);
+      if (d) Row::zero(d, in.V, lane);
       if (lane == 0 && a.kl) a.kl[row] = 0.f;
       continue;
     }
@@ -463,11 +568,11 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
     double cross = 0.0, lse_q = 0.0, mass64 = 0.0;
     float mass = 0.f;
     bool twice = false;
-    if (lane < LL) {
+    if (holds) {
       float tv[TeacherList<LL>::N], most = -INFINITY;
 #pragma unroll
       for (int i = 0; i < TeacherList<LL>::N; ++i) {
-        const int e = i * LL + lane;
+        const int e = i * LL + ll;
         list.id[i] = -1;
         list.zt[i] = 0.f;
         tv[i] = -INFINITY;
@@ -527,11 +632,11 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
         mass = mass64 > 0.0 ? 1.f : mass;
         mass64 = mass;
       }
-      if (GL > 64 && lane == 0) mass_sh = mass;
+      if (GL > 64 && ll == 0) mass_sh = mass;
       if (twice) {
 #pragma unroll
         for (int i = 0; i < TeacherList<LL>::N; ++i) {
-          const int e = i * LL + lane;
+          const int e = i * LL + ll;
           if (e < a.K) {
             ids_sh[group][e] = list.id[i];
             qs[group][e] = list.q[i];
@@ -539,17 +644,11 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
         }
       }
     }
-    float top = -INFINITY;
-    r.values([&](float x) { top = fmaxf(top, x); });
-    top = group_max<GL>(top, sh[0]);
-    r.keep();
-    float s = 0.f;
-    r.values([&](float x) { s += exp_of(x, top, scale); });
-    s = group_add<GL>(s, sh[1]);
-    r.keep();
+    float top, s;
+    row_stats<GL>(r, scale, sh, top, s);
     if constexpr (GL > 64) mass = mass_sh;
     const double share = static_cast<double>(w) * w_all * a.tau;
-    if (lane == 0) {
+    if (ll == 0) {
       // sum q (log q - log p) = sum q (t - z) / tau + Q (lse_p - lse_q)
       const double kl = mass == 0.f ? 0.0
                                     : cross + mass64 * (static_cast<double>(top) * a.inv_tau + log_of(s) - lse_q);
@@ -560,14 +659,14 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
       const float c = static_cast<float>(share * static_cast<double>(factor));
       const float k = mass == 0.f ? 0.f : c * mass / s;
       if (mass == 0.f)
-        zero_row<T, GL>(d, in.V, lane);
+        Row::zero(d, in.V, lane);
       else
-        r.write(d, lane, [&](float x) { return exp_of(x, top, scale) * k; });
+        r.write(d, lane, top, scale, k);
       group_sync<GL>();
-      if (lane < LL) {
+      if (holds) {
 #pragma unroll
         for (int i = 0; i < TeacherList<LL>::N; ++i) {
-          const int id = list.id[i], e = i * LL + lane;
+          const int id = list.id[i], e = i * LL + ll;
           if (id < 0) continue;
           float q = list.q[i];
           bool mine = true;
@@ -587,7 +686,7 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
     group_sync<GL>();  // before the next row's list
   }
   if (!a.loss_parts) return;
-  if (GROUPS > 1) loss = block_sum64(loss, loss_sh);
+  loss = block_sum64<group_threads(GL)>(loss, loss_sh);
   if (threadIdx.x == 0) a.loss_parts[blockIdx.x] = loss;
 }
 
@@ -600,6 +699,13 @@ inline unsigned row_blocks(int64_t n, int gl) {
   int64_t most = static_cast<int64_t>(device_cus_cached()) * (2048 / threads);
   if (most > OBJ_BLOCKS) most = OBJ_BLOCKS;
   return static_cast<unsigned>(want < most ? want : most);
+}
+
+// Whether the rows' kernel counts the tokens itself: a launch less (2.7 us of the host, 1.6 on the GPU and the gap), for N
+// numbers read by every workgroup or T by every row. 148 tokens of 37: 24.0 -> 21.3 us. Calls whose rows are more than the
+// chip holds at once keep the launch, which is nothing beside them.
+inline bool count_here(int64_t n, int64_t T, int gl, bool per_sequence) {
+  return gl > 1 && n <= 2048 && (!per_sequence || T <= 4 * gl);
 }
 
 template <typename T, bool LANES, typename F>
@@ -670,19 +776,28 @@ extern "C" int vk_policy_score(const void *logits, int32_t dtype, int64_t ld_b, 
   const Upstream up{upstream, unless_one};
   unsigned blocks = 0;
   if (N > 0) {
-    if (per == VK_PER_SEQUENCE)
-      sequence_counts_kernel<<<static_cast<unsigned>((B + 3) / 4), 256, 0, st>>>(mask, targets, counts, B, T, V, up);
-    else if (per == VK_PER_TOKEN_MEAN)
-      weight_parts_kernel<<<OBJ_PARTS, 256, 0, st>>>(mask, targets, nullptr, weight_parts, N, V, up);
-    rc = launch_status("policy_score counts");
-    if (rc != VK_OK) return rc;
     const LogitRows in{logits, ld_b, ld_t, N, static_cast<uint32_t>(T), V};
-    const PolicyArgs a{targets, mask, old_lp, adv, ref_lp, adv_per_token, 1.0 - eps_lo, 1.0 + eps_hi, kl_coef, per, inv_n,
+    PolicyArgs a{targets, mask, old_lp, adv, ref_lp, adv_per_token, 1.0 - eps_lo, 1.0 + eps_hi, kl_coef, per, inv_n,
                        counts, weight_parts, pg, kl, lp, dlogits, loss ? loss_parts : nullptr, up};
     rc = with_row<true>(dtype, V, [&](auto *form) {
       typedef typename std::remove_pointer<decltype(form)>::type Row;
       blocks = row_blocks(N, Row::GL);
-      policy_rows_kernel<Row><<<blocks, group_threads(Row::GL), 0, st>>>(in, a);
+      if (per != VK_PER_TOKEN && count_here(N, T, Row::GL, per == VK_PER_SEQUENCE)) {
+        a.weight_parts = nullptr;
+        if (per == VK_PER_SEQUENCE) {
+          if constexpr (Row::GL > 1) {
+            policy_rows_kernel<Row, true><<<blocks, group_threads(Row::GL), 0, st>>>(in, a);
+            return launch_status("policy_score");
+          }
+        }
+      } else if (per == VK_PER_SEQUENCE) {
+        sequence_counts_kernel<<<static_cast<unsigned>((B + 3) / 4), 256, 0, st>>>(mask, targets, counts, B, T, V, up);
+      } else if (per == VK_PER_TOKEN_MEAN) {
+        weight_parts_kernel<<<OBJ_PARTS, 256, 0, st>>>(mask, targets, nullptr, weight_parts, N, V, up);
+      }
+      const int rc2 = launch_status("policy_score counts");
+      if (rc2 != VK_OK) return rc2;
+      policy_rows_kernel<Row, false><<<blocks, group_threads(Row::GL), 0, st>>>(in, a);
       return launch_status("policy_score");
     });
     if (rc != VK_OK) return rc;
@@ -727,14 +842,19 @@ extern "C" int vk_preference_score(const void *logits, int32_t dtype, int64_t ld
       });
       if (rc != VK_OK) return rc;
     }
-    if (B > 0) sequence_ratio_kernel<<<static_cast<unsigned>(B), 256, 0, st>>>(token_ratio, lengths, ratio, T);
-    rc = launch_status("preference_score sequences");
-    if (rc != VK_OK) return rc;
-    pair_loss_kernel<<<1, 256, 0, st>>>(ratio, pairs, P, B, beta, target, smoothing, inv_n, margin, slope, loss);
-    rc = launch_status("preference_score pairs");
-    if (rc != VK_OK) return rc;
-    if (B > 0)
-      sequence_slope_kernel<<<static_cast<unsigned>((B + 3) / 4), 256, 0, st>>>(slope, pairs, lengths, P, B, coef);
+    if (B > 0 && B <= 64 && N <= PAIRS_AT_ONCE_TOKENS && P <= PAIRS_AT_ONCE_PAIRS) {
+      pairs_at_once_kernel<<<1, 1024, 0, st>>>(token_ratio, lengths, pairs, static_cast<int>(P), static_cast<int>(B), T, beta,
+                                               target, smoothing, inv_n, ratio, slope, margin, loss, coef);
+    } else {
+      if (B > 0) sequence_ratio_kernel<<<static_cast<unsigned>(B), 256, 0, st>>>(token_ratio, lengths, ratio, T);
+      rc = launch_status("preference_score sequences");
+      if (rc != VK_OK) return rc;
+      pair_loss_kernel<<<1, 256, 0, st>>>(ratio, pairs, P, B, beta, target, smoothing, inv_n, margin, slope, loss);
+      rc = launch_status("preference_score pairs");
+      if (rc != VK_OK) return rc;
+      if (B > 0)
+        sequence_slope_kernel<<<static_cast<unsigned>((B + 3) / 4), 256, 0, st>>>(slope, pairs, lengths, P, B, coef);
+    }
     rc = launch_status("preference_score slopes");
     if (rc != VK_OK) return rc;
   }
@@ -769,23 +889,19 @@ extern "C" int vk_distill_score(const void *logits, int32_t dtype, int64_t ld_b,
   const Upstream up{upstream, unless_one};
   unsigned blocks = 0;
   if (N > 0) {
-    bool parts = false;
-    double scale = inv_n;
-    if (mean) {
-      if (weights) {
-        weight_parts_kernel<<<OBJ_PARTS, 256, 0, st>>>(nullptr, nullptr, weights, weight_parts, N, V, up);
-        rc = launch_status("distill_score weights");
-        if (rc != VK_OK) return rc;
-        parts = true;
-      } else {
-        scale = 1.0 / static_cast<double>(N);
-      }
-    }
+    const bool sums = mean && weights;
+    const double scale = mean ? 1.0 / static_cast<double>(N) : inv_n;
     const LogitRows in{logits, ld_b, ld_t, N, static_cast<uint32_t>(T), V};
-    const DistillArgs a{values, values_dtype == VK_DTYPE_BF16, ids, ids_64, K, t_lse, weights, temperature,
-                        1.0 / temperature, ExpScale::of(temperature), parts, scale, weight_parts, kl, dlogits, loss ? loss_parts : nullptr, up};
+    DistillArgs a{values, values_dtype == VK_DTYPE_BF16, ids, ids_64, K, t_lse, weights, temperature,
+                        1.0 / temperature, ExpScale::of(temperature), sums, scale, weight_parts, kl, dlogits, loss ? loss_parts : nullptr, up};
     rc = with_row<false>(dtype, V, [&](auto *form) {
       typedef typename std::remove_pointer<decltype(form)>::type Row;
+      if (sums && count_here(N, T, Row::GL, false))
+        a.weight_parts = nullptr;
+      else if (sums)
+        weight_parts_kernel<<<OBJ_PARTS, 256, 0, st>>>(nullptr, nullptr, weights, weight_parts, N, V, up);
+      const int rc2 = launch_status("distill_score weights");
+      if (rc2 != VK_OK) return rc2;
       blocks = row_blocks(N, Row::GL);
       distill_rows_kernel<Row><<<blocks, group_threads(Row::GL), 0, st>>>(in, a);
       return launch_status("distill_score");

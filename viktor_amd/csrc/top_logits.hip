@@ -1,14 +1,15 @@
 // The k largest logits of each row with their ids, in falling order (equal values: the lower id first), and the row's
 // log-sum-exp: a teacher's list for distillation.
 //
-// The row stays in the registers of a wavefront (up to 512 logits, element lane + 64 i with lane `lane`) or of a workgroup.
-// A bound that at least k logits reach comes from one value a thread: each wavefront finds the ceil(k / wavefronts)-th
-// largest of its lanes' maxima, bit by bit with ballots, and the least of these bounds the row's k-th logit from below. What
-// reaches it (a little more than k logits of most rows) goes to shared memory with its id, and one wavefront sorts it in
-// registers. Rows with more candidates than fit (many equal logits, lists nearly as long as the row) have their k-th logit
-// searched bit by bit over all of it, then the id up to which equal ones are taken. Rows of up to 16 logits go one a thread:
-// each logit counts the ones before it.
+// The row stays in the registers of a wavefront (up to 512 logits, element lane + 64 i with lane `lane`; to 704 vectors of 16
+// bytes, whole vectors) or of a workgroup. A bound that at least k logits reach comes from one or a few maxima a thread: bit
+// by bit with ballots, the largest number that k of the maxima reach. What reaches it in the row (a little more than k logits
+// of most rows) goes to shared memory with its id, and one wavefront sorts it in registers. Rows with more candidates than fit
+// (many equal logits) have their k-th logit searched bit by bit over all of it, then the id up to which equal ones are taken.
+// Rows of up to 16 logits go one a thread: each logit counts the ones before it.
 // Logits of -inf and NaN are no entries: a list that runs out ends in id -1, value -inf.
+#include <float.h>
+
 #include "common.h"
 #include "vocab_rows.h"
 
@@ -50,8 +51,15 @@ __device__ __forceinline__ int id_of(uint32_t e) { return static_cast<int>(0xfff
 template <typename T, int NE>
 struct RowStrided {
   typedef T type;
-  static constexpr int GL = 64;
+  static constexpr int GL = 64, TOP_WAVES = 8, TOP_MAXIMA = NE;
   float z[NE];
+
+  template <int M>
+  __device__ __forceinline__ void maxima(float (&m)[M]) const {
+    static_assert(M == NE, "its elements");
+#pragma unroll
+    for (int i = 0; i < M; ++i) m[i] = z[i];
+  }
 
   __device__ __forceinline__ void load(const T *p, int V, int lane) {
 #pragma unroll
@@ -84,6 +92,22 @@ __device__ __forceinline__ int group_count(int v, int *sh) {
     __syncthreads();
   }
   return v;
+}
+
+// A bound that k of a wavefront's keys reach, R keys a lane: the largest with zeros in its low half (BF16: the keys are of bf16
+// values, which have nothing there) or in its low 12 bits, from its highest bit down; 0 where fewer than k keys are above 0.
+template <int R, bool BF16>
+__device__ __forceinline__ uint32_t kth_key(const uint32_t (&key)[R], int k) {
+  uint32_t bound = 0;
+#pragma unroll
+  for (int bit = 31; bit >= (BF16 ? 16 : 12); --bit) {
+    const uint32_t trial = bound | (1u << bit);
+    int n = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) n += __popcll(__ballot(key[r] >= trial));
+    if (n >= k) bound = trial;
+  }
+  return BF16 && bound && !(bound & 0x80000000u) ? bound | 0xffffu : bound;  // (a negative bf16's key has ones there)
 }
 
 // Sorts 64 R entries of a wavefront, entry 64 r + lane with e[r], the largest first (bitonic).
@@ -122,11 +146,12 @@ __device__ __forceinline__ void write_entry(T *values, int32_t *ids, int64_t at,
   ids[at] = id;
 }
 
-template <typename T, typename Entry, int R>
-__device__ __forceinline__ void sort_and_write(const Entry *cand, int C, int K, T *values, int32_t *ids, int64_t at, int lane) {
+// Entries entry(0), ... of a wavefront, 64 R at most (0 where there is none), sorted; the first K written.
+template <typename T, typename Entry, int R, typename F>
+__device__ __forceinline__ void sort_and_write(F entry, int K, T *values, int32_t *ids, int64_t at, int lane) {
   Entry e[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) e[r] = 64 * r + lane < C ? cand[64 * r + lane] : 0;
+  for (int r = 0; r < R; ++r) e[r] = entry(64 * r + lane);
   sort_entries<Entry, R>(e, lane);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -137,86 +162,126 @@ __device__ __forceinline__ void sort_and_write(const Entry *cand, int C, int K, 
 }
 
 template <typename Row, typename Entry>
-__global__ __launch_bounds__(group_threads(Row::GL)) void top_rows_kernel(const void *logits, int64_t ld_b, int64_t ld_t,
+__global__ __launch_bounds__(group_threads(Row::GL), Row::TOP_WAVES) void top_rows_kernel(const void *logits, int64_t ld_b, int64_t ld_t,
                                                                          int64_t N, uint32_t T_, int V, int K, ExpScale scale,
                                                                          double inv_tau, void *values_, int32_t *ids,
                                                                          float *lse) {
   typedef typename Row::type T;
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL, WAVES = GL / 64;
-  constexpr int CAP = 512;  // candidates
-  __shared__ Entry cand[GROUPS][CAP];
-  __shared__ int taken[GROUPS];
-  __shared__ float sh[2][WAVES];
+  // candidates of a wavefront
+  constexpr int OWN = WAVES == 1 ? 512 : WAVES <= 4 ? 256 : 128;
+  __shared__ Entry cand[GROUPS * WAVES][OWN];
+  __shared__ int found[GROUPS * WAVES], taken[GROUPS];
+  __shared__ float sh[WAVES], sums[WAVES];
   __shared__ int shc[WAVES];
-  __shared__ uint32_t shk[WAVES];
-  const int lane = lane_of<GL>(), group = group_of<GL>();
+  __shared__ uint32_t maxima[GL > 64 ? GL : 1], bound_sh;
+  const int lane = lane_of<GL>(), group = group_of<GL>(), l64 = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Entry *own = cand[wave];
   T *values = static_cast<T *>(values_);
+  int turn = 0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < N;
        row += static_cast<int64_t>(gridDim.x) * GROUPS) {
     const uint32_t b = static_cast<uint32_t>(row) / T_, t = static_cast<uint32_t>(row) % T_;
     const T *z = static_cast<const T *>(logits) + b * ld_b + t * ld_t;
     Row r;
     r.load(z, V, lane);
-    if (GL > 64 && lane == 0) taken[group] = 0;
     float mine = -INFINITY;
     r.values([&](float x) { mine = fmaxf(mine, x); });
-    const float top = group_max<GL>(mine, sh[0]);
     r.keep();
-    // the wavefront's bound
-    const int share = (K + WAVES - 1) / WAVES;
+    // A bound from the threads' maxima: by the wavefront itself or, in a workgroup, by one of its wavefronts in turn while the
+    // others are at their sums.
+    float top, s;
     uint32_t bound = 0;
-    if (share <= 64) {
-      const uint32_t key = key_of(mine);
-      constexpr int LOW = sizeof(T) == 2 ? 16 : 0;  // (a bf16's low bits say nothing)
-#pragma unroll
-      for (int bit = 31; bit >= LOW; --bit) {
-        const uint32_t trial = bound | (1u << bit);
-        if (__popcll(__ballot(key >= trial)) >= share) bound = trial;
-      }
-      if (LOW && bound && !(bound & 0x80000000u)) bound |= 0xffffu;  // (a negative bf16's key has ones there)
-    }
-    if constexpr (GL > 64) {
-      if ((threadIdx.x & 63) == 0) shk[threadIdx.x >> 6] = bound;
-    }
-    float s = 0.f;
-    r.values([&](float x) { s += exp_of(x, top, scale); });
-    s = group_add<GL>(s, sh[1]);
-    r.keep();
-    if constexpr (GL > 64) {
-      bound = shk[0];
-#pragma unroll
-      for (int w = 1; w < WAVES; ++w) bound = min(bound, shk[w]);
-    }
-    if (lane == 0) lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (top == -INFINITY ? 0.0 : log_of(s)));
-    // candidates
-    const float least = bound ? of_key(bound) : -INFINITY;
-    auto reaches = [&](float x) { return x >= least && x > -INFINITY; };
-    int C = 0;
     if constexpr (GL == 64) {
-      r.each(lane, [&](int i, float x) {
-        const uint64_t m = __ballot(reaches(x));
-        if (m) {
-          const int at = C + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(m >> 32),
-                                                       __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(m), 0));
-          if (reaches(x) && at < CAP) cand[group][at] = entry_of<Entry>(x, i);
-          C += __popcll(m);
-        }
-      });
+      top = group_max<GL>(mine, sh);
+      // from one maximum a lane for short lists, from several for longer ones (a bound from M maxima leaves some
+      // -M log(1 - K / M) candidates)
+      if (K <= 24) {
+        const uint32_t key[1] = {key_of(mine)};
+        bound = kth_key<1, sizeof(T) == 2>(key, K);
+      } else {
+        constexpr int M = Row::TOP_MAXIMA;
+        float m[M];
+        r.maxima(m);
+        r.keep();
+        uint32_t key[M];
+#pragma unroll
+        for (int i = 0; i < M; ++i) key[i] = key_of(m[i]);
+        bound = kth_key<M, sizeof(T) == 2>(key, K);
+      }
     } else {
-      int n = 0;
-      r.values([&](float x) { n += reaches(x) ? 1 : 0; });
-      r.keep();
-      int at = n ? atomicAdd(&taken[group], n) : 0;
-      if (n && at + n <= CAP)
-        r.each(lane, [&](int i, float x) {
-          if (reaches(x)) cand[group][at++] = entry_of<Entry>(x, i);
-        });
-      __syncthreads();
-      C = taken[group];
+      maxima[threadIdx.x] = key_of(mine);
+      top = group_max<GL>(mine, sh);  // (a barrier for the maxima too)
+      if (wave == turn) {
+        uint32_t key[WAVES];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) key[w] = maxima[64 * w + l64];
+        const uint32_t k = kth_key<WAVES, sizeof(T) == 2>(key, K);
+        if (l64 == 0) bound_sh = k;
+      }
+      turn = (turn + 1) % WAVES;
     }
-    if (C > CAP) {
-      // the k-th key, bit by bit over the row (more than CAP >= K logits are above -inf), then the ids of its equals. (Walked in
-      // memory: the registers of a form for this rare case would be every row's.)
+    s = 0.f;
+    r.values([&](float x) { s += exp_near(x, top, scale); });
+    r.keep();
+    s = group_add<GL>(s, sums);
+    if constexpr (GL > 64) bound = bound_sh;
+    if (lane == 0)
+      lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (isinf(top) ? 0.0 : log_of(s)));
+    // each wavefront's candidates, in its own part of the list
+    const float least = bound ? of_key(bound) : -FLT_MAX;
+    int n = 0;
+    r.each(lane, [&](int i, float x) {
+      const uint64_t m = __ballot(x >= least);
+      if (m) {
+        const int at = n + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(m >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(m), 0));
+        if (x >= least && at < OWN) own[at] = entry_of<Entry>(x, i);
+        n += __popcll(m);
+      }
+    });
+    int C = n;
+    bool fits = n <= OWN;
+    if constexpr (GL > 64) {
+      if (l64 == 0) found[wave] = n;
+      __syncthreads();
+      C = 0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const int f = found[w];
+        fits &= f <= OWN;
+        C += f;
+      }
+    }
+    const int64_t at = row * K;
+    if (fits && C <= 256) {
+      group_sync<64>();
+      if (lane < 64) {
+        // entry e of all wavefronts' parts together
+        auto entry = [&](int e) -> Entry {
+          if (WAVES == 1) return e < C ? own[e] : 0;
+          int w = 0;
+#pragma unroll
+          for (int k = 0; k < WAVES - 1; ++k) {
+            const int f = found[k];
+            if (w == k && e >= f) {
+              e -= f;
+              w = k + 1;
+            }
+          }
+          return e < found[w] ? cand[w][e] : 0;
+        };
+        if (C <= 64)
+          sort_and_write<T, Entry, 1>(entry, K, values, ids, at, lane);
+        else if (C <= 128)
+          sort_and_write<T, Entry, 2>(entry, K, values, ids, at, lane);
+        else
+          sort_and_write<T, Entry, 4>(entry, K, values, ids, at, lane);
+      }
+    } else {
+      // the k-th key, bit by bit over the row (more than 256 > K logits are above -inf), then the ids of its equals. (Walked
+      // in memory: the registers of a form for this rare case would be every row's.)
       RowWalk<T, GL> w;
       w.load(z, V, lane);
       uint32_t kth = 0;
@@ -240,30 +305,14 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void top_rows_kernel(const 
       }
       if (lane == 0) taken[group] = 0;
       group_sync<GL>();
+      Entry *first = cand[group * WAVES];  // (K <= 128 <= OWN)
       w.each(lane, [&](int i, float x) {
-        if (x > f || (x == f && static_cast<uint32_t>(i) <= last))
-          cand[group][atomicAdd(&taken[group], 1)] = entry_of<Entry>(x, i);
+        if (x > f || (x == f && static_cast<uint32_t>(i) <= last)) first[atomicAdd(&taken[group], 1)] = entry_of<Entry>(x, i);
       });
-      C = K;
-    }
-    group_sync<GL>();
-    const int64_t at = row * K;
-    if (C <= 256) {
+      group_sync<GL>();
       if (lane < 64) {
-        if (C <= 64)
-          sort_and_write<T, Entry, 1>(cand[group], C, K, values, ids, at, lane);
-        else if (C <= 128)
-          sort_and_write<T, Entry, 2>(cand[group], C, K, values, ids, at, lane);
-        else
-          sort_and_write<T, Entry, 4>(cand[group], C, K, values, ids, at, lane);
-      }
-    } else {
-      // each candidate's place: how many are before it (C > 256 > K: no places are left over)
-      for (int i = lane; i < C; i += GL) {
-        const Entry me = cand[group][i];
-        int place = 0;
-        for (int j = 0; j < C; ++j) place += cand[group][j] > me ? 1 : 0;
-        if (place < K) write_entry(values, ids, at + place, value_of(me), id_of(me));
+        auto entry = [&](int e) -> Entry { return e < K ? first[e] : 0; };
+        sort_and_write<T, Entry, 2>(entry, K, values, ids, at, lane);
       }
     }
     group_sync<GL>();
@@ -283,7 +332,7 @@ __global__ __launch_bounds__(256) void top_lanes_kernel(const void *logits, int6
   float top = -INFINITY, s = 0.f;
   r.values([&](float x) { top = fmaxf(top, x); });
   r.values([&](float x) { s += exp_of(x, top, scale); });
-  lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (top == -INFINITY ? 0.0 : log_of(s)));
+  lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (isinf(top) ? 0.0 : log_of(s)));
   uint32_t key[NE];
   int entries = 0;
 #pragma unroll
@@ -299,6 +348,24 @@ __global__ __launch_bounds__(256) void top_lanes_kernel(const void *logits, int6
     if (key[i] && place < K) write_entry(static_cast<T *>(values), ids, row * K + place, of_key(key[i]), i);
   }
   for (int place = entries; place < K; ++place) write_entry(static_cast<T *>(values), ids, row * K + place, -INFINITY, -1);
+}
+
+// row_form for rows of more than 512 logits, with 512 threads where 1024 would do: two workgroups a CU, of which one loads
+// while the other sorts (2064 x 87383 bf16, lists of 64: 105 us; 1024 threads 199).
+template <typename F>
+int top_form(int64_t vectors, F f) {
+#define VK_FORM(GL, NV) \
+  if (vectors <= GL * NV) return f(std::integral_constant<int, GL>{}, std::integral_constant<int, NV>{})
+  VK_FORM(64, 3);
+  VK_FORM(64, 6);
+  VK_FORM(64, 11);
+  VK_FORM(256, 6);
+  VK_FORM(256, 11);
+  VK_FORM(512, 11);
+  VK_FORM(512, 22);
+  VK_FORM(1024, 22);
+#undef VK_FORM
+  return f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 0>{});
 }
 
 }  // namespace vk
@@ -331,10 +398,9 @@ extern "C" int vk_top_logits(const void *logits, int32_t dtype, int64_t ld_b, in
     if (V <= 16) return run(top_lanes_kernel<E, 16>, 256, 256, true);
     if (V <= 256) return run(top_rows_kernel<RowStrided<E, 4>, Short>, 256, 4, false);
     if (V <= 512) return run(top_rows_kernel<RowStrided<E, 8>, Short>, 256, 4, false);
-    return row_form((V + kVec<E> - 1) / kVec<E>, [&](auto gl, auto nv) {
-      constexpr int G = decltype(gl)::value < 64 ? 64 : decltype(gl)::value;
-      constexpr int NV = decltype(gl)::value < 64 ? 3 : decltype(nv)::value;
-      typedef typename RowForm<E, G, NV>::type Row;
+    return top_form((V + kVec<E> - 1) / kVec<E>, [&](auto gl, auto nv) {
+      constexpr int G = decltype(gl)::value;
+      typedef typename RowForm<E, G, decltype(nv)::value>::type Row;
       if (V <= 65536) return run(top_rows_kernel<Row, Short>, group_threads(G), group_threads(G) / G, false);
       return run(top_rows_kernel<Row, uint64_t>, group_threads(G), group_threads(G) / G, false);
     });

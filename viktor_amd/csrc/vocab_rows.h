@@ -4,6 +4,7 @@
 // (objectives.hip, top_logits.hip).
 #pragma once
 
+#include <float.h>
 #include <math.h>
 
 #include <type_traits>
@@ -53,6 +54,17 @@ __device__ __forceinline__ int owner_of(const Span &s, int i) {
   return j < s.nv ? j % GL : i - s.nv * kVec<T>;
 }
 
+// Vector c GL + lane behind p, as a row's first part that is the same for a wavefront (a scalar register there), and the
+// lane's 32-bit offset: no 64-bit address a vector in the vector registers.
+template <int GL, typename T>
+__device__ __forceinline__ const T *vector_at(const T *p, int c, int lane) {
+  return reinterpret_cast<const T *>(reinterpret_cast<const char *>(p) + c * GL * 16 + static_cast<uint32_t>(lane) * 16u);
+}
+template <int GL, typename T>
+__device__ __forceinline__ T *vector_at(T *p, int c, int lane) {
+  return reinterpret_cast<T *>(reinterpret_cast<char *>(p) + c * GL * 16 + static_cast<uint32_t>(lane) * 16u);
+}
+
 // ---- reductions over a group ------------------------------------------------------------------------------------------
 // GL <= 64: lanes of one wavefront. GL > 64: the whole workgroup, through sh [GL / 64]; two calls with the same sh need
 // a barrier between them (another reduction's, for instance).
@@ -94,30 +106,68 @@ __device__ __forceinline__ void group_sync() {
   }
 }
 
+// exp((z - top) / temperature) as a power of two: log2 e / temperature in two parts. (Rounded to one, its error has the same
+// sign for every term: 1e-8 of |z - top|, which a sum over a sequence's tokens keeps. Both parts are positive: -inf stays
+// -inf in their sum.)
+struct ExpScale {
+  float hi, lo;
+  static ExpScale of(double temperature) {
+    const double s = 1.4426950408889634 / temperature;
+    float h = static_cast<float>(s);
+    if (static_cast<double>(h) >= s) h = nextafterf(h, 0.f);
+    return {h, static_cast<float>(s - static_cast<double>(h))};
+  }
+};
+__device__ __forceinline__ float exp_of(float z, float top, ExpScale s) {
+  const float t = z - top;
+  return __builtin_amdgcn_exp2f(fmaf(t, s.lo, t * s.hi));
+}
+
 // ---- rows ---------------------------------------------------------------------------------------------------------------
 // In registers: NV vectors a thread, up to GL * NV vectors. Places behind the row's end hold -inf.
 template <typename T, int GL_, int NV>
 struct RowRegs {
   typedef T type;
+  static constexpr bool WALKS = false;
   static constexpr int GL = GL_;
+  // Exponentials stay in registers from the sum to the gradient: in the logits' place (fp32), or beside them up to 6 vectors
+  // of bf16. Beyond that they are computed again.
+  static constexpr bool KEEPS = sizeof(T) == 4 || NV <= 6;
+  // Wavefronts a SIMD that the objectives' kernels are compiled for: rows of up to 3 vectors a thread gain more from 8 of them
+  // than the ten registers that go to memory around the 64-bit numbers cost (16416 x 5463 bf16: 86 -> 79 us).
+  static constexpr int WAVES_A_SIMD = GL_ >= 64 && NV <= 3 ? 8 : GL_ == 1024 ? 4 : 1;
+  // ... that top_logits is, and the maxima a lane of a wavefront's row that its bound comes from
+  static constexpr int TOP_WAVES = GL_ > 64 ? 4 : NV <= 3 ? 8 : NV <= 6 ? 6 : NV <= 11 ? 4 : 3, TOP_MAXIMA = NV <= 6 ? NV : 4;
   Span s;
   u32x4 v[NV];
-  float edge;
+  float edge, e[sizeof(T) == 2 && KEEPS ? NV * 8 : 1];
 
   __device__ __forceinline__ void load(const T *p, int V, int lane) {
     s = span_of(p, V);
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       const int j = c * GL + lane;
-      v[c] = j < s.nv ? stream_16(p + s.head + j * kVec<T>) : nothing(p);
+      v[c] = j < s.nv ? stream_16(vector_at<GL>(p + s.head, c, lane)) : nothing(p);
     }
-    edge = lane < s.edges ? load_one(p + edge_index<T>(s, lane)) : -INFINITY;
+    // (an element of the row for every lane: a load under a branch would be waited for there)
+    const float x = load_one(p + (lane < s.edges ? edge_index<T>(s, lane) : 0));
+    edge = lane < s.edges ? x : -INFINITY;
   }
   // Between two walks: the vectors stay as they are. (The compiler keeps every element of the first walk unpacked for the
   // next ones otherwise, twice the registers.)
   __device__ __forceinline__ void keep() {
 #pragma unroll
     for (int c = 0; c < NV; ++c) asm("" : "+v"(v[c]));
+  }
+  // The largest of every M-th of the thread's vectors.
+  template <int M>
+  __device__ __forceinline__ void maxima(float (&m)[M]) const {
+#pragma unroll
+    for (int i = 0; i < M; ++i) m[i] = i ? -INFINITY : edge;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int k = 0; k < kVec<T>; ++k) m[c % M] = fmaxf(m[c % M], vec_at(v[c], k, static_cast<const T *>(nullptr)));
   }
   // f(value) for each element, with -inf for places behind the end
   template <typename F>
@@ -138,20 +188,66 @@ struct RowRegs {
         f(s.head + (c * GL + lane) * kVec<T> + k, vec_at(v[c], k, static_cast<const T *>(nullptr)));
     f(edge_index<T>(s, lane), edge);
   }
-  // d[i] = f(value i), in the row's type
-  template <typename F>
-  __device__ __forceinline__ void write(T *d, int lane, F f) const {
+  // Zeros for a row that counts nothing.
+  static __device__ __forceinline__ void zero(T *d, int V, int lane) {
+    const Span s = span_of(d, V);
+    const float o[kVec<T>] = {};
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+      if (c * GL + lane < s.nv) store_row(vector_at<GL>(d + s.head, c, lane), o);
+    if (lane < s.edges) store_one(d + edge_index<T>(s, lane), 0.f);
+  }
+  // The thread's sum of exp((z - top) / temperature).
+  __device__ __forceinline__ float exps(float top, ExpScale scale) {
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int k = 0; k < kVec<T>; ++k) {
+        const float x = exp_of(vec_at(v[c], k, static_cast<const T *>(nullptr)), top, scale);
+        sum += x;
+        if constexpr (sizeof(T) == 4)
+          v[c][k] = __float_as_uint(x);
+        else if constexpr (KEEPS)
+          e[c * 8 + k] = x;
+      }
+    const float x = exp_of(edge, top, scale);
+    if constexpr (KEEPS) edge = x;
+    return sum + x;
+  }
+  // d[i] = factor exp((z_i - top) / temperature), in the row's type, after exps.
+  __device__ __forceinline__ void write(T *d, int lane, float top, ExpScale scale, float factor) const {
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       const int j = c * GL + lane;
       if (j < s.nv) {
         float o[kVec<T>];
 #pragma unroll
-        for (int k = 0; k < kVec<T>; ++k) o[k] = f(vec_at(v[c], k, static_cast<const T *>(nullptr)));
-        store_row(d + s.head + j * kVec<T>, o);
+        for (int k = 0; k < kVec<T>; ++k) {
+          const float x = vec_at(v[c], k, static_cast<const T *>(nullptr));
+          if constexpr (sizeof(T) == 2 && KEEPS)
+            o[k] = e[c * 8 + k] * factor;
+          else
+            o[k] = (KEEPS ? x : exp_of(x, top, scale)) * factor;
+        }
+        store_row(vector_at<GL>(d + s.head, c, lane), o);
       }
     }
-    if (lane < s.edges) store_one(d + edge_index<T>(s, lane), f(edge));
+    if (lane < s.edges) store_one(d + edge_index<T>(s, lane), (KEEPS ? edge : exp_of(edge, top, scale)) * factor);
+  }
+  // ... where another pass had the row's maximum and sum: without exps before.
+  __device__ __forceinline__ void write_fresh(T *d, int lane, float top, ExpScale scale, float factor) const {
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      const int j = c * GL + lane;
+      if (j < s.nv) {
+        float o[kVec<T>];
+#pragma unroll
+        for (int k = 0; k < kVec<T>; ++k) o[k] = exp_of(vec_at(v[c], k, static_cast<const T *>(nullptr)), top, scale) * factor;
+        store_row(vector_at<GL>(d + s.head, c, lane), o);
+      }
+    }
+    if (lane < s.edges) store_one(d + edge_index<T>(s, lane), exp_of(edge, top, scale) * factor);
   }
 };
 
@@ -160,6 +256,8 @@ struct RowRegs {
 template <typename T, int NE>
 struct RowLane {
   typedef T type;
+  static constexpr int WAVES_A_SIMD = 1;
+  static constexpr bool WALKS = false;
   static constexpr int GL = 1;
   Span s;
   float z[NE];
@@ -176,11 +274,22 @@ struct RowLane {
 #pragma unroll
     for (int k = 0; k < NE; ++k) f(z[k]);
   }
-  template <typename F>
-  __device__ __forceinline__ void write(T *d, int lane, F f) const {
+  static __device__ __forceinline__ void zero(T *d, int V, int lane) {
+    for (int k = 0; k < V; ++k) store_one(d + k, 0.f);
+  }
+  __device__ __forceinline__ float exps(float top, ExpScale scale) const {
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < NE; ++k) sum += exp_of(z[k], top, scale);
+    return sum;
+  }
+  __device__ __forceinline__ void write(T *d, int lane, float top, ExpScale scale, float factor) const {
 #pragma unroll
     for (int k = 0; k < NE; ++k)
-      if (k < n) store_one(d + k, f(z[k]));
+      if (k < n) store_one(d + k, exp_of(z[k], top, scale) * factor);
+  }
+  __device__ __forceinline__ void write_fresh(T *d, int lane, float top, ExpScale scale, float factor) const {
+    write(d, lane, top, scale, factor);
   }
 };
 
@@ -188,7 +297,9 @@ struct RowLane {
 template <typename T, int GL_>
 struct RowWalk {
   typedef T type;
-  static constexpr int GL = GL_;
+  static constexpr int WAVES_A_SIMD = 1;
+  static constexpr bool WALKS = true;
+  static constexpr int GL = GL_, TOP_WAVES = 1, TOP_MAXIMA = 1;
   Span s;
   const T *p;
   float edge;
@@ -201,10 +312,12 @@ struct RowWalk {
     edge = lane < s.edges ? load_one(p + edge_index<T>(s, lane)) : -INFINITY;
   }
   __device__ __forceinline__ void keep() {}
+  // (every thread makes every step, with -inf behind the end: f may vote)
   template <typename F>
   __device__ __forceinline__ void values(F f) const {
-    for (int j = lane; j < s.nv; j += GL) {
-      const u32x4 r = stream_16(p + s.head + static_cast<int64_t>(j) * kVec<T>);
+    for (int j0 = 0; j0 < s.nv; j0 += GL) {
+      const int j = j0 + lane;
+      const u32x4 r = j < s.nv ? stream_16(p + s.head + static_cast<int64_t>(j) * kVec<T>) : nothing(p);
 #pragma unroll
       for (int k = 0; k < kVec<T>; ++k) f(vec_at(r, k, p));
     }
@@ -212,50 +325,94 @@ struct RowWalk {
   }
   template <typename F>
   __device__ __forceinline__ void each(int l, F f) const {
-    for (int j = lane; j < s.nv; j += GL) {
-      const u32x4 r = stream_16(p + s.head + static_cast<int64_t>(j) * kVec<T>);
+    for (int j0 = 0; j0 < s.nv; j0 += GL) {
+      const int j = j0 + lane;
+      const u32x4 r = j < s.nv ? stream_16(p + s.head + static_cast<int64_t>(j) * kVec<T>) : nothing(p);
 #pragma unroll
       for (int k = 0; k < kVec<T>; ++k) f(s.head + j * kVec<T> + k, vec_at(r, k, p));
     }
     f(edge_index<T>(s, lane), edge);
   }
-  template <typename F>
-  __device__ __forceinline__ void write(T *d, int l, F f) const {
-    for (int j = lane; j < s.nv; j += GL) {
-      const u32x4 r = stream_16(p + s.head + static_cast<int64_t>(j) * kVec<T>);
-      float o[kVec<T>];
+  static __device__ __forceinline__ void zero(T *d, int V, int lane) {
+    const Span s = span_of(d, V);
+    const float o[kVec<T>] = {};
+    for (int j = lane; j < s.nv; j += GL) store_row(d + s.head + static_cast<int64_t>(j) * kVec<T>, o);
+    if (lane < s.edges) store_one(d + edge_index<T>(s, lane), 0.f);
+  }
+  // Steps of a walk that are loaded together.
+  static constexpr int U = 4;
+  // d[i] = factor exp((z_i - top) / temperature)
+  __device__ __forceinline__ void write_fresh(T *d, int l, float top, ExpScale scale, float factor) const {
+    for (int j0 = 0; j0 < s.nv; j0 += GL * U) {
+      u32x4 r[U];
 #pragma unroll
-      for (int k = 0; k < kVec<T>; ++k) o[k] = f(vec_at(r, k, p));
-      store_row(d + s.head + static_cast<int64_t>(j) * kVec<T>, o);
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * GL + lane;
+        r[u] = j < s.nv ? stream_16(p + s.head + static_cast<int64_t>(j) * kVec<T>) : nothing(p);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * GL + lane;
+        float o[kVec<T>];
+#pragma unroll
+        for (int k = 0; k < kVec<T>; ++k) o[k] = exp_of(vec_at(r[u], k, p), top, scale) * factor;
+        if (j < s.nv) store_row(d + s.head + static_cast<int64_t>(j) * kVec<T>, o);
+      }
     }
-    if (lane < s.edges) store_one(d + edge_index<T>(s, lane), f(edge));
+    if (lane < s.edges) store_one(d + edge_index<T>(s, lane), exp_of(edge, top, scale) * factor);
+  }
+  __device__ __forceinline__ void write(T *d, int l, float top, ExpScale scale, float factor) const {
+    write_fresh(d, l, top, scale, factor);
   }
 };
 
-// exp((z - top) / temperature) as a power of two: log2 e / temperature in two parts. (Rounded to one, its error has the same
-// sign for every term: 1e-8 of |z - top|, which a sum over a sequence's tokens keeps. Both parts are positive: -inf stays
-// -inf in their sum.)
-struct ExpScale {
-  float hi, lo;
-  static ExpScale of(double temperature) {
-    const double s = 1.4426950408889634 / temperature;
-    float h = static_cast<float>(s);
-    if (static_cast<double>(h) >= s) h = nextafterf(h, 0.f);
-    return {h, static_cast<float>(s - static_cast<double>(h))};
+// A walked row in one pass: each thread has its own maximum so far, and its sum by that.
+template <int GL, typename T>
+__device__ __forceinline__ void walk_stats(RowWalk<T, GL> &r, ExpScale scale, float (*sh)[GL > 64 ? GL / 64 : 1], float &top,
+                                          float &s) {
+  constexpr int U = RowWalk<T, GL>::U;
+  float m = fmaxf(r.edge, -FLT_MAX);  // (finite: -inf - m stays -inf)
+  float sum = exp_of(r.edge, m, scale);
+  for (int j0 = 0; j0 < r.s.nv; j0 += GL * U) {
+    u32x4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * GL + r.lane;
+      v[u] = j < r.s.nv ? stream_16(r.p + r.s.head + static_cast<int64_t>(j) * kVec<T>) : nothing(r.p);
+    }
+    float n = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < kVec<T>; ++k) n = fmaxf(n, vec_at(v[u], k, r.p));
+    sum *= exp_of(m, n, scale);
+    m = n;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < kVec<T>; ++k) sum += exp_of(vec_at(v[u], k, r.p), m, scale);
   }
-};
-__device__ __forceinline__ float exp_of(float z, float top, ExpScale s) {
-  const float t = z - top;
-  return __builtin_amdgcn_exp2f(fmaf(t, s.lo, t * s.hi));
+  top = group_max<GL>(m, sh[0]);
+  s = group_add<GL>(sum * exp_of(m, top, scale), sh[1]);
 }
 
-// Zeros where a row counts nothing.
-template <typename T, int GL>
-__device__ __forceinline__ void zero_row(T *d, int V, int lane) {
-  const Span s = span_of(d, V);
-  const float o[kVec<T>] = {};
-  for (int j = lane; j < s.nv; j += GL) store_row(d + s.head + static_cast<int64_t>(j) * kVec<T>, o);
-  for (int l = lane; l < s.edges; l += GL) store_one(d + edge_index<T>(s, l), 0.f);
+// A row's maximum and its sum of exp((z - maximum) / temperature), in every thread of the group. sh: two numbers a wavefront.
+template <int GL, typename Row>
+__device__ __forceinline__ void row_stats(Row &r, ExpScale scale, float (*sh)[GL > 64 ? GL / 64 : 1], float &top, float &s) {
+  if constexpr (Row::WALKS) {
+    walk_stats<GL>(r, scale, sh, top, s);
+    return;
+  }
+  top = -INFINITY;
+  r.values([&](float x) { top = fmaxf(top, x); });
+  top = group_max<GL>(top, sh[0]);
+  r.keep();
+  if constexpr (!Row::WALKS) s = group_add<GL>(r.exps(top, scale), sh[1]);
+  r.keep();
+}
+// The same for a log-sum-exp alone: off by 2^-24 |z - top| of a term more, all to one side, which is no more of the result.
+__device__ __forceinline__ float exp_near(float z, float top, ExpScale s) {
+  return __builtin_amdgcn_exp2f((z - top) * s.hi);
 }
 
 // log s of a sum of exponentials, off by some 3e-8 whatever its size: the exponent's part in 64 bits, the mantissa's
@@ -270,28 +427,28 @@ __device__ __forceinline__ double log_of(float s) {
   return static_cast<double>(ex) * 0.6931471805599453 + static_cast<double>(log1pf(m - 1.f));
 }
 
-// exp(x) - 1, off by a few 1e-16 of it (and of x near 0): a series on x halved until it is under 1/2, then
-// expm1(2 y) = expm1(y) (expm1(y) + 2). A dozen registers, where the library's takes thirty from the row.
-__device__ __forceinline__ double series_beyond_line(double x) {  // exp(x) - 1 - x for |x| < 1/2
+// exp(x) - 1 - x for |x| < 1/2, off by 1e-10 of it: nine terms.
+__device__ __forceinline__ double series_beyond_line(double x) {
   double t = 1.0;
 #pragma unroll
-  for (int n = 14; n >= 3; --n) t = fma(t * x, 1.0 / n, 1.0);
+  for (int n = 11; n >= 3; --n) t = fma(t * x, 1.0 / n, 1.0);
   return 0.5 * x * x * t;
 }
-__device__ __forceinline__ double expm1_of(double x) {
+// exp(x) - 1 - x beyond: x halved until it is under 1/2, then expm1(2 y) = expm1(y) (expm1(y) + 2). A call: few tokens need
+// it, and its registers would be taken from every row.
+__device__ __attribute__((noinline)) double exp_far_beyond_line(double x) {
   int m;
   frexp(x, &m);
-  if (!(fabs(x) >= 0.5) || fabs(x) > 800.0) m = -1;
-  const double y = ldexp(fabs(x) > 800.0 ? 0.0 : x, -(m + 1));
+  const bool huge = !(fabs(x) <= 800.0);
+  if (huge) return x > 0.0 ? INFINITY : x < 0.0 ? -1.0 - x : x;
+  const double y = ldexp(x, -(m + 1));
   double e = y + series_beyond_line(y);
   for (; m >= 0; --m) e *= e + 2.0;
-  if (x > 800.0) e = INFINITY;
-  if (x < -800.0) e = -1.0;
-  return e;
+  return e - x;
 }
 // exp(x) - 1 - x without cancellation
 __device__ __forceinline__ double exp_beyond_line(double x) {
-  return fabs(x) < 0.5 ? series_beyond_line(x) : expm1_of(x) - x;
+  return fabs(x) < 0.5 ? series_beyond_line(x) : exp_far_beyond_line(x);
 }
 
 // Threads of a workgroup that holds groups of GL; a thread's group, known to be the same for a wavefront where it is (row
@@ -319,8 +476,8 @@ inline int row_form(int64_t vectors, F f) {
   VK_FORM(16, 6);
   VK_FORM(64, 3);
   VK_FORM(64, 6);
-  VK_FORM(256, 3);
-  VK_FORM(256, 6);
+  VK_FORM(64, 11);
+  VK_FORM(64, 22);
   VK_FORM(256, 11);
   VK_FORM(512, 11);
   VK_FORM(1024, 11);

@@ -1177,12 +1177,14 @@ def choose_update(logits, bias, is_tail, is_homo, homo_stop, tok, run, pos, plen
 
 # ---- objectives on logits and their gradients --------------------------------------------------------------------------
 _PER_SEQUENCE, _PER_TOKEN, _PER_TOKEN_MEAN = 0, 1, 2
+_F32 = torch.float32
 
 
 def _logit_rows(what, logits):
     """B, T, V and the C entry points' first arguments of logits [B, T, V]: rows of contiguous logits, apart from each
     other, at any strides."""
-    if logits.dim() != 3 or logits.dtype not in (BF16, torch.float32):
+    dt = logits.dtype
+    if logits.dim() != 3 or not (dt is BF16 or dt is _F32):
         _refuse(what, "logits [B, T, V] bf16 or fp32")
     B, T, V = logits.shape
     if not 0 < V <= _WIDEST or B * T >= 1 << 31:
@@ -1190,23 +1192,23 @@ def _logit_rows(what, logits):
     sb, st, sv = logits.stride()
     if (V > 1 and sv != 1) or (T > 1 and st < V) or (B > 1 and sb < V):
         _refuse(what, "logits whose rows are contiguous and do not overlap")
-    return B, T, V, (logits.data_ptr(), _vk_dtype(logits.dtype), sb if B > 1 else 0, st if T > 1 else 0)
+    return B, T, V, (logits.data_ptr(), _vk_dtype(dt), sb if B > 1 else 0, st if T > 1 else 0)
 
 
 def _tokens_and_mask(what, targets, mask, shape):
-    if targets.dtype != torch.long or targets.shape != shape:
+    if targets.dtype is not torch.long or targets.shape != shape:
         _refuse(what, "targets int64 [B, T]")
-    if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != shape:
+    if not (mask.dtype is torch.bool or mask.dtype is torch.uint8) or mask.shape != shape:
         _refuse(what, "mask bool [B, T]")
     return targets.contiguous(), mask.contiguous()
 
 
-def _floats(what, name, t, *shapes):
-    """fp32 of one of the shapes, contiguous; None stays None."""
+def _floats(what, name, t, shape):
+    """fp32 of that shape, contiguous; None stays None."""
     if t is None:
         return None
-    if not isinstance(t, _Tensor) or t.dtype is not torch.float32 or t.shape not in shapes:
-        _refuse(what, f"{name} fp32 {' or '.join(str(list(s)) for s in shapes)}")
+    if not isinstance(t, _Tensor) or t.dtype is not _F32 or t.shape != shape:
+        _refuse(what, f"{name} fp32 {list(shape)}")
     return t.contiguous()
 
 
@@ -1214,7 +1216,7 @@ def _gradient_buffer(what, logits, out, grad):
     """The buffer of dlogits: a new one, the caller's, or None."""
     if out is None:
         return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
-    if not grad or out.dtype != logits.dtype or out.shape != logits.shape or not out.is_contiguous():
+    if not grad or out.dtype is not logits.dtype or out.shape != logits.shape or not out.is_contiguous():
         _refuse(what, "out contiguous [B, T, V] of the logits' type, with grad")
     if logits.numel():
         lo, size = logits.data_ptr(), logits.element_size()
@@ -1224,12 +1226,8 @@ def _gradient_buffer(what, logits, out, grad):
     return out
 
 
-def _upstream_ptr(what, upstream, unless_one, dl):
-    if upstream is None:
-        if unless_one:
-            _refuse(what, "unless_one needs the upstream gradient")
-        return None
-    if upstream.dtype is not torch.float32 or upstream.numel() != 1 or dl is None:
+def _upstream(what, upstream, grad):
+    if upstream.dtype is not _F32 or upstream.numel() != 1 or not grad:
         _refuse(what, "upstream: one fp32 number on the device, with grad")
     return upstream.data_ptr()
 
@@ -1241,8 +1239,28 @@ def _objective_workspace(B, T, P):
     return nb.value
 
 
+class _Launch:
+    """A call of an objective's entry point: its arguments, and the places among them of what a second pass over the same
+    inputs replaces (the gradient's buffer, its factor, the outputs, which that pass leaves alone)."""
+    __slots__ = ("name", "args", "outputs", "at", "keep")
+
+    def __init__(self, name, args, outputs, at, keep):
+        self.name, self.args, self.outputs, self.at, self.keep = name, args, outputs, at, keep
+
+    def again(self, dl, upstream, unless_one):
+        """dlogits times the fp32 number `upstream` into dl; unless_one: dl holds it for a factor of 1, in which case nothing
+        is done. On the current device's current stream."""
+        args, at = list(self.args), self.at
+        for i in self.outputs:
+            args[i] = None
+        args[at], args[at + 1], args[at + 2] = dl.data_ptr(), upstream.data_ptr(), unless_one
+        if self.name == "vk_preference_score":
+            args[at + 3] = 2  # (from the workspace's coefficients)
+        call(self.name, *args, stream_handle())
+
+
 def policy_score(logits, targets, mask, old_lp, adv, ref_lp=None, eps_lo=0.2, eps_hi=0.2, kl_coef=0.0, per="sequence",
-                 inv_n=None, grad=True, out=None, upstream=None, unless_one=False):
+                 inv_n=None, grad=True, out=None, upstream=None):
     """Clipped policy loss per token with a KL term to a reference policy, and its gradient in the same pass. For each token
     with mask[b, t] and a target in [0, V): lp = log softmax(logits)[target], r = exp(lp - old_lp),
       pg = -min(r A, clip(r, 1 - eps_lo, 1 + eps_hi) A), kl = exp(ref_lp - lp) - (ref_lp - lp) - 1,
@@ -1251,16 +1269,22 @@ def policy_score(logits, targets, mask, old_lp, adv, ref_lp=None, eps_lo=0.2, ep
     tokens by default). Other tokens have zeros, whatever their inputs hold. logits [B, T, V] bf16 or fp32 with rows of unit
     stride; targets int64, mask bool, old_lp, ref_lp fp32 [B, T]; adv fp32 [B] or [B, T].
     Returns dict(loss [], pg, kl (None without ref_lp), lp [B, T] fp32, dlogits [B, T, V] of the logits' type when grad).
-    out: the caller's buffer of dlogits; upstream: one fp32 number on the device that dlogits is multiplied by; unless_one:
-    only dlogits is written, and only where upstream is not 1. Beside gspo_score, whose ratio is per sequence."""
+    out: the caller's buffer of dlogits, apart from the logits; upstream: one fp32 number on the device that dlogits is
+    multiplied by. Beside gspo_score, whose ratio is per sequence."""
+    return _policy(logits, targets, mask, old_lp, adv, ref_lp, eps_lo, eps_hi, kl_coef, per, inv_n, grad, out, upstream)[0]
+
+
+def _policy(logits, targets, mask, old_lp, adv, ref_lp, eps_lo, eps_hi, kl_coef, per, inv_n, grad=True, out=None, upstream=None):
     what = "policy_score"
     _here(what, (logits, targets, mask, old_lp, adv, ref_lp, out, upstream))
     B, T, V, rows = _logit_rows(what, logits)
-    targets, mask = _tokens_and_mask(what, targets, mask, (B, T))
+    shape = (B, T)
+    targets, mask = _tokens_and_mask(what, targets, mask, shape)
     if old_lp is None or adv is None:
         _refuse(what, "old_lp and adv")
-    old_lp, ref_lp = _floats(what, "old_lp", old_lp, (B, T)), _floats(what, "ref_lp", ref_lp, (B, T))
-    adv = _floats(what, "adv", adv, (B,), (B, T))
+    old_lp, ref_lp = _floats(what, "old_lp", old_lp, shape), _floats(what, "ref_lp", ref_lp, shape)
+    adv_2 = int(adv.dim() == 2)
+    adv = _floats(what, "adv", adv, shape if adv_2 else (B,))
     if ref_lp is None and kl_coef != 0:
         _refuse(what, "the KL term needs ref_lp")
     if not (eps_lo >= 0 and eps_hi >= 0):
@@ -1273,36 +1297,41 @@ def policy_score(logits, targets, mask, old_lp, adv, ref_lp=None, eps_lo=0.2, ep
         _refuse(what, "per is 'sequence' or 'token'")
     dev = logits.device
     dl = _gradient_buffer(what, logits, out, grad)
-    up = _upstream_ptr(what, upstream, unless_one, dl)
-    loss = pg = kl = lp = None
-    if not unless_one:
-        pg, lp = torch.empty(B, T, dtype=torch.float32, device=dev), torch.empty(B, T, dtype=torch.float32, device=dev)
-        kl = torch.empty(B, T, dtype=torch.float32, device=dev) if ref_lp is not None else None
-        loss = torch.empty((), dtype=torch.float32, device=dev)
+    up = None if upstream is None else _upstream(what, upstream, grad)
+    if ref_lp is None:
+        pg, lp = torch.empty(2, B, T, dtype=_F32, device=dev).unbind(0)
+        kl = None
+    else:
+        pg, lp, kl = torch.empty(3, B, T, dtype=_F32, device=dev).unbind(0)
+    loss = torch.empty((), dtype=_F32, device=dev)
     nb = _objective_workspace(B, T, 0)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    call("vk_policy_score", *rows, targets.data_ptr(), mask.data_ptr(), old_lp.data_ptr(), adv.data_ptr(),
-         int(adv.dim() == 2), ptr(ref_lp), float(eps_lo), float(eps_hi), float(kl_coef), mode, inv, ptr(loss), ptr(pg), ptr(kl),
-         ptr(lp), ptr(dl), up, int(bool(unless_one)), B, T, V, ws.data_ptr(), nb, stream_handle())
+    args = (*rows, targets.data_ptr(), mask.data_ptr(), old_lp.data_ptr(), adv.data_ptr(), adv_2, ptr(ref_lp), eps_lo, eps_hi,
+            kl_coef, mode, inv, loss.data_ptr(), pg.data_ptr(), ptr(kl), lp.data_ptr(), ptr(dl), up, 0, B, T, V, ws.data_ptr(), nb)
+    call("vk_policy_score", *args, stream_handle())
     res = {"loss": loss, "pg": pg, "kl": kl, "lp": lp}
-    if dl is not None:
+    if grad:
         res["dlogits"] = dl
-    return res
+    return res, _Launch("vk_policy_score", args, (15, 16, 17, 18), 19, (targets, mask, old_lp, adv, ref_lp, ws))
 
 
 def preference_score(logits, targets, mask, ref_lp=None, pairs=None, beta=0.1, target=0.0, smoothing=0.0, lengths=None,
-                     inv_n=None, grad=True, out=None, upstream=None, unless_one=False, workspace=None):
+                     inv_n=None, grad=True, out=None, upstream=None):
     """Loss of paired log ratios, and its gradient. S_b = the sum of lp - ref_lp over sequence b's tokens (mask set, target
     in [0, V); ref_lp fp32 [B, T], None: 0), over lengths[b] where given (fp32 [B], positive); for pair p of a preferred and
     a lesser sequence (pairs int64 [P, 2]; None: sequences 2 p and 2 p + 1)
       margin_p = beta (S_preferred - S_lesser) - target
       loss = inv_n sum_p -(1 - smoothing) log sigma(margin_p) - smoothing log sigma(-margin_p)     (inv_n 1 / P by default)
     A sequence may be in any number of pairs, or none; a pair with an index outside [0, B) counts nothing (margin 0).
-    Returns dict(loss [], margin [P], lp [B, T] fp32 with zeros where a token does not count, workspace, dlogits [B, T, V] of
-    the logits' type when grad). logits, targets, mask, out, upstream, unless_one as in policy_score; workspace: of an
-    earlier call with the same arguments, whose loss and coefficients are then taken (dlogits alone is computed)."""
+    Returns dict(loss [], margin [P], lp [B, T] fp32 with zeros where a token does not count, dlogits [B, T, V] of the
+    logits' type when grad). logits, targets, mask, out, upstream as in policy_score."""
+    return _preference(logits, targets, mask, ref_lp, pairs, beta, target, smoothing, lengths, inv_n, grad, out, upstream)[0]
+
+
+def _preference(logits, targets, mask, ref_lp, pairs, beta, target, smoothing, lengths, inv_n, grad=True, out=None,
+                upstream=None):
     what = "preference_score"
-    _here(what, (logits, targets, mask, ref_lp, pairs, lengths, out, upstream, workspace))
+    _here(what, (logits, targets, mask, ref_lp, pairs, lengths, out, upstream))
     B, T, V, rows = _logit_rows(what, logits)
     targets, mask = _tokens_and_mask(what, targets, mask, (B, T))
     ref_lp, lengths = _floats(what, "ref_lp", ref_lp, (B, T)), _floats(what, "lengths", lengths, (B,))
@@ -1311,39 +1340,31 @@ def preference_score(logits, targets, mask, ref_lp=None, pairs=None, beta=0.1, t
             _refuse(what, "without pairs an even number of sequences")
         P = B // 2
     else:
-        if pairs.dtype != torch.long or pairs.dim() != 2 or pairs.shape[1] != 2:
+        if pairs.dtype is not torch.long or pairs.dim() != 2 or pairs.shape[1] != 2:
             _refuse(what, "pairs int64 [P, 2]")
         P, pairs = pairs.shape[0], pairs.contiguous()
     if not 0 <= smoothing <= 1:
         _refuse(what, "smoothing from 0 to 1")
     dev = logits.device
     dl = _gradient_buffer(what, logits, out, grad)
-    up = _upstream_ptr(what, upstream, unless_one, dl)
+    up = None if upstream is None else _upstream(what, upstream, grad)
+    loss = torch.empty((), dtype=_F32, device=dev)
+    margin = torch.empty(P, dtype=_F32, device=dev)
+    lp = torch.empty(B, T, dtype=_F32, device=dev)
     nb = _objective_workspace(B, T, max(P, 1))
-    loss = margin = lp = None
-    forward = workspace is None
-    if forward:
-        if unless_one:
-            _refuse(what, "unless_one needs the workspace of the first call")
-        workspace = torch.empty(nb, dtype=torch.uint8, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        margin = torch.empty(P, dtype=torch.float32, device=dev)
-        lp = torch.empty(B, T, dtype=torch.float32, device=dev)
-    elif workspace.dtype is not torch.uint8 or workspace.numel() != nb or not workspace.is_contiguous() or dl is None:
-        _refuse(what, "the workspace of an earlier call, with grad")
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
     inv = (1.0 / max(P, 1)) if inv_n is None else float(inv_n)
-    parts = int(forward) + 2 * int(dl is not None)
-    call("vk_preference_score", *rows, targets.data_ptr(), mask.data_ptr(), ptr(ref_lp), ptr(lengths), ptr(pairs), P,
-         float(beta), float(target), float(smoothing), inv, ptr(loss), ptr(margin), ptr(lp), ptr(dl), up,
-         int(bool(unless_one)), parts, B, T, V, workspace.data_ptr(), nb, stream_handle())
-    res = {"loss": loss, "margin": margin, "lp": lp, "workspace": workspace}
-    if dl is not None:
+    args = (*rows, targets.data_ptr(), mask.data_ptr(), ptr(ref_lp), ptr(lengths), ptr(pairs), P, beta, target, smoothing, inv,
+            loss.data_ptr(), margin.data_ptr(), lp.data_ptr(), ptr(dl), up, 0, 1 if dl is None else 3, B, T, V, ws.data_ptr(), nb)
+    call("vk_preference_score", *args, stream_handle())
+    res = {"loss": loss, "margin": margin, "lp": lp}
+    if grad:
         res["dlogits"] = dl
-    return res
+    return res, _Launch("vk_preference_score", args, (14, 15, 16), 17, (targets, mask, ref_lp, lengths, pairs, ws))
 
 
 def distill_score(logits, values, ids, t_lse=None, weights=None, temperature=1.0, inv_n=None, grad=True, out=None,
-                  upstream=None, unless_one=False):
+                  upstream=None):
     """Divergence of each token's softmax from a teacher's list of top logits, and its gradient in the same pass. values
     bf16 or fp32 and ids int32 or int64 [B, T, K], K up to 128 (top_logits' outputs): the teacher's logits and their tokens;
     entries of value -inf or an id outside [0, V) are none, equal ids add. With p = softmax(logits / temperature) and
@@ -1352,15 +1373,22 @@ def distill_score(logits, values, ids, t_lse=None, weights=None, temperature=1.0
       kl = sum over the entries of q (log q - log p[id]),  loss = temperature^2 sum of w kl
     w = weights (fp32 [B, T]; None: 1) over their sum, or times inv_n where that is given. Tokens whose weight is not
     positive are left out (not read, zeros); a token without an entry has kl 0 and no gradient.
-    Returns dict(loss [], kl [B, T] fp32, dlogits [B, T, V] of the logits' type when grad). logits, out, upstream, unless_one
-    as in policy_score. Beside the weighted cross-entropy of viktor/model.py:153-177."""
+    Returns dict(loss [], kl [B, T] fp32, dlogits [B, T, V] of the logits' type when grad). logits, out, upstream as in
+    policy_score. Beside the weighted cross-entropy of viktor/model.py:153-177."""
+    return _distill(logits, values, ids, t_lse, weights, temperature, inv_n, grad, out, upstream)[0]
+
+
+def _distill(logits, values, ids, t_lse, weights, temperature, inv_n, grad=True, out=None, upstream=None):
     what = "distill_score"
     _here(what, (logits, values, ids, t_lse, weights, out, upstream))
     B, T, V, rows = _logit_rows(what, logits)
-    if values.dim() != 3 or values.shape[:2] != (B, T) or values.dtype not in (BF16, torch.float32) \
-            or not 1 <= values.shape[2] <= 128:
-        _refuse(what, "values [B, T, K] bf16 or fp32, K from 1 to 128")
-    if ids.shape != values.shape or ids.dtype not in (torch.int32, torch.long):
+    vdt, idt = values.dtype, ids.dtype
+    if values.dim() != 3 or not (vdt is BF16 or vdt is _F32):
+        _refuse(what, "values [B, T, K] bf16 or fp32")
+    K = values.shape[2]
+    if not 1 <= K <= 128 or values.shape != (B, T, K):
+        _refuse(what, "values [B, T, K], K from 1 to 128")
+    if ids.shape != (B, T, K) or not (idt is torch.int32 or idt is torch.long):
         _refuse(what, "ids int32 or int64 [B, T, K]")
     values, ids = values.contiguous(), ids.contiguous()
     t_lse, weights = _floats(what, "t_lse", t_lse, (B, T)), _floats(what, "weights", weights, (B, T))
@@ -1368,21 +1396,19 @@ def distill_score(logits, values, ids, t_lse=None, weights=None, temperature=1.0
         _refuse(what, "the temperature must be positive")
     dev = logits.device
     dl = _gradient_buffer(what, logits, out, grad)
-    up = _upstream_ptr(what, upstream, unless_one, dl)
-    loss = kl = None
-    if not unless_one:
-        kl = torch.empty(B, T, dtype=torch.float32, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
+    up = None if upstream is None else _upstream(what, upstream, grad)
+    kl = torch.empty(B, T, dtype=_F32, device=dev)
+    loss = torch.empty((), dtype=_F32, device=dev)
     nb = _objective_workspace(B, T, 0)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    call("vk_distill_score", *rows, values.data_ptr(), _vk_dtype(values.dtype), ids.data_ptr(), int(ids.dtype is torch.long),
-         values.shape[2], ptr(t_lse), ptr(weights), float(temperature), int(inv_n is None),
-         1.0 if inv_n is None else float(inv_n), ptr(loss), ptr(kl), ptr(dl), up, int(bool(unless_one)), B, T, V,
-         ws.data_ptr(), nb, stream_handle())
+    args = (*rows, values.data_ptr(), _vk_dtype(vdt), ids.data_ptr(), int(idt is torch.long), K, ptr(t_lse), ptr(weights),
+            temperature, int(inv_n is None), 1.0 if inv_n is None else float(inv_n), loss.data_ptr(), kl.data_ptr(), ptr(dl), up, 0,
+            B, T, V, ws.data_ptr(), nb)
+    call("vk_distill_score", *args, stream_handle())
     res = {"loss": loss, "kl": kl}
-    if dl is not None:
+    if grad:
         res["dlogits"] = dl
-    return res
+    return res, _Launch("vk_distill_score", args, (14, 15), 16, (values, ids, t_lse, weights, ws))
 
 
 def top_logits(logits, k, temperature=1.0):
@@ -1392,20 +1418,20 @@ def top_logits(logits, k, temperature=1.0):
     list that runs out ends in value -inf, id -1. What distill_score takes as a teacher's list."""
     what = "top_logits"
     _here(what, (logits,))
-    if logits.dim() not in (2, 3):
+    nd = logits.dim()
+    if nd not in (2, 3):
         _refuse(what, "logits [B, V] or [B, T, V]")
-    shape = logits.shape[:-1]
-    B, T, V, rows = _logit_rows(what, logits if logits.dim() == 3 else logits.unsqueeze(0))
+    B, T, V, rows = _logit_rows(what, logits if nd == 3 else logits.unsqueeze(0))
     if not 1 <= k <= min(128, V):
         _refuse(what, "k from 1 to 128, and no more than V")
     if not 1e-30 <= temperature <= 1e30:
         _refuse(what, "the temperature must be positive")
     dev = logits.device
-    values = torch.empty(*shape, k, dtype=logits.dtype, device=dev)
-    ids = torch.empty(*shape, k, dtype=torch.int32, device=dev)
-    lse = torch.empty(shape, dtype=torch.float32, device=dev)
-    call("vk_top_logits", *rows, int(k), float(temperature), values.data_ptr(), ids.data_ptr(), lse.data_ptr(), B, T, V,
-         stream_handle())
+    lead = (B, T) if nd == 3 else (T,)
+    values = torch.empty(*lead, k, dtype=logits.dtype, device=dev)
+    ids = torch.empty(*lead, k, dtype=torch.int32, device=dev)
+    lse = torch.empty(*lead, dtype=_F32, device=dev)
+    call("vk_top_logits", *rows, k, temperature, values.data_ptr(), ids.data_ptr(), lse.data_ptr(), B, T, V, stream_handle())
     return values, ids, lse
 
 
