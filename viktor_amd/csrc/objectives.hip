@@ -9,8 +9,8 @@
 // (16 lanes to a whole workgroup, by its length) through its maximum, its sum and its gradient, and the few elements that
 // differ from c' p_v are written by themselves afterwards. Rows that count nothing are not read.
 //
-// Sums of exponentials are fp32 (each term off by about an ulp); their logarithm, log-ratios, objectives and sums over
-// tokens are 64 bits. The gradient is rounded once, to the logits' type. Every sum runs in a fixed order.
+// Exponentials are fp32 (each off by about an ulp); their sums, the logarithm, log-ratios, objectives and sums over tokens are
+// 64 bits. The gradient is rounded once, to the logits' type. Every sum runs in a fixed order.
 #include "common.h"
 #include "vocab_rows.h"
 
@@ -210,7 +210,8 @@ template <typename Row, bool COUNTS>
 __global__ __launch_bounds__(group_threads(Row::GL), Row::WAVES_A_SIMD) void policy_rows_kernel(LogitRows in, PolicyArgs a) {
   typedef typename Row::type T;
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL;
-  __shared__ float sh[2][GL > 64 ? GL / 64 : 1], count_sh[COUNTS && GL > 64 ? GL / 64 : 1];
+  __shared__ RowSums<GL> sh;
+  __shared__ float count_sh[COUNTS && GL > 64 ? GL / 64 : 1];
   __shared__ float coef_sh;
   __shared__ double total_sh, loss_sh[group_threads(GL) / 64];
   const float factor = a.up.get();
@@ -255,7 +256,8 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::WAVES_A_SIMD) void pol
     r.load(z, in.V, lane);
     int among = 1;
     if constexpr (COUNTS) among = count_sequence<GL>(a.mask, a.targets, b, in.T, in.V, lane, count_sh);
-    float top, s;
+    float top;
+    double s;
     row_stats<GL>(r, kUnit, sh, top, s);
     float c = 0.f;
     if (GL <= 64 || lane == lead) {
@@ -281,7 +283,7 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::WAVES_A_SIMD) void pol
       __syncthreads();
       c = coef_sh;
     }
-    const float k = -c / s;
+    const float k = -c / static_cast<float>(s);
     r.write(d, lane, top, kUnit, k);
     // (after this thread's own vector that holds it)
     if (lane == owner_of<T, GL>(r.s, y)) store_one(d + y, c + exp_of(zy, top, kUnit) * k);
@@ -310,7 +312,7 @@ template <typename Row>
 __global__ __launch_bounds__(group_threads(Row::GL)) void token_ratio_kernel(LogitRows in, PairArgs a) {
   typedef typename Row::type T;
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL;
-  __shared__ float sh[2][GL > 64 ? GL / 64 : 1];
+  __shared__ RowSums<GL> sh;
   const int lane = lane_of<GL>(), group = group_of<GL>();
   const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
   int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group;
@@ -331,14 +333,15 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void token_ratio_kernel(Log
     const float zy = load_one(z + static_cast<int>(token.target)), ref_lp = a.ref_lp ? a.ref_lp[row] : 0.f;
     Row r;
     r.load(z, in.V, lane);
-    float top, s;
+    float top;
+    double s;
     row_stats<GL>(r, kUnit, sh, top, s);
     if (lane == 0) {
       const double lp = static_cast<double>(zy) - static_cast<double>(top) - log_of(s);
       a.lp[row] = static_cast<float>(lp);
       // (rounded to 32 bits after the difference: off by 2^-24 of the ratio, not of lp)
       a.ratio[row] = static_cast<float>(lp - static_cast<double>(ref_lp));
-      if (a.stats) a.stats[row] = RowStats{top, 1.f / s};
+      if (a.stats) a.stats[row] = RowStats{top, 1.f / static_cast<float>(s)};
     }
   }
 }
@@ -520,7 +523,7 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL;
   constexpr int LL = GL < 64 ? GL : 64;                       // lanes that hold the list
   constexpr int BITS = GL == 16 ? 1024 : GL == 64 ? 4096 : 65536;  // ids seen, by their low bits
-  __shared__ float sh[2][GL > 64 ? GL / 64 : 1];
+  __shared__ RowSums<GL> sh;
   __shared__ uint32_t seen[GROUPS * BITS / 32];
   __shared__ double total_sh, loss_sh[group_threads(GL) / 64];
   __shared__ float qs[GROUPS][LIST_MAX];
@@ -624,8 +627,7 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
       mass = static_cast<float>(mass64);
       if (!a.t_lse && mass64 != 0.0) {
         cross /= mass64;
-        const float m32 = static_cast<float>(mass64);
-        lse_q = static_cast<double>(most) * a.inv_tau + log_of(m32) + (mass64 - m32) / mass64;
+        lse_q = static_cast<double>(most) * a.inv_tau + log_of(mass64);
         const float rs = static_cast<float>(1.0 / mass64);
 #pragma unroll
         for (int i = 0; i < TeacherList<LL>::N; ++i) list.q[i] *= rs;
@@ -644,7 +646,8 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
         }
       }
     }
-    float top, s;
+    float top;
+    double s;
     row_stats<GL>(r, scale, sh, top, s);
     if constexpr (GL > 64) mass = mass_sh;
     const double share = static_cast<double>(w) * w_all * a.tau;
@@ -657,7 +660,7 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
     }
     if (d) {
       const float c = static_cast<float>(share * static_cast<double>(factor));
-      const float k = mass == 0.f ? 0.f : c * mass / s;
+      const float k = mass == 0.f ? 0.f : c * mass / static_cast<float>(s);
       if (mass == 0.f)
         Row::zero(d, in.V, lane);
       else

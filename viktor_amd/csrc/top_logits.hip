@@ -197,7 +197,7 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::TOP_WAVES) void top_ro
       top = group_max<GL>(mine, sh);
       // from one maximum a lane for short lists, from several for longer ones (a bound from M maxima leaves some
       // -M log(1 - K / M) candidates)
-      if (K <= 24) {
+      if (K <= 32) {
         const uint32_t key[1] = {key_of(mine)};
         bound = kth_key<1, sizeof(T) == 2>(key, K);
       } else {
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::TOP_WAVES) void top_ro
     s = group_add<GL>(s, sums);
     if constexpr (GL > 64) bound = bound_sh;
     if (lane == 0)
-      lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (isinf(top) ? 0.0 : log_of(s)));
+      lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (isinf(top) ? 0.0 : log_near(s)));
     // each wavefront's candidates, in its own part of the list
     const float least = bound ? of_key(bound) : -FLT_MAX;
     int n = 0;
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(256) void top_lanes_kernel(const void *logits, int6
   float top = -INFINITY, s = 0.f;
   r.values([&](float x) { top = fmaxf(top, x); });
   r.values([&](float x) { s += exp_of(x, top, scale); });
-  lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (isinf(top) ? 0.0 : log_of(s)));
+  lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (isinf(top) ? 0.0 : log_near(s)));
   uint32_t key[NE];
   int entries = 0;
 #pragma unroll

@@ -94,6 +94,19 @@ __device__ __forceinline__ float group_add(float v, float *sh) {
   }
   return v;
 }
+template <int GL>
+__device__ __forceinline__ double group_add(double v, double *sh) {
+#pragma unroll
+  for (int o = (GL < 64 ? GL : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+  if constexpr (GL > 64) {
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < GL / 64; ++w) v += sh[w];
+  }
+  return v;
+}
 // Orders the group's accesses to shared memory and to what it has written. Within a wavefront they are in order as they
 // are: the fence keeps the compiler from moving them.
 template <int GL>
@@ -197,15 +210,16 @@ struct RowRegs {
       if (c * GL + lane < s.nv) store_row(vector_at<GL>(d + s.head, c, lane), o);
     if (lane < s.edges) store_one(d + edge_index<T>(s, lane), 0.f);
   }
-  // The thread's sum of exp((z - top) / temperature).
-  __device__ __forceinline__ float exps(float top, ExpScale scale) {
-    float sum = 0.f;
+  // The thread's sum of exp((z - top) / temperature). In 64 bits: 32 round at the largest term's last place with every term
+  // that follows it, 3e-7 of the sum after 88 of them, where the terms' own errors are 1e-7 of the small ones alone.
+  __device__ __forceinline__ double exps(float top, ExpScale scale) {
+    double sum = 0.0;
 #pragma unroll
     for (int c = 0; c < NV; ++c)
 #pragma unroll
       for (int k = 0; k < kVec<T>; ++k) {
         const float x = exp_of(vec_at(v[c], k, static_cast<const T *>(nullptr)), top, scale);
-        sum += x;
+        sum += static_cast<double>(x);
         if constexpr (sizeof(T) == 4)
           v[c][k] = __float_as_uint(x);
         else if constexpr (KEEPS)
@@ -213,7 +227,7 @@ struct RowRegs {
       }
     const float x = exp_of(edge, top, scale);
     if constexpr (KEEPS) edge = x;
-    return sum + x;
+    return sum + static_cast<double>(x);
   }
   // d[i] = factor exp((z_i - top) / temperature), in the row's type, after exps.
   __device__ __forceinline__ void write(T *d, int lane, float top, ExpScale scale, float factor) const {
@@ -277,8 +291,8 @@ struct RowLane {
   static __device__ __forceinline__ void zero(T *d, int V, int lane) {
     for (int k = 0; k < V; ++k) store_one(d + k, 0.f);
   }
-  __device__ __forceinline__ float exps(float top, ExpScale scale) const {
-    float sum = 0.f;
+  __device__ __forceinline__ double exps(float top, ExpScale scale) const {
+    double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < NE; ++k) sum += exp_of(z[k], top, scale);
     return sum;
@@ -366,13 +380,18 @@ struct RowWalk {
   }
 };
 
+template <int GL>
+struct RowSums {  // a number a wavefront, in shared memory
+  float top[GL > 64 ? GL / 64 : 1];
+  double sum[GL > 64 ? GL / 64 : 1];
+};
 // A walked row in one pass: each thread has its own maximum so far, and its sum by that.
 template <int GL, typename T>
-__device__ __forceinline__ void walk_stats(RowWalk<T, GL> &r, ExpScale scale, float (*sh)[GL > 64 ? GL / 64 : 1], float &top,
-                                          float &s) {
+__device__ __forceinline__ void walk_stats(RowWalk<T, GL> &r, ExpScale scale, RowSums<GL> &sh, float &top,
+                                           double &s) {
   constexpr int U = RowWalk<T, GL>::U;
   float m = fmaxf(r.edge, -FLT_MAX);  // (finite: -inf - m stays -inf)
-  float sum = exp_of(r.edge, m, scale);
+  double sum = exp_of(r.edge, m, scale);
   for (int j0 = 0; j0 < r.s.nv; j0 += GL * U) {
     u32x4 v[U];
 #pragma unroll
@@ -385,29 +404,29 @@ __device__ __forceinline__ void walk_stats(RowWalk<T, GL> &r, ExpScale scale, fl
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int k = 0; k < kVec<T>; ++k) n = fmaxf(n, vec_at(v[u], k, r.p));
-    sum *= exp_of(m, n, scale);
+    sum *= static_cast<double>(exp_of(m, n, scale));
     m = n;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int k = 0; k < kVec<T>; ++k) sum += exp_of(vec_at(v[u], k, r.p), m, scale);
+      for (int k = 0; k < kVec<T>; ++k) sum += static_cast<double>(exp_of(vec_at(v[u], k, r.p), m, scale));
   }
-  top = group_max<GL>(m, sh[0]);
-  s = group_add<GL>(sum * exp_of(m, top, scale), sh[1]);
+  top = group_max<GL>(m, sh.top);
+  s = group_add<GL>(sum * static_cast<double>(exp_of(m, top, scale)), sh.sum);
 }
 
-// A row's maximum and its sum of exp((z - maximum) / temperature), in every thread of the group. sh: two numbers a wavefront.
+// A row's maximum and its sum of exp((z - maximum) / temperature), in every thread of the group.
 template <int GL, typename Row>
-__device__ __forceinline__ void row_stats(Row &r, ExpScale scale, float (*sh)[GL > 64 ? GL / 64 : 1], float &top, float &s) {
+__device__ __forceinline__ void row_stats(Row &r, ExpScale scale, RowSums<GL> &sh, float &top, double &s) {
   if constexpr (Row::WALKS) {
     walk_stats<GL>(r, scale, sh, top, s);
     return;
   }
   top = -INFINITY;
   r.values([&](float x) { top = fmaxf(top, x); });
-  top = group_max<GL>(top, sh[0]);
+  top = group_max<GL>(top, sh.top);
   r.keep();
-  if constexpr (!Row::WALKS) s = group_add<GL>(r.exps(top, scale), sh[1]);
+  if constexpr (!Row::WALKS) s = group_add<GL>(r.exps(top, scale), sh.sum);
   r.keep();
 }
 // The same for a log-sum-exp alone: off by 2^-24 |z - top| of a term more, all to one side, which is no more of the result.
@@ -415,9 +434,24 @@ __device__ __forceinline__ float exp_near(float z, float top, ExpScale s) {
   return __builtin_amdgcn_exp2f((z - top) * s.hi);
 }
 
-// log s of a sum of exponentials, off by some 3e-8 whatever its size: the exponent's part in 64 bits, the mantissa's
-// (in [1 / sqrt 2, sqrt 2]) from log1p. A float log is off by half a step of the result, 5e-7 at a vocabulary of 87383.
-__device__ __forceinline__ double log_of(float s) {
+// log s, off by 1e-12: s = 2^ex m with m in [1 / sqrt 2, sqrt 2], log m = 2 atanh f, f = (m - 1) / (m + 1), |f| < 0.172.
+__device__ __forceinline__ double log_of(double s) {
+  int ex;
+  double m = frexp(s, &ex);
+  if (m < 0.70710678) {
+    m += m;
+    ex -= 1;
+  }
+  const double f = (m - 1.0) / (m + 1.0), g = f * f;
+  double t = 1.0 / 15.0;
+#pragma unroll
+  for (int n = 13; n >= 1; n -= 2) t = fma(t, g, 1.0 / n);
+  t = fma(static_cast<double>(ex), 0.6931471805599453, 2.0 * f * t);
+  return s > 0.0 ? t : s == 0.0 ? -INFINITY : s;  // (NaN stays)
+}
+
+// The same of a sum in 32 bits, off by 3e-8 whatever its size: the exponent's part in 64 bits, the mantissa's from log1p.
+__device__ __forceinline__ double log_near(float s) {
   int ex;
   float m = frexpf(s, &ex);
   if (m < 0.70710678f) {
