@@ -309,7 +309,7 @@ struct PairArgs {
 
 // Each token's log-probability, its log-ratio and what its gradient will need.
 template <typename Row>
-__global__ __launch_bounds__(group_threads(Row::GL)) void token_ratio_kernel(LogitRows in, PairArgs a) {
+__global__ __launch_bounds__(group_threads(Row::GL), Row::RATIO_WAVES) void token_ratio_kernel(LogitRows in, PairArgs a) {
   typedef typename Row::type T;
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL;
   __shared__ RowSums<GL> sh;

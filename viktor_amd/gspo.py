@@ -6,6 +6,7 @@
   bf16_copy(model), sync(inf, model)              scripts/gspo.py:113-126
   advantages(reward, std_floor | eps)             scripts/gspo.py:446-450
   sequence_ratio_loss(...)                        scripts/gspo.py:451, 474-477 (one kernel, + dL/dlogits)
+  teacher_lists(model, frames, plens, seqs, k)    no reference counterpart: a teacher's top logits for distillation
 
 Rewards (edit distance against labels), data loading, the optimiser loop and the gradient all-reduce of
 the reference driver are outside this path.
@@ -86,6 +87,15 @@ def token_logprobs(model, frames, plens, seqs, ended, group_size=1):
     lp = ops.gspo_score(logits.contiguous(), targets.clamp(min=0).contiguous())["lp"]
     mask = sampled_mask(targets, seqs, ended, model.tokenizer.k)
     return lp, mask
+
+
+@torch.no_grad()
+def teacher_lists(model, frames, plens, seqs, k=32, temperature=1.0, group_size=1):
+    """A teacher's lists for train.distill_frame_loss: each teacher-forced token's k largest logits with their ids, and the
+    log-sum-exp at the temperature (hip_ops.top_logits): values bf16, ids int32 [B, T, k], lse fp32 [B, T]; k <= the vocabulary.
+    No counterpart in the reference; tokens as viktor/model.py:153-177 batches them."""
+    tokens_in = model.batch(seqs)[0]
+    return ops.top_logits(model.logits(frames, tokens_in, plens, group_size=group_size), k, temperature)
 
 
 def advantages(reward, std_floor=0.003, eps=None):

@@ -30,6 +30,7 @@ import torch
 
 from . import hip_ops as ops
 from .gspo import sequence_ratio_loss
+from .objectives import distill_loss, preference_loss, token_policy_loss
 
 BF16 = torch.bfloat16
 # The embedding's gradient goes by sorted tokens past this vocabulary. Sorted is the faster way for the 343 ids too (16384
@@ -482,6 +483,29 @@ def frame_loss(model, frames, seqs, weights=None, plens=None):
     return (ce * w).sum() / w.sum()
 
 
+def pair_loss(model, frames, plens, seqs, ended, ref_lp=None, pairs=None, beta=0.1, target=0.0, smoothing=0.0, lengths=None,
+              inv_n=None, group_size=1):
+    """The micro-batch's loss of paired log ratios (objectives.preference_loss) with its autograd graph into the model:
+    returns (loss, margin [P], lp [B, T]). ref_lp [B, T] fp32: the reference policy's token log-probabilities
+    (gspo.token_logprobs' first output for the same calls); pairs int64 [P, 2] of a preferred and a lesser call (None: calls
+    2 p and 2 p + 1), for instance the best and the worst call of each window. Beside gspo_loss; the sampled tokens count, as
+    there (scripts/gspo.py:349-352)."""
+    logits, targets, mask = token_logprobs_train(model, frames, plens, seqs, ended, group_size)
+    return preference_loss(logits, targets, mask, ref_lp, pairs, beta, target, smoothing, lengths, inv_n)
+
+
+def distill_frame_loss(model, frames, seqs, lists, weights=None, plens=None, temperature=1.0, renormalise=False):
+    """Divergence of the model from a teacher on teacher-forced sequences, the distillation counterpart of frame_loss:
+    returns (loss, kl [B, T]), the loss weighted as frame_loss weighs its cross-entropy (viktor/model.py:153-177; PAD left
+    out). lists: gspo.teacher_lists' output for the same sequences and temperature; renormalise: the teacher's probabilities
+    over its list instead of the whole vocabulary."""
+    tokens_in, targets, w = model.batch(seqs, weights)
+    values, ids, lse = lists
+    logits = train_logits(model, frames, tokens_in, plens)
+    w = torch.where(targets != 0, w, torch.zeros_like(w)).to(frames.device)
+    return distill_loss(logits, values, ids, None if renormalise else lse, w, temperature)
+
+
 def _old_row(vals, mask_row):
     """Scatter one sequence's per-token values (its sampled positions, in order) into a row of mask_row's shape."""
     row = torch.zeros(mask_row.shape, dtype=torch.float32, device=mask_row.device)
@@ -489,17 +513,36 @@ def _old_row(vals, mask_row):
     return row
 
 
+def _token_lp(logits, targets, mask):
+    """The log-probabilities that token_policy_loss computes, [B, T] fp32 (0 where the mask is not set)."""
+    zero = torch.zeros(targets.shape, dtype=torch.float32, device=logits.device)
+    return ops.policy_score(logits, targets, mask, zero, zero, grad=False)["lp"]
+
+
 def gspo_update(model, opt: HipAdamW, frames, plens, calls, ended, reward, G, updates=2, micro=32, eps=4e-4,
-                std_floor=0.003, labels=None, weights=None, sft_weight=0.0):
+                std_floor=0.003, labels=None, weights=None, sft_weight=0.0, objective="sequence", eps_hi=None,
+                ref_model=None, kl_coef=0.0):
     """The GSPO policy update of one rollout (scripts/gspo.py:446-493 on one GPU, without the all-reduce):
     advantages over each window's G calls (live windows: reward std > 1e-6); pi_old of every live call before
     any update; then `updates` optimiser steps, step u over the calls of windows b % updates == u: micro-batches
     of the sequence-ratio loss summed / len(mine), plus sft_weight x the weighted cross-entropy of the windows'
     labels (when given), backward, clip + AdamW (opt). frames [windows, P, d_enc], plens [windows]; calls /
     ended: the G calls of window b at b * G .. b * G + G - 1; reward [windows, G]. Returns the step statistics
-    (pg, ce, clip, ratio, n as the reference's, and each step's gradient norm)."""
+    (pg, ce, clip, ratio, n as the reference's, and each step's gradient norm).
+
+    objective "token": the clipped policy loss per token instead (objectives.token_policy_loss: each call's tokens averaged,
+    then the calls), with kl_coef times the KL term to ref_model, a frozen policy, where one is given; its statistics are
+    sums over the calls of their tokens' means, kl among them. eps_hi: the clip's upper border (eps by default)."""
     from .gspo import advantages
     import numpy as np
+    if objective not in ("sequence", "token"):
+        raise ValueError("gspo_update: objective is 'sequence' or 'token'")
+    per_token = objective == "token"
+    if not per_token and (ref_model is not None or kl_coef):
+        raise ValueError("gspo_update: the KL term goes with objective 'token'")
+    if kl_coef and ref_model is None:
+        raise ValueError("gspo_update: the KL term needs ref_model")
+    eps_hi = eps if eps_hi is None else eps_hi
     B = frames.shape[0]
     adv, live = advantages(np.asarray(reward, dtype=np.float64).reshape(B, G), std_floor=std_floor)
     seqs = [(b, j) for b in live for j in range(G)]
@@ -516,15 +559,24 @@ def gspo_update(model, opt: HipAdamW, frames, plens, calls, ended, reward, G, up
         whole = len(mb) % G == 0 and all(mb[i][0] == mb[i - i % G][0] and mb[i][1] == i % G for i in range(len(mb)))
         return G if G > 1 and whole else 1
 
-    old = {}
+    old, ref = {}, {}
     with torch.no_grad():  # pi_old through the same forward as the update's (scripts/gspo.py:455-462)
         for i in range(0, len(seqs), micro):
             mb = seqs[i:i + micro]
             logits, targets, m = token_logprobs_train(model, *batch_of(mb), group_size=group_of(mb))
-            lp = ops.gspo_score(logits.contiguous(), targets.clamp(min=0).contiguous())["lp"]
+            if per_token:
+                lp = _token_lp(logits, targets, m)
+            else:
+                lp = ops.gspo_score(logits.contiguous(), targets.clamp(min=0).contiguous())["lp"]
             for k, bj in enumerate(mb):
                 old[bj] = lp[k][m[k]].clone()
+            if ref_model is not None:
+                lp = _token_lp(*token_logprobs_train(ref_model, *batch_of(mb), group_size=group_of(mb)))
+                for k, bj in enumerate(mb):
+                    ref[bj] = lp[k][m[k]].clone()
     stats = {"pg": 0.0, "ce": 0.0, "clip": 0.0, "ratio": 0.0, "n": 0, "grad_norm": []}
+    if per_token:
+        stats["kl"] = 0.0
     for u in range(updates):
         mine = [bj for bj in seqs if bj[0] % updates == u]
         wins = [b for b in range(B) if b % updates == u]
@@ -533,9 +585,22 @@ def gspo_update(model, opt: HipAdamW, frames, plens, calls, ended, reward, G, up
             mb = mine[i:i + micro]
             logits, targets, mask = token_logprobs_train(model, *batch_of(mb), group_size=group_of(mb))
             old_lp = torch.stack([_old_row(old[bj], mask[k]) for k, bj in enumerate(mb)])
-            nb = torch.tensor([float(n_bases[bj]) for bj in mb], device=dev)
             a = torch.tensor([adv[b, j] for b, j in mb], device=dev, dtype=torch.float32)
-            loss, s, pg, _ = sequence_ratio_loss(logits, targets, mask, old_lp, nb, a, eps, eps, 1.0 / len(mine))
+            if per_token:
+                ref_lp = torch.stack([_old_row(ref[bj], mask[k]) for k, bj in enumerate(mb)]) if ref else None
+                loss, pg, kl, lp = token_policy_loss(logits, targets, mask, old_lp, a, ref_lp, eps, eps_hi, kl_coef,
+                                                     inv_n=1.0 / len(mine))
+                loss.backward()
+                count = mask.sum(1).clamp(min=1)
+                away = torch.where(mask, (lp - old_lp).exp() - 1, torch.zeros_like(lp))
+                stats["pg"] += float((pg.sum(1) / count).sum())
+                stats["n"] += len(mb)
+                stats["clip"] += float((((away < -eps) | (away > eps_hi)).sum(1) / count).sum())
+                stats["ratio"] += float((away.abs().sum(1) / count).sum())
+                stats["kl"] += 0.0 if kl is None else float((kl.sum(1) / count).sum())
+                continue
+            nb = torch.tensor([float(n_bases[bj]) for bj in mb], device=dev)
+            loss, s, pg, _ = sequence_ratio_loss(logits, targets, mask, old_lp, nb, a, eps, eps_hi, 1.0 / len(mine))
             loss.backward()
             stats["pg"] += float(pg.sum())
             stats["n"] += len(mb)
