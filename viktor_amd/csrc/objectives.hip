@@ -509,16 +509,18 @@ struct DistillArgs {
 };
 
 // What the lanes of the list's wavefront (or of a group of 16) hold of it: entry i with lane i % LL.
-template <int LL>
+template <int LL, int LONGEST>
 struct TeacherList {
-  static constexpr int N = LIST_MAX / LL;
+  static constexpr int N = LONGEST < LL ? 1 : LONGEST / LL;
   float q[N];   // the entry's weight, 0 where there is none
   float zt[N];  // the student's logit there
   int id[N];    // -1 where there is none
 };
 
-template <typename Row>
-__global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(LogitRows in, DistillArgs a) {
+// LONGEST: the longest list. (Rows of 16 lanes hold lists of up to 32 in two entries a lane and longer ones in eight, which
+// cost registers: 131072 x 343 bf16, lists of 32: 97 -> 81 us.)
+template <typename Row, int LONGEST>
+__global__ __launch_bounds__(group_threads(Row::GL), Row::DISTILL_WAVES) void distill_rows_kernel(LogitRows in, DistillArgs a) {
   typedef typename Row::type T;
   constexpr int GL = Row::GL, GROUPS = group_threads(GL) / GL;
   constexpr int LL = GL < 64 ? GL : 64;                       // lanes that hold the list
@@ -526,8 +528,8 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
   __shared__ RowSums<GL> sh;
   __shared__ uint32_t seen[GROUPS * BITS / 32];
   __shared__ double total_sh, loss_sh[group_threads(GL) / 64];
-  __shared__ float qs[GROUPS][LIST_MAX];
-  __shared__ int ids_sh[GROUPS][LIST_MAX];
+  __shared__ float qs[GROUPS][LONGEST];
+  __shared__ int ids_sh[GROUPS][LONGEST];
   __shared__ float mass_sh;
   const float factor = a.up.get();
   if (a.up.done(factor)) return;
@@ -567,18 +569,20 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
     Row r;
     r.load(z, in.V, lane);
     // the list, with the group's first lanes: weights q, their sum, and sum q (t - z) / tau
-    TeacherList<LL> list;
+    TeacherList<LL, LONGEST> list;
     double cross = 0.0, lse_q = 0.0, mass64 = 0.0;
     float mass = 0.f;
     bool twice = false;
     if (holds) {
-      float tv[TeacherList<LL>::N], most = -INFINITY;
+      float tv[TeacherList<LL, LONGEST>::N], most = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < TeacherList<LL>::N; ++i) {
+      for (int i = 0; i < TeacherList<LL, LONGEST>::N; ++i) {
         const int e = i * LL + ll;
         list.id[i] = -1;
         list.zt[i] = 0.f;
+        list.q[i] = 0.f;
         tv[i] = -INFINITY;
+        if (i * LL >= a.K) continue;  // (the same for all: nothing of it runs for shorter lists)
         if (e >= a.K) continue;
         const int64_t at = row * a.K + e;
         const int64_t id = a.ids_64 ? static_cast<const int64_t *>(a.ids)[at] : static_cast<const int32_t *>(a.ids)[at];
@@ -595,7 +599,8 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
       if (a.t_lse) {
         lse_q = static_cast<double>(a.t_lse[row]);
 #pragma unroll
-        for (int i = 0; i < TeacherList<LL>::N; ++i) {
+        for (int i = 0; i < TeacherList<LL, LONGEST>::N; ++i) {
+          if (i * LL >= a.K) break;
           const double x = static_cast<double>(tv[i]) * a.inv_tau - lse_q;
           const float xf = static_cast<float>(x), e = expf(xf);
           list.q[i] = list.id[i] >= 0 ? fmaf(e, static_cast<float>(x - static_cast<double>(xf)), e) : 0.f;
@@ -604,10 +609,14 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
 #pragma unroll
         for (int o = LL / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, kWave));
 #pragma unroll
-        for (int i = 0; i < TeacherList<LL>::N; ++i) list.q[i] = list.id[i] >= 0 ? exp_of(tv[i], most, scale) : 0.f;
+        for (int i = 0; i < TeacherList<LL, LONGEST>::N; ++i) {
+          if (i * LL >= a.K) break;
+          list.q[i] = list.id[i] >= 0 ? exp_of(tv[i], most, scale) : 0.f;
+        }
       }
 #pragma unroll
-      for (int i = 0; i < TeacherList<LL>::N; ++i) {
+      for (int i = 0; i < TeacherList<LL, LONGEST>::N; ++i) {
+        if (i * LL >= a.K) break;
         if (list.id[i] < 0) continue;
         mass64 += static_cast<double>(list.q[i]);
         if (list.q[i] != 0.f)
@@ -630,14 +639,14 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
         lse_q = static_cast<double>(most) * a.inv_tau + log_of(mass64);
         const float rs = static_cast<float>(1.0 / mass64);
 #pragma unroll
-        for (int i = 0; i < TeacherList<LL>::N; ++i) list.q[i] *= rs;
+        for (int i = 0; i < TeacherList<LL, LONGEST>::N; ++i) list.q[i] *= rs;
         mass = mass64 > 0.0 ? 1.f : mass;
         mass64 = mass;
       }
       if (GL > 64 && ll == 0) mass_sh = mass;
       if (twice) {
 #pragma unroll
-        for (int i = 0; i < TeacherList<LL>::N; ++i) {
+        for (int i = 0; i < TeacherList<LL, LONGEST>::N; ++i) {
           const int e = i * LL + ll;
           if (e < a.K) {
             ids_sh[group][e] = list.id[i];
@@ -668,8 +677,9 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void distill_rows_kernel(Lo
       group_sync<GL>();
       if (holds) {
 #pragma unroll
-        for (int i = 0; i < TeacherList<LL>::N; ++i) {
+        for (int i = 0; i < TeacherList<LL, LONGEST>::N; ++i) {
           const int id = list.id[i], e = i * LL + ll;
+          if (i * LL >= a.K) break;
           if (id < 0) continue;
           float q = list.q[i];
           bool mine = true;
@@ -716,13 +726,14 @@ int with_form(int V, F f) {
   if constexpr (LANES) {
     if (V <= 8) return f(static_cast<RowLane<T, 8> *>(nullptr));
     if (V <= 16) return f(static_cast<RowLane<T, 16> *>(nullptr));
+    if (V <= 32) return f(static_cast<RowLane<T, 32> *>(nullptr));
   }
   return row_form((V + kVec<T> - 1) / kVec<T>, [&](auto gl, auto nv) {
     typedef typename RowForm<T, decltype(gl)::value, decltype(nv)::value>::type Row;
     return f(static_cast<Row *>(nullptr));
   });
 }
-// LANES: rows of up to 16 logits a thread each
+// LANES: rows of up to 32 logits a thread each
 template <bool LANES, typename F>
 int with_row(int dtype, int V, F f) {
   return dtype == VK_DTYPE_BF16 ? with_form<bf16_t, LANES>(V, f) : with_form<float, LANES>(V, f);
@@ -906,7 +917,13 @@ extern "C" int vk_distill_score(const void *logits, int32_t dtype, int64_t ld_b,
       const int rc2 = launch_status("distill_score weights");
       if (rc2 != VK_OK) return rc2;
       blocks = row_blocks(N, Row::GL);
-      distill_rows_kernel<Row><<<blocks, group_threads(Row::GL), 0, st>>>(in, a);
+      if constexpr (Row::GL == 16) {
+        if (K <= 32) {
+          distill_rows_kernel<Row, 32><<<blocks, group_threads(Row::GL), 0, st>>>(in, a);
+          return launch_status("distill_score");
+        }
+      }
+      distill_rows_kernel<Row, LIST_MAX><<<blocks, group_threads(Row::GL), 0, st>>>(in, a);
       return launch_status("distill_score");
     });
     if (rc != VK_OK) return rc;

@@ -6,7 +6,7 @@
 // by bit with ballots, the largest number that k of the maxima reach. What reaches it in the row (a little more than k logits
 // of most rows) goes to shared memory with its id, and one wavefront sorts it in registers. Rows with more candidates than fit
 // (many equal logits) have their k-th logit searched bit by bit over all of it, then the id up to which equal ones are taken.
-// Rows of up to 16 logits go one a thread: each logit counts the ones before it.
+// Rows of up to 32 logits go one a thread: each logit counts the ones before it.
 // Logits of -inf and NaN are no entries: a list that runs out ends in id -1, value -inf.
 #include <float.h>
 
@@ -110,6 +110,40 @@ __device__ __forceinline__ uint32_t kth_key(const uint32_t (&key)[R], int k) {
   return BF16 && bound && !(bound & 0x80000000u) ? bound | 0xffffu : bound;  // (a negative bf16's key has ones there)
 }
 
+// The lane's partner's word across j lanes (xor): data-parallel moves within rows of 16, one swizzle for 4, gfx950's lane swaps
+// for 16 and 32. (ds_bpermute, which __shfl_xor is, goes through the LDS pipe with an address each time.)
+template <int J>
+__device__ __forceinline__ uint32_t across(uint32_t x) {
+  if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(x, 0xb1, 0xf, 0xf, true);        // quads 1 0 3 2
+  if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(x, 0x4e, 0xf, 0xf, true);        // quads 2 3 0 1
+  if constexpr (J == 4) return __builtin_amdgcn_ds_swizzle(x, 0x101f);                   // lane ^ 4 of 32
+  if constexpr (J == 8) return __builtin_amdgcn_mov_dpp(x, 0x128, 0xf, 0xf, true);       // rows of 16 turned by 8
+  if constexpr (J == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return (threadIdx.x & 16) ? r[0] : r[1];
+  }
+  if constexpr (J == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return (threadIdx.x & 32) ? r[0] : r[1];
+  }
+  return x;
+}
+template <int J>
+__device__ __forceinline__ uint64_t across(uint64_t x) {
+  return (static_cast<uint64_t>(across<J>(static_cast<uint32_t>(x >> 32))) << 32) | across<J>(static_cast<uint32_t>(x));
+}
+template <typename Entry>
+__device__ __forceinline__ Entry across(Entry x, int j) {  // (j is a constant where it is unrolled)
+  switch (j) {
+    case 1: return across<1>(x);
+    case 2: return across<2>(x);
+    case 4: return across<4>(x);
+    case 8: return across<8>(x);
+    case 16: return across<16>(x);
+    default: return across<32>(x);
+  }
+}
+
 // Sorts 64 R entries of a wavefront, entry 64 r + lane with e[r], the largest first (bitonic).
 template <typename Entry, int R>
 __device__ __forceinline__ void sort_entries(Entry (&e)[R], int lane) {
@@ -132,7 +166,7 @@ __device__ __forceinline__ void sort_entries(Entry (&e)[R], int lane) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const bool falls = ((64 * r + lane) & k) == 0 || k == 64 * R, first = (lane & j) == 0;
-          const Entry o = __shfl_xor(e[r], j, kWave);
+          const Entry o = across(e[r], j);
           e[r] = (falls == first) == (e[r] > o) ? e[r] : o;
         }
       }
@@ -396,7 +430,9 @@ extern "C" int vk_top_logits(const void *logits, int32_t dtype, int64_t ld_b, in
     typedef typename std::conditional<sizeof(E) == 2, uint32_t, uint64_t>::type Short;
     if (V <= 8) return run(top_lanes_kernel<E, 8>, 256, 256, true);
     if (V <= 16) return run(top_lanes_kernel<E, 16>, 256, 256, true);
+    if (V <= 32) return run(top_lanes_kernel<E, 32>, 256, 256, true);
     if (V <= 256) return run(top_rows_kernel<RowStrided<E, 4>, Short>, 256, 4, false);
+    if (V <= 384) return run(top_rows_kernel<RowStrided<E, 6>, Short>, 256, 4, false);
     if (V <= 512) return run(top_rows_kernel<RowStrided<E, 8>, Short>, 256, 4, false);
     return top_form((V + kVec<E> - 1) / kVec<E>, [&](auto gl, auto nv) {
       constexpr int G = decltype(gl)::value;

@@ -146,11 +146,13 @@ struct RowRegs {
   // Exponentials stay in registers from the sum to the gradient: in the logits' place (fp32), or beside them up to 6 vectors
   // of bf16. Beyond that they are computed again.
   static constexpr bool KEEPS = sizeof(T) == 4 || NV <= 6;
-  // Wavefronts a SIMD that the objectives' kernels are compiled for: rows of up to 3 vectors a thread gain more from 8 of them
-  // than the ten registers that go to memory around the 64-bit numbers cost (16416 x 5463 bf16: 86 -> 79 us).
-  static constexpr int WAVES_A_SIMD = GL_ >= 64 && NV <= 3 ? 8 : GL_ == 1024 ? 4 : 1;
+  // Wavefronts a SIMD that the policy's kernel is compiled for: rows of 22 vectors a lane come out a few registers over three
+  // (8192 x 11000 bf16: 82 -> 72 us); a workgroup of 1024 needs four.
+  static constexpr int WAVES_A_SIMD = GL_ == 1024 ? 4 : GL_ == 64 && NV == 22 ? 3 : 1;
   // ... that the log-ratios are: 85 registers are enough (32 x 147 x 21847 bf16, 256 threads a row: 39 -> 35 us)
   static constexpr int RATIO_WAVES = GL_ == 256 || GL_ == 512 ? 6 : GL_ == 64 && NV > 3 ? 4 : 1;
+  // ... that the distillation is: one register short of four
+  static constexpr int DISTILL_WAVES = GL_ > 64 ? 4 : 1;
   // ... that top_logits is, and the maxima a lane of a wavefront's row that its bound comes from
   static constexpr int TOP_WAVES = GL_ > 64 ? 4 : NV <= 3 ? 8 : NV <= 6 ? 6 : NV <= 11 ? 4 : 3, TOP_MAXIMA = NV <= 6 ? NV : 4;
   Span s;
@@ -272,7 +274,7 @@ struct RowRegs {
 template <typename T, int NE>
 struct RowLane {
   typedef T type;
-  static constexpr int WAVES_A_SIMD = 1, RATIO_WAVES = 1;
+  static constexpr int WAVES_A_SIMD = 1, RATIO_WAVES = 1, DISTILL_WAVES = 1;
   static constexpr bool WALKS = false;
   static constexpr int GL = 1;
   Span s;
@@ -313,7 +315,7 @@ struct RowLane {
 template <typename T, int GL_>
 struct RowWalk {
   typedef T type;
-  static constexpr int WAVES_A_SIMD = 1, RATIO_WAVES = 1;
+  static constexpr int WAVES_A_SIMD = 1, RATIO_WAVES = 1, DISTILL_WAVES = 1;
   static constexpr bool WALKS = true;
   static constexpr int GL = GL_, TOP_WAVES = 1, TOP_MAXIMA = 1;
   Span s;
@@ -510,6 +512,7 @@ inline int row_form(int64_t vectors, F f) {
   if (vectors <= GL * NV) return f(std::integral_constant<int, GL>{}, std::integral_constant<int, NV>{})
   VK_FORM(16, 3);
   VK_FORM(16, 6);
+  VK_FORM(64, 2);
   VK_FORM(64, 3);
   VK_FORM(64, 6);
   VK_FORM(64, 11);
