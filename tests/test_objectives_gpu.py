@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from viktor_amd import hip_ops as ops, objectives
 
@@ -450,11 +451,53 @@ def test_backward_hands_out_what_score_computes(which):
         assert torch.equal(got, score(z, **kw, upstream=up)["dlogits"])
         f = score(z.float(), **kw)["dlogits"].double() * float(up)
         near(got, f, torch.finfo(BF16).eps / 2 * f.abs() * (1 + 1e-4) + 1e-9 * f.abs().max() + 1e-37, "factor")
-    with torch.no_grad():
-        assert not loss_fn(leaf, **kw)[0].requires_grad
+    with torch.no_grad():  # no gradient, nor its memory
+        before = torch.cuda.memory_allocated()
+        off = loss_fn(leaf, **kw)
+        assert not off[0].requires_grad and torch.cuda.memory_allocated() - before < leaf.numel()
+        assert torch.equal(off[0], want["loss"])
     leaf.grad = None
     (loss_fn(leaf, **kw)[0] + loss_fn(leaf, **kw)[0]).backward()
     near(leaf.grad, 2 * want["dlogits"].double(), torch.finfo(BF16).eps * want["dlogits"].double().abs() + 1e-37, "sum of two")
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("layout", ["plain", "sliced"])
+def test_backward_of_moved_tensors(which, layout):
+    """Saved tensors that hooks move to the host and back (contiguous then), and a checkpointed region that is computed
+    anew: the gradient of a scaled loss, and of a kept graph's second backward, reads what the hooks give."""
+    z, calls = objective_calls()
+    if layout == "sliced":
+        big = torch.zeros(4, 15, 348, dtype=BF16, device=DEV)
+        big[:, 2:14, 3:346] = z
+        z = big[:, 2:14, 3:346]
+    loss_fn, score, _, kw = calls[which]
+    want = score(z, **kw, upstream=torch.tensor(0.37, device=DEV))["dlogits"]
+    leaf = z.detach().requires_grad_(True)
+    with torch.autograd.graph.save_on_cpu():
+        loss = loss_fn(leaf * 1, **kw)[0]
+        view = loss_fn(leaf, **kw)[0]
+    torch.empty(4, 12, 343, dtype=BF16, device=DEV).fill_(math.nan)  # (memory that the product's result may have had)
+    assert torch.equal(torch.autograd.grad(0.37 * loss, leaf, retain_graph=True)[0], want)
+    assert torch.equal(torch.autograd.grad(0.37 * loss, leaf)[0], want)
+    assert torch.equal(torch.autograd.grad(0.37 * view, leaf)[0], want)
+    again = torch.utils.checkpoint.checkpoint(lambda x: loss_fn(x * 1, **kw)[0], leaf, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(0.37 * again, leaf)[0], want)
+
+
+def test_inputs_written_to_before_the_backward():
+    """Autograd's own refusal: an input of the loss that changed in between."""
+    z, calls = objective_calls()
+    for loss_fn, _, _, kw in calls:
+        leaf = z.clone().requires_grad_(True)
+        x = leaf * 1
+        loss = loss_fn(x, **kw)[0]
+        x.data.add_(0)  # (no version: still good)
+        loss.backward(retain_graph=True)
+        with torch.no_grad():
+            x.add_(1)
+        with pytest.raises(RuntimeError):
+            loss.backward()
 
 
 @pytest.mark.parametrize("which", [0, 1, 2])

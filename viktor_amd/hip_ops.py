@@ -1240,17 +1240,22 @@ def _objective_workspace(B, T, P):
 
 
 class _Launch:
-    """A call of an objective's entry point: its arguments, and the places among them of what a second pass over the same
-    inputs replaces (the gradient's buffer, its factor, the outputs, which that pass leaves alone)."""
-    __slots__ = ("name", "args", "outputs", "at", "keep")
+    """A call of an objective's entry point, for another pass over the same inputs: its arguments; the places among them of
+    the outputs (which that pass leaves alone), of the gradient's buffer with its factor behind it, and of each tensor that
+    the pass reads beside the logits (`tensors`, at `places`; contiguous)."""
+    __slots__ = ("name", "args", "outputs", "at", "tensors", "places")
 
-    def __init__(self, name, args, outputs, at, keep):
-        self.name, self.args, self.outputs, self.at, self.keep = name, args, outputs, at, keep
+    def __init__(self, name, args, outputs, at, tensors, places):
+        self.name, self.args, self.outputs, self.at, self.tensors, self.places = name, args, outputs, at, tensors, places
 
-    def again(self, dl, upstream, unless_one):
+    def again(self, logits, tensors, dl, upstream, unless_one):
         """dlogits times the fp32 number `upstream` into dl; unless_one: dl holds it for a factor of 1, in which case nothing
-        is done. On the current device's current stream."""
+        is done. logits and tensors: the inputs as autograd kept them (hooks may have moved them). On the current device's
+        current stream."""
         args, at = list(self.args), self.at
+        args[:4] = _logit_rows(self.name, logits)[3]
+        for i, t in zip(self.places, tensors):
+            args[i] = ptr(t)
         for i in self.outputs:
             args[i] = None
         args[at], args[at + 1], args[at + 2] = dl.data_ptr(), upstream.data_ptr(), unless_one
@@ -1312,7 +1317,8 @@ def _policy(logits, targets, mask, old_lp, adv, ref_lp, eps_lo, eps_hi, kl_coef,
     res = {"loss": loss, "pg": pg, "kl": kl, "lp": lp}
     if grad:
         res["dlogits"] = dl
-    return res, _Launch("vk_policy_score", args, (15, 16, 17, 18), 19, (targets, mask, old_lp, adv, ref_lp, ws))
+    return res, _Launch("vk_policy_score", args, (15, 16, 17, 18), 19, (targets, mask, old_lp, adv, ref_lp, ws),
+                        (4, 5, 6, 7, 9, 25))
 
 
 def preference_score(logits, targets, mask, ref_lp=None, pairs=None, beta=0.1, target=0.0, smoothing=0.0, lengths=None,
@@ -1360,7 +1366,7 @@ def _preference(logits, targets, mask, ref_lp, pairs, beta, target, smoothing, l
     res = {"loss": loss, "margin": margin, "lp": lp}
     if grad:
         res["dlogits"] = dl
-    return res, _Launch("vk_preference_score", args, (14, 15, 16), 17, (targets, mask, ref_lp, lengths, pairs, ws))
+    return res, _Launch("vk_preference_score", args, (14, 15, 16), 17, (targets, mask, ws), (4, 5, 24))
 
 
 def distill_score(logits, values, ids, t_lse=None, weights=None, temperature=1.0, inv_n=None, grad=True, out=None,
@@ -1408,7 +1414,7 @@ def _distill(logits, values, ids, t_lse, weights, temperature, inv_n, grad=True,
     res = {"loss": loss, "kl": kl}
     if grad:
         res["dlogits"] = dl
-    return res, _Launch("vk_distill_score", args, (14, 15), 16, (values, ids, t_lse, weights, ws))
+    return res, _Launch("vk_distill_score", args, (14, 15), 16, (values, ids, t_lse, weights, ws), (4, 6, 9, 10, 22))
 
 
 def top_logits(logits, k, temperature=1.0):

@@ -19,12 +19,12 @@ from . import hip_ops as ops
 
 class _Objective(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, op, outputs, args):
-        grad = ctx.needs_input_grad[0]
+    def forward(ctx, logits, op, outputs, args, grad):
         res, launch = op(logits.detach(), *args, grad)
         if grad:
+            ctx.save_for_backward(logits, *launch.tensors)
+            launch.tensors = None
             ctx.launch, ctx.dlogits = launch, res["dlogits"]
-            ctx.save_for_backward(logits, *launch.keep)
         others = [res[name] for name in outputs]
         ctx.mark_non_differentiable(*(t for t in others if t is not None))
         ctx.set_materialize_grads(False)
@@ -34,31 +34,35 @@ class _Objective(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_loss, *unused):
         if g_loss is None:
-            return None, None, None, None
-        logits = ctx.saved_tensors[0]  # (raises if an input has been written to since)
-        dl, ctx.dlogits = ctx.dlogits, None  # (handed out once: a caller may keep it as its gradient)
+            return None, None, None, None, None
+        logits, *tensors = ctx.saved_tensors  # (raises if an input has been written to since)
+        dl, ctx.dlogits = ctx.dlogits, None   # (handed out once: a caller may keep it as its gradient)
         there = dl is not None
         if not there:
             dl = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        ctx.launch.again(dl, g_loss, there)
-        return dl, None, None, None
+        ctx.launch.again(logits, tensors, dl, g_loss, there)
+        return dl, None, None, None, None
+
+
+def _objective(logits, op, outputs, args):
+    return _Objective.apply(logits, op, outputs, args, logits.requires_grad and torch.is_grad_enabled())
 
 
 def token_policy_loss(logits, targets, mask, old_lp, adv, ref_lp=None, eps_lo=0.2, eps_hi=0.2, kl_coef=0.0, per="sequence",
                       inv_n=None):
     """hip_ops.policy_score, differentiable in logits: (loss, pg, kl, lp); kl is None without ref_lp. The per-token
     counterpart of gspo.sequence_ratio_loss. pg, kl and lp are values to read."""
-    return _Objective.apply(logits, ops._policy, ("pg", "kl", "lp"),
+    return _objective(logits, ops._policy, ("pg", "kl", "lp"),
                             (targets, mask, old_lp, adv, ref_lp, eps_lo, eps_hi, kl_coef, per, inv_n))
 
 
 def preference_loss(logits, targets, mask, ref_lp=None, pairs=None, beta=0.1, target=0.0, smoothing=0.0, lengths=None,
                     inv_n=None):
     """hip_ops.preference_score, differentiable in logits: (loss, margin, lp). margin and lp are values to read."""
-    return _Objective.apply(logits, ops._preference, ("margin", "lp"),
+    return _objective(logits, ops._preference, ("margin", "lp"),
                             (targets, mask, ref_lp, pairs, beta, target, smoothing, lengths, inv_n))
 
 
 def distill_loss(logits, values, ids, t_lse=None, weights=None, temperature=1.0, inv_n=None):
     """hip_ops.distill_score, differentiable in logits: (loss, kl). kl is a value to read."""
-    return _Objective.apply(logits, ops._distill, ("kl",), (values, ids, t_lse, weights, temperature, inv_n))
+    return _objective(logits, ops._distill, ("kl",), (values, ids, t_lse, weights, temperature, inv_n))
