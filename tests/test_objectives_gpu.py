@@ -246,6 +246,15 @@ def test_preference_pairs(B, T, V):
     assert float(one["loss"]) == 0 and one["margin"].shape == (0,) and bool((one["dlogits"] == 0).all())
 
 
+@pytest.mark.parametrize("B,T,P", [(64, 5, 1024), (64, 5, 1025), (66, 5, 40), (200, 50, 900), (2, 8192, 3), (2, 8193, 3)])
+def test_preference_both_ways_of_the_pairs(B, T, P):
+    """The pairs in one workgroup and in three launches, on both sides of the borders between them."""
+    z, y, mask, old, ref, g = policy_inputs(B, T, 20, F32, B + P, far=0.05)
+    pairs = torch.randint(0, B, (P, 2), generator=g, device=DEV)
+    check_preference(z, y, mask, ref, pairs=pairs, beta=0.05)
+    check_preference(z, y, mask, ref, beta=0.05, lengths=1 + torch.rand(B, generator=g, device=DEV))
+
+
 def test_preference_far_margins_and_what_does_not_count():
     """Margins of hundreds either way (no overflow), NaN where nothing counts."""
     z, y, mask, old, ref, g = policy_inputs(6, 20, 343, BF16, 8)
@@ -318,6 +327,30 @@ def test_distill_lists(K, V):
         got = check_distill(z, val, ids, temperature=tau)
         assert float(got["kl"][0, 6]) == 0 and bool((got["dlogits"][0, 6:8] == 0).all())
         check_distill(z, val, ids, temperature=tau, t_lse=lse, inv_n=0.05)
+
+
+@pytest.mark.parametrize("V", [25000, 87383, 190000])
+def test_distill_long_lists_of_long_rows(V):
+    """Lists of 128 of rows that a workgroup holds or walks: ids that share their low 16 bits, ids that repeat, and both."""
+    for dtype in (BF16, F32):
+        z, y, mask, g = logits_of(2, 3, V, dtype, V)
+        val, ids, lse = lists(z, 128, g, F32, torch.int64)
+        if V > 70000:
+            ids[0, 0, 1] = ids[0, 0, 0] % 65536
+            ids[0, 0, 2] = ids[0, 0, 0] % 65536 + 65536 if int(ids[0, 0, 0]) % 65536 + 65536 < V else ids[0, 0, 0] % 65536
+        ids[0, 1, 7:9] = ids[0, 1, 100].clone()
+        ids[0, 2, ::2] = ids[0, 2, 127].clone()
+        ids[1, 0, 5], ids[1, 0, 6] = 2 ** 40, -2 ** 40
+        check_distill(z, val, ids)
+        check_distill(z, val, ids, t_lse=lse, temperature=1.0, inv_n=0.2)
+
+
+def test_distill_many_tokens():
+    """More tokens than one pass of the rows' kernel counts by itself: the weights summed in a launch of their own."""
+    for B, T, V in ((2, 1024, 50), (1, 2049, 50), (70, 60, 343)):
+        z, y, mask, g = logits_of(B, T, V, BF16, B + T)
+        val, ids, lse = lists(z, 8, g, BF16, torch.int32)
+        check_distill(z, val, ids, weights=torch.where(mask, torch.rand(B, T, generator=g, device=DEV), 0.0))
 
 
 def test_distill_what_does_not_count():
@@ -597,6 +630,24 @@ def test_side_stream():
     for a, b in zip(wants, gots):
         assert all(torch.equal(a[k], b[k]) for k in a if a[k] is not None)
     assert all(torch.equal(a, b) for a, b in zip(top, top2))
+
+
+def test_two_streams_at_once():
+    """Calls of different inputs on two streams, nothing between them: each as alone."""
+    sets = [objective_calls(BF16, 5463, seed) for seed in (1, 2)]
+    wants = [[score(z, **kw) for _, score, _, kw in calls] for z, calls in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    gots = [[], []]
+    for _ in range(3):
+        for i, (z, calls) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                gots[i] += [score(z, **kw) for _, score, _, kw in calls]
+    torch.cuda.synchronize()
+    for want, got in zip(wants, gots):
+        for k, b in enumerate(got):
+            a = want[k % 3]
+            assert all(torch.equal(a[n], b[n]) for n in a if a[n] is not None)
 
 
 def test_captured_and_replayed():

@@ -136,6 +136,12 @@ __device__ __forceinline__ float exp_of(float z, float top, ExpScale s) {
   return __builtin_amdgcn_exp2f(fmaf(t, s.lo, t * s.hi));
 }
 
+// ... of a gradient of type T: a bf16's last place is far above the scale's low part.
+template <typename T>
+__device__ __forceinline__ float exp_out(float z, float top, ExpScale s) {
+  return sizeof(T) == 2 ? __builtin_amdgcn_exp2f((z - top) * s.hi) : exp_of(z, top, s);
+}
+
 // ---- rows ---------------------------------------------------------------------------------------------------------------
 // In registers: NV vectors a thread, up to GL * NV vectors. Places behind the row's end hold -inf.
 template <typename T, int GL_, int NV>
@@ -246,7 +252,7 @@ struct RowRegs {
           if constexpr (sizeof(T) == 2 && KEEPS)
             o[k] = e[c * 8 + k] * factor;
           else
-            o[k] = (KEEPS ? x : exp_of(x, top, scale)) * factor;
+            o[k] = (KEEPS ? x : exp_out<T>(x, top, scale)) * factor;
         }
         store_row(vector_at<GL>(d + s.head, c, lane), o);
       }
@@ -261,7 +267,7 @@ struct RowRegs {
       if (j < s.nv) {
         float o[kVec<T>];
 #pragma unroll
-        for (int k = 0; k < kVec<T>; ++k) o[k] = exp_of(vec_at(v[c], k, static_cast<const T *>(nullptr)), top, scale) * factor;
+        for (int k = 0; k < kVec<T>; ++k) o[k] = exp_out<T>(vec_at(v[c], k, static_cast<const T *>(nullptr)), top, scale) * factor;
         store_row(vector_at<GL>(d + s.head, c, lane), o);
       }
     }
@@ -270,7 +276,8 @@ struct RowRegs {
 };
 
 // A row of up to NE elements in one thread. (Its loads and stores are 2 or 4 bytes a lane, a row's length apart; the lines
-// they share stay in the caches: 512 x 1024 rows of 7 bf16 move 4.9 TB/s so.)
+// they share stay in the caches. 512 x 1024 rows of 7 bf16 with the policy's 64-bit numbers: 16 us, 133 with 16 lanes a row;
+// 131072 rows of 20: 28 and 52; of 64, lists of 32: 138 and 85.)
 template <typename T, int NE>
 struct RowLane {
   typedef T type;
@@ -453,6 +460,9 @@ __device__ __forceinline__ double log_of(double s) {
   t = fma(static_cast<double>(ex), 0.6931471805599453, 2.0 * f * t);
   return s > 0.0 ? t : s == 0.0 ? -INFINITY : s;  // (NaN stays)
 }
+// The same as a call, beside a row that fills the registers: the constants of the series stay out of them
+// (2064 x 87383 fp32, distillation: 300 us inlined, 285 called).
+static __device__ __attribute__((noinline)) double log_called(double s) { return log_of(s); }
 
 // The same of a sum in 32 bits, off by 3e-8 whatever its size: the exponent's part in 64 bits, the mantissa's from log1p.
 __device__ __forceinline__ double log_near(float s) {
@@ -504,8 +514,13 @@ __device__ __forceinline__ int lane_of() {
   return threadIdx.x % GL;
 }
 
-// The smallest register form of at least 16 lanes that holds that many vectors: calls f(GL, NV), both as integral constants; NV = 0 for rows
-// that are walked.
+// The smallest register form of at least 16 lanes that holds that many vectors: calls f(GL, NV), both as integral constants;
+// NV = 0 for rows that are walked. A wavefront a row (no barriers) as far as its registers go: 16416 x 5463 bf16, policy and
+// distillation, 71 and 91 us with 64 lanes of 11 vectors, 84 and 111 with 256 of 3, 116 and 185 with 512 of 2; beyond 22
+// vectors a lane it loses (4704 x 21847 bf16, preference: 108 us with 64 lanes of 43, 100 with 256 of 11). 16 lanes where four
+// rows to a wavefront share the 64-bit numbers: 131072 x 343 fp32, policy, 83 us with 16 lanes of 6, 144 with 64 of 2; the
+// other way round from 100 vectors on (112500 x 800 bf16: 153 and 128). Rows past 22528 vectors are read twice: 2064 x 87383 fp32,
+// distillation, 390 us walked, 285 in registers.
 template <typename F>
 inline int row_form(int64_t vectors, F f) {
 #define VK_FORM(GL, NV) \

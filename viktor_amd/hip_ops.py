@@ -1253,9 +1253,11 @@ class _Launch:
         is done. logits and tensors: the inputs as autograd kept them (hooks may have moved them). On the current device's
         current stream."""
         args, at = list(self.args), self.at
-        args[:4] = _logit_rows(self.name, logits)[3]
+        if logits.data_ptr() != args[0]:
+            args[:4] = _logit_rows(self.name, logits)[3]
         for i, t in zip(self.places, tensors):
-            args[i] = ptr(t)
+            if t is not None:
+                args[i] = t.data_ptr()
         for i in self.outputs:
             args[i] = None
         args[at], args[at + 1], args[at + 2] = dl.data_ptr(), upstream.data_ptr(), unless_one
