@@ -518,6 +518,46 @@ def test_backward_of_moved_tensors(which, layout):
     assert torch.equal(torch.autograd.grad(0.37 * again, leaf)[0], want)
 
 
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_backward_of_logits_laid_out_anew_at_their_address(which):
+    """Hooks that give the logits back at the address they had, their rows packed: the strides are the packed ones. Kept
+    inputs of another type or size, or on the host, are refused."""
+    z, calls = objective_calls()
+    loss_fn, score, _, kw = calls[which]
+    want = score(z, **kw, upstream=torch.tensor(0.37, device=DEV))["dlogits"]
+    big = torch.zeros(4, 15, 348, dtype=BF16, device=DEV)
+    view = big[:, 2:14, 3:346]
+    view.copy_(z)
+    leaf = view.detach().requires_grad_(True)
+
+    def pack(t):
+        return t.clone(memory_format=torch.contiguous_format)
+
+    def unpack(t):
+        if t.shape != z.shape or t.dtype is not BF16:
+            return t
+        big.zero_()
+        there = big.view(-1)[view.storage_offset():][:t.numel()].view(t.shape)
+        assert there.data_ptr() == view.data_ptr()
+        return there.copy_(t)
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        loss = loss_fn(leaf, **kw)[0]
+    assert torch.equal(torch.autograd.grad(0.37 * loss, leaf, retain_graph=True)[0], want)
+    assert torch.equal(torch.autograd.grad(0.37 * loss, leaf)[0], want)
+
+    def halves(t):
+        return t.bfloat16() if t.dtype is torch.float32 else t[:2] if t.dtype is torch.uint8 else t
+
+    for give in (halves, lambda t: t[:, :-1] if t.shape == z.shape else t, lambda t: t.cpu() if t.dim() == 2 else t,
+                 lambda t: t.cpu()):
+        leaf = z.detach().requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, give):
+            loss = loss_fn(leaf, **kw)[0]
+        with pytest.raises(AssertionError, match="kept"):
+            loss.backward()
+
+
 def test_inputs_written_to_before_the_backward():
     """Autograd's own refusal: an input of the loss that changed in between."""
     z, calls = objective_calls()

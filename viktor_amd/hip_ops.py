@@ -1242,21 +1242,32 @@ def _objective_workspace(B, T, P):
 class _Launch:
     """A call of an objective's entry point, for another pass over the same inputs: its arguments; the places among them of
     the outputs (which that pass leaves alone), of the gradient's buffer with its factor behind it, and of each tensor that
-    the pass reads beside the logits (`tensors`, at `places`; contiguous)."""
-    __slots__ = ("name", "args", "outputs", "at", "tensors", "places")
+    the pass reads beside the logits (`tensors`, at `places`; contiguous). `like`, `kinds`: types, sizes and devices of the
+    logits and of these."""
+    __slots__ = ("name", "args", "outputs", "at", "tensors", "places", "like", "kinds")
 
     def __init__(self, name, args, outputs, at, tensors, places):
         self.name, self.args, self.outputs, self.at, self.tensors, self.places = name, args, outputs, at, tensors, places
 
+    def keep(self, logits):
+        """The tensors, for autograd to keep: none of them is held here any more."""
+        tensors, self.tensors = self.tensors, None
+        self.like = (logits.dtype, logits.shape, logits.get_device())
+        self.kinds = [t if t is None else (t.dtype, t.numel(), t.get_device()) for t in tensors]
+        return tensors
+
     def again(self, logits, tensors, dl, upstream, unless_one):
         """dlogits times the fp32 number `upstream` into dl; unless_one: dl holds it for a factor of 1, in which case nothing
-        is done. logits and tensors: the inputs as autograd kept them (hooks may have moved them). On the current device's
-        current stream."""
+        is done. logits and tensors: the inputs as autograd kept them (hooks may have moved them, to rows of other strides at
+        the same address too). On the current device's current stream."""
         args, at = list(self.args), self.at
-        if logits.data_ptr() != args[0]:
-            args[:4] = _logit_rows(self.name, logits)[3]
-        for i, t in zip(self.places, tensors):
+        args[:4] = _logit_rows(self.name, logits)[3]
+        if (logits.dtype, logits.shape, logits.get_device()) != self.like:
+            _refuse(self.name, "kept logits of the type, shape and device they had")
+        for i, t, kind in zip(self.places, tensors, self.kinds):
             if t is not None:
+                if (t.dtype, t.numel(), t.get_device()) != kind or not t.is_contiguous():
+                    _refuse(self.name, "kept inputs of the types, shapes and devices they had")
                 args[i] = t.data_ptr()
         for i in self.outputs:
             args[i] = None

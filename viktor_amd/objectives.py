@@ -22,8 +22,7 @@ class _Objective(torch.autograd.Function):
     def forward(ctx, logits, op, outputs, args, grad):
         res, launch = op(logits.detach(), *args, grad)
         if grad:
-            ctx.save_for_backward(logits, *launch.tensors)
-            launch.tensors = None
+            ctx.save_for_backward(logits, *launch.keep(logits))
             ctx.launch, ctx.dlogits = launch, res["dlogits"]
         others = [res[name] for name in outputs]
         ctx.mark_non_differentiable(*(t for t in others if t is not None))
