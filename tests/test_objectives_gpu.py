@@ -724,6 +724,22 @@ def test_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(got, want)), k
 
 
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_backward_captured_without_its_forward_computes_the_gradient(which, monkeypatch):
+    """Its replays would find what the last user of the gradient left in it: it is not taken from the forward then."""
+    z, calls = objective_calls()
+    loss_fn, score, _, kw = calls[which]
+    want = score(z, **kw)["dlogits"]
+    leaf = z.clone().requires_grad_(True)
+    for captured in (True, False):
+        monkeypatch.setattr(objectives, "_capturing", lambda: False)
+        loss = loss_fn(leaf, **kw)[0]
+        loss.grad_fn.dlogits.zero_()
+        monkeypatch.setattr(objectives, "_capturing", lambda: captured)
+        got = torch.autograd.grad(loss, leaf)[0]
+        assert torch.equal(got, want if captured else torch.zeros_like(want))
+
+
 # ---- refusals that need device tensors ----------------------------------------------------------------------------------
 
 def test_refusals():

@@ -8,7 +8,9 @@
 Each is one autograd node whose forward computes the gradient beside the loss, in the logits' type: a row of logits is read
 once and its gradient written once. The first backward hands that gradient out; where the loss's own gradient is not 1 (a
 scaled or summed loss) the kernel runs again with that factor in its place, so that the result is rounded once. It looks at
-the factor on the device: nothing waits. A second backward through a kept graph computes the gradient anew.
+the factor on the device: nothing waits. A second backward through a kept graph computes the gradient anew, and so does one
+that is captured without its forward. (One captured in a graph of its own, apart from its forward's, is replayed once for each
+replay of that.)
 """
 
 import torch
@@ -17,13 +19,16 @@ from torch.autograd.function import once_differentiable
 from . import hip_ops as ops
 
 
+_capturing = torch.cuda.is_current_stream_capturing
+
+
 class _Objective(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, op, outputs, args, grad):
         res, launch = op(logits.detach(), *args, grad)
         if grad:
             ctx.save_for_backward(logits, *launch.keep(logits))
-            ctx.launch, ctx.dlogits = launch, res["dlogits"]
+            ctx.launch, ctx.dlogits, ctx.captured = launch, res["dlogits"], _capturing()
         others = [res[name] for name in outputs]
         ctx.mark_non_differentiable(*(t for t in others if t is not None))
         ctx.set_materialize_grads(False)
@@ -36,8 +41,9 @@ class _Objective(torch.autograd.Function):
             return None, None, None, None, None
         logits, *tensors = ctx.saved_tensors  # (raises if an input has been written to since)
         dl, ctx.dlogits = ctx.dlogits, None   # (handed out once: a caller may keep it as its gradient)
-        there = dl is not None
-        if not there:
+        # (a backward captured without its forward writes the gradient at every replay: nothing else would)
+        there = dl is not None and ctx.captured == _capturing()
+        if dl is None:
             dl = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         ctx.launch.again(logits, tensors, dl, g_loss, there)
         return dl, None, None, None, None
