@@ -165,6 +165,44 @@ def test_policy_masked_vocabulary_entries():
         check_gradient(got["dlogits"], leaf, want["loss"], BF16, 8 * plain.lp_tolerance(z[z > -1e30], 343), "masked entries")
 
 
+@pytest.mark.parametrize("V", [20, 343])
+def test_policy_of_far_and_impossible_tokens(V):
+    """A target's logit far below the row's maximum, or -inf: the ratio exp(lp - old_lp) keeps its 32 bits down to the type's
+    smallest numbers and is 0 at last; a reference policy that rules a token out has an infinite kl with a finite slope."""
+    B, T = 2, 8
+    z, _, _, g = logits_of(B, T, V, F32, 77, sure=False)
+    y = torch.randint(0, V, (B, T), generator=g, device=DEV)
+    mask = torch.ones(B, T, dtype=torch.bool, device=DEV)
+    far = torch.tensor([0.0, -12.0, -25.0, -45.0, -80.0, -70.0, -700.0, -math.inf], device=DEV)
+    z = z.scatter(2, y[..., None], (z.gather(2, y[..., None])[..., 0] + far)[..., None])
+    old = torch.full((B, T), -3.0, device=DEV)
+    adv = torch.tensor([1.0, -2.0], device=DEV)
+    _, want = plain.policy(z, y, mask, old, adv)
+    got = ops.policy_score(z, y, mask, old, adv)
+    assert bool(torch.isfinite(got["loss"])) and not bool(got["dlogits"].isnan().any())
+    assert bool(((got["lp"] == -math.inf) == (far == -math.inf)).all())
+    # the ratio's error: that of lp, 5e-7 of the sum's logarithm in 32-bit terms at most, and 2^-24 of its rounding
+    inner = want["pg"][0, :7].abs() > 1e-37
+    off = ((got["pg"][0, :7] - want["pg"][0, :7]).abs() / want["pg"][0, :7].abs().clamp(min=1e-300))[inner]
+    assert bool((off < 1e-6).all())
+    # the gradient: c (onehot - p), c = A r / n below the clip's border for A > 0, 0 for A < 0 (the clip's side is the lesser)
+    lp = torch.log_softmax(z.double(), -1)
+    c = (torch.exp(lp.gather(2, y[..., None])[..., 0] + 3.0) * 1.0 / (B * T))[0, 1:]
+    one = torch.nn.functional.one_hot(y, V).double()
+    grad = -c[:, None] * (one - lp.exp())[0, 1:]
+    # (p: |z - top| < 24 rounded to 32 bits twice, 2^-24 of 24 and 0.69 of 2^-24 of 35, 2.9e-6; c and the exponential, 6e-7)
+    assert bool(((got["dlogits"][0, 1:].double() - grad).abs() <= 4e-6 * grad.abs() + 1e-37).all())
+    assert not bool(got["dlogits"][1, 1:].any())
+    ref = torch.full((B, T), -math.inf, device=DEV)
+    ref[:, 4:] = -3.0
+    got = ops.policy_score(z[:, :6].contiguous(), y[:, :6].contiguous(), mask[:, :6], old[:, :6], adv * 0, ref[:, :6], kl_coef=0.5)
+    x = ref[:, :6].double() - lp.gather(2, y[..., None])[:, :6, 0]
+    c = 0.5 * -torch.expm1(x) / (B * 6)
+    grad = c[..., None] * (one - lp.exp())[:, :6]
+    assert bool((got["kl"][:, :4] == math.inf).all()) and float(got["loss"]) == math.inf
+    assert bool(((got["dlogits"].double() - grad).abs() <= 4e-6 * grad.abs() + 1e-37).all())
+
+
 def test_policy_clip_and_its_borders():
     """Ratios of exactly 1, inside, and past each border with both signs: clipped tokens have no gradient from the
     objective. Two logits, where log-probabilities are known."""

@@ -189,7 +189,7 @@ __device__ __forceinline__ PolicyTerms policy_terms(double lp, float old_lp, flo
   PolicyTerms t;
   t.lp = lp;
   const double d = lp - static_cast<double>(old_lp), A = static_cast<double>(adv);
-  const double r = exp_beyond_line(d) + 1.0 + d;
+  const double r = exp_64(d);
   const double cut = r < lo ? lo : r > hi ? hi : r;
   const double a1 = r * A, a2 = cut * A;
   const double inner = (r >= lo && r <= hi) ? A : 0.0;
@@ -204,7 +204,7 @@ __device__ __forceinline__ PolicyTerms policy_terms(double lp, float old_lp, flo
     t.kl = exp_beyond_line(x);
     if (kl_coef != 0.0) {
       t.loss += kl_coef * t.kl;
-      g -= kl_coef * (t.kl + x);
+      g -= kl_coef * (x < -40.0 ? -1.0 : t.kl + x);  // (exp(x) - 1: of -inf too)
     }
   }
   t.g = static_cast<float>(g);

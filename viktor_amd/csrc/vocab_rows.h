@@ -484,7 +484,7 @@ __device__ __forceinline__ double series_beyond_line(double x) {
 }
 // exp(x) - 1 - x beyond: x halved until it is under 1/2, then expm1(2 y) = expm1(y) (expm1(y) + 2). A call: few tokens need
 // it, and its registers would be taken from every row.
-__device__ __attribute__((noinline)) double exp_far_beyond_line(double x) {
+static __device__ __attribute__((noinline)) double exp_far_beyond_line(double x) {
   int m;
   frexp(x, &m);
   const bool huge = !(fabs(x) <= 800.0);
@@ -494,9 +494,22 @@ __device__ __attribute__((noinline)) double exp_far_beyond_line(double x) {
   for (; m >= 0; --m) e *= e + 2.0;
   return e - x;
 }
+// exp(x) for |x| >= 1/2: halved likewise, then squared (off by 1e-10 of it at 10, 1e-8 at 700).
+static __device__ __attribute__((noinline)) double exp_far(double x) {
+  int m;
+  frexp(x, &m);
+  if (!(fabs(x) <= 800.0)) return x > 0.0 ? INFINITY : x < 0.0 ? 0.0 : x;
+  const double y = ldexp(x, -(m + 1));
+  double e = 1.0 + (y + series_beyond_line(y));
+  for (; m >= 0; --m) e *= e;
+  return e;
+}
 // exp(x) - 1 - x without cancellation
 __device__ __forceinline__ double exp_beyond_line(double x) {
   return fabs(x) < 0.5 ? series_beyond_line(x) : exp_far_beyond_line(x);
+}
+__device__ __forceinline__ double exp_64(double x) {
+  return fabs(x) < 0.5 ? 1.0 + (x + series_beyond_line(x)) : exp_far(x);
 }
 
 // Threads of a workgroup that holds groups of GL; a thread's group, known to be the same for a wavefront where it is (row
