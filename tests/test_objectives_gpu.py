@@ -293,6 +293,25 @@ def test_preference_both_ways_of_the_pairs(B, T, P):
     check_preference(z, y, mask, ref, beta=0.05, lengths=1 + torch.rand(B, generator=g, device=DEV))
 
 
+def test_preference_of_impossible_calls():
+    """A call with a token of probability 0 has a log-ratio of -inf: its pair's margin is infinite, and the loss of a pair that
+    is as sure as that on the right side is 0 without smoothing, infinite with it."""
+    z, y, _, _ = logits_of(4, 6, 343, BF16, 78)
+    mask = torch.ones(4, 6, dtype=torch.bool, device=DEV)
+    for call, smoothing, loss in ((1, 0.0, None), (1, 0.1, math.inf), (0, 0.0, math.inf), (0, 1.0, None), (1, 1.0, math.inf)):
+        x = z.clone()
+        x[call, 2, y[call, 2]] = -math.inf
+        got = ops.preference_score(x, y, mask, smoothing=smoothing)
+        assert got["margin"][0] == (math.inf if call else -math.inf)
+        _, want = plain.preference(z[2:], y[2:], mask[2:], smoothing=smoothing)
+        if loss is None:  # the other pair's alone
+            near(got["loss"], want["loss"] / 2, 1e-6 * (1 + float(want["loss"].detach())), "loss")
+            assert not bool(got["dlogits"][:2].any())
+        else:
+            assert float(got["loss"]) == loss
+        assert not bool(got["dlogits"].isnan().any())
+
+
 def test_preference_far_margins_and_what_does_not_count():
     """Margins of hundreds either way (no overflow), NaN where nothing counts."""
     z, y, mask, old, ref, g = policy_inputs(6, 20, 343, BF16, 8)

@@ -379,7 +379,8 @@ __device__ __forceinline__ double pair_terms(const double *ratio, const int64_t 
   double h = 0.0, dh = 0.0, loss = 0.0;
   if (c >= 0 && c < B && r >= 0 && r < B) {
     h = beta * (ratio[c] - ratio[r]) - target;
-    loss = (1.0 - smoothing) * softplus(-h) + smoothing * softplus(h);
+    // (a side without weight is left out: the margin may be infinite)
+    loss = (smoothing < 1.0 ? (1.0 - smoothing) * softplus(-h) : 0.0) + (smoothing > 0.0 ? smoothing * softplus(h) : 0.0);
     // sigma(h) - (1 - smoothing), without cancellation where the margin is far
     dh = inv_n * beta * (smoothing * logistic(h) - (1.0 - smoothing) * logistic(-h));
   }
