@@ -479,6 +479,23 @@ def test_top_equal_logits(V, dtype):
         check_top(z, k)
 
 
+@pytest.mark.parametrize("V", [7, 343, 5463, 87383, 200001])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_top_log_sum_exp_of_rows_with_nan(V, dtype):
+    """NaN wherever a logit is, whatever the others are; the lists are of the others."""
+    z = torch.zeros(6, V, dtype=dtype, device=DEV)
+    z[0] = math.nan
+    z[1, V // 2:] = math.nan
+    z[2] = -math.inf
+    z[2, V - 1] = math.nan
+    z[3, 0], z[3, 3] = math.inf, math.nan
+    z[4] = -math.inf
+    z[5, 1] = math.inf
+    values, ids, lse = ops.top_logits(z, 2)
+    assert bool(lse[:4].isnan().all()) and lse[4] == -math.inf and lse[5] == math.inf
+    assert ids.tolist() == [[-1, -1], [0, 1], [-1, -1], [0, 1], [-1, -1], [1, 0]]
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("V", [7, 343, 5463, 45000])
 def test_top_nothing_and_infinities(V, dtype):

@@ -177,6 +177,10 @@ __device__ __forceinline__ void sort_entries(Entry (&e)[R], int lane) {
   }
 }
 
+// What a row's log-sum-exp has beyond its maximum, from the sum of exponentials by it (by 0 where it is infinite: NaN then if
+// a logit is).
+__device__ __forceinline__ double log_beyond(float top, float s) { return isinf(top) && !isnan(s) ? 0.0 : log_near(s); }
+
 template <typename T>
 __device__ __forceinline__ void write_entry(T *values, int32_t *ids, int64_t at, float value, int id) {
   store_one(values + at, value);
@@ -259,12 +263,13 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::TOP_WAVES) void top_ro
       turn = (turn + 1) % WAVES;
     }
     s = 0.f;
-    r.values([&](float x) { s += exp_near(x, top, scale); });
+    const float base = isinf(top) ? 0.f : top;
+    r.values([&](float x) { s += exp_near(x, base, scale); });
     r.keep();
     s = group_add<GL>(s, sums);
     if constexpr (GL > 64) bound = bound_sh;
     if (lane == 0)
-      lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (isinf(top) ? 0.0 : log_near(s)));
+      lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + log_beyond(top, s));
     // each wavefront's candidates, in its own part of the list
     const float least = bound ? of_key(bound) : -FLT_MAX;
     int n = 0;
@@ -367,8 +372,9 @@ __global__ __launch_bounds__(256) void top_lanes_kernel(const void *logits, int6
   r.load(static_cast<const T *>(logits) + b * ld_b + t * ld_t, V, 0);
   float top = -INFINITY, s = 0.f;
   r.values([&](float x) { top = fmaxf(top, x); });
-  r.values([&](float x) { s += exp_of(x, top, scale); });
-  lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + (isinf(top) ? 0.0 : log_near(s)));
+  const float base = isinf(top) ? 0.f : top;
+  r.values([&](float x) { s += exp_of(x, base, scale); });
+  lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + log_beyond(top, s));
   uint32_t key[NE];
   int entries = 0;
 #pragma unroll

@@ -1434,7 +1434,7 @@ def top_logits(logits, k, temperature=1.0):
     """Each row's k (1 to 128) largest logits in falling order, equal ones the lower id first, with their ids and the
     log-sum-exp: logits [..., V] bf16 or fp32 (two or three dimensions, rows of unit stride) -> (values [..., k] of their
     type, ids int32 [..., k], lse fp32 [...] = log sum exp(logits / temperature)). Logits of -inf and NaN are no entries; a
-    list that runs out ends in value -inf, id -1. What distill_score takes as a teacher's list."""
+    list that runs out ends in value -inf, id -1; lse is NaN where a logit is. What distill_score takes as a teacher's list."""
     what = "top_logits"
     _here(what, (logits,))
     nd = logits.dim()
