@@ -203,6 +203,26 @@ def test_policy_of_far_and_impossible_tokens(V):
     assert bool(((got["dlogits"].double() - grad).abs() <= 4e-6 * grad.abs() + 1e-37).all())
 
 
+@pytest.mark.parametrize("V", [7, 20, 343, 5463, 21847, 87383, 250001])
+def test_gradient_of_rows_sure_of_their_target(V):
+    """c (1 - p) where p is next to 1 keeps its 32 bits, in the policy's gradient and in the pairs'."""
+    B, T = 2, 5
+    z, y, _, g = logits_of(B, T, V, F32, 79, sure=False)
+    mask = torch.ones(B, T, dtype=torch.bool, device=DEV)
+    z = z.clamp(-9, 9).scatter(2, y[..., None], 20.0)
+    lp = torch.log_softmax(z.double(), -1).gather(2, y[..., None])[..., 0]
+    old = lp.float()
+    adv = torch.tensor([1.0, -2.0], device=DEV)
+    zp, want = plain.policy(z, y, mask, old, adv, eps_lo=0.3, eps_hi=0.3)
+    zq, pairs = plain.preference(z, y, mask)
+    for got, leaf, loss in ((ops.policy_score(z, y, mask, old, adv, eps_lo=0.3, eps_hi=0.3), zp, want["loss"]),
+                            (ops.preference_score(z, y, mask), zq, pairs["loss"])):
+        grad = torch.autograd.grad(loss, leaf)[0].gather(2, y[..., None])
+        # (the others' exponentials: |z - top| < 30 rounded to 32 bits, and 0.69 of 43; c, 1 / s and the products: 2.7e-6)
+        off = (got["dlogits"].gather(2, y[..., None]).double() - grad).abs()
+        assert bool((grad != 0).all()) and bool((off <= 4e-6 * grad.abs()).all()), float((off / grad.abs()).max())
+
+
 def test_policy_clip_and_its_borders():
     """Ratios of exactly 1, inside, and past each border with both signs: clipped tokens have no gradient from the
     objective. Two logits, where log-probabilities are known."""

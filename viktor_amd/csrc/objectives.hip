@@ -80,6 +80,12 @@ __device__ __forceinline__ bool counts(const uint8_t *mask, const int64_t *targe
   return mask[row] != 0 && t >= 0 && t < V;
 }
 
+// The sum of a row's exponentials without its target's: 1 - p_y = that over s, which keeps its 32 bits where p_y is next to 1
+// (c - c p_y is off by 2e-7 c there).
+__device__ __forceinline__ float beyond_target(double s, float zy, float top) {
+  return static_cast<float>(s - static_cast<double>(exp_of(zy, top, kUnit)));
+}
+
 // A token's target and mask as loaded, ahead of their use.
 struct Token {
   int64_t target;
@@ -290,9 +296,10 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::WAVES_A_SIMD) void pol
       c = coef_sh;
     }
     const float k = -c / static_cast<float>(s);
+    const float rest = beyond_target(s, zy, top);
     r.write(d, lane, top, kUnit, k);
     // (after this thread's own vector that holds it)
-    if (lane == owner_of<T, GL>(r.s, y)) store_one(d + y, c + exp_of(zy, top, kUnit) * k);
+    if (lane == owner_of<T, GL>(r.s, y)) store_one(d + y, -k * rest);
   }
   if (!a.loss_parts) return;
   loss = block_sum64<group_threads(GL)>(loss, loss_sh);
@@ -302,7 +309,7 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::WAVES_A_SIMD) void pol
 // ---- paired log ratios --------------------------------------------------------------------------------------------------
 
 struct RowStats {
-  float top, rs;  // a row's maximum, one over its sum of exponentials
+  float top, rs, rest;  // a row's maximum, one over its sum of exponentials, that sum without its target's
 };
 
 struct PairArgs {
@@ -347,7 +354,7 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::RATIO_WAVES) void toke
       a.lp[row] = static_cast<float>(lp);
       // (rounded to 32 bits after the difference: off by 2^-24 of the ratio, not of lp)
       a.ratio[row] = static_cast<float>(lp - static_cast<double>(ref_lp));
-      if (a.stats) a.stats[row] = RowStats{top, 1.f / static_cast<float>(s)};
+      if (a.stats) a.stats[row] = RowStats{top, 1.f / static_cast<float>(s), beyond_target(s, zy, top)};
     }
   }
 }
@@ -483,13 +490,12 @@ __global__ __launch_bounds__(group_threads(Row::GL)) void softmax_grad_kernel(Lo
     }
     const T *z = in.row<T>(b, t);
     const int y = static_cast<int>(token.target);
-    const float zy = load_one(z + y);
     const RowStats st = a.stats[row];
     Row r;
     r.load(z, in.V, lane);
     const float k = -c * st.rs;
     r.write_fresh(d, lane, st.top, kUnit, k);
-    if (lane == owner_of<T, GL>(r.s, y)) store_one(d + y, c + exp_of(zy, st.top, kUnit) * k);
+    if (lane == owner_of<T, GL>(r.s, y)) store_one(d + y, -k * st.rest);
   }
 }
 
@@ -769,8 +775,8 @@ extern "C" int vk_objective_workspace(int64_t B, int64_t T, int64_t P, int64_t *
                    B * T < (int64_t(1) << 31),
                "objective_workspace: bad arguments");
   // partial sums of weights and loss, then per sequence a 64-bit and a 32-bit number, per pair a 64-bit one, per token a
-  // log-ratio and the row's maximum and sum
-  *bytes = 8 * (OBJ_PARTS + OBJ_BLOCKS) + 16 * B + (P > 0 ? 8 * P + 12 * B * T : 0) + 16;
+  // log-ratio and what the row's gradient needs
+  *bytes = 8 * (OBJ_PARTS + OBJ_BLOCKS) + 16 * B + (P > 0 ? 8 * P + 16 * B * T : 0) + 16;
   return VK_OK;
 }
 
