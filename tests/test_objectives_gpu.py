@@ -223,6 +223,25 @@ def test_gradient_of_rows_sure_of_their_target(V):
         assert bool((grad != 0).all()) and bool((off <= 4e-6 * grad.abs()).all()), float((off / grad.abs()).max())
 
 
+@pytest.mark.parametrize("V", [7, 20, 343, 5463, 21847, 87383])
+def test_exponentials_far_below_the_top(V):
+    """A row of one logit t above all others: 1 - p is the others' exponentials alone, and so is the target's gradient."""
+    T = 128
+    z = torch.zeros(1, T, V, device=DEV)
+    z[0, :, 3] = 10 + torch.arange(T, device=DEV) * 0.109375  # (differences without a rounding)
+    y = torch.full((1, T), 3, device=DEV)
+    mask = torch.ones(1, T, dtype=torch.bool, device=DEV)
+    old = torch.log_softmax(z.double(), -1)[..., 3].float()
+    adv = torch.ones(1, device=DEV)
+    # 1 - p without the cancellation of p in 64 bits: 2^-53 is 4e-7 of the six others' 2.8e-10
+    rest = (V - 1) * torch.exp(-z[0, :, 3].double())
+    grad = -torch.exp(-torch.log1p(rest) - old[0].double()) * rest / (1 + rest) / T
+    off = ((ops.policy_score(z, y, mask, old, adv)["dlogits"][0, :, 3].double() - grad) / grad).abs()
+    # an exponential's ulp 1.2e-7, log 2 in 32 bits 7e-8, six roundings of 2^-24; and what the others' sum loses in one of 64
+    # bits that the top's 1 is part of: 2^-53 with each addition behind it, V or a thread's 176 and the group's 16 at most
+    assert bool((off <= 6e-7 + min(V, 192) * 2.0 ** -53 / rest).all()), float(off.max())
+
+
 def test_policy_clip_and_its_borders():
     """Ratios of exactly 1, inside, and past each border with both signs: clipped tokens have no gradient from the
     objective. Two logits, where log-probabilities are known."""

@@ -9,9 +9,9 @@
 // (16 lanes to a whole workgroup, by its length) through its maximum, its sum and its gradient, and the few elements that
 // differ from c' p_v are written by themselves afterwards. Rows that count nothing are not read.
 //
-// Exponentials are fp32 (each off by about an ulp); their sums, the logarithm, log-ratios, objectives and sums over tokens are
-// 64 bits. The gradient is rounded once, to the logits' type. Every sum runs in a fixed order, which a row's address
-// modulo 16 bytes is part of.
+// Exponentials are fp32 (each off by 2e-7 at temperature 1, for distillation by up to 1e-6 far below the top); their sums,
+// the logarithm, log-ratios, objectives and sums over tokens are 64 bits. The gradient is rounded once, to the logits' type.
+// Every sum runs in a fixed order, which a row's address modulo 16 bytes is part of.
 //
 // What it reaches, of the 5.2 TB/s that a copy does: fp32 rows of 2500 to 45000 logits 4.5 to 5.3 (policy), 4.5 to 4.9
 // (distillation, lists of 32), bf16 rows 4.2 to 4.4 and 3.6 to 4.0 (their exponentials are computed twice past 6 vectors a lane,
@@ -26,7 +26,7 @@ constexpr int OBJ_BLOCKS = 2048;  // most workgroups of a pass over the rows: on
 constexpr int OBJ_PARTS = 256;    // partial sums of the tokens' weights
 
 // (temperature 1)
-constexpr ExpScale kUnit = {1.4426950216293335f, 1.925963e-8f};
+constexpr UnitScale kUnit = {};
 
 struct LogitRows {
   const void *logits;
@@ -316,7 +316,8 @@ struct PairArgs {
   const int64_t *targets;
   const uint8_t *mask;
   const float *ref_lp;
-  float *lp, *ratio;
+  float *lp;
+  double *ratio;
   RowStats *stats;
 };
 
@@ -338,7 +339,7 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::RATIO_WAVES) void toke
     if (!token.counts(in.V)) {
       if (lane == 0) {
         a.lp[row] = 0.f;
-        a.ratio[row] = 0.f;
+        a.ratio[row] = 0.0;
       }
       continue;
     }
@@ -350,23 +351,22 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::RATIO_WAVES) void toke
     double s;
     row_stats<GL>(r, kUnit, sh, top, s);
     if (lane == 0) {
-      const double lp = static_cast<double>(zy) - static_cast<double>(top) - log_of(s);
+      const double lp = static_cast<double>(zy) - static_cast<double>(top) - log_called(s);
       a.lp[row] = static_cast<float>(lp);
-      // (rounded to 32 bits after the difference: off by 2^-24 of the ratio, not of lp)
-      a.ratio[row] = static_cast<float>(lp - static_cast<double>(ref_lp));
+      a.ratio[row] = lp - static_cast<double>(ref_lp);
       if (a.stats) a.stats[row] = RowStats{top, 1.f / static_cast<float>(s), beyond_target(s, zy, top)};
     }
   }
 }
 
 // A workgroup per sequence: its log-ratio over all tokens that count, over its length where one is given.
-__global__ __launch_bounds__(256) void sequence_ratio_kernel(const float *__restrict__ ratio,
+__global__ __launch_bounds__(256) void sequence_ratio_kernel(const double *__restrict__ ratio,
                                                             const float *__restrict__ lengths, double *__restrict__ out,
                                                             int64_t T) {
   __shared__ double sh[4];
   const int64_t b = blockIdx.x;
   double v = 0.0;
-  for (int64_t t = threadIdx.x; t < T; t += 256) v += static_cast<double>(ratio[b * T + t]);
+  for (int64_t t = threadIdx.x; t < T; t += 256) v += ratio[b * T + t];
   v = block_sum64(v, sh);
   if (threadIdx.x == 0) out[b] = lengths ? v / static_cast<double>(lengths[b]) : v;
 }
@@ -437,7 +437,7 @@ __global__ __launch_bounds__(256) void sequence_slope_kernel(const double *__res
 // The three steps above in one workgroup, for calls of few tokens: two launches less. 260 tokens in 2 pairs: 28.1 -> 22.8 us;
 // 32 sequences of 147 tokens in 48 pairs take it 7 us, as long as the launches do.
 constexpr int64_t PAIRS_AT_ONCE_TOKENS = 8192, PAIRS_AT_ONCE_PAIRS = 1024;
-__global__ __launch_bounds__(1024) void pairs_at_once_kernel(const float *__restrict__ token_ratio,
+__global__ __launch_bounds__(1024) void pairs_at_once_kernel(const double *__restrict__ token_ratio,
                                                              const float *__restrict__ lengths, const int64_t *__restrict__ pairs,
                                                              int P, int B, int64_t T, double beta, double target,
                                                              double smoothing, double inv_n, double *ratio, double *slope,
@@ -447,7 +447,7 @@ __global__ __launch_bounds__(1024) void pairs_at_once_kernel(const float *__rest
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (int b = wave; b < B; b += 16) {
     double v = 0.0;
-    for (int64_t t = lane; t < T; t += 64) v += static_cast<double>(token_ratio[b * T + t]);
+    for (int64_t t = lane; t < T; t += 64) v += token_ratio[b * T + t];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
     if (lane == 0) ratio[b] = lengths ? v / static_cast<double>(lengths[b]) : v;
@@ -776,7 +776,7 @@ extern "C" int vk_objective_workspace(int64_t B, int64_t T, int64_t P, int64_t *
                "objective_workspace: bad arguments");
   // partial sums of weights and loss, then per sequence a 64-bit and a 32-bit number, per pair a 64-bit one, per token a
   // log-ratio and what the row's gradient needs
-  *bytes = 8 * (OBJ_PARTS + OBJ_BLOCKS) + 16 * B + (P > 0 ? 8 * P + 16 * B * T : 0) + 16;
+  *bytes = 8 * (OBJ_PARTS + OBJ_BLOCKS) + 16 * B + (P > 0 ? 8 * P + 20 * B * T : 0) + 16;
   return VK_OK;
 }
 
@@ -856,8 +856,9 @@ extern "C" int vk_preference_score(const void *logits, int32_t dtype, int64_t ld
   VK_CHECK_ARG(!backward || N == 0 || dlogits, "preference_score: null gradient");
   hipStream_t st = VK_STREAM(stream);
   double *ratio = static_cast<double *>(ws), *slope = ratio + B;
-  RowStats *stats = reinterpret_cast<RowStats *>(slope + (P > 0 ? P : 1));
-  float *token_ratio = reinterpret_cast<float *>(stats + N), *coef = token_ratio + N;
+  double *token_ratio = slope + (P > 0 ? P : 1);
+  RowStats *stats = reinterpret_cast<RowStats *>(token_ratio + N);
+  float *coef = reinterpret_cast<float *>(stats + N);
   const LogitRows in{logits, ld_b, ld_t, N, static_cast<uint32_t>(T), V};
   const PairArgs a{targets, mask, ref_lp, lp, token_ratio, stats};
   if (forward) {
