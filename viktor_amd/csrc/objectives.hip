@@ -616,7 +616,9 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::DISTILL_WAVES) void di
           if (i * LL >= a.K) break;
           const double x = static_cast<double>(tv[i]) * a.inv_tau - lse_q;
           const float xf = static_cast<float>(x), e = expf(xf);
-          list.q[i] = list.id[i] >= 0 ? fmaf(e, static_cast<float>(x - static_cast<double>(xf)), e) : 0.f;
+          // (beyond 32 bits, as the type's lowest value over a small temperature is, the narrowing leaves no remainder)
+          const float exact = e > 0.f && e < INFINITY ? fmaf(e, static_cast<float>(x - static_cast<double>(xf)), e) : e;
+          list.q[i] = list.id[i] >= 0 ? exact : 0.f;
         }
       } else {
 #pragma unroll
