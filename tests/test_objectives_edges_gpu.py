@@ -47,3 +47,26 @@ def test_distill_lists_that_end_in_the_lowest_value(V, vdtype, tau):
     val, ids, lse = ops.top_logits(t, K, tau)
     check_distill(z, val, ids, temperature=tau)
     check_distill(z, val, ids, temperature=tau, t_lse=lse)
+
+
+@pytest.mark.parametrize("tau", [0.7, 1.0, 2.0])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [7, 343, 5463, 25000, 190000])
+def test_distill_rows_of_the_lowest_value(V, dtype, tau):
+    """A row whose mask leaves nothing, written as the type's lowest value, is a uniform one: of the student, of the list, of
+    both. So is a row of one far value, and one of a large common size keeps its differences."""
+    z, _, _, _, _, g = policy_inputs(2, 5, V, dtype, V)
+    K = min(V, 16)
+    val, ids, lse = lists(z, K, g, dtype, torch.int32, tau)
+    low = torch.finfo(dtype).min
+    z[0, 0], z[0, 1], z[0, 2] = low, 1e30, -1e37
+    z[1, 0] = low
+    z[1, 1] = 2.0 ** 20 + 8192 * torch.randint(0, 2, (V,), generator=g, device=DEV)  # (in either type without a rounding)
+    z[1, 2] = low
+    z[1, 2, ids[1, 2].long()] = 1.0  # (what the list does not name is masked)
+    val[1, 0] = low
+    val[1, 3] = low
+    val[1, 4] = -1e33
+    check_distill(z, val, ids, temperature=tau)
+    lse[1, 0], lse[1, 3], lse[1, 4] = 5.0, 6.0, 7.0  # (no weight at all against a teacher's sum)
+    check_distill(z, val, ids, temperature=tau, t_lse=lse, inv_n=0.1)

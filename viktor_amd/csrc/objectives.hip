@@ -581,10 +581,11 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::DISTILL_WAVES) void di
     const T *z = in.row<T>(b, t);
     Row r;
     r.load(z, in.V, lane);
-    // the list, with the group's first lanes: weights q, their sum, and sum q (t - z) / tau
+    // the list, with the group's first lanes: weights q, their sum, and sum q (log q - (z - near) / tau) by its largest student
+    // logit, `near` (not by 0: a row masked by the type's lowest value would lose its logarithms beside 1e38)
     TeacherList<LL, LONGEST> list;
-    double cross = 0.0, lse_q = 0.0, mass64 = 0.0;
-    float mass = 0.f;
+    double cross = 0.0, mass64 = 0.0;
+    float mass = 0.f, near = -FLT_MAX;
     bool twice = false;
     if (holds) {
       float tv[TeacherList<LL, LONGEST>::N], most = -INFINITY;
@@ -609,8 +610,8 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::DISTILL_WAVES) void di
         most = fmaxf(most, x);
       }
       // weights q: the entries' exponentials over their sum, or over the teacher's
+      const double lse_q = a.t_lse ? static_cast<double>(a.t_lse[row]) : 0.0;
       if (a.t_lse) {
-        lse_q = static_cast<double>(a.t_lse[row]);
 #pragma unroll
         for (int i = 0; i < TeacherList<LL, LONGEST>::N; ++i) {
           if (i * LL >= a.K) break;
@@ -620,6 +621,7 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::DISTILL_WAVES) void di
           const float exact = e > 0.f && e < INFINITY ? fmaf(e, static_cast<float>(x - static_cast<double>(xf)), e) : e;
           list.q[i] = list.id[i] >= 0 ? exact : 0.f;
         }
+        most = 0.f;
       } else {
 #pragma unroll
         for (int o = LL / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, kWave));
@@ -632,10 +634,19 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::DISTILL_WAVES) void di
 #pragma unroll
       for (int i = 0; i < TeacherList<LL, LONGEST>::N; ++i) {
         if (i * LL >= a.K) break;
+        if (list.q[i] != 0.f) near = fmaxf(near, list.zt[i]);
+      }
+#pragma unroll
+      for (int o = LL / 2; o > 0; o >>= 1) near = fmaxf(near, __shfl_xor(near, o, kWave));
+#pragma unroll
+      for (int i = 0; i < TeacherList<LL, LONGEST>::N; ++i) {
+        if (i * LL >= a.K) break;
         if (list.id[i] < 0) continue;
         mass64 += static_cast<double>(list.q[i]);
         if (list.q[i] != 0.f)
-          cross += static_cast<double>(list.q[i]) * (static_cast<double>(tv[i]) - static_cast<double>(list.zt[i]));
+          cross += static_cast<double>(list.q[i]) *
+                   (((static_cast<double>(tv[i]) - static_cast<double>(most)) * a.inv_tau - lse_q) -
+                    (static_cast<double>(list.zt[i]) - static_cast<double>(near)) * a.inv_tau);
         if (d) {
           const uint32_t bit = 1u << (list.id[i] & 31);
           twice |= (atomicOr(&bits[(list.id[i] & (BITS - 1)) >> 5], bit) & bit) != 0;
@@ -647,11 +658,9 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::DISTILL_WAVES) void di
         cross += __shfl_xor(cross, o, kWave);
         twice |= __shfl_xor(static_cast<int>(twice), o, kWave) != 0;
       }
-      cross *= a.inv_tau;
       mass = static_cast<float>(mass64);
       if (!a.t_lse && mass64 != 0.0) {
-        cross /= mass64;
-        lse_q = static_cast<double>(most) * a.inv_tau + log_called(mass64);
+        cross = cross / mass64 - log_called(mass64);
         const float rs = static_cast<float>(1.0 / mass64);
 #pragma unroll
         for (int i = 0; i < TeacherList<LL, LONGEST>::N; ++i) list.q[i] *= rs;
@@ -676,9 +685,10 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::DISTILL_WAVES) void di
     if constexpr (GL > 64) mass = mass_sh;
     const double share = static_cast<double>(w) * w_all * a.tau;
     if (ll == 0) {
-      // sum q (log q - log p) = sum q (t - z) / tau + Q (lse_p - lse_q)
-      const double kl = mass == 0.f ? 0.0
-                                    : cross + mass64 * (static_cast<double>(top) * a.inv_tau + log_called(s) - lse_q);
+      // sum q (log q - log p), log p = (z - top) / tau - log s
+      const double kl =
+          mass == 0.f ? 0.0
+                      : cross + mass64 * ((static_cast<double>(top) - static_cast<double>(near)) * a.inv_tau + log_called(s));
       loss += share * a.tau * kl;
       if (a.kl) a.kl[row] = static_cast<float>(kl);
     }
