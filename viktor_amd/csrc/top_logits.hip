@@ -74,6 +74,12 @@ struct RowStrided {
 #pragma unroll
     for (int i = 0; i < NE; ++i) f(z[i]);
   }
+  __device__ __forceinline__ float sum_near(float top, ExpScale scale) const {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) sum += exp_near(z[i], top, scale);
+    return sum;
+  }
   template <typename F>
   __device__ __forceinline__ void each(int lane, F f) const {
 #pragma unroll
@@ -212,7 +218,8 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::TOP_WAVES) void top_ro
   constexpr int OWN = WAVES == 1 ? 512 : WAVES <= 4 ? 256 : 128;
   __shared__ Entry cand[GROUPS * WAVES][OWN];
   __shared__ int found[GROUPS * WAVES], taken[GROUPS];
-  __shared__ float sh[WAVES], sums[WAVES];
+  __shared__ float sh[WAVES];
+  __shared__ decltype(Row().sum_near(0.f, ExpScale())) sums[WAVES];
   __shared__ int shc[WAVES];
   __shared__ uint32_t maxima[GL > 64 ? GL : 1], bound_sh;
   const int lane = lane_of<GL>(), group = group_of<GL>(), l64 = threadIdx.x & 63;
@@ -231,7 +238,7 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::TOP_WAVES) void top_ro
     r.keep();
     // A bound from the threads' maxima: by the wavefront itself or, in a workgroup, by one of its wavefronts in turn while the
     // others are at their sums.
-    float top, s;
+    float top;
     uint32_t bound = 0;
     if constexpr (GL == 64) {
       top = group_max<GL>(mine, sh);
@@ -262,11 +269,9 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::TOP_WAVES) void top_ro
       }
       turn = (turn + 1) % WAVES;
     }
-    s = 0.f;
-    const float base = isinf(top) ? 0.f : top;
-    r.values([&](float x) { s += exp_near(x, base, scale); });
+    const auto part = r.sum_near(isinf(top) ? 0.f : top, scale);
     r.keep();
-    s = group_add<GL>(s, sums);
+    const float s = static_cast<float>(group_add<GL>(part, sums));
     if constexpr (GL > 64) bound = bound_sh;
     if (lane == 0)
       lse[row] = static_cast<float>(static_cast<double>(top) * inv_tau + log_beyond(top, s));
