@@ -604,7 +604,7 @@ def gspo_update(model, opt: HipAdamW, frames, plens, calls, ended, reward, G, up
             loss.backward()
             stats["pg"] += float(pg.sum())
             stats["n"] += len(mb)
-            stats["clip"] += float(((s - 1).abs() > eps).sum())
+            stats["clip"] += float(((s - 1 < -eps) | (s - 1 > eps_hi)).sum())
             stats["ratio"] += float((s - 1).abs().sum())
         if sft_weight and labels is not None:
             for i in range(0, len(wins), micro):
