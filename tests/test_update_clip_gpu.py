@@ -28,3 +28,18 @@ def test_sequence_objective_counts_what_its_borders_clip(eps, eps_hi, each, monk
     kw = {} if eps_hi is None else {"eps_hi": eps_hi}
     st = TR.gspo_update(m, opt, fr, plens, calls, ended, reward, G, updates=1, micro=3, eps=eps, **kw)
     assert st["n"] == 6 and st["clip"] == 2 * each
+
+
+@pytest.mark.parametrize("kw,want", [({}, 4e-4), ({"objective": "token"}, 0.2), ({"objective": "token", "eps": 0.1}, 0.1),
+                                     ({"eps": 0.1}, 0.1)])
+def test_clip_by_default(kw, want, monkeypatch):
+    """A sequence's ratio is a mean over its length, a token's is not: each objective's clip is its own by default."""
+    fr, plens, calls, ended, reward, G = _inputs(11)
+    seen = []
+    for name, at in (("sequence_ratio_loss", 6), ("token_policy_loss", 6)):
+        real = getattr(TR, name)
+        monkeypatch.setattr(TR, name, lambda *args, _real=real, _at=at, **more: (seen.append(args[_at:_at + 2]),
+                                                                                 _real(*args, **more))[1])
+    m = make_model(1, n_layers=1, seed=71).to(DEV)
+    TR.gspo_update(m, TR.HipAdamW(list(m.parameters()), lr=1e-4), fr, plens, calls, ended, reward, G, updates=1, micro=3, **kw)
+    assert seen and all(s == (want, want) for s in seen)

@@ -519,7 +519,7 @@ def _token_lp(logits, targets, mask):
     return ops.policy_score(logits, targets, mask, zero, zero, grad=False)["lp"]
 
 
-def gspo_update(model, opt: HipAdamW, frames, plens, calls, ended, reward, G, updates=2, micro=32, eps=4e-4,
+def gspo_update(model, opt: HipAdamW, frames, plens, calls, ended, reward, G, updates=2, micro=32, eps=None,
                 std_floor=0.003, labels=None, weights=None, sft_weight=0.0, objective="sequence", eps_hi=None,
                 ref_model=None, kl_coef=0.0):
     """The GSPO policy update of one rollout (scripts/gspo.py:446-493 on one GPU, without the all-reduce):
@@ -532,7 +532,9 @@ def gspo_update(model, opt: HipAdamW, frames, plens, calls, ended, reward, G, up
 
     objective "token": the clipped policy loss per token instead (objectives.token_policy_loss: each call's tokens averaged,
     then the calls), with kl_coef times the KL term to ref_model, a frozen policy, where one is given; its statistics are
-    sums over the calls of their tokens' means, kl among them. eps_hi: the clip's upper border (eps by default)."""
+    sums over the calls of their tokens' means, kl among them. eps: the clip's borders 1 - eps and 1 + eps, by default 4e-4
+    for a sequence's ratio (scripts/gspo.py's, a mean over its length) and 0.2 for a token's, which moves by far more; eps_hi:
+    the upper one (eps by default)."""
     from .gspo import advantages
     import numpy as np
     if objective not in ("sequence", "token"):
@@ -542,6 +544,8 @@ def gspo_update(model, opt: HipAdamW, frames, plens, calls, ended, reward, G, up
         raise ValueError("gspo_update: the KL term goes with objective 'token'")
     if kl_coef and ref_model is None:
         raise ValueError("gspo_update: the KL term needs ref_model")
+    if eps is None:
+        eps = 0.2 if per_token else 4e-4
     eps_hi = eps if eps_hi is None else eps_hi
     B = frames.shape[0]
     adv, live = advantages(np.asarray(reward, dtype=np.float64).reshape(B, G), std_floor=std_floor)
