@@ -705,7 +705,8 @@ int vk_policy_score(const void *logits, int32_t dtype, int64_t ld_b, int64_t ld_
  * fp32 [B], positive, NULL: 1); pair p = (chosen, rejected) = pairs[2 p], pairs[2 p + 1] (int64; NULL: sequences 2 p and
  * 2 p + 1, B = 2 P): margin_p = beta (S_chosen - S_rejected) - target,
  * loss = inv_n sum_p (1 - smoothing) softplus(-margin_p) + smoothing softplus(margin_p).
- * A sequence may be in any number of pairs; a pair with an index outside [0, B) has margin 0 and counts nothing.
+ * A sequence may be in any number of pairs; a pair with an index outside [0, B) has margin 0 and counts nothing. Every
+ * sequence looks at every pair: made for some thousand of them.
  * parts: 1 = loss, margin [P], lp [B, T]; 2 = dlogits, from what part 1 left in the workspace; 3 = both. No counterpart in
  * the reference.
  */

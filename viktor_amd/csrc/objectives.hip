@@ -396,7 +396,9 @@ __device__ __forceinline__ double pair_terms(const double *ratio, const int64_t 
   return loss;
 }
 
-// The derivative of the loss by the tokens' log-probabilities of sequence b, from all pairs that name it, by a wavefront.
+// The derivative of the loss by the tokens' log-probabilities of sequence b, from all pairs that name it, by a wavefront: each
+// sequence looks at every pair, and one workgroup has the pairs' own numbers. For up to some thousand pairs: 512 sequences with
+// 1024, 8192, 65536 and 2^20 of them, 28, 72, 490 and 8350 us a call of short rows.
 __device__ __forceinline__ double sequence_slope(const double *slope, const int64_t *pairs, int64_t b, int64_t P, int lane) {
   if (!pairs) return b / 2 < P ? ((b & 1) ? -slope[b / 2] : slope[b / 2]) : 0.0;
   double v = 0.0;

@@ -4,8 +4,13 @@
 // The row stays in the registers of a wavefront (up to 512 logits, element lane + 64 i with lane `lane`; to 704 vectors of 16
 // bytes, whole vectors) or of a workgroup. A bound that at least k logits reach comes from one or a few maxima a thread: bit
 // by bit with ballots, the largest number that k of the maxima reach. What reaches it in the row (a little more than k logits
-// of most rows) goes to shared memory with its id, and one wavefront sorts it in registers. Rows with more candidates than fit
-// (many equal logits) have their k-th logit searched bit by bit over all of it, then the id up to which equal ones are taken.
+// of most rows) goes to shared memory with its id, and one wavefront sorts it in registers. Rows with more than 256 candidates
+// have their k-th logit searched bit by bit over all of it, in memory, then the id up to which equal ones are taken: some 65
+// walks. Those are rows of many equal logits, and any row just past 512 logits with a list that is long for it: a maximum of 16
+// bytes bounds little where there are hardly more vectors than entries (bf16 rows of 513 to some 1250 logits with lists of nine
+// tenths of their vectors or more, fp32 rows of 513 to 560 with lists of 120 or more). 16416 rows of 640 bf16: lists of 64 in 34
+// us, of 100 in 254; of 1000: 39 for 100, 275 for 128; of 1200 and 1367: 319 and 107 for 128; of 520 fp32: 302 for 128; of 512
+// bf16, whose bound is of single logits, 35 for 128.
 // Rows of up to 32 logits go one a thread: each logit counts the ones before it.
 // Logits of -inf and NaN are no entries: a list that runs out ends in id -1, value -inf.
 //
@@ -326,8 +331,8 @@ __global__ __launch_bounds__(group_threads(Row::GL), Row::TOP_WAVES) void top_ro
           sort_and_write<T, Entry, 4>(entry, K, values, ids, at, lane);
       }
     } else {
-      // the k-th key, bit by bit over the row (more than 256 > K logits are above -inf), then the ids of its equals. (Walked
-      // in memory: the registers of a form for this rare case would be every row's.)
+      // the k-th key, bit by bit over the row (more candidates than K, all above -inf), then the ids of its equals. (Walked in
+      // memory: the registers of a form for this would be every row's.)
       RowWalk<T, GL> w;
       w.load(z, V, lane);
       uint32_t kth = 0;

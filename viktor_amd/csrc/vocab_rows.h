@@ -312,7 +312,8 @@ struct RowRegs {
 
 // A row of up to NE elements in one thread. (Its loads and stores are 2 or 4 bytes a lane, a row's length apart; the lines
 // they share stay in the caches. 512 x 1024 rows of 7 bf16 with the policy's 64-bit numbers: 16 us, 133 with 16 lanes a row;
-// 131072 rows of 20: 28 and 52; of 64, lists of 32: 138 and 85.)
+// 131072 rows of 20: 28 and 52; of 64, lists of 32: 138 and 85. The distillation has no such form: its rows of 7 and 20 take 16
+// lanes, 512 x 1024 of them 187 and 218 us.)
 template <typename T, int NE>
 struct RowLane {
   typedef T type;
@@ -502,7 +503,9 @@ __device__ __forceinline__ double log_of(double s) {
   return s > 0.0 ? t : s == 0.0 ? -INFINITY : s;  // (NaN stays)
 }
 // The same as a call, beside a row that fills the registers: the constants of the series stay out of them
-// (2064 x 87383 fp32, distillation: 300 us inlined, 285 called; 32 x 147 x 21847 bf16, preference: 111 and 107).
+// (2064 x 87383 fp32, distillation: 300 us inlined, 285 called; 32 x 147 x 21847 bf16, preference: 111 and 107). Not all of them:
+// rows of 1024 threads of 22 vectors still have 44 (bf16) and 46 (fp32) registers in memory there, and 22 to 44 in the
+// policy's kernel, which has the logarithm inlined.
 static __device__ __attribute__((noinline)) double log_called(double s) { return log_of(s); }
 
 // The same of a sum in 32 bits, off by 3e-8 whatever its size: the exponent's part in 64 bits, the mantissa's from log1p.
@@ -574,7 +577,9 @@ __device__ __forceinline__ int lane_of() {
 // vectors a lane it loses (4704 x 21847 bf16, preference: 108 us with 64 lanes of 43, 100 with 256 of 11). 16 lanes where four
 // rows to a wavefront share the 64-bit numbers: 131072 x 343 fp32, policy, 83 us with 16 lanes of 6, 144 with 64 of 2; the
 // other way round from 100 vectors on (112500 x 800 bf16: 153 and 128). Rows past 22528 vectors are read twice: 2064 x 87383 fp32,
-// distillation, 390 us walked, 285 in registers.
+// distillation, 390 us walked, 288 in registers; of 90112 and 90300 logits, 289 and 411.
+// A row pays the exponentials of all the vectors of its form, so that one just past a form's end costs more than its bytes:
+// policy, 16416 rows of 5632 and 5640 bf16 75 and 98 us, 4704 of 11264 and 11300 51 and 65.
 template <typename F>
 inline int row_form(int64_t vectors, F f) {
 #define VK_FORM(GL, NV) \
